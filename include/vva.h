@@ -306,6 +306,92 @@ VVA_API vva_status vva_qkv_proj(vva_context* ctx, const vva_tensor* x, const vva
 VVA_API vva_status vva_out_proj_residual(vva_context* ctx, const vva_tensor* o, const vva_tensor* w_o,
                                          const vva_tensor* x, const vva_tensor* h);
 
+/* ---------------------------------------------------- many requests at once */
+
+/* Largest number of sequences of a vva_batch. */
+#define VVA_MAX_BATCH_SEQ 1024
+
+/* The sequences of one call over a paged cache.  All three tensors live on the
+ * device and are read by the kernels, so a captured step can be replayed while
+ * the sequences grow and change: only the shapes are fixed.
+ *   q_start: I32 ne = [n_seq + 1]: the packed token rows of sequence s are
+ *            q_start[s] .. q_start[s + 1] - 1 (n_s of them, 0 allowed);
+ *   kv_len:  I32 ne = [n_seq]: keys of the sequence, its n_s new ones included;
+ *            new token t is key kv_len[s] - n_s + t;
+ *   table:   I32 ne = [max_pages, n_seq], contiguous rows of any stride: page
+ *            table[s][i / page_size] of the pool holds key i in its slot
+ *            i % page_size.  Entries past a sequence's keys are not read.
+ *   max_new: no sequence of the call brings more new tokens (the rows of one
+ *            that does are computed up to here).
+ * n_seq <= VVA_MAX_BATCH_SEQ.  Values that point outside are kept inside:
+ * q_start is cut to the token rows there are, kv_len to the table's row. */
+typedef struct {
+    vva_tensor q_start;
+    vva_tensor kv_len;
+    vva_tensor table;
+    int32_t    max_new;
+} vva_batch;
+
+/* A layer's cache in pages is two tensors of the caller's, one for K and one
+ * for V: ne = [head_dim, page_size, n_kv_heads, n_pages], F16 or BF16, rows
+ * contiguous, any other strides (of 16 bytes' multiples; the memory order
+ * [page][head][slot][dim] of a contiguous tensor streams best).  head_dim is 64
+ * or 128, page_size a power of two from 16 to 1024 (otherwise
+ * VVA_ERR_NOT_IMPLEMENTED).  Sequences may share pages they only read. */
+
+/* RoPE of packed rows and their append into the pages: vva_rope_append for
+ * the tokens of a batch.
+ *   q: ne = [d, Hq, N]   k, v: ne = [d, Hkv, N]   (F32 / F16 / BF16, 16-byte
+ *      aligned rows);
+ *   rope: F32 ne = [d, n_pos], 16-byte aligned rows: the cosines of a
+ *      position's d / 2 angles, then the sines.  vva_rope_ext of rows that
+ *      hold d / 2 ones, then zeros, writes them, with the angles of
+ *      vva_rope_append (the results are then the same bits);
+ *   pos: I32 ne = [N], or NULL: each token's index in its sequence;
+ *   q_out: ne = [d, Hq, N], F32 / F16 / BF16 (may be q itself where the types
+ *      match), receives RoPE(q).
+ * Writes RoPE(k) and v, rounded to the pages' type, to the tokens' slots.
+ * A token whose page id is outside the pool, or which belongs to no sequence,
+ * or lies before key 0, is not appended; a position outside the table gives
+ * NaN.  q_out rows of no sequence are left as they were. */
+VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, const vva_tensor* k,
+                                         const vva_tensor* v, const vva_tensor* rope, const vva_tensor* pos,
+                                         const vva_batch* batch, const vva_tensor* k_pages,
+                                         const vva_tensor* v_pages, const vva_tensor* q_out);
+
+/* Causal grouped-query attention of a batch's new tokens over the pages:
+ * vva_attn for packed sequences, each with any number of new tokens behind any
+ * number of keys (whole prompts, chunks and single tokens in one call).
+ *   q:   ne = [d, Hq, N], already RoPE'd, in the pages' type;
+ *   out: ne = [d, Hq, N], in that type too, apart from q's memory;
+ *   scale: a finite number above 0.
+ * Token t of sequence s sees keys 0 .. kv_len[s] - n_s + t; one that sees none
+ * gets zeros.  Rows of no sequence are left as they were; a sequence with a
+ * page id outside the pool among its keys gets NaN.  What is stored behind the
+ * keys of a sequence (NaN included) does not matter.  The products run on the
+ * matrix cores in the pages' type with F32 sums, the probabilities rounded to
+ * that type; the softmax is F32.
+ * Every row of q and out and every page row starts on 16 bytes. */
+VVA_API vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, const vva_tensor* k_pages,
+                                  const vva_tensor* v_pages, const vva_batch* batch, float scale,
+                                  const vva_tensor* out);
+
+/* Residual addition and root-mean-square norm, the ggml_add and the
+ * ggml_rms_norm + ggml_mul before the projections (src/qwen2.cpp:250-275):
+ *   h = x + add,  y = h / sqrt(mean(h^2) + eps) * w
+ *   x, add: ne = [hidden, T, B], F32 / F16 / BF16; add may be NULL (h = x);
+ *   w:   F32 ne = [hidden];
+ *   sum: ne = [hidden, T, B], F32 / F16 / BF16, receives h (NULL: not kept);
+ *        may be x or add itself where the types match;
+ *   y:   ne = [hidden, T, B], F32 / F16 / BF16, or Q8_0 blocks along hidden
+ *        (then hidden is a multiple of 32; scale amax / 127, codes
+ *        round(y * 127 / amax), as in the Q8_0 caches); may be x or add itself
+ *        where the types match.
+ * Everything is computed in F32 from the unrounded h.  hidden <= 16384, rows
+ * contiguous, any strides between them; eps >= 0. */
+VVA_API vva_status vva_add_rms_norm(vva_context* ctx, const vva_tensor* x, const vva_tensor* add, const vva_tensor* w,
+                                    float eps, const vva_tensor* sum, const vva_tensor* y);
+
 /* Capability probe — analogue of backend_supports_flash_attn()
  * (src/backend.cpp:157-196).  Returns 1 if vva_attn / vva_flash_attn_ext can
  * run this combination on the context's device, 0 otherwise. */

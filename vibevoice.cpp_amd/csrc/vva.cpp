@@ -1460,3 +1460,190 @@ extern "C" vva_status vva_decode_step(vva_context* ctx, vva_kv* kv, int layer, c
     ctx->last_splits = n_splits;
     return VVA_OK;
 }
+
+// ---------------------------------------------------- many requests at once
+
+namespace {
+
+bool al16(const vva_tensor* t, int dims) {
+    bool ok = (uintptr_t)t->data % 16 == 0;
+    for (int i = 1; i <= dims; ++i) ok = ok && (t->ne[i] == 1 || t->nb[i] % 16 == 0);
+    return ok;
+}
+
+// Packed token rows ne = [d, H, N]: a float type, contiguous 16-byte aligned rows.
+vva_status check_packed(vva_context* ctx, const vva_tensor* t, const char* name, int64_t d, int64_t H, int64_t N) {
+    vva_status st = check_rows(ctx, t, name, d, H, N, 1);
+    if (st != VVA_OK) return st;
+    if (!al16(t, 2)) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: rows must be 16-byte aligned", name);
+    return VVA_OK;
+}
+
+// A contiguous I32 row of n elements.
+vva_status check_ints(vva_context* ctx, const vva_tensor* t, const char* name, int64_t n) {
+    vva_status st = check_tensor(ctx, t, name);
+    if (st != VVA_OK) return st;
+    if (t->type != VVA_TYPE_I32 || t->nb[0] != 4 || (uintptr_t)t->data % 4)
+        return fail(ctx, VVA_ERR_INVALID_ARG, "%s must be contiguous I32", name);
+    if (t->ne[0] != n || t->ne[1] * t->ne[2] * t->ne[3] != 1)
+        return fail(ctx, VVA_ERR_INVALID_ARG, "%s: ne[0]=%lld, expected %lld (one row)", name, (long long)t->ne[0], (long long)n);
+    return VVA_OK;
+}
+
+// Pages and batch of a call over N packed tokens, into p (all but q and out).
+vva_status fill_paged(vva_context* ctx, const char* what, const vva_tensor* kp, const vva_tensor* vp, const vva_batch* b,
+                      int64_t Hq, int64_t N, PagedArgs& p) {
+    vva_status st;
+    if ((st = check_tensor(ctx, kp, "k_pages")) != VVA_OK) return st;
+    if ((st = check_tensor(ctx, vp, "v_pages")) != VVA_OK) return st;
+    const int64_t d = kp->ne[0], ps = kp->ne[1], Hkv = kp->ne[2], n_pages = kp->ne[3];
+    if (kp->type != vp->type || (kp->type != VVA_TYPE_F16 && kp->type != VVA_TYPE_BF16))
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: pages must be F16 or BF16, K and V alike", what);
+    for (int i = 0; i < 4; ++i)
+        if (kp->ne[i] != vp->ne[i]) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: k_pages and v_pages differ in ne[%d]", what, i);
+    if (kp->nb[0] != 2 || vp->nb[0] != 2 || !al16(kp, 3) || !al16(vp, 3))
+        return fail(ctx, VVA_ERR_INVALID_ARG, "%s: page rows must be contiguous and 16-byte aligned", what);
+    if (d != 64 && d != 128) return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: head_dim %lld, needs 64 or 128", what, (long long)d);
+    if (ps < 16 || ps > 1024 || (ps & (ps - 1)))
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: page_size %lld, needs a power of two from 16 to 1024", what, (long long)ps);
+    if (Hq % Hkv) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: Hq %% Hkv != 0", what);
+    // lane offsets inside a page are 32-bit; pages and heads are 64-bit
+    if ((uint64_t)kp->nb[1] * ps >= ((uint64_t)1 << 31) || (uint64_t)vp->nb[1] * ps >= ((uint64_t)1 << 31) ||
+        n_pages > 0x7fffffff || Hq > 65535)
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: pages too large", what);
+    if (N > (1 << 24)) return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: %lld tokens, at most 2^24", what, (long long)N);
+    if (!b) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: batch is null", what);
+    const int64_t n_seq = b->kv_len.ne[0];
+    if (n_seq < 1 || n_seq > VVA_MAX_BATCH_SEQ)
+        return fail(ctx, VVA_ERR_INVALID_ARG, "%s: %lld sequences, at most %d", what, (long long)n_seq, VVA_MAX_BATCH_SEQ);
+    if ((st = check_ints(ctx, &b->kv_len, "kv_len", n_seq)) != VVA_OK) return st;
+    if ((st = check_ints(ctx, &b->q_start, "q_start", n_seq + 1)) != VVA_OK) return st;
+    const vva_tensor* t = &b->table;
+    if ((st = check_tensor(ctx, t, "table")) != VVA_OK) return st;
+    if (t->type != VVA_TYPE_I32 || t->nb[0] != 4 || (uintptr_t)t->data % 4 || t->nb[1] % 4 || t->ne[1] != n_seq ||
+        t->ne[2] * t->ne[3] != 1)
+        return fail(ctx, VVA_ERR_INVALID_ARG, "table must be I32 ne=[max_pages,%lld] with contiguous rows", (long long)n_seq);
+    if (t->ne[0] * ps > (1 << 30))
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: a table row of %lld pages of %lld keys", what, (long long)t->ne[0], (long long)ps);
+    if (b->max_new < 1) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: max_new %d", what, b->max_new);
+    p.q_start = (const int32_t*)b->q_start.data;
+    p.kv_len = (const int32_t*)b->kv_len.data;
+    p.table = (const int32_t*)t->data;
+    p.table_stride = (int64_t)(t->nb[1] / 4);
+    p.n_seq = (int)n_seq; p.n_tok = (int)N; p.n_pages = (int)n_pages; p.max_pages = (int)t->ne[0];
+    p.max_new = (int)std::min<int64_t>(b->max_new, N);
+    p.page_shift = __builtin_ctz((unsigned)ps);
+    p.d = (int)d; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv);
+    p.k = (char*)kp->data; p.v = (char*)vp->data; p.type = kp->type;
+    p.k_nb_slot = kp->nb[1]; p.k_nb_head = kp->nb[2]; p.k_nb_page = kp->nb[3];
+    p.v_nb_slot = vp->nb[1]; p.v_nb_head = vp->nb[2]; p.v_nb_page = vp->nb[3];
+    return VVA_OK;
+}
+
+}  // namespace
+
+extern "C" vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, const vva_tensor* k,
+                                            const vva_tensor* v, const vva_tensor* rope, const vva_tensor* pos,
+                                            const vva_batch* batch, const vva_tensor* k_pages,
+                                            const vva_tensor* v_pages, const vva_tensor* q_out) {
+    if (!ctx) return VVA_ERR_INVALID_ARG;
+    vva_status st;
+    if ((st = check_tensor(ctx, q, "q")) != VVA_OK) return st;
+    const int64_t Hq = q->ne[1], N = q->ne[2];
+    PagedAppendArgs a{};
+    if ((st = fill_paged(ctx, "paged_rope_append", k_pages, v_pages, batch, Hq, N, a.p)) != VVA_OK) return st;
+    const int64_t d = a.p.d, Hkv = a.p.Hkv;
+    if ((st = check_packed(ctx, q, "q", d, Hq, N)) != VVA_OK) return st;
+    if ((st = check_packed(ctx, k, "k", d, Hkv, N)) != VVA_OK) return st;
+    if ((st = check_packed(ctx, v, "v", d, Hkv, N)) != VVA_OK) return st;
+    if ((st = check_packed(ctx, q_out, "q_out", d, Hq, N)) != VVA_OK) return st;
+    if ((st = check_tensor(ctx, rope, "rope")) != VVA_OK) return st;
+    if (rope->type != VVA_TYPE_F32 || rope->ne[0] != d || rope->nb[0] != 4 || rope->ne[2] * rope->ne[3] != 1 ||
+        !al16(rope, 1) || rope->ne[1] > 0x7fffffff)
+        return fail(ctx, VVA_ERR_INVALID_ARG, "rope must be F32 ne=[%lld,n_pos] with 16-byte aligned rows", (long long)d);
+    if (pos && (st = check_ints(ctx, pos, "pos", N)) != VVA_OK) return st;
+    // q_out: q itself, row for row, or memory of its own
+    const bool same = q_out->data == q->data && q_out->type == q->type && q_out->nb[1] == q->nb[1] && q_out->nb[2] == q->nb[2];
+    if ((!same && overlaps(q_out, q)) || overlaps(q_out, k) || overlaps(q_out, v) || overlaps(q_out, k_pages) ||
+        overlaps(q_out, v_pages) || overlaps(q_out, rope))
+        return fail(ctx, VVA_ERR_INVALID_ARG, "paged_rope_append: q_out overlaps another tensor (only q_out == q may alias)");
+    a.p.q = (const char*)q->data; a.q_type = q->type; a.p.q_nb_h = q->nb[1]; a.p.q_nb_t = q->nb[2];
+    a.k_new = (const char*)k->data; a.k_type = k->type; a.k_nb_h = k->nb[1]; a.k_nb_t = k->nb[2];
+    a.v_new = (const char*)v->data; a.v_type = v->type; a.v_nb_h = v->nb[1]; a.v_nb_t = v->nb[2];
+    a.p.out = (char*)q_out->data; a.qo_type = q_out->type; a.p.o_nb_h = q_out->nb[1]; a.p.o_nb_t = q_out->nb[2];
+    a.rope = (const char*)rope->data; a.rope_nb = rope->nb[1]; a.n_pos = (int)rope->ne[1];
+    a.pos = pos ? (const int32_t*)pos->data : nullptr;
+    DeviceGuard g(ctx->device);
+    const hipError_t e = launch_paged_append(a, ctx->stream);
+    return e == hipSuccess ? VVA_OK : hip_fail(ctx, e, "paged_rope_append launch");
+}
+
+extern "C" vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, const vva_tensor* k_pages,
+                                     const vva_tensor* v_pages, const vva_batch* batch, float scale,
+                                     const vva_tensor* out) {
+    if (!ctx) return VVA_ERR_INVALID_ARG;
+    vva_status st;
+    if ((st = check_tensor(ctx, q, "q")) != VVA_OK) return st;
+    const int64_t Hq = q->ne[1], N = q->ne[2];
+    PagedArgs a{};
+    if ((st = fill_paged(ctx, "paged_attn", k_pages, v_pages, batch, Hq, N, a)) != VVA_OK) return st;
+    if ((st = check_packed(ctx, q, "q", a.d, Hq, N)) != VVA_OK) return st;
+    if ((st = check_packed(ctx, out, "out", a.d, Hq, N)) != VVA_OK) return st;
+    if (q->type != a.type || out->type != a.type)
+        return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: q and out must have the pages' type (%d)", a.type);
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: scale must be finite and > 0");
+    if (overlaps(out, q) || overlaps(out, k_pages) || overlaps(out, v_pages))
+        return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: out overlaps q or the pages");
+    a.q = (const char*)q->data; a.q_nb_h = q->nb[1]; a.q_nb_t = q->nb[2];
+    a.out = (char*)out->data; a.o_nb_h = out->nb[1]; a.o_nb_t = out->nb[2];
+    a.scale = scale;
+    DeviceGuard g(ctx->device);
+    const hipError_t e = launch_paged_attn(a, ctx->stream);
+    return e == hipSuccess ? VVA_OK : hip_fail(ctx, e, "paged_attn launch");
+}
+
+extern "C" vva_status vva_add_rms_norm(vva_context* ctx, const vva_tensor* x, const vva_tensor* add, const vva_tensor* w,
+                                       float eps, const vva_tensor* sum, const vva_tensor* y) {
+    if (!ctx) return VVA_ERR_INVALID_ARG;
+    vva_status st;
+    if ((st = check_tensor(ctx, x, "x")) != VVA_OK) return st;
+    if ((st = check_tensor(ctx, y, "y")) != VVA_OK) return st;
+    const int64_t K = x->ne[0], T = x->ne[1], B = x->ne[2], N = T * B;
+    if ((st = check_act(ctx, x, "x", K, T, B)) != VVA_OK) return st;
+    if (add && (st = check_act(ctx, add, "add", K, T, B)) != VVA_OK) return st;
+    if (sum && (st = check_act(ctx, sum, "sum", K, T, B)) != VVA_OK) return st;
+    if ((st = check_tensor(ctx, w, "w")) != VVA_OK) return st;
+    if (w->type != VVA_TYPE_F32 || w->ne[0] != K || w->nb[0] != 4 || w->ne[1] * w->ne[2] * w->ne[3] != 1)
+        return fail(ctx, VVA_ERR_INVALID_ARG, "add_rms_norm: w must be F32 ne=[%lld]", (long long)K);
+    if (y->type == VVA_TYPE_Q8_0) {
+        if (y->ne[0] != K || y->ne[1] != T || y->ne[2] != B || y->ne[3] != 1 || K % kQK8 || y->nb[0] != kQ8Bytes)
+            return fail(ctx, VVA_ERR_INVALID_ARG, "add_rms_norm: Q8_0 y needs ne=[%lld,%lld,%lld,1] in whole blocks of 32",
+                        (long long)K, (long long)T, (long long)B);
+        if ((uintptr_t)y->data % 2 || y->nb[1] % 2 || y->nb[2] % 2)
+            return fail(ctx, VVA_ERR_INVALID_ARG, "add_rms_norm: Q8_0 y rows must be 2-byte aligned");
+    } else if ((st = check_act(ctx, y, "y", K, T, B)) != VVA_OK) {
+        return st;
+    }
+    if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(ctx, VVA_ERR_INVALID_ARG, "add_rms_norm: eps must be finite and >= 0");
+    if (K > 16384 || N > 0x7fffffff)
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "add_rms_norm: %lld rows of %lld", (long long)N, (long long)K);
+    // an output may be an input itself, row for row; other overlaps would be
+    // read by one workgroup while another writes
+    auto same = [](const vva_tensor* o, const vva_tensor* i) {
+        return o->data == i->data && o->type == i->type && (o->ne[1] == 1 || o->nb[1] == i->nb[1]) && (o->ne[2] == 1 || o->nb[2] == i->nb[2]);
+    };
+    auto clash = [&](const vva_tensor* o, const vva_tensor* i) { return o && i && !same(o, i) && overlaps(o, i); };
+    if (clash(y, x) || clash(y, add) || clash(sum, x) || clash(sum, add) || overlaps(y, w) || (sum && overlaps(sum, w)) ||
+        (sum && overlaps(sum, y)))
+        return fail(ctx, VVA_ERR_INVALID_ARG, "add_rms_norm: outputs overlap each other or an input (only an input itself may alias)");
+    NormArgs a{};
+    a.x = (const char*)x->data; a.x_type = x->type; a.x_nb_t = x->nb[1]; a.x_nb_b = x->nb[2];
+    if (add) { a.add = (const char*)add->data; a.add_type = add->type; a.add_nb_t = add->nb[1]; a.add_nb_b = add->nb[2]; }
+    if (sum) { a.sum = (char*)sum->data; a.sum_type = sum->type; a.sum_nb_t = sum->nb[1]; a.sum_nb_b = sum->nb[2]; }
+    a.y = (char*)y->data; a.y_type = y->type; a.y_nb_t = y->nb[1]; a.y_nb_b = y->nb[2];
+    a.w = (const float*)w->data;
+    a.K = (int)K; a.T = (int)T; a.N = (int)N; a.eps = eps;
+    DeviceGuard g(ctx->device);
+    const hipError_t e = launch_norm(a, ctx->stream);
+    return e == hipSuccess ? VVA_OK : hip_fail(ctx, e, "add_rms_norm launch");
+}

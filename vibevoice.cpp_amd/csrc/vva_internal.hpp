@@ -193,7 +193,46 @@ ProjPlan proj_plan(const ProjArgs& a, int n_cu);
 // bytes of the pieces' partials
 size_t proj_part_bytes(const ProjArgs& a, const ProjPlan& p);
 
+// Packed tokens of many sequences over a cache in pages (paged.hip).  Row
+// (slot, head, page) of K at k + page * k_nb_page + head * k_nb_head + slot *
+// k_nb_slot; token rows n of q, out at base + n * nb_t + h * nb_h.
+struct PagedArgs {
+    const int32_t* q_start; const int32_t* kv_len; const int32_t* table;
+    int64_t table_stride;                          // in elements
+    int n_seq, n_tok, n_pages, max_pages, max_new;
+    int page_shift;                                // page size = 1 << page_shift
+    int d, Hq, Hkv, G;                             // G = Hq / Hkv
+    char* k; char* v; int type;
+    int64_t k_nb_slot, k_nb_head, k_nb_page, v_nb_slot, v_nb_head, v_nb_page;
+    const char* q; int64_t q_nb_h, q_nb_t;
+    char* out; int64_t o_nb_h, o_nb_t;
+    float scale;
+};
+// RoPE + append: q, k, v rows in, q_out = PagedArgs::out
+struct PagedAppendArgs {
+    PagedArgs p;
+    const char* k_new; const char* v_new;
+    int q_type, k_type, v_type, qo_type;
+    int64_t k_nb_h, k_nb_t, v_nb_h, v_nb_t;
+    const char* rope; int64_t rope_nb; int n_pos;  // rows of d floats, cos then sin
+    const int32_t* pos;                            // [n_tok] or null
+};
+// Residual addition + RMS norm (norm.hip)
+struct NormArgs {
+    const char* x; int x_type; int64_t x_nb_t, x_nb_b;
+    const char* add; int add_type; int64_t add_nb_t, add_nb_b;    // null: none
+    char* sum; int sum_type; int64_t sum_nb_t, sum_nb_b;          // null: not kept
+    char* y; int y_type; int64_t y_nb_t, y_nb_b;
+    const float* w;
+    int K, T, N;                                   // row n = b * T + t
+    float eps;
+};
+
 // --------------------------------------------------------- host launchers
+
+hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s);
+hipError_t launch_paged_attn(const PagedArgs& a, hipStream_t s);
+hipError_t launch_norm(const NormArgs& a, hipStream_t s);
 
 hipError_t launch_rope_append(const RopeAppendArgs& a, hipStream_t s);
 hipError_t launch_attn_rows(const AttnArgs& a, hipStream_t s);

@@ -33,6 +33,7 @@ EXPORTS = [
     "vva_flash_attn_ext", "vva_supports", "vva_set_attn_path", "vva_last_decode_splits",
     "vva_set_schedule", "vva_attn_noalloc", "vva_qkv_rope_append", "vva_out_proj_residual",
     "vva_set_flash_attn", "vva_decode_step", "vva_qkv_proj", "vva_set_log_callback",
+    "vva_paged_rope_append", "vva_paged_attn", "vva_add_rms_norm",
 ]
 
 LOG_ERROR, LOG_WARN, LOG_INFO, LOG_DEBUG = 0, 1, 2, 3
@@ -55,6 +56,10 @@ class KVDesc(ctypes.Structure):
     _fields_ = [("n_layers", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
                 ("head_dim", ctypes.c_int32), ("max_seq", ctypes.c_int32),
                 ("n_seq", ctypes.c_int32), ("type", ctypes.c_int32)]
+
+
+class BatchDesc(ctypes.Structure):
+    _fields_ = [("q_start", Tensor), ("kv_len", Tensor), ("table", Tensor), ("max_new", ctypes.c_int32)]
 
 
 _lib = None
@@ -112,6 +117,9 @@ def load_library(path: str = LIB_PATH):
         "vva_set_flash_attn": (I, [P, I]),
         "vva_decode_step": (I, [P, P, I, TP, TP, TP, TP, P, F, F, TP, TP]),
         "vva_set_log_callback": (None, [LOG_CB, P, I]),
+        "vva_paged_rope_append": (I, [P, TP, TP, TP, TP, TP, ctypes.POINTER(BatchDesc), TP, TP, TP]),
+        "vva_paged_attn": (I, [P, TP, TP, TP, ctypes.POINTER(BatchDesc), F, TP]),
+        "vva_add_rms_norm": (I, [P, TP, TP, TP, F, TP, TP]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -168,6 +176,22 @@ def view(t, ggml_ne=None, ggml_nb=None, type_=None) -> Tensor:
         tv.ne[i] = int(ggml_ne[i])
         tv.nb[i] = int(ggml_nb[i])
     return tv
+
+
+def q8_view(raw) -> Tensor:
+    """View of uint8 blocks [B, T, hidden / 32, 34] (rows contiguous) as Q8_0 rows ne = [hidden, T, B]."""
+    B, T, n, _ = raw.shape
+    return view(raw, ggml_ne=[n * 32, T, B, 1],
+                ggml_nb=[Q8_BLOCK_BYTES, raw.stride(1), raw.stride(0), raw.stride(0) * B], type_=Q8_0)
+
+
+class Batch:
+    """vva_batch: the sequences of a call over a paged cache.  q_start int32 [n_seq + 1], kv_len int32 [n_seq], table
+    int32 [n_seq, max_pages], all on the device; max_new: the most new tokens a sequence brings."""
+
+    def __init__(self, q_start, kv_len, table, max_new: int):
+        self.tensors = (q_start, kv_len, table)
+        self.c = BatchDesc(view(q_start), view(kv_len), view(table), int(max_new))
 
 
 class Context:
@@ -300,6 +324,48 @@ class Context:
             o = o.reshape(o.shape[0], o.shape[1], -1)
         self.check(self.lib.vva_out_proj_residual(self.h, ctypes.byref(view(o)), ctypes.byref(w_o.t),
                                                   ctypes.byref(view(x)), ctypes.byref(view(h))))
+
+    def _bound(self, fn, keep, *args):
+        """The call fn(h, *args) with its descriptors made once: for callers that repeat it over the same tensors
+        (kept alive by the returned function)."""
+        refs = [ctypes.byref(a) if isinstance(a, ctypes.Structure) else a for a in args]
+
+        def call():
+            self.check(fn(self.h, *refs))
+        call.keep = (keep, args)
+        return call
+
+    def bind_paged_rope_append(self, q, k, v, rope, batch: Batch, k_pages, v_pages, q_out, pos=None):
+        """q, q_out: [N, Hq, d]; k, v: [N, Hkv, d] packed tokens; rope f32 [n_pos, d] (cos, then sin); pos int32 [N] or
+        None; k_pages, v_pages: [n_pages, Hkv, page_size, d].  Returns the call."""
+        return self._bound(self.lib.vva_paged_rope_append, (q, k, v, rope, pos, batch, k_pages, v_pages, q_out), view(q),
+                           view(k), view(v), view(rope), view(pos) if pos is not None else None, batch.c, view(k_pages),
+                           view(v_pages), view(q_out))
+
+    def paged_rope_append(self, *args, **kw):
+        """bind_paged_rope_append's call, once."""
+        self.bind_paged_rope_append(*args, **kw)()
+
+    def bind_paged_attn(self, q, k_pages, v_pages, batch: Batch, scale: float, out):
+        """q, out: [N, Hq, d] packed tokens in the pages' dtype; k_pages, v_pages: [n_pages, Hkv, page_size, d].  Returns
+        the call."""
+        return self._bound(self.lib.vva_paged_attn, (q, k_pages, v_pages, batch, out), view(q), view(k_pages),
+                           view(v_pages), batch.c, scale, view(out))
+
+    def paged_attn(self, *args, **kw):
+        """bind_paged_attn's call, once."""
+        self.bind_paged_attn(*args, **kw)()
+
+    def bind_add_rms_norm(self, x, w, y, add=None, total=None, eps: float = 1.0e-6):
+        """x, add, total (receives x + add): [B, T, hidden]; w f32 [hidden]; y: a tensor like x or q8_view(...) of Q8_0
+        blocks.  Returns the call."""
+        return self._bound(self.lib.vva_add_rms_norm, (x, w, y, add, total), view(x),
+                           view(add) if add is not None else None, view(w), eps,
+                           view(total) if total is not None else None, y if isinstance(y, Tensor) else view(y))
+
+    def add_rms_norm(self, *args, **kw):
+        """bind_add_rms_norm's call, once."""
+        self.bind_add_rms_norm(*args, **kw)()
 
     def flash_attn_ext(self, q, k, v, out, scale: float, mask=None, k_view=None, v_view=None):
         """ggml layout: q torch [B, Hq, T, d] (ne=[d,T,Hq,B]); k, v torch [B, Hkv, L, d] or
