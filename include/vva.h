@@ -366,8 +366,8 @@ VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, 
  *   out: ne = [d, Hq, N], in that type too, apart from q's memory;
  *   scale: a finite number above 0.
  * Token t of sequence s sees keys 0 .. kv_len[s] - n_s + t; one that sees none
- * gets zeros.  Rows of no sequence are left as they were; a sequence with a
- * page id outside the pool among its keys gets NaN.  What is stored behind the
+ * gets zeros.  Rows of no sequence are left as they were; rows that see a key
+ * whose page id is outside the pool get NaN (other rows of that sequence may).  What is stored behind the
  * keys of a sequence (NaN included) does not matter.  The products run on the
  * matrix cores in the pages' type with F32 sums, the probabilities rounded to
  * that type; the softmax is F32.

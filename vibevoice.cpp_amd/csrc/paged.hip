@@ -1,7 +1,7 @@
-// paged.hip — packed tokens of many sequences over a cache in pages: RoPE +
-// append, and causal grouped-query attention.
+// paged.hip — RoPE + append of packed tokens of many sequences into a cache in
+// pages.
 //
-// What a call covers is on the device (vva_batch): the kernels find their
+// What a call covers is on the device (vva_batch): the kernel finds its
 // sequence in q_start, its keys in kv_len and their places in the page table,
 // so the same launch serves any lengths of the same shapes.
 #include "vva_internal.hpp"
@@ -10,31 +10,7 @@ namespace vva {
 
 namespace {
 
-#include "wave_ops.hpp"
-
-// A sequence of the batch, kept inside the rows and the table there are.
-struct Seq {
-    int q0, n;          // first token row, new tokens
-    int L;              // keys
-};
-__device__ __forceinline__ Seq seq_of(const PagedArgs& a, int s) {
-    Seq r;
-    r.q0 = min(max(a.q_start[s], 0), a.n_tok);
-    r.n = min(max(a.q_start[s + 1], r.q0), a.n_tok) - r.q0;
-    r.L = min(max(a.kv_len[s], 0), a.max_pages << a.page_shift);
-    return r;
-}
-
-// The sequence whose rows hold token row n, or n_seq.  Called by whole waves.
-__device__ __forceinline__ int seq_of_token(const PagedArgs& a, int n) {
-    const int lane = threadIdx.x & 63;
-    for (int i = 0; i < a.n_seq; i += 64) {
-        const int s = min(i + lane, a.n_seq - 1);
-        const uint64_t hit = __ballot(a.q_start[s] <= n && n < a.q_start[s + 1]);
-        if (hit) return min(i + __ffsll((unsigned long long)hit) - 1, a.n_seq - 1);
-    }
-    return a.n_seq;
-}
+#include "paged_ops.hpp"
 
 // One workgroup per token row.
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppendArgs a) {
@@ -85,54 +61,10 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppendArgs a) {
     }
 }
 
-// One wave per (token row, query head): the keys one after the other, the
-// softmax's running maximum and sum beside the output.
-template <int D>
-__global__ void __launch_bounds__(256) paged_attn_kernel(PagedArgs a) {
-    constexpr int E = D / 64;                      // dims per lane
-    const int lane = threadIdx.x & 63;
-    const int n = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (h >= a.Hq) return;
-    const int s = seq_of_token(a, n);
-    if (s >= a.n_seq) return;
-    const Seq q = seq_of(a, s);
-    const int t = n - q.q0;
-    if (t < 0 || t >= min(q.n, a.max_new)) return;
-    const int last = q.L - q.n + t, kvh = h / a.G;
-    float x[E], o[E] = {};
-    for (int e = 0; e < E; ++e) x[e] = load_elem(a.q + n * a.q_nb_t + h * a.q_nb_h + (lane * E + e) * 2, a.type) * a.scale * kLog2e;
-    float m = -INFINITY, l = 0.0f;
-    for (int j = 0; j <= last; ++j) {
-        const int page = a.table[s * a.table_stride + (j >> a.page_shift)];
-        const int slot = j & ((1 << a.page_shift) - 1);
-        if (page < 0 || page >= a.n_pages) { l = __builtin_nanf(""); continue; }
-        const char* kr = a.k + page * a.k_nb_page + kvh * a.k_nb_head + slot * a.k_nb_slot + lane * E * 2;
-        const char* vr = a.v + page * a.v_nb_page + kvh * a.v_nb_head + slot * a.v_nb_slot + lane * E * 2;
-        float sc = 0.0f;
-        for (int e = 0; e < E; ++e) sc = fmaf(x[e], load_elem(kr + e * 2, a.type), sc);
-        sc = wave_sum(sc);
-        const float mn = fmaxf(m, sc);
-        const float base = mn == -INFINITY ? 0.0f : mn;
-        const float f = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(sc - base);
-        l = l * f + p;
-        for (int e = 0; e < E; ++e) o[e] = fmaf(p, load_elem(vr + e * 2, a.type), o[e] * f);
-        m = mn;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int e = 0; e < E; ++e) store_elem(a.out + n * a.o_nb_t + h * a.o_nb_h + (lane * E + e) * 2, a.type, o[e] * inv);
-}
-
 }  // namespace
 
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
     hipLaunchKernelGGL(paged_append_kernel, dim3(a.p.n_tok), dim3(256), 0, s, a);
-    return hipGetLastError();
-}
-
-hipError_t launch_paged_attn(const PagedArgs& a, hipStream_t s) {
-    const dim3 grid(a.n_tok, (a.Hq + 3) / 4);
-    if (a.d == 64) hipLaunchKernelGGL(paged_attn_kernel<64>, grid, dim3(256), 0, s, a);
-    else           hipLaunchKernelGGL(paged_attn_kernel<128>, grid, dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

@@ -1,0 +1,39 @@
+// paged_ops.hpp — what the kernels over a cache in pages share: a sequence of
+// the batch, kept inside the rows and the table there are, and the lookups by
+// whole waves.  Included inside an anonymous namespace of each kernel file.
+#pragma once
+
+struct Seq {
+    int q0, n;          // first token row, new tokens
+    int L;              // keys
+};
+__device__ __forceinline__ Seq seq_of(const PagedArgs& a, int s) {
+    Seq r;
+    r.q0 = min(max(a.q_start[s], 0), a.n_tok);
+    r.n = min(max(a.q_start[s + 1], r.q0), a.n_tok) - r.q0;
+    r.L = min(max(a.kv_len[s], 0), a.max_pages << a.page_shift);
+    return r;
+}
+
+// The sequence whose rows hold token row n, or n_seq.  Called by whole waves.
+__device__ __forceinline__ int seq_of_token(const PagedArgs& a, int n) {
+    const int lane = threadIdx.x & 63;
+    for (int i = 0; i < a.n_seq; i += 64) {
+        const int s = min(i + lane, a.n_seq - 1);
+        const uint64_t hit = __ballot(a.q_start[s] <= n && n < a.q_start[s + 1]);
+        if (hit) return min(i + __ffsll((unsigned long long)hit) - 1, a.n_seq - 1);
+    }
+    return a.n_seq;
+}
+
+__device__ __forceinline__ int lane_of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+// Sum of x over the lanes up to and with this one
+__device__ __forceinline__ int wave_scan(int x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const int y = __shfl_up(x, m, 64);
+        x += lane >= m ? y : 0;
+    }
+    return x;
+}

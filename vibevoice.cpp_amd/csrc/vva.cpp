@@ -1523,8 +1523,10 @@ vva_status fill_paged(vva_context* ctx, const char* what, const vva_tensor* kp, 
     if (t->type != VVA_TYPE_I32 || t->nb[0] != 4 || (uintptr_t)t->data % 4 || t->nb[1] % 4 || t->ne[1] != n_seq ||
         t->ne[2] * t->ne[3] != 1)
         return fail(ctx, VVA_ERR_INVALID_ARG, "table must be I32 ne=[max_pages,%lld] with contiguous rows", (long long)n_seq);
-    if (t->ne[0] * ps > (1 << 30))
-        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: a table row of %lld pages of %lld keys", what, (long long)t->ne[0], (long long)ps);
+    // keys of a sequence, and tiles of 32 keys of all of them, in 32 bits
+    if (t->ne[0] > (1 << 30) / ps || t->ne[0] * ps * n_seq > ((int64_t)1 << 34))
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: table of %lld sequences x %lld pages of %lld keys", what,
+                    (long long)n_seq, (long long)t->ne[0], (long long)ps);
     if (b->max_new < 1) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: max_new %d", what, b->max_new);
     p.q_start = (const int32_t*)b->q_start.data;
     p.kv_len = (const int32_t*)b->kv_len.data;
@@ -1598,7 +1600,9 @@ extern "C" vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, cons
     a.out = (char*)out->data; a.o_nb_h = out->nb[1]; a.o_nb_t = out->nb[2];
     a.scale = scale;
     DeviceGuard g(ctx->device);
-    const hipError_t e = launch_paged_attn(a, ctx->stream);
+    const PagedPlan plan = paged_plan(a, ctx->n_cu);
+    if ((st = ensure_ws(ctx, paged_ws_bytes(a, plan))) != VVA_OK) return st;
+    const hipError_t e = launch_paged_attn(a, plan, ctx->ws, ctx->stream);
     return e == hipSuccess ? VVA_OK : hip_fail(ctx, e, "paged_attn launch");
 }
 
