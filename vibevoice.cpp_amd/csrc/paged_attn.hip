@@ -160,6 +160,7 @@ __device__ __forceinline__ void load_q(const PagedArgs& a, int q0, int kvh, int 
 
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 __device__ __forceinline__ lds_u32x4* lds_vec(uint32_t addr) { return (lds_u32x4*)(uintptr_t)addr; }
+__device__ __forceinline__ u32x4 lds_read(uint32_t addr) { return *lds_vec(addr); }
 template <int KT>
 __device__ __forceinline__ bool chunk_not_finite(u32x4 x) {
     return not_finite2<KT>(x.x) || not_finite2<KT>(x.y) || not_finite2<KT>(x.z) || not_finite2<KT>(x.w);
@@ -170,7 +171,7 @@ __device__ __forceinline__ bool tile_not_finite(uint32_t v_lds, int lane) {
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < N * 2 * D / 1024; ++i) {
-        bad = bad || chunk_not_finite<KT>(*lds_vec(v_lds + i * 1024 + lane * 16));
+        bad = bad || chunk_not_finite<KT>(lds_read(v_lds + i * 1024 + lane * 16));
     }
     return __any(bad);
 }
@@ -214,30 +215,32 @@ __device__ __forceinline__ int few_tiles(const PagedArgs& a, const Seq& q) {
     const int n = min(q.n, a.max_new);
     return n > 0 && n * a.G <= kFewRows ? max(1, (q.L + kFewTile - 1) / kFewTile) : 0;
 }
-// Piece `item` of the call (SEQ: the pieces of sequence `item`, part = 0).
-// All sequences are cut into pieces of one length, the whole work over
-// `target`, so a long sequence among short ones gets its share of the chip.
-// By whole waves.
-template <bool SEQ>
-__device__ __forceinline__ FewItem few_item(const PagedArgs& a, int item, int target) {
+// Piece `item` of the call.  All sequences are cut into pieces of at most
+// `chunk` tiles, the least for which the pieces are no more than `slots` (the
+// workgroups that run at once, per kv head), so a long sequence among short
+// ones gets its share of the chip and no piece waits for a second round: tried
+// from the even share up in steps of an eighth, for up to 64 sequences; more
+// of them leave many pieces, whose rounds even out.  By whole waves.
+__device__ __forceinline__ FewItem few_item(const PagedArgs& a, int item, int slots) {
     const int lane = threadIdx.x & 63;
-    int total = 0;
-    for (int i = 0; i < a.n_seq; i += 64) {
-        const int s = i + lane;
-        total += s < a.n_seq ? few_tiles(a, seq_of(a, s)) : 0;
-    }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) total += __shfl_xor(total, m, 64);
-    const int chunk = max(kFewMin, (total + target - 1) / target);
+    Seq q = seq_of(a, min(lane, a.n_seq - 1));
+    int t = lane < a.n_seq ? few_tiles(a, q) : 0;
+    int total = t;
+    for (int s = lane + 64; s < a.n_seq; s += 64) total += few_tiles(a, seq_of(a, s));
+    total = wave_total(total);
+    int chunk = max(kFewMin, (total + slots - 1) / slots);
+    if (a.n_seq <= 64)
+        for (int i = 0; i < 12 && wave_total((t + chunk - 1) / chunk) > slots; ++i) chunk += (chunk + 7) / 8;
     FewItem r{};
     int base = 0;
     for (int i = 0; i < a.n_seq; i += 64) {
-        const int s = i + lane;
-        const Seq q = seq_of(a, min(s, a.n_seq - 1));
-        const int t = s < a.n_seq ? few_tiles(a, q) : 0;
+        if (i > 0) {
+            q = seq_of(a, min(i + lane, a.n_seq - 1));
+            t = i + lane < a.n_seq ? few_tiles(a, q) : 0;
+        }
         const int c = (t + chunk - 1) / chunk;
         const int end = wave_scan(c);
-        const uint64_t hit = __ballot(SEQ ? s == item : (item >= base + end - c && item < base + end));
+        const uint64_t hit = __ballot(item >= base + end - c && item < base + end);
         if (hit) {
             const int l = __ffsll((unsigned long long)hit) - 1;
             r.q.q0 = lane_of(q.q0, l);
@@ -246,7 +249,7 @@ __device__ __forceinline__ FewItem few_item(const PagedArgs& a, int item, int ta
             r.s = i + l;
             r.parts = lane_of(c, l);
             r.first = base + lane_of(end - c, l);
-            r.part = SEQ ? 0 : item - r.first;
+            r.part = item - r.first;
             return r;
         }
         base += lane_of(end, 63);
@@ -254,32 +257,33 @@ __device__ __forceinline__ FewItem few_item(const PagedArgs& a, int item, int ta
     return r;
 }
 
-// Partial of a piece and kv head in the workspace: [rows][D] sums, then
-// [rows] (exponent base, row sum)
-__device__ __forceinline__ float* few_partial(float* ws, int piece, int kvh, int Hkv, int rows, int D) {
-    return ws + ((int64_t)piece * Hkv + kvh) * rows * (D + 2);
-}
+constexpr int kSc1 = 16;           // cache policy of the partials: agent scope
+constexpr int kMergeBatch = 16;    // pieces whose partials are loaded together
 
-// One workgroup per (piece of a sequence's keys, kv head); each wave streams
-// every fourth tile of it through LDS of its own, two tiles deep, without a
-// barrier, and the waves' sums meet at the end.
+// One workgroup per (piece of a sequence's keys, kv head), two of them (D = 64:
+// four) on a CU.  Each wave streams every fourth tile of the piece through LDS of its
+// own, without a barrier: the next K goes out when K is read, the next V when V
+// is, so 16 KB of the wave's loads fly while it waits and 8 while it computes.
+// The waves' sums meet at the end.  Partials in the workspace, per
+// piece and kv head: [cap rows][D] sums, then [cap] (exponent base, row sum).
 template <int D, int KT>
-__global__ void __launch_bounds__(kFewWaves * 64) paged_few_kernel(PagedArgs a, float* __restrict__ ws, int target, int cap) {
+__global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets, int slots, int cap) {
     prefetch_kernargs<sizeof(PagedArgs)>();
     using F = Frag<KT>;
     using QF = typename F::type;
     constexpr int DS = D / 16, DT = D / 32;
     constexpr int NC = kFewTile * 2 * D / 1024;    // loads of a K (V) tile
     constexpr int RC = 1024 / (2 * D);             // rows of a load
-    constexpr int TB = kFewTile * 2 * D;           // bytes of a K (V) tile
+    constexpr int TB = kFewTile * 2 * D;           // bytes of a K (V) tile, and of the rows of Q
     constexpr int OP = D + 4;                      // pitch of a row of sums
-    __shared__ __attribute__((aligned(1024))) char lds[kFewWaves * 2 * 2 * TB];
-    static_assert(sizeof(lds) >= kFewWaves * kFewRows * (OP + 2) * sizeof(float), "the sums fit the ring");
+    constexpr int SUMS = kFewWaves * kFewRows * (OP + 2) * (int)sizeof(float);
+    constexpr int RING = (kFewWaves * 2 + 1) * TB;
+    __shared__ __attribute__((aligned(1024))) char lds[RING > SUMS ? RING : SUMS];
 
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x % a.Hkv, piece = blockIdx.x / a.Hkv;
-    const FewItem it = few_item<false>(a, piece, target);
+    const FewItem it = few_item(a, piece, slots);
     if (it.parts == 0) return;
     const int n = min(it.q.n, a.max_new), L = it.q.L, rows = n * a.G, past = L - it.q.n;
     const int tiles = (L + kFewTile - 1) / kFewTile;
@@ -288,7 +292,7 @@ __global__ void __launch_bounds__(kFewWaves * 64) paged_few_kernel(PagedArgs a, 
     // ---- this wave's tiles: t0 + w, + 4, ...
     const ConstInts table = (ConstInts)(uintptr_t)(a.table + (int64_t)it.s * a.table_stride);
     const int last_page = (L - 1) >> a.page_shift;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)lds + w * 4 * TB;
+    const uint32_t qs = (uint32_t)(uintptr_t)(lds_char*)lds, ks = qs + (1 + 2 * w) * TB, vs = ks + TB;
     int koff[4], voff[4];                          // by row group: the swizzles repeat every 16 rows
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -301,58 +305,66 @@ __global__ void __launch_bounds__(kFewWaves * 64) paged_few_kernel(PagedArgs a, 
 #pragma unroll
         for (int i = 0; i < 2; ++i) ids[i] = table[min((t * kFewTile + 16 * i) >> a.page_shift, last_page)];
     };
-    auto issue = [&](int t, int stage) {
-        uint64_t kb[2], vb[2];
+    auto issue = [&](int t, uint32_t dst, const char* pool, int64_t nb_page, int64_t nb_head, int64_t nb_slot, const int (&off)[4]) {
+        uint64_t base[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const bool ok = (uint32_t)ids[i] < (uint32_t)a.n_pages;
             bad = bad || !ok;
             const int64_t id = ok ? ids[i] : 0;
             const int64_t slot = (t * kFewTile + 16 * i) & ((1 << a.page_shift) - 1);
-            kb[i] = uniform64((uint64_t)(uintptr_t)a.k + id * a.k_nb_page + kvh * a.k_nb_head + slot * a.k_nb_slot);
-            vb[i] = uniform64((uint64_t)(uintptr_t)a.v + id * a.v_nb_page + kvh * a.v_nb_head + slot * a.v_nb_slot);
+            base[i] = uniform64((uint64_t)(uintptr_t)pool + id * nb_page + kvh * nb_head + slot * nb_slot);
         }
-        const uint32_t st = lds0 + stage * 2 * TB;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int r = c * RC;                  // first row of the load, in its 16-key half r % 16
-            dma16(kb[r / 16] + (uint64_t)(r % 16) * a.k_nb_slot, koff[c % 4], st + c * 1024);
-        }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int r = c * RC;
-            dma16(vb[r / 16] + (uint64_t)(r % 16) * a.v_nb_slot, voff[c % 4], st + TB + c * 1024);
+            dma16(base[r / 16] + (uint64_t)(r % 16) * nb_slot, off[c % 4], dst + c * 1024);
         }
     };
+    auto issue_k = [&](int t) { issue(t, ks, a.k, a.k_nb_page, a.k_nb_head, a.k_nb_slot, koff); };
+    auto issue_v = [&](int t) { issue(t, vs, a.v, a.v_nb_page, a.v_nb_head, a.v_nb_slot, voff); };
     int t = t0 + w;
-    if (t < t1) {
-        fetch(t);
-        issue(t, 0);
-        if (t + kFewWaves < t1) {
-            fetch(t + kFewWaves);
-            issue(t + kFewWaves, 1);
+    if (t < t1) fetch(t);
+    // the rows of Q, a quarter by each wave, laid out as K is; rows that are
+    // not there are row 0 again (no one reads their results)
+    {
+        const uint64_t qb = uniform64((uint64_t)(uintptr_t)a.q + (int64_t)it.q.q0 * a.q_nb_t + (int64_t)kvh * a.G * a.q_nb_h);
+#pragma unroll
+        for (int i = 0; i < NC / kFewWaves; ++i) {
+            const int c = w * (NC / kFewWaves) + i;
+            const int r = c * RC + lane / (D / 8), row = r < rows ? r : 0;
+            const int off = (row / a.G) * (int)a.q_nb_t + (row % a.G) * (int)a.q_nb_h;
+            dma16(qb, off + (((lane % (D / 8)) ^ k_swz<D>(r)) << 4), qs + c * 1024);
         }
     }
+    if (t < t1) {
+        issue_k(t);
+        issue_v(t);
+        wait_vm<2 * NC>();                         // Q
+    } else {
+        wait_vm<0>();
+    }
+    asm volatile("s_barrier" : : : "memory");
+    const int k_off = k_lane_off<D>(lane), v_off = v_lane_off<D>(lane);
     QF qf[DS];
-    load_q<D>(a, it.q.q0, kvh, l32, rows, half, qf);
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) qf[ds] = as_vec<QF>(lds_read((qs + k_off) ^ (ds << 5)));
     const int lim = l32 < rows ? min(L - 1, past + l32 / a.G) : -1;   // the last key the lane's row sees
     const float sl2 = a.scale * kLog2e;
     float m = -INFINITY, lsum = 0.0f;
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
-    const int k_off = k_lane_off<D>(lane), v_off = v_lane_off<D>(lane);
-    for (int stage = 0; t < t1; t += kFewWaves, stage ^= 1) {
-        const bool more = t + 2 * kFewWaves < t1;
-        if (more) fetch(t + 2 * kFewWaves);
-        if (t + kFewWaves < t1) wait_vm<2 * NC>();
-        else wait_vm<0>();
-        const uint32_t ks = lds0 + stage * 2 * TB, vs = ks + TB;
+    for (; t < t1; t += kFewWaves) {
+        const bool more = t + kFewWaves < t1;
+        if (more) fetch(t + kFewWaves);
+        wait_vm<NC>();                             // K; V may still fly
         f32x16 s{};
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds) {
-            const u32x4 kf = *lds_vec((ks + k_off) ^ (ds << 5));
-            s = F::mma(as_vec<QF>(kf), qf[ds], s);
+        for (int ds = 0; ds < DS; ++ds) s = F::mma(as_vec<QF>(lds_read((ks + k_off) ^ (ds << 5))), qf[ds], s);
+        if (more) {
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // K is read
+            issue_k(t + kFewWaves);
         }
         const int k0 = t * kFewTile;
         const bool masked = k0 + kFewTile - 1 > min(L - 1, past);      // some row must not see some key
@@ -380,6 +392,8 @@ __global__ void __launch_bounds__(kFewWaves * 64) paged_few_kernel(PagedArgs a, 
             p[r] = pack2<KT>(__builtin_amdgcn_exp2f(fmaf(s[2 * r], sl2, nb)), __builtin_amdgcn_exp2f(fmaf(s[2 * r + 1], sl2, nb)));
             lsum = sum2<KT>(p[r], lsum);
         }
+        if (more) wait_vm<NC>();                   // V; the next K may still fly
+        else wait_vm<0>();
         const bool fix = masked && tile_not_finite<D, KT, kFewTile>(vs, lane);
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
@@ -394,8 +408,8 @@ __global__ void __launch_bounds__(kFewWaves * 64) paged_few_kernel(PagedArgs a, 
         }
         if (fix) add_not_finite<D, KT, kFewTile>(vs, k0, lim, half, o);
         if (more) {
-            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // the tile's reads are done
-            issue(t + 2 * kFewWaves, stage);
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // V is read
+            issue_v(t + kFewWaves);
         }
     }
     // ---- the waves' sums, in LDS, added in wave order
@@ -411,6 +425,10 @@ __global__ void __launch_bounds__(kFewWaves * 64) paged_few_kernel(PagedArgs a, 
                 make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
     if (half == 0) *(float2*)(ml + (w * kFewRows + l32) * 2) = make_float2(m, lt);
     const bool any_bad = __syncthreads_or(bad);
+    auto piece_rsrc = [&](int part) {
+        const uint32_t bytes = cap * (D + 2) * sizeof(float);
+        return make_rsrc((const char*)ws + ((int64_t)(it.first + part) * a.Hkv + kvh) * bytes, bytes);
+    };
     for (int i = tid; i < rows * (D / 4); i += kFewWaves * 64) {
         const int row = i / (D / 4), c = i % (D / 4);
         float M = -INFINITY;
@@ -428,10 +446,13 @@ __global__ void __launch_bounds__(kFewWaves * 64) paged_few_kernel(PagedArgs a, 
             num.z = fmaf(f, v.z, num.z); num.w = fmaf(f, v.w, num.w);
         }
         if (it.parts > 1) {
-            float* const pr = few_partial(ws, piece, kvh, a.Hkv, cap, D);
-            *(float4*)(pr + row * D + 4 * c) = num;
+            // agent-scope stores: coherent across the XCDs' L2 caches
+            __builtin_amdgcn_raw_buffer_store_b128(
+                u32x4{__float_as_uint(num.x), __float_as_uint(num.y), __float_as_uint(num.z), __float_as_uint(num.w)},
+                piece_rsrc(it.part), (row * D + 4 * c) * 4, 0, kSc1);
             if (c == 0)
-                *(uint2*)(pr + cap * D + row * 2) = make_uint2(any_bad ? kNanBits : __float_as_uint(M), __float_as_uint(den));
+                __builtin_amdgcn_raw_buffer_store_b64(u32x2{any_bad ? kNanBits : __float_as_uint(M), __float_as_uint(den)},
+                                                      piece_rsrc(it.part), (cap * D + row * 2) * 4, 0, kSc1);
             continue;
         }
         const float inv = den > 0.0f ? 1.0f / den : 0.0f;
@@ -439,57 +460,68 @@ __global__ void __launch_bounds__(kFewWaves * 64) paged_few_kernel(PagedArgs a, 
         if (any_bad) y.x = y.y = 0x7fff7fffu;
         *(uint2*)(a.out + (int64_t)(it.q.q0 + row / a.G) * a.o_nb_t + (int64_t)(kvh * a.G + row % a.G) * a.o_nb_h + 8 * c) = y;
     }
-}
-
-// The pieces' sums of one row: groups of D / 4 threads take every NG-th piece,
-// their sums meet in LDS.
-template <int D, int KT>
-__global__ void __launch_bounds__(256) paged_few_merge_kernel(PagedArgs a, const float* __restrict__ ws, int target, int cap) {
-    prefetch_kernargs<sizeof(PagedArgs)>();
-    constexpr int C = D / 4, NG = 256 / C;
-    __shared__ float4 sums[256];
-    __shared__ float2 mls[NG];
-    const int kvh = blockIdx.x % a.Hkv, s = blockIdx.x / a.Hkv, row = blockIdx.y;
-    const FewItem it = few_item<true>(a, s, target);
-    if (it.parts <= 1 || row >= min(it.q.n, a.max_new) * a.G) return;
-    const int c = threadIdx.x % C, g = threadIdx.x / C;
-    float M = -INFINITY, den = 0.0f;
-    float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    bool bad = false;
-    for (int p = g; p < it.parts; p += NG) {
-        const float* pr = few_partial(const_cast<float*>(ws), it.first + p, kvh, a.Hkv, cap, D);
-        const float2 e = *(const float2*)(pr + cap * D + row * 2);
-        const float4 v = *(const float4*)(pr + row * D + 4 * c);
-        bad = bad || __float_as_uint(e.x) == kNanBits;
-        const float mn = fmaxf(M, bad ? -INFINITY : e.x), base = mn == -INFINITY ? 0.0f : mn;
-        const float f0 = __builtin_amdgcn_exp2f(M - base), f = __builtin_amdgcn_exp2f(e.x - base);
-        den = den * f0 + e.y * f;
-        num.x = num.x * f0 + v.x * f; num.y = num.y * f0 + v.y * f;
-        num.z = num.z * f0 + v.z * f; num.w = num.w * f0 + v.w * f;
-        M = mn;
+    if (it.parts == 1) return;
+    // ---- the last of the sequence's pieces adds their partials, in order:
+    // every store of this workgroup is done before its ticket
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    int* const last = (int*)lds;
+    if (tid == 0) {
+        unsigned* tk = tickets + it.s * a.Hkv + kvh;
+        const unsigned old = __hip_atomic_fetch_add(tk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *last = old == (unsigned)(it.parts - 1);
+        if (*last) __hip_atomic_store(tk, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    sums[threadIdx.x] = num;
-    if (c == 0) mls[g] = make_float2(M, den);
-    bad = __syncthreads_or(bad);
-    if (g != 0) return;
-    M = -INFINITY;
+    __syncthreads();
+    if (!*last) return;
+    for (int i = tid; i < rows * (D / 4); i += kFewWaves * 64) {
+        const int row = i / (D / 4), c = i % (D / 4);
+        float M = -INFINITY, den = 0.0f;
+        float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        bool nan = false;
+        for (int p0 = 0; p0 < it.parts; p0 += kMergeBatch) {
+            // a batch's loads go out together: one round trip each
+            u32x2 e[kMergeBatch];
+            u32x4 v[kMergeBatch];
 #pragma unroll
-    for (int k = 0; k < NG; ++k) M = fmaxf(M, mls[k].x);
-    const float base = M == -INFINITY ? 0.0f : M;
-    den = 0.0f;
-    num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int u = 0; u < kMergeBatch; ++u) {
+                const BufRsrc rs = piece_rsrc(min(p0 + u, it.parts - 1));
+                e[u] = __builtin_amdgcn_raw_buffer_load_b64(rs, (cap * D + row * 2) * 4, 0, kSc1);
+                v[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, (row * D + 4 * c) * 4, 0, kSc1);
+            }
 #pragma unroll
-    for (int k = 0; k < NG; ++k) {
-        const float f = __builtin_amdgcn_exp2f(mls[k].x - base);
-        const float4 v = sums[k * C + c];
-        den = fmaf(f, mls[k].y, den);
-        num.x = fmaf(f, v.x, num.x); num.y = fmaf(f, v.y, num.y);
-        num.z = fmaf(f, v.z, num.z); num.w = fmaf(f, v.w, num.w);
+            for (int u = 0; u < kMergeBatch; ++u) asm volatile("" : "+v"(e[u]), "+v"(v[u]));
+            float mb = M;
+#pragma unroll
+            for (int u = 0; u < kMergeBatch; ++u) {
+                const bool hit = e[u].x == kNanBits;
+                nan = nan || hit;
+                if (hit || p0 + u >= it.parts) {              // nothing to add
+                    e[u] = u32x2{0xff800000u, 0u};
+                    v[u] = u32x4{0u, 0u, 0u, 0u};
+                }
+                mb = fmaxf(mb, __uint_as_float(e[u].x));
+            }
+            const float base = mb == -INFINITY ? 0.0f : mb;
+            const float f0 = __builtin_amdgcn_exp2f(M - base);
+            M = mb;
+            den *= f0;
+            num.x *= f0; num.y *= f0; num.z *= f0; num.w *= f0;
+#pragma unroll
+            for (int u = 0; u < kMergeBatch; ++u) {
+                const float f = __builtin_amdgcn_exp2f(__uint_as_float(e[u].x) - base);
+                den = fmaf(f, __uint_as_float(e[u].y), den);
+                num.x = fmaf(f, __uint_as_float(v[u].x), num.x);
+                num.y = fmaf(f, __uint_as_float(v[u].y), num.y);
+                num.z = fmaf(f, __uint_as_float(v[u].z), num.z);
+                num.w = fmaf(f, __uint_as_float(v[u].w), num.w);
+            }
+        }
+        const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+        uint2 y = {pack2<KT>(num.x * inv, num.y * inv), pack2<KT>(num.z * inv, num.w * inv)};
+        if (nan) y.x = y.y = 0x7fff7fffu;
+        *(uint2*)(a.out + (int64_t)(it.q.q0 + row / a.G) * a.o_nb_t + (int64_t)(kvh * a.G + row % a.G) * a.o_nb_h + 8 * c) = y;
     }
-    const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-    uint2 y = {pack2<KT>(num.x * inv, num.y * inv), pack2<KT>(num.z * inv, num.w * inv)};
-    if (bad) y.x = y.y = 0x7fff7fffu;
-    *(uint2*)(a.out + (int64_t)(it.q.q0 + row / a.G) * a.o_nb_t + (int64_t)(kvh * a.G + row % a.G) * a.o_nb_h + 8 * c) = y;
 }
 
 // ----------------------------------------------------------- many rows
@@ -672,7 +704,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         const int lim = min(L - 1, past + tcol);              // the last key the lane's row sees
         auto stage = [&](int j) { return lds0 + (j % kStages) * STAGE; };
         auto read_k128 = [&](uint32_t ka, int ds, int kt) {
-            return *lds_vec((ka ^ (ds << 5)) + kt * 32 * ROW);
+            return lds_read((ka ^ (ds << 5)) + kt * 32 * ROW);
         };
         auto scores = [&](uint32_t ka, f32x16 (&s)[2]) {
 #pragma unroll
@@ -774,7 +806,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
             constexpr int NF = TB / 1024 / kWaves;
             bool nf = false;
 #pragma unroll
-            for (int i = 0; i < NF; ++i) nf = nf || chunk_not_finite<KT>(*lds_vec(vs + (i * kWaves + w) * 1024 + lane * 16));
+            for (int i = 0; i < NF; ++i) nf = nf || chunk_not_finite<KT>(lds_read(vs + (i * kWaves + w) * 1024 + lane * 16));
             if (__any(nf)) *(volatile __attribute__((address_space(3))) int*)&fix = j;
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
             if (*(volatile __attribute__((address_space(3))) int*)&fix != j) return;
@@ -895,7 +927,7 @@ __global__ void __launch_bounds__(256) paged_many_merge_kernel(PagedArgs a, cons
 }
 
 template <int D, int KT>
-hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, float* ws, hipStream_t s) {
+hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s) {
     hipError_t e = hipSuccess;
     if (p.many_tiles > 0) {
         hipLaunchKernelGGL((paged_many_kernel<D, KT>), dim3(p.many_pieces * a.Hkv), dim3(kWaves * 64), 0, s, a, ws, p.n_cu, p.max_wgs);
@@ -906,12 +938,8 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, float* ws, hipSt
         }
     }
     if (p.few_pieces > 0) {
-        hipLaunchKernelGGL((paged_few_kernel<D, KT>), dim3(p.few_pieces * a.Hkv), dim3(kFewWaves * 64), 0, s, a, ws, p.few_target, p.few_cap);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-        if (p.few_split) {
-            hipLaunchKernelGGL((paged_few_merge_kernel<D, KT>), dim3(a.n_seq * a.Hkv, p.few_cap), dim3(256), 0, s, a, ws, p.few_target, p.few_cap);
-            e = hipGetLastError();
-        }
+        hipLaunchKernelGGL((paged_few_kernel<D, KT>), dim3(p.few_pieces * a.Hkv), dim3(kFewWaves * 64), 0, s, a, ws, tickets, p.few_slots, p.few_cap);
+        e = hipGetLastError();
     }
     return e;
 }
@@ -940,11 +968,10 @@ PagedPlan paged_plan(const PagedArgs& a, int n_cu) {
     }
     if (rows <= kFewRows || !even) {
         p.few_cap = (int)std::min<int64_t>(rows, kFewRows);
-        // a workgroup per CU (D = 64: two), shared by the kv heads
-        p.few_target = std::max(1, n_cu * (a.d == 64 ? 2 : 1) / a.Hkv);
+        p.few_slots = std::max(1, n_cu * (a.d == 64 ? 4 : 2) / a.Hkv);
         const int64_t seq_tiles = (max_keys + kFewTile - 1) / kFewTile;
         p.few_split = seq_tiles > kFewMin;
-        p.few_pieces = (int)std::min<int64_t>(p.few_target + (int64_t)a.n_seq, a.n_seq * ((seq_tiles + kFewMin - 1) / kFewMin));
+        p.few_pieces = (int)std::min<int64_t>(p.few_slots + (int64_t)a.n_seq, a.n_seq * ((seq_tiles + kFewMin - 1) / kFewMin));
     }
     return p;
 }
@@ -954,10 +981,10 @@ size_t paged_ws_bytes(const PagedArgs& a, const PagedPlan& p) {
     return std::max(many, few);                    // one after the other on the stream
 }
 
-hipError_t launch_paged_attn(const PagedArgs& a, const PagedPlan& p, float* ws, hipStream_t s) {
+hipError_t launch_paged_attn(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s) {
     if (a.d == 64)
-        return a.type == VVA_TYPE_F16 ? launch_paged<64, VVA_TYPE_F16>(a, p, ws, s) : launch_paged<64, VVA_TYPE_BF16>(a, p, ws, s);
-    return a.type == VVA_TYPE_F16 ? launch_paged<128, VVA_TYPE_F16>(a, p, ws, s) : launch_paged<128, VVA_TYPE_BF16>(a, p, ws, s);
+        return a.type == VVA_TYPE_F16 ? launch_paged<64, VVA_TYPE_F16>(a, p, ws, tickets, s) : launch_paged<64, VVA_TYPE_BF16>(a, p, ws, tickets, s);
+    return a.type == VVA_TYPE_F16 ? launch_paged<128, VVA_TYPE_F16>(a, p, ws, tickets, s) : launch_paged<128, VVA_TYPE_BF16>(a, p, ws, tickets, s);
 }
 
 }  // namespace vva

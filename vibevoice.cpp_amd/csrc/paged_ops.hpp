@@ -37,3 +37,14 @@ __device__ __forceinline__ int wave_scan(int x) {
     }
     return x;
 }
+// Sum of x over the wave (DPP within rows of 16 lanes, permlane swaps across)
+__device__ __forceinline__ int wave_total(int x) {
+    x += __builtin_amdgcn_mov_dpp(x, 0xB1, 0xf, 0xf, true);
+    x += __builtin_amdgcn_mov_dpp(x, 0x4E, 0xf, 0xf, true);
+    x += __builtin_amdgcn_mov_dpp(x, 0x141, 0xf, 0xf, true);
+    x += __builtin_amdgcn_mov_dpp(x, 0x140, 0xf, 0xf, true);
+    const auto a = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)x, false, false);
+    x = (int)(a[0] + a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
+    return __builtin_amdgcn_readfirstlane((int)(b[0] + b[1]));
+}

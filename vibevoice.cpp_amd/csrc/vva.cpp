@@ -42,7 +42,8 @@ struct vva_context {
     float* scratch = nullptr;            // this device's `scratch` (vva_attn_noalloc)
     // merge tickets, zeroed once: vva_decode_step's [kMaxStepTickets], then the
     // prefill's in-launch merge [kMaxPrefillTickets], then the projection
-    // GEMM's split along K [kMaxProjTickets]
+    // GEMM's split along K [kMaxProjTickets], then vva_paged_attn's
+    // [kMaxPagedTickets]
     unsigned* tickets = nullptr;
     // the f16 window of a Q8_0 prefill flags an out-of-range value here
     // with the call's epoch; the call's gated fp32 fallback then runs
@@ -541,7 +542,7 @@ extern "C" vva_status vva_create(int device, void* stream, vva_context** out) {
     ctx->stream = (hipStream_t)stream;
     ctx->scratch = scr;
     ctx->err.reserve(512);               // error messages (< 512 bytes) then never allocate
-    constexpr size_t ticket_bytes = sizeof(unsigned) * (kMaxStepTickets + kMaxPrefillTickets + kMaxProjTickets);
+    constexpr size_t ticket_bytes = sizeof(unsigned) * (kMaxStepTickets + kMaxPrefillTickets + kMaxProjTickets + kMaxPagedTickets);
     e = hipMalloc(&ctx->tickets, ticket_bytes);
     if (e == hipSuccess) e = hipMemset(ctx->tickets, 0, ticket_bytes);
     if (e == hipSuccess) e = hipMalloc(&ctx->ovf, 256);
@@ -1591,6 +1592,8 @@ extern "C" vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, cons
     if ((st = fill_paged(ctx, "paged_attn", k_pages, v_pages, batch, Hq, N, a)) != VVA_OK) return st;
     if ((st = check_packed(ctx, q, "q", a.d, Hq, N)) != VVA_OK) return st;
     if ((st = check_packed(ctx, out, "out", a.d, Hq, N)) != VVA_OK) return st;
+    if ((Hq > 1 && q->nb[1] >= ((size_t)1 << 25)) || (N > 1 && q->nb[2] >= ((size_t)1 << 25)))
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "paged_attn: rows of q 32 MiB apart");   // 32 rows in 32-bit offsets
     if (q->type != a.type || out->type != a.type)
         return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: q and out must have the pages' type (%d)", a.type);
     if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: scale must be finite and > 0");
@@ -1600,9 +1603,12 @@ extern "C" vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, cons
     a.out = (char*)out->data; a.o_nb_h = out->nb[1]; a.o_nb_t = out->nb[2];
     a.scale = scale;
     DeviceGuard g(ctx->device);
+    if ((int64_t)a.n_seq * a.Hkv > kMaxPagedTickets)
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "paged_attn: %d sequences x %d kv heads, at most %d", a.n_seq, a.Hkv, kMaxPagedTickets);
     const PagedPlan plan = paged_plan(a, ctx->n_cu);
     if ((st = ensure_ws(ctx, paged_ws_bytes(a, plan))) != VVA_OK) return st;
-    const hipError_t e = launch_paged_attn(a, plan, ctx->ws, ctx->stream);
+    const hipError_t e = launch_paged_attn(a, plan, ctx->ws, ctx->tickets + kMaxStepTickets + kMaxPrefillTickets + kMaxProjTickets,
+                                           ctx->stream);
     return e == hipSuccess ? VVA_OK : hip_fail(ctx, e, "paged_attn launch");
 }
 

@@ -236,12 +236,14 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s);
 struct PagedPlan {
     int n_cu, max_wgs;
     int many_tiles, many_pieces;   // row tiles, pieces of their keys (per kv head; 0: no launch)
-    int few_pieces, few_target, few_cap;
+    int few_pieces, few_slots, few_cap;
     bool many_split, few_split;    // whether a second launch may have partials to add
 };
 PagedPlan paged_plan(const PagedArgs& a, int n_cu);
 size_t paged_ws_bytes(const PagedArgs& a, const PagedPlan& p);
-hipError_t launch_paged_attn(const PagedArgs& a, const PagedPlan& p, float* ws, hipStream_t s);
+// tickets: [n_seq * Hkv], zero between calls
+constexpr int kMaxPagedTickets = 65536;
+hipError_t launch_paged_attn(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s);
 hipError_t launch_norm(const NormArgs& a, hipStream_t s);
 
 hipError_t launch_rope_append(const RopeAppendArgs& a, hipStream_t s);
