@@ -59,11 +59,20 @@ typedef const __attribute__((address_space(4))) int32_t* ConstInts;
 // 64 lanes' 16 bytes from base + voff to LDS lds .. lds + 1023.  Inline asm so
 // that the compiler does not fence LDS reads on it: completion is waited for
 // explicitly.  The address is uniform but for the lane's 32-bit offset.
+// NT: non-temporal, for rows that the call reads once (64 x 4096 keys 5.4 ->
+// 6.0 TB/s, 128 x 4096 5.8 -> 6.5).
+template <bool NT>
 __device__ __forceinline__ void dma16(uint64_t base, int voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(base)
-                 : "memory", "m0");
+    if constexpr (NT)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                     :
+                     : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(base)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(base)
+                     : "memory", "m0");
 }
 __device__ __forceinline__ uint64_t uniform64(uint64_t x) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x) |
@@ -258,7 +267,9 @@ __device__ __forceinline__ FewItem few_item(const PagedArgs& a, int item, int sl
 }
 
 constexpr int kSc1 = 16;           // cache policy of the partials: agent scope
-constexpr int kMergeBatch = 16;    // pieces whose partials are loaded together
+// pieces whose partials are loaded together (16: 8 x 1024 keys 9.4 -> 10.0 us, two
+// streams of 1k keys 6.8 -> 7.3, 1 x 32768 keys 23.2 -> 22.2)
+constexpr int kMergeBatch = 8;
 
 // One workgroup per (piece of a sequence's keys, kv head), two of them (D = 64:
 // four) on a CU.  Each wave streams every fourth tile of the piece through LDS of its
@@ -318,7 +329,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int r = c * RC;                  // first row of the load, in its 16-key half r % 16
-            dma16(base[r / 16] + (uint64_t)(r % 16) * nb_slot, off[c % 4], dst + c * 1024);
+            dma16<true>(base[r / 16] + (uint64_t)(r % 16) * nb_slot, off[c % 4], dst + c * 1024);
         }
     };
     auto issue_k = [&](int t) { issue(t, ks, a.k, a.k_nb_page, a.k_nb_head, a.k_nb_slot, koff); };
@@ -334,7 +345,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
             const int c = w * (NC / kFewWaves) + i;
             const int r = c * RC + lane / (D / 8), row = r < rows ? r : 0;
             const int off = (row / a.G) * (int)a.q_nb_t + (row % a.G) * (int)a.q_nb_h;
-            dma16(qb, off + (((lane % (D / 8)) ^ k_swz<D>(r)) << 4), qs + c * 1024);
+            dma16<false>(qb, off + (((lane % (D / 8)) ^ k_swz<D>(r)) << 4), qs + c * 1024);
         }
     }
     if (t < t1) {
@@ -480,14 +491,16 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
         float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         bool nan = false;
         for (int p0 = 0; p0 < it.parts; p0 += kMergeBatch) {
-            // a batch's loads go out together: one round trip each
+            // a batch's loads go out together, one round trip each; those past
+            // the last piece lie outside their buffer and read nothing
             u32x2 e[kMergeBatch];
             u32x4 v[kMergeBatch];
 #pragma unroll
             for (int u = 0; u < kMergeBatch; ++u) {
-                const BufRsrc rs = piece_rsrc(min(p0 + u, it.parts - 1));
-                e[u] = __builtin_amdgcn_raw_buffer_load_b64(rs, (cap * D + row * 2) * 4, 0, kSc1);
-                v[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, (row * D + 4 * c) * 4, 0, kSc1);
+                const bool in = p0 + u < it.parts;
+                const BufRsrc rs = piece_rsrc(in ? p0 + u : 0);
+                e[u] = __builtin_amdgcn_raw_buffer_load_b64(rs, in ? (cap * D + row * 2) * 4 : 0x7ffffff0, 0, kSc1);
+                v[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, in ? (row * D + 4 * c) * 4 : 0x7ffffff0, 0, kSc1);
             }
 #pragma unroll
             for (int u = 0; u < kMergeBatch; ++u) asm volatile("" : "+v"(e[u]), "+v"(v[u]));
@@ -676,9 +689,9 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
             vb[i] = uniform64((uint64_t)(uintptr_t)a.v + id * a.v_nb_page + kvh * a.v_nb_head + slot * a.v_nb_slot);
         }
 #pragma unroll
-        for (int i = 0; i < NI; ++i) dma16(kb[i], koff, st + i * kWaves * 1024);
+        for (int i = 0; i < NI; ++i) dma16<false>(kb[i], koff, st + i * kWaves * 1024);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) dma16(vb[i], voff, st + TB + i * kWaves * 1024);
+        for (int i = 0; i < NI; ++i) dma16<false>(vb[i], voff, st + TB + i * kWaves * 1024);
     };
     const int row = wr0 + l32;
     const bool qok = row < rows;
@@ -968,7 +981,12 @@ PagedPlan paged_plan(const PagedArgs& a, int n_cu) {
     }
     if (rows <= kFewRows || !even) {
         p.few_cap = (int)std::min<int64_t>(rows, kFewRows);
-        p.few_slots = std::max(1, n_cu * (a.d == 64 ? 4 : 2) / a.Hkv);
+        // Half the workgroups that fit a CU, so that fewer partials are added and
+        // no CU's share of the bytes is less (1 x 32768 keys 29.3 -> 22.3 us, 64 x 4096
+        // 88.8 -> 83.8); all of them where the sequences are too many to be cut evenly
+        // into that few (48 of 500 to 8000 keys: 94.2 -> 79.3)
+        const int slots = n_cu * (a.d == 64 ? 2 : 1);
+        p.few_slots = std::max(1, (2 * a.n_seq * a.Hkv > slots ? 2 : 1) * slots / a.Hkv);
         const int64_t seq_tiles = (max_keys + kFewTile - 1) / kFewTile;
         p.few_split = seq_tiles > kFewMin;
         p.few_pieces = (int)std::min<int64_t>(p.few_slots + (int64_t)a.n_seq, a.n_seq * ((seq_tiles + kFewMin - 1) / kFewMin));
