@@ -74,6 +74,14 @@ __device__ __forceinline__ void dma16(uint64_t base, int voff, uint32_t lds) {
                      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(base)
                      : "memory", "m0");
 }
+// this lane, from the hardware: no register holds it meanwhile
+__device__ __forceinline__ int lane_id() {
+    int x;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+    return x;
+}
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float uni(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
 __device__ __forceinline__ uint64_t uniform64(uint64_t x) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x) |
            ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32)) << 32);
@@ -152,19 +160,6 @@ __device__ __forceinline__ int v_lane_off(int lane) {
     const int r = (lane & 15) >> 2;
     const int c = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_swz<D>(r);
     return (r + 4 * (lane >> 5)) * 2 * D + (c << 4) + 8 * (lane & 1);
-}
-
-// Q^T fragments of the lane's row (zeros where there is none)
-template <int D, typename QF>
-__device__ __forceinline__ void load_q(const PagedArgs& a, int q0, int kvh, int row, int rows, int half, QF (&qf)[D / 16]) {
-    const bool ok = row < rows;
-    const int t = ok ? row / a.G : 0, h = ok ? row % a.G : 0;
-    const char* p = a.q + (int64_t)(q0 + t) * a.q_nb_t + (int64_t)(kvh * a.G + h) * a.q_nb_h + half * 16;
-#pragma unroll
-    for (int ds = 0; ds < D / 16; ++ds) {
-        const u32x4 r = *(const u32x4*)(p + ds * 32);
-        qf[ds] = as_vec<QF>(ok ? r : u32x4{0u, 0u, 0u, 0u});
-    }
 }
 
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
@@ -381,7 +376,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
         const bool masked = k0 + kFewTile - 1 > min(L - 1, past);      // some row must not see some key
         if (masked) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = k0 + 8 * (r / 4) + 4 * half + r % 4 > lim ? -INFINITY : s[r];
+            for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + r % 4 > lim - k0 - 4 * half ? -INFINITY : s[r];
         }
         float mx = fmaxf(s[0], s[1]);
 #pragma unroll
@@ -544,91 +539,108 @@ constexpr int kRowsWave = 32;
 constexpr int kWaves = 8;          // two per SIMD
 constexpr int kRowsWG = kRowsWave * kWaves;
 constexpr int kStages = 4;         // LDS ring: tile j + 3 loads while tile j is computed
-constexpr int kMaxKs = 16;         // key splits per row tile
-constexpr int kMinPiece = 8;       // key tiles of a piece at least
+constexpr int kMinShare = 4;       // key tiles of a workgroup's share at least
+constexpr int kRowTileCost = 4;    // what a row tile costs beside its keys, in key tiles
+constexpr int kMaxWgs = 256;       // workgroups of a call at most
+constexpr int kGroup = 8;          // pieces whose partials are added at once
+constexpr int kManyTickets = kMaxWgs * kWaves * (1 + kMaxWgs / kGroup);
 
-// A piece of a row tile's keys: row tile rt of the sequence, piece `ks` of
-// `n_ks`; n_ks = 0: none.  first: the row tile's piece 0 of the call.
-struct ManyItem {
-    Seq q;
-    int s, rt, ks, n_ks, first;
-};
+// Row tiles of a sequence, and the key tiles that one sees
 __device__ __forceinline__ int many_row_tiles(const PagedArgs& a, const Seq& q) {
     const int n = min(q.n, a.max_new);
     return n * a.G > kFewRows ? (n * a.G + kRowsWG - 1) / kRowsWG : 0;
 }
-// Key tiles that row tile rt of a sequence sees
 __device__ __forceinline__ int many_key_tiles(const PagedArgs& a, const Seq& q, int rt) {
     const int n = min(q.n, a.max_new);
     const int t_hi = min(n * a.G, (rt + 1) * kRowsWG) - 1;
     return (max(0, min(q.L, q.L - q.n + t_hi / a.G + 1)) + kBN - 1) / kBN;
 }
-// Item `item` of the call: a row tile (TILE) or a piece of one; the last row
-// tiles of a sequence (the longest) come first.  Every row tile is cut into the same number of
-// pieces, the one that leaves the least for the fullest CU (one workgroup at a
-// time each): rounds of workgroups times their share of the keys and what a
-// piece costs beside them, about kMinPiece tiles.  max_wgs: the most workgroups
-// that the launch's grid and workspace hold of split row tiles (0: none is
-// split).  By whole waves.
-template <bool TILE>
-__device__ __forceinline__ ManyItem many_item(const PagedArgs& a, int item, int n_cu, int max_wgs) {
+
+// The call's work on one axis: kv heads, in them the sequences, in them the
+// row tiles, each as long as the keys that it sees: first + slope * (rt + 1)
+// sixteenths of a key tile (more, where 2^30 of them would not hold the call).
+// The axis is cut into equal shares, one per workgroup, wherever that falls in
+// a row tile: a chunk over a long cache, prompts of unlike lengths and a few
+// row tiles all leave every CU the same work.
+struct ManyWeight {
+    int r, first, slope;
+    __device__ __forceinline__ int before(int rt) const { return rt * first + (int)((int64_t)slope * rt * (rt + 1) / 2); }
+    __device__ __forceinline__ int of(int rt) const { return first + slope * (rt + 1); }
+};
+__device__ __forceinline__ ManyWeight many_weight(const PagedArgs& a, const Seq& q, int slope, int shift) {
+    ManyWeight w;
+    w.r = many_row_tiles(a, q);
+    w.first = max((max(q.L - q.n, 0) / (kBN / 16) + 16 * kRowTileCost) >> shift, 1);
+    w.slope = slope >> shift;
+    return w;
+}
+struct ManyAxis {
+    int slope;              // of a row tile, in sixteenths
+    int shift;              // the unit's power of two above a sixteenth
+    int head;               // length of a kv head's part (0: no work)
+};
+// `mine`: the lane's own of the first 64 sequences.  By whole waves.
+__device__ __forceinline__ ManyAxis many_axis(const PagedArgs& a, const Seq& mine) {
     const int lane = threadIdx.x & 63;
-    int rts = 0;
-    float work = 0.0f;
-    for (int i = 0; i < a.n_seq; i += 64) {
-        const int s = i + lane;
-        const Seq q = seq_of(a, min(s, a.n_seq - 1));
-        const int r = s < a.n_seq ? many_row_tiles(a, q) : 0;
-        rts += r;
-        work += r > 0 ? (float)r * (float)many_key_tiles(a, q, r - 1) : 0.0f;
+    ManyAxis x;
+    x.slope = uni(kRowsWG * 16 / kBN / a.G);
+    float all = 0.0f;
+    for (int s = lane; s < a.n_seq; s += 64) {
+        const ManyWeight w = many_weight(a, s == lane ? mine : seq_of(a, s), x.slope, 0);
+        all += (float)w.r * ((float)w.first + 0.5f * (float)w.slope * (float)(w.r + 1));
     }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-        rts += __shfl_xor(rts, m, 64);
-        work += __shfl_xor(work, m, 64);
+    all = wave_sum(all) * (float)a.Hkv;
+    int shift = 0;
+    for (; all > 1.0e9f; all *= 0.5f) ++shift;
+    x.shift = uni(shift);
+    int total = 0;
+    for (int s = lane; s < a.n_seq; s += 64) {
+        const ManyWeight w = many_weight(a, s == lane ? mine : seq_of(a, s), x.slope, x.shift);
+        total += w.before(w.r);
     }
-    ManyItem it{};
-    if (rts == 0) return it;
-    const int kt = (int)(work / (float)rts);       // key tiles of a row tile
-    const int wgs = rts * a.Hkv;
-    // lane x: x + 1 pieces
-    const int x = min(lane, kMaxKs - 1) + 1;
-    int cost = 0x7fffffff;
-    if (x == 1 || (wgs * x <= max_wgs && kt >= kMinPiece * x))
-        cost = ((wgs * x + n_cu - 1) / n_cu) * ((kt + x - 1) / x + (x > 1 ? kMinPiece : 0));
-    int best = cost;
-#pragma unroll
-    for (int m = 8; m >= 1; m >>= 1) best = min(best, __shfl_xor(best, m, 64));
-    const int sp = __ffsll((unsigned long long)__ballot(cost == best));
-    const int tile = TILE ? item : item / sp;
-    it.ks = TILE ? 0 : item - tile * sp;
+    x.head = wave_total(total);
+    return x;
+}
+// The sequence at place p of a kv head's part, and where it starts and ends
+struct ManySeq {
+    Seq q;
+    int s, start, end;
+};
+__device__ __forceinline__ ManySeq many_seq(const PagedArgs& a, const ManyAxis& x, const Seq& mine, int p) {
+    const int lane = threadIdx.x & 63;
+    ManySeq r{};
+    Seq q = mine;
     int base = 0;
     for (int i = 0; i < a.n_seq; i += 64) {
-        const int s = i + lane;
-        const Seq q = seq_of(a, min(s, a.n_seq - 1));
-        const int r = s < a.n_seq ? many_row_tiles(a, q) : 0;
-        const int end = wave_scan(r);
-        const uint64_t hit = __ballot(tile >= base + end - r && tile < base + end);
+        if (i > 0) q = seq_of(a, min(i + lane, a.n_seq - 1));
+        const ManyWeight w = many_weight(a, q, x.slope, x.shift);
+        const int len = i + lane < a.n_seq ? w.before(w.r) : 0;
+        const int end = base + wave_scan(len);
+        const uint64_t hit = __ballot(p >= end - len && p < end);
         if (hit) {
             const int l = __ffsll((unsigned long long)hit) - 1;
-            it.q.q0 = lane_of(q.q0, l);
-            it.q.n = lane_of(q.n, l);
-            it.q.L = lane_of(q.L, l);
-            it.s = i + l;
-            it.rt = base + lane_of(end, l) - 1 - tile;
-            it.first = tile * sp;
-            it.n_ks = sp;
-            return it;
+            r.q.q0 = lane_of(q.q0, l);
+            r.q.n = lane_of(q.n, l);
+            r.q.L = lane_of(q.L, l);
+            r.s = i + l;
+            r.end = lane_of(end, l);
+            r.start = r.end - lane_of(len, l);
+            return r;
         }
-        base += lane_of(end, 63);
+        base = lane_of(end, 63);
     }
-    return it;
+    return r;
 }
 
-// One workgroup per (piece of a row tile's keys, kv head): 8 waves x 32 rows
-// that share every K / V tile.
+// One workgroup per share of the work: 8 waves x 32 rows that share every K / V
+// tile.  A row tile that lies in one share is written at once; of one that
+// several workgroups share, each leaves its rows' sums in the workspace, wave
+// by wave ([wave][16-byte group][lane], then (exponent base, row sum)), and
+// takes the wave's ticket: the last of up to kGroup pieces adds them, and of
+// more groups the last adds the groups, in the order of the keys whoever it is
+// (its own sums are read back too, so that they need no registers meanwhile).
 template <int D, int KT>
-__global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, float* __restrict__ ws, int n_cu, int max_wgs) {
+__global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets) {
     prefetch_kernargs<sizeof(PagedArgs)>();
     using F = Frag<KT>;
     using QF = typename F::type;
@@ -639,99 +651,196 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     constexpr int RC = 1024 / ROW;                 // rows of a load
     constexpr int STAGE = 2 * TB;
     constexpr int NLD = 2 * NI;
+    constexpr int WAVE_O = DT * 16 * 64 * 4;       // bytes of a wave's sums
+    constexpr int WAVE = WAVE_O + 64 * 8;
     __shared__ __attribute__((aligned(1024))) char lds[kStages * STAGE];
-    __shared__ int fix;                            // the last tile found to hold a V that is not finite
+    __shared__ int fix, bad_seg;                   // the last tile with a V that is not finite, the last share with a bad page
 
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kvh = blockIdx.x % a.Hkv;
-    if (tid == 0) fix = -1;                        // before the first tile's barrier
-    const ManyItem it = many_item<false>(a, blockIdx.x / a.Hkv, n_cu, max_wgs);
-    if (it.n_ks == 0) return;
-    const int L = it.q.L, past = L - it.q.n, G = a.G;
-    const int rows = min(it.q.n, a.max_new) * G;
-    const int wr0 = it.rt * kRowsWG + w * kRowsWave;
-    const int n_tiles_rt = many_key_tiles(a, it.q, it.rt);
-    const int j_lo = (int)((int64_t)it.ks * n_tiles_rt / it.n_ks);
-    const int n_tiles = (int)((int64_t)(it.ks + 1) * n_tiles_rt / it.n_ks) - j_lo;
-    const int kb0 = j_lo * kBN;
-    // keys [0, kend_w) are seen by some row of the wave, keys up to lim_w by every row
-    const bool wave_live = wr0 < rows;
-    const int kend_w = wave_live ? max(0, min(L, past + (min(wr0 + kRowsWave, rows) - 1) / G + 1)) : 0;
-    const int lim_w = min(L - 1, past + min(wr0, rows - 1) / G);
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (threadIdx.x == 0) fix = bad_seg = -1;      // before the first tile's barrier
+    ManySeq sq{};                                  // the sequence at hand, and its end on the axis
+    int sq_kvh = 0, sq_end = -1;
+    int head, axis_shift, axis_slope;
+    int g, wgs, share, more;
+    {
+    const Seq mine = seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1));
+    const ManyAxis axis = many_axis(a, mine);
+    head = axis.head;
+    axis_shift = axis.shift;
+    axis_slope = axis.slope;
+    if (head <= 0) return;
+    const int total = head * a.Hkv;
+    wgs = uni(min((int)gridDim.x, max(1, total / max((16 * kMinShare) >> axis_shift, 1))));
+    if ((int)blockIdx.x >= wgs) return;
+    // neighbouring shares on one XCD (workgroups go round its 8): they read the same keys
+    g = wgs % 8 == 0 ? (int)(blockIdx.x % 8) * (wgs / 8) + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+    share = uni(total / wgs);
+    more = uni(total - share * wgs);
+    const int p = g * share + min(g, more);
+    sq_kvh = uni(p / head);
+    sq = many_seq(a, axis, mine, p - sq_kvh * head);
+    sq_end = sq_kvh * head + sq.end;
+    }
+    // the workgroup whose share holds place p
+    auto owner = [&](int p) {
+        const int cut = more * (share + 1);
+        return uni(min(wgs - 1, p < cut ? p / (share + 1) : more + (p - cut) / max(share, 1)));
+    };
+    const int p_end = (g + 1) * share + min(g + 1, more);
+    const int G = a.G;
+    const float inv_g = uni(1.0f / (float)G);
+
+    // ---- the row tile at place p of the axis, and this workgroup's keys of it
+    struct Cut {
+        int s, kvh, q0, rows, L, past;             // the sequence; rows of its kv group
+        int rt, n_tiles, kb0;                      // row tile, key tiles from key kb0 on
+        int place, len;                            // the row tile on the axis
+        bool whole;
+        int next;                                  // the place after this part
+    };
+    auto find = [&](int p) {
+        Cut c;
+        if (p >= sq_end) {
+            sq_kvh = uni(p / head);
+            sq = many_seq(a, ManyAxis{axis_slope, axis_shift, head}, seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1)), p - sq_kvh * head);
+            sq_end = sq.end > sq.start ? sq_kvh * head + sq.end : p_end;   // no sequence: a batch that changed meanwhile
+        }
+        ManyWeight wt = many_weight(a, sq.q, axis_slope, axis_shift);
+        wt.r = uni(wt.r);
+        const int ps = p - sq_kvh * head - sq.start;           // place in the sequence
+        const float s2 = 0.5f * (float)wt.slope, f1 = (float)wt.first + s2;
+        int rt = (int)(wt.slope > 0 ? (sqrtf(f1 * f1 + 4.0f * s2 * (float)ps) - f1) * __builtin_amdgcn_rcpf(2.0f * s2)
+                                    : (float)ps * __builtin_amdgcn_rcpf((float)wt.first));
+        rt = uni(max(0, min(rt, wt.r - 1)));
+        while (rt > 0 && wt.before(rt) > ps) --rt;
+        while (rt + 1 < wt.r && wt.before(rt + 1) <= ps) ++rt;
+        c.rt = rt;
+        c.s = sq.s;
+        c.kvh = sq_kvh;
+        c.q0 = sq.q.q0;
+        c.rows = min(sq.q.n, a.max_new) * G;
+        c.L = sq.q.L;
+        c.past = sq.q.L - sq.q.n;
+        c.len = wt.of(rt);
+        const int off = ps - wt.before(rt), off_end = min(c.len, off + p_end - p);
+        c.place = p - off;
+        c.whole = off <= 0 && off_end == c.len;
+        c.next = p + max(1, off_end - off);
+        // keys in proportion: a function of the place alone, so that a part ends where the next begins
+        const int tiles = uni(many_key_tiles(a, sq.q, rt));
+        const float r = (float)tiles * __builtin_amdgcn_rcpf((float)c.len);
+        const int lo = uni(min(tiles, (int)((float)max(off, 0) * r)));
+        c.n_tiles = (off_end == c.len ? tiles : uni(min(tiles, (int)((float)off_end * r)))) - lo;
+        c.kb0 = lo * kBN;
+        return c;
+    };
 
     // ---- tile loads: load i of K (V) covers rows RC * (i * 8 + w) .. of the
     // tile, inside one 16-key group
-    const ConstInts table = (ConstInts)(uintptr_t)(a.table + (int64_t)it.s * a.table_stride);
-    const int last_page = max(0, (L - 1) >> a.page_shift);
-    const int r0w = RC * w;                                   // first row of the wave's loads, + i * 8 * RC
-    const int koff = dma_off<D, false>(lane, r0w, (int)a.k_nb_slot);
-    const int voff = dma_off<D, true>(lane, r0w, (int)a.v_nb_slot);
+    const int r0w = RC * w;                        // first row of the wave's loads, + i * 8 * RC
+    const int koff = dma_off<D, false>(lane_id(), r0w, (int)a.k_nb_slot);
+    const int voff = dma_off<D, true>(lane_id(), r0w, (int)a.v_nb_slot);
+    const int k_off = k_lane_off<D>(lane_id()), v_off = v_lane_off<D>(lane_id());
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)lds;
+    const float sl2 = uni(a.scale * kLog2e);
     bool bad = false;
     int ids[NI];
-    auto fetch = [&](int j) {
+    auto fetch = [&](const Cut& c, int j, int (&id)[NI]) {
+        const ConstInts table = (ConstInts)(uintptr_t)(a.table + (int64_t)c.s * a.table_stride);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) ids[i] = table[min((kb0 + j * kBN + i * kWaves * RC + r0w) >> a.page_shift, last_page)];
+        for (int i = 0; i < NI; ++i)
+            id[i] = table[min((c.kb0 + j * kBN + i * kWaves * RC + r0w) >> a.page_shift, max(0, (c.L - 1) >> a.page_shift))];
     };
-    // the loads of tile j (K, then V); past the last tile the last one's again,
-    // to a stage that nobody reads any more, so that every tile counts the same
-    auto issue = [&](int j) {
+    // the loads of tile j (K, then V); past the last tile further ones of the
+    // sequence, to a stage that nobody reads any more, so that every tile
+    // counts the same
+    auto issue = [&](const Cut& c, int j, const int (&id)[NI]) {
         const uint32_t st = lds0 + (j % kStages) * STAGE + w * 1024;
         uint64_t kb[NI], vb[NI];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const bool ok = (uint32_t)ids[i] < (uint32_t)a.n_pages;
+            const bool ok = (uint32_t)id[i] < (uint32_t)a.n_pages;
             bad = bad || !ok;
-            const int64_t id = ok ? ids[i] : 0;
-            const int64_t slot = (kb0 + j * kBN + i * kWaves * RC + r0w) & ((1 << a.page_shift) - 1);
-            kb[i] = uniform64((uint64_t)(uintptr_t)a.k + id * a.k_nb_page + kvh * a.k_nb_head + slot * a.k_nb_slot);
-            vb[i] = uniform64((uint64_t)(uintptr_t)a.v + id * a.v_nb_page + kvh * a.v_nb_head + slot * a.v_nb_slot);
+            const int64_t page = ok ? id[i] : 0;
+            const int64_t slot = (c.kb0 + j * kBN + i * kWaves * RC + r0w) & ((1 << a.page_shift) - 1);
+            kb[i] = uniform64((uint64_t)(uintptr_t)a.k + page * a.k_nb_page + c.kvh * a.k_nb_head + slot * a.k_nb_slot);
+            vb[i] = uniform64((uint64_t)(uintptr_t)a.v + page * a.v_nb_page + c.kvh * a.v_nb_head + slot * a.v_nb_slot);
         }
 #pragma unroll
         for (int i = 0; i < NI; ++i) dma16<false>(kb[i], koff, st + i * kWaves * 1024);
 #pragma unroll
         for (int i = 0; i < NI; ++i) dma16<false>(vb[i], voff, st + TB + i * kWaves * 1024);
     };
-    const int row = wr0 + l32;
-    const bool qok = row < rows;
-    const int tcol = (qok ? row : rows - 1) / G;
-    QF qf[DS];
+    // x = t * G + h for small x (below G + 32): one product
+    auto small_divide = [&](int x, int& t, int& h) {
+        t = (int)(((float)x + 0.5f) * inv_g);
+        h = x - t * G;
+    };
+    // a part's first loads: the wave's rows of Q (laid out as K is, in the
+    // stages of tiles 2 and 3; rows past the last: one that is there), two tiles
+    auto start = [&](const Cut& c) {
+        bad = false;
+        const int ln = lane_id();                  // offsets made here, not held from one part to the next
+        int id0[NI], id1[NI];
+        fetch(c, 0, id0);
+        fetch(c, 1, id1);
+        fetch(c, 2, ids);
+        const int wr0 = min(c.rt * kRowsWG + w * kRowsWave, c.rows - 1), live = min(kRowsWave, c.rows - wr0);
+        const int t0 = wr0 / G, h0 = wr0 - t0 * G;
+        const uint64_t qb = uniform64((uint64_t)(uintptr_t)a.q + (int64_t)(c.q0 + t0) * a.q_nb_t + (int64_t)c.kvh * G * a.q_nb_h);
+#pragma unroll
+        for (int i = 0; i < kRowsWave / RC; ++i) {
+            const int r = i * RC + ln / (D / 8);
+            int t, h;
+            small_divide(h0 + (r < live ? r : 0), t, h);
+            dma16<false>(qb, t * (int)a.q_nb_t + h * (int)a.q_nb_h + (((ln % (D / 8)) ^ k_swz<D>(r)) << 4),
+                         lds0 + 2 * STAGE + w * kRowsWave * ROW + i * 1024);
+        }
+        issue(c, 0, id0);
+        issue(c, 1, id1);
+    };
+
+    int fix_id = 0;
+    for (int p = g * share + min(g, more), seg = 0, p_next; p < p_end; p = p_next, ++seg) {
+    const Cut c = find(p);
+    p_next = c.next;
+    if (c.n_tiles > 0) start(c);
+    const int L = c.L, past = c.past, kb0 = c.kb0, n_tiles = c.n_tiles, rows = c.rows;
+    const int wr0 = c.rt * kRowsWG + w * kRowsWave;
+    const bool wave_live = wr0 < rows;
     float m = -INFINITY, lsum = 0.0f;
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
     if (n_tiles > 0) {                                        // uniform
-        fetch(0);
-        issue(0);
-        load_q<D>(a, it.q.q0, kvh, row, rows, half, qf);
+        // keys [0, kend_w) are seen by some row of the wave, keys up to lim_w by every row
+        const int kend_w = uni(wave_live ? max(0, min(L, past + (min(wr0 + kRowsWave, rows) - 1) / G + 1)) : 0);
+        const int lim_w = uni(min(L - 1, past + min(wr0, rows - 1) / G));
+        int lim, hcol;                                        // the last key the lane's row sees
+        const int wr = min(wr0, rows - 1), t0 = wr / G;
+        const int l32 = lane_id() & 31;
+        small_divide(wr - t0 * G + (wr0 + l32 < rows ? l32 : 0), lim, hcol);
+        lim = min(L - 1, past + t0 + lim);
+        wait_vm<2 * NLD>();                                   // Q has landed
+        QF qf[DS];
+        {
+            const uint32_t qa = lds0 + 2 * STAGE + w * kRowsWave * ROW + k_lane_off<D>(lane_id());
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds) asm volatile("" : "+v"(qf[ds]));   // Q has landed, and tile 0
-        fetch(1);
-        issue(1);
-        fetch(2);
-        issue(2);
-        fetch(3);
-        const float sl2 = a.scale * kLog2e;
-        const int k_off = k_lane_off<D>(lane), v_off = v_lane_off<D>(lane);
-        const int lim = min(L - 1, past + tcol);              // the last key the lane's row sees
+            for (int ds = 0; ds < DS; ++ds) qf[ds] = as_vec<QF>(lds_read(qa ^ (ds << 5)));
+        }
+        // K of tile 0 has landed (its V and tile 1 may still fly), and every wave has its Q
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(NI + NLD) : "memory");
+        issue(c, 2, ids);
+        fetch(c, 3, ids);
         auto stage = [&](int j) { return lds0 + (j % kStages) * STAGE; };
-        auto read_k128 = [&](uint32_t ka, int ds, int kt) {
-            return lds_read((ka ^ (ds << 5)) + kt * 32 * ROW);
-        };
-        auto scores = [&](uint32_t ka, f32x16 (&s)[2]) {
-#pragma unroll
-            for (int ds = 0; ds < DS; ++ds)
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-                    s[kt] = F::mma(as_vec<QF>(read_k128(ka, ds, kt)), qf[ds], ds == 0 ? f32x16{} : s[kt]);
-        };
+        auto read_k = [&](uint32_t ka, int ds, int kt) { return lds_read((ka ^ (ds << 5)) + kt * 32 * ROW); };
         auto apply_mask = [&](f32x16 (&s)[2], int k0) {
+            const int x = lim - k0 - 4 * (lane_id() >> 5);
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    s[kt][r] = k0 + kt * 32 + 8 * (r / 4) + 4 * half + r % 4 > lim ? -INFINITY : s[kt][r];
+                    s[kt][r] = kt * 32 + 8 * (r / 4) + r % 4 > x ? -INFINITY : s[kt][r];
         };
         auto rowmax = [&](const f32x16 (&s)[2]) {
             float mr = fmaxf(fmaxf(s[0][0], s[0][1]), s[0][2]);
@@ -755,21 +864,20 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         };
         // Software pipeline over the key tiles: a step raises the running max
         // to tile j's, then runs one straight line of matrix-core slots, the
-        // scores of tile j + 1, then P.V of tile j, with the softmax of tile j
-        // and the operand reads placed between them by scheduling fences so
-        // that the VALU issues while the matrix cores run.
+        // scores of tile j + 1, then P.V of tile j, with the softmax of tile j and the operand reads placed between them by
+        // scheduling fences so that the VALU issues while the matrix cores run.
         const int n_live = max(0, min(n_tiles, (kend_w - kb0 + kBN - 1) / kBN));   // the wave's tiles
         auto needs_mask = [&](int j) { return kb0 + j * kBN + kBN - 1 > lim_w; };
-        constexpr int NQ = 2 * DS, NP = 4 * DT, NS = NQ + NP;
-        constexpr int KAHEAD = 2, VAHEAD = 2;                 // operand reads ahead of their slot
         auto block = [&](const f32x16 (&cur)[2], f32x16 (&nxt)[2], uint32_t ka, uint32_t va) {
+            constexpr int NQ = 2 * DS, NP = 4 * DT, NS = NQ + NP;
+            constexpr int KAHEAD = 2, VAHEAD = 2;             // operand reads ahead of their slot
             const float nb = m == -INFINITY ? 0.0f : -m;      // no visible key yet: every s is -inf
             u32x4 kf[NQ], vf[NP];
             float pe[32];
             uint32_t pp[16];
             float ps = lsum;
-            auto read_k = [&](int i) { kf[i] = read_k128(ka, i >> 1, i & 1); };
-            auto read_v = [&](int p) {
+            auto get_k = [&](int i) { kf[i] = read_k(ka, i >> 1, i & 1); };
+            auto get_v = [&](int p) {
                 const uint32_t v = (va ^ ((p % DT) << 6)) + (p / DT) * 16 * ROW;
                 vf[p] = v_bits<KT>(lds_at(v), lds_at(v + 8 * ROW));
             };
@@ -791,19 +899,19 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
                 }
             };
 #pragma unroll
-            for (int i = 0; i < KAHEAD; ++i) read_k(i);
+            for (int i = 0; i < KAHEAD; ++i) get_k(i);
 #pragma unroll
             for (int sl = 0; sl < NS; ++sl) {
                 if (sl < NQ) {
                     const int ds = sl >> 1, kt = sl & 1;
                     nxt[kt] = F::mma(as_vec<QF>(kf[sl]), qf[ds], ds == 0 ? f32x16{} : nxt[kt]);
-                    if (sl + KAHEAD < NQ) read_k(sl + KAHEAD);
+                    if (sl + KAHEAD < NQ) get_k(sl + KAHEAD);
                 } else {
-                    const int p = sl - NQ, c = p / DT;
-                    const QF pf = as_vec<QF>(u32x4{pp[4 * c], pp[4 * c + 1], pp[4 * c + 2], pp[4 * c + 3]});
+                    const int p = sl - NQ, ch = p / DT;
+                    const QF pf = as_vec<QF>(u32x4{pp[4 * ch], pp[4 * ch + 1], pp[4 * ch + 2], pp[4 * ch + 3]});
                     o[p % DT] = F::mma(as_vec<QF>(vf[p]), pf, o[p % DT]);
                 }
-                if (sl - NQ + VAHEAD >= 0 && sl - NQ + VAHEAD < NP) read_v(sl - NQ + VAHEAD);
+                if (sl - NQ + VAHEAD >= 0 && sl - NQ + VAHEAD < NP) get_v(sl - NQ + VAHEAD);
                 valu_slot(sl);
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -813,17 +921,19 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         // looks at its share of V, and where a value is not finite every row adds
         // the ones that it sees and the tile goes on with zeros in their places
         // (the order of the barriers is the workgroup's; seen by no other tile).
-        const int lim_wg = min(L - 1, past + min(it.rt * kRowsWG, rows - 1) / G);
+        const int lim_wg = uni(min(L - 1, past + min(c.rt * kRowsWG, rows - 1) / G));
         auto fix_tile = [&](int j) {
+            const int lane = lane_id();
             const uint32_t vs = stage(j) + TB;
             constexpr int NF = TB / 1024 / kWaves;
             bool nf = false;
 #pragma unroll
             for (int i = 0; i < NF; ++i) nf = nf || chunk_not_finite<KT>(lds_read(vs + (i * kWaves + w) * 1024 + lane * 16));
-            if (__any(nf)) *(volatile __attribute__((address_space(3))) int*)&fix = j;
+            ++fix_id;
+            if (__any(nf)) *(volatile __attribute__((address_space(3))) int*)&fix = fix_id;
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
-            if (*(volatile __attribute__((address_space(3))) int*)&fix != j) return;
-            add_not_finite<D, KT, kBN>(vs, kb0 + j * kBN, qok ? lim : -1, half, o);
+            if (*(volatile __attribute__((address_space(3))) int*)&fix != fix_id) return;
+            add_not_finite<D, KT, kBN>(vs, kb0 + j * kBN, lim, lane >> 5, o);
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
 #pragma unroll
             for (int i = 0; i < NF; ++i) {
@@ -833,12 +943,15 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
             }
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
         };
-        // K of tile 0 has landed (its V and tiles 1, 2 may still fly)
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(NI + 2 * NLD) : "memory");
         f32x16 sa[2], sb[2];
         float mx = 0.0f;
         if (n_live > 0) {
-            scores(stage(0) + k_off, sa);
+            uint32_t ka = stage(0) + k_off;
+            asm volatile("" : "+v"(ka));                      // its variants are made here, not held
+#pragma unroll
+            for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) sa[kt] = F::mma(as_vec<QF>(read_k(ka, ds, kt)), qf[ds], ds == 0 ? f32x16{} : sa[kt]);
             if (needs_mask(0)) apply_mask(sa, kb0);
             mx = rowmax(sa);
         }
@@ -846,8 +959,8 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
             // K of tile j + 1 and V of tile j have landed, and every wave is done
             // with tile j - 1, whose stage tile j + 3 now takes
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(NI + NLD) : "memory");
-            issue(j + 3);
-            fetch(j + 4);
+            issue(c, j + 3, ids);
+            fetch(c, j + 4, ids);
             if (j < n_live) rescale(mx);                      // wave-uniform
             if (kb0 + j * kBN + kBN - 1 > lim_wg) fix_tile(j);
             if (j < n_live) {
@@ -860,95 +973,132 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
                 mx = rowmax(nxt);
             }
         };
-        int j = 0;
-        for (; j + 1 < n_tiles; j += 2) {
+        for (int j = 0; j < n_tiles; j += 2) {
             step(j, sa, sb);
-            step(j + 1, sb, sa);
+            if (j + 1 < n_tiles) step(j + 1, sb, sa);
         }
-        if (j < n_tiles) step(j, sa, sb);
+        if (__any(bad)) *(volatile __attribute__((address_space(3))) int*)&bad_seg = seg;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");   // the padding tiles' loads
     }
-    // ---- normalize and write (lanes l and l ^ 32 summed different keys), or
-    // the piece's partial: sums, and (exponent base, row sum)
-    const float lt = add_swap32(lsum);
-    const bool any_bad = __syncthreads_or(bad);
-    if (!qok) return;
-    if (it.n_ks == 1) {
-        char* const orow = a.out + (int64_t)(it.q.q0 + row / G) * a.o_nb_t + (int64_t)(kvh * G + row % G) * a.o_nb_h;
+    if (!wave_live) continue;
+    // ---- this workgroup's sums of the wave's rows (lanes l and l ^ 32 summed
+    // different keys); with the other pieces' where the row tile has several
+    const int ln = lane_id();
+    float lt = add_swap32(lsum);
+    bool nan = c.n_tiles > 0 && *(volatile __attribute__((address_space(3))) int*)&bad_seg == seg;
+    bool done = true;
+    if (!c.whole) {
+        const int g0 = owner(c.place), pieces = owner(c.place + c.len - 1) - g0 + 1;
+        // piece k's slot: workgroup g0's second, the others' first
+        auto piece_rsrc = [&](int k) {
+            const int slot = k == 0 ? 2 * g0 + 1 : 2 * min(g0 + k, wgs - 1);
+            return make_rsrc((const char*)(uintptr_t)uniform64((uint64_t)(uintptr_t)ws + (uint64_t)(slot * kWaves + w) * WAVE), WAVE);
+        };
+        auto store = [&](int k) {
+            const BufRsrc rs = piece_rsrc(k);
+#pragma unroll
+            for (int i = 0; i < DT * 4; ++i)
+                __builtin_amdgcn_raw_buffer_store_b128(
+                    u32x4{__float_as_uint(o[i / 4][4 * (i % 4)]), __float_as_uint(o[i / 4][4 * (i % 4) + 1]),
+                          __float_as_uint(o[i / 4][4 * (i % 4) + 2]), __float_as_uint(o[i / 4][4 * (i % 4) + 3])},
+                    rs, ln * 16 + i * 1024, 0, kSc1);
+            __builtin_amdgcn_raw_buffer_store_b64(u32x2{nan ? kNanBits : __float_as_uint(m), __float_as_uint(lt)}, rs,
+                                                  WAVE_O + ln * 8, 0, kSc1);
+        };
+        // whether this wave is the last of n at the ticket; its stores are done before
+        auto last_of = [&](unsigned* tk, int n) {
+            __builtin_amdgcn_s_waitcnt(0);
+            unsigned old = 0;
+            if (ln == 0) {
+                old = __hip_atomic_fetch_add(tk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (old == (unsigned)(n - 1)) __hip_atomic_store(tk, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            return __builtin_amdgcn_readfirstlane((int)old) == n - 1;
+        };
+        // pieces first, first + by, ... (n of them) added in this order
+        auto add = [&](int first, int by, int n) {
+            float M = -INFINITY, den = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+                const BufRsrc rs = piece_rsrc(first + i * by);
+                const u32x2 e = __builtin_amdgcn_raw_buffer_load_b64(rs, WAVE_O + ln * 8, 0, kSc1);
+                u32x4 v[DT * 4];                   // loaded together: one round trip
+#pragma unroll
+                for (int k = 0; k < DT * 4; ++k) v[k] = __builtin_amdgcn_raw_buffer_load_b128(rs, ln * 16 + k * 1024, 0, kSc1);
+                __builtin_amdgcn_sched_barrier(0);
+                const bool hit = e.x == kNanBits;
+                nan = nan || hit;
+                const float mi = hit ? -INFINITY : __uint_as_float(e.x);
+                const float mn = fmaxf(M, mi), base = mn == -INFINITY ? 0.0f : mn;
+                const float f0 = __builtin_amdgcn_exp2f(M - base), f = __builtin_amdgcn_exp2f(mi - base);
+                den = den * f0 + __uint_as_float(e.y) * f;
+#pragma unroll
+                for (int k = 0; k < DT * 4; ++k) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int t = k / 4, r = 4 * (k % 4) + x;
+                        o[t][r] = fmaf(__uint_as_float(v[k][x]), f, o[t][r] * f0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                M = mn;
+            }
+            m = M;
+            lt = den;
+        };
+        const int k = g - g0, grp = k / kGroup, groups = (pieces + kGroup - 1) / kGroup;
+        store(k);
+        unsigned* tk = tickets + kMaxWgs * kWaves + ((g0 * kWaves + w) * (kMaxWgs / kGroup) + grp);
+        int first = grp * kGroup, by = 1, n = min(kGroup, pieces - first);
+#pragma unroll 1
+        for (int level = 0; level < 2; ++level) {
+            if (n > 1) {
+                done = last_of(tk, n);
+                if (!done) break;
+                add(first, by, n);
+            }
+            if (level > 0 || groups == 1) break;
+            if (n > 1) store(first);               // its pieces have been added: the group's slot is the first one's
+            tk = tickets + (g0 * kWaves + w);
+            first = 0;
+            by = kGroup;
+            n = groups;
+        }
+    }
+    if (done) {
+        const int t0 = wr0 / G;
+        int t, h;
+        small_divide(wr0 - t0 * G + (ln & 31), t, h);
+        // lanes l and l + 32 have 4 dims each of 8: they trade halves of pairs
+        // of such groups, so that each stores 16 bytes
+        char* const op = a.out + (int64_t)(c.q0 + t0 + t) * a.o_nb_t + (int64_t)(c.kvh * G + h) * a.o_nb_h + 16 * (ln >> 5);
         const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+        for (int i = 0; i < DT * 2; ++i) {
+            uint32_t y[2][2];
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                uint2 y = {pack2<KT>(o[dt][4 * q4] * inv, o[dt][4 * q4 + 1] * inv),
-                           pack2<KT>(o[dt][4 * q4 + 2] * inv, o[dt][4 * q4 + 3] * inv)};
-                if (any_bad) y.x = y.y = 0x7fff7fffu;
-                *(uint2*)(orow + (dt * 32 + 8 * q4 + 4 * half) * 2) = y;
+            for (int x = 0; x < 4; ++x) {
+                const int q4 = 2 * (i % 2) + x / 2, r = 4 * q4 + 2 * (x % 2);
+                y[x / 2][x % 2] = pack2<KT>(o[i / 2][r] * inv, o[i / 2][r + 1] * inv);
             }
-        return;
+            const auto s0 = __builtin_amdgcn_permlane32_swap(y[0][0], y[1][0], false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(y[0][1], y[1][1], false, false);
+            u32x4 z = {s0[0], s1[0], s0[1], s1[1]};
+            if (nan) z = u32x4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+            if (wr0 + (ln & 31) < c.rows) *(u32x4*)(op + i * 32) = z;
+        }
     }
-    float* const pr = ws + ((int64_t)(it.first + it.ks) * a.Hkv + kvh) * kRowsWG * (D + 2);
-    const int r = w * kRowsWave + l32;
-    if (half == 0) *(uint2*)(pr + kRowsWG * D + 2 * r) = make_uint2(any_bad ? kNanBits : __float_as_uint(m), __float_as_uint(lt));
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4)
-            *(float4*)(pr + r * D + dt * 32 + 8 * q4 + 4 * half) =
-                make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
-}
-
-// The pieces' sums of a row tile's rows: D / 4 threads a row.
-template <int D, int KT>
-__global__ void __launch_bounds__(256) paged_many_merge_kernel(PagedArgs a, const float* __restrict__ ws, int n_cu, int max_wgs) {
-    prefetch_kernargs<sizeof(PagedArgs)>();
-    constexpr int C = D / 4, R = 256 / C;          // rows of a workgroup
-    const int kvh = blockIdx.x % a.Hkv;
-    const ManyItem it = many_item<true>(a, blockIdx.x / a.Hkv, n_cu, max_wgs);
-    if (it.n_ks <= 1) return;
-    const int r = blockIdx.y * R + threadIdx.x / C, c = threadIdx.x % C;
-    const int row = it.rt * kRowsWG + r;
-    if (row >= min(it.q.n, a.max_new) * a.G) return;
-    constexpr int64_t PS = kRowsWG * (D + 2);
-    const float* pr = ws + ((int64_t)it.first * a.Hkv + kvh) * PS;
-    float2 e[kMaxKs];
-#pragma unroll
-    for (int k = 0; k < kMaxKs; ++k) e[k] = *(const float2*)(pr + (int64_t)min(k, it.n_ks - 1) * a.Hkv * PS + kRowsWG * D + 2 * r);
-    float M = -INFINITY;
-    bool bad = false;
-#pragma unroll
-    for (int k = 0; k < kMaxKs; ++k) {
-        const bool b = __float_as_uint(e[k].x) == kNanBits;
-        bad = bad || b;
-        M = fmaxf(M, b ? -INFINITY : e[k].x);
     }
-    const float base = M == -INFINITY ? 0.0f : M;
-    float den = 0.0f;
-    float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = 0; k < it.n_ks; ++k) {
-        const float2 ek = *(const float2*)(pr + (int64_t)k * a.Hkv * PS + kRowsWG * D + 2 * r);
-        const float f = __builtin_amdgcn_exp2f(ek.x - base);
-        const float4 v = *(const float4*)(pr + (int64_t)k * a.Hkv * PS + r * D + 4 * c);
-        den = fmaf(f, ek.y, den);
-        num.x = fmaf(f, v.x, num.x); num.y = fmaf(f, v.y, num.y);
-        num.z = fmaf(f, v.z, num.z); num.w = fmaf(f, v.w, num.w);
-    }
-    const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-    uint2 y = {pack2<KT>(num.x * inv, num.y * inv), pack2<KT>(num.z * inv, num.w * inv)};
-    if (bad) y.x = y.y = 0x7fff7fffu;
-    *(uint2*)(a.out + (int64_t)(it.q.q0 + row / a.G) * a.o_nb_t + (int64_t)(kvh * a.G + row % a.G) * a.o_nb_h + 8 * c) = y;
 }
 
 template <int D, int KT>
 hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s) {
     hipError_t e = hipSuccess;
-    if (p.many_tiles > 0) {
-        hipLaunchKernelGGL((paged_many_kernel<D, KT>), dim3(p.many_pieces * a.Hkv), dim3(kWaves * 64), 0, s, a, ws, p.n_cu, p.max_wgs);
+    if (p.many_wgs > 0) {
+        hipLaunchKernelGGL((paged_many_kernel<D, KT>), dim3(p.many_wgs), dim3(kWaves * 64), 0, s, a, ws, tickets);
         if ((e = hipGetLastError()) != hipSuccess) return e;
-        if (p.many_split) {
-            hipLaunchKernelGGL((paged_many_merge_kernel<D, KT>), dim3(p.many_tiles * a.Hkv, kRowsWG * D / 4 / 256), dim3(256), 0, s, a, ws, p.n_cu, p.max_wgs);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
-        }
     }
     if (p.few_pieces > 0) {
         hipLaunchKernelGGL((paged_few_kernel<D, KT>), dim3(p.few_pieces * a.Hkv), dim3(kFewWaves * 64), 0, s, a, ws, tickets, p.few_slots, p.few_cap);
@@ -957,6 +1107,8 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, float* ws, unsig
     return e;
 }
 
+static_assert(kManyTickets <= kMaxPagedTickets, "the context holds the tickets");
+
 }  // namespace
 
 // What a call of these shapes may need: the lengths are on the device, so
@@ -964,21 +1116,11 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, float* ws, unsig
 // there is end at once.
 PagedPlan paged_plan(const PagedArgs& a, int n_cu) {
     PagedPlan p{};
-    p.n_cu = n_cu;
-    const int64_t rows = (int64_t)a.max_new * a.G, all = (int64_t)a.n_tok * a.G;
+    const int64_t rows = (int64_t)a.max_new * a.G;
     const int64_t max_keys = (int64_t)a.max_pages << a.page_shift;
     // every sequence brings max_new tokens where their number says so
     const bool even = (int64_t)a.n_seq * a.max_new == a.n_tok;
-    if (rows > kFewRows) {
-        const int64_t seqs = std::min<int64_t>(a.n_seq, all / (kFewRows + 1));
-        const int64_t tiles = even ? (int64_t)a.n_seq * ((rows + kRowsWG - 1) / kRowsWG) : all / kRowsWG + seqs;
-        const int64_t key_tiles = (max_keys + kBN - 1) / kBN;
-        p.many_tiles = (int)tiles;
-        // at most four workgroups per CU in all where row tiles are split
-        p.many_split = key_tiles >= 2 * kMinPiece && (!even || 2 * tiles * a.Hkv <= 4 * n_cu);
-        p.max_wgs = p.many_split ? 4 * n_cu : 0;
-        p.many_pieces = (int)std::max<int64_t>(tiles, p.max_wgs / a.Hkv);
-    }
+    if (rows > kFewRows) p.many_wgs = std::min(n_cu, kMaxWgs);
     if (rows <= kFewRows || !even) {
         p.few_cap = (int)std::min<int64_t>(rows, kFewRows);
         // Half the workgroups that fit a CU, so that fewer partials are added and
@@ -994,7 +1136,7 @@ PagedPlan paged_plan(const PagedArgs& a, int n_cu) {
     return p;
 }
 size_t paged_ws_bytes(const PagedArgs& a, const PagedPlan& p) {
-    const size_t many = p.many_split ? (size_t)p.many_pieces * a.Hkv * kRowsWG * (a.d + 2) * sizeof(float) : 0;
+    const size_t many = (size_t)p.many_wgs * 2 * kWaves * (a.d * kRowsWave * sizeof(float) + 64 * 8);
     const size_t few = p.few_split ? (size_t)p.few_pieces * a.Hkv * p.few_cap * (a.d + 2) * sizeof(float) : 0;
     return std::max(many, few);                    // one after the other on the stream
 }

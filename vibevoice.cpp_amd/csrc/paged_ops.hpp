@@ -27,15 +27,17 @@ __device__ __forceinline__ int seq_of_token(const PagedArgs& a, int n) {
 }
 
 __device__ __forceinline__ int lane_of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
-// Sum of x over the lanes up to and with this one
+// Sum of x over the lanes up to and with this one (DPP: shifts within rows of
+// 16 lanes, then the rows' totals broadcast upwards)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int x) { return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
 __device__ __forceinline__ int wave_scan(int x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const int y = __shfl_up(x, m, 64);
-        x += lane >= m ? y : 0;
-    }
-    return x;
+    x = dpp_add<0x111, 0xf>(x);
+    x = dpp_add<0x112, 0xf>(x);
+    x = dpp_add<0x114, 0xf>(x);
+    x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);                    // row 0's total to row 1, row 2's to row 3
+    return dpp_add<0x143, 0xc>(x);                 // the lower half's to the upper
 }
 // Sum of x over the wave (DPP within rows of 16 lanes, permlane swaps across)
 __device__ __forceinline__ int wave_total(int x) {

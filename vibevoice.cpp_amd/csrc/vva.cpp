@@ -1510,9 +1510,11 @@ vva_status fill_paged(vva_context* ctx, const char* what, const vva_tensor* kp, 
     if (Hq % Hkv) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: Hq %% Hkv != 0", what);
     // lane offsets inside a page are 32-bit; pages and heads are 64-bit
     if ((uint64_t)kp->nb[1] * ps >= ((uint64_t)1 << 31) || (uint64_t)vp->nb[1] * ps >= ((uint64_t)1 << 31) ||
-        n_pages > 0x7fffffff || Hq > 65535)
+        n_pages > 0x7fffffff)
         return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: pages too large", what);
-    if (N > (1 << 24)) return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: %lld tokens, at most 2^24", what, (long long)N);
+    if (Hq / Hkv > 256 || Hkv > 65535 || N > (1 << 22))
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: %lld tokens, %lld / %lld heads: at most 2^22 tokens and 256 query heads per kv head",
+                    what, (long long)N, (long long)Hq, (long long)Hkv);
     if (!b) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: batch is null", what);
     const int64_t n_seq = b->kv_len.ne[0];
     if (n_seq < 1 || n_seq > VVA_MAX_BATCH_SEQ)
@@ -1592,8 +1594,9 @@ extern "C" vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, cons
     if ((st = fill_paged(ctx, "paged_attn", k_pages, v_pages, batch, Hq, N, a)) != VVA_OK) return st;
     if ((st = check_packed(ctx, q, "q", a.d, Hq, N)) != VVA_OK) return st;
     if ((st = check_packed(ctx, out, "out", a.d, Hq, N)) != VVA_OK) return st;
-    if ((Hq > 1 && q->nb[1] >= ((size_t)1 << 25)) || (N > 1 && q->nb[2] >= ((size_t)1 << 25)))
-        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "paged_attn: rows of q 32 MiB apart");   // 32 rows in 32-bit offsets
+    // 32 tokens' rows of up to 256 heads in 32-bit offsets
+    if ((Hq > 1 && q->nb[1] >= ((size_t)1 << 22)) || (N > 1 && q->nb[2] >= ((size_t)1 << 22)))
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "paged_attn: rows of q 4 MiB apart");
     if (q->type != a.type || out->type != a.type)
         return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: q and out must have the pages' type (%d)", a.type);
     if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: scale must be finite and > 0");

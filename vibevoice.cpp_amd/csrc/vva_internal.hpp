@@ -234,15 +234,14 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s);
 // Launches of a paged_attn call of these shapes, whatever its lengths are
 // (upper bounds; paged_attn.hip)
 struct PagedPlan {
-    int n_cu, max_wgs;
-    int many_tiles, many_pieces;   // row tiles, pieces of their keys (per kv head; 0: no launch)
-    int few_pieces, few_slots, few_cap;
-    bool many_split, few_split;    // whether a second launch may have partials to add
+    int many_wgs;                              // workgroups of paged_many_kernel (0: no launch)
+    int few_pieces, few_slots, few_cap;        // pieces per kv head (0: no launch), how many run at once, rows of a partial
+    bool few_split;                            // whether pieces may leave partials
 };
 PagedPlan paged_plan(const PagedArgs& a, int n_cu);
 size_t paged_ws_bytes(const PagedArgs& a, const PagedPlan& p);
-// tickets: [n_seq * Hkv], zero between calls
-constexpr int kMaxPagedTickets = 65536;
+// tickets: [kMaxPagedTickets], zero between launches; n_seq * Hkv of them at most are used for sequences
+constexpr int kMaxPagedTickets = 67584;
 hipError_t launch_paged_attn(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s);
 hipError_t launch_norm(const NormArgs& a, hipStream_t s);
 
