@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
         for (int i = 0; i < NC / kFewWaves; ++i) {
             const int c = w * (NC / kFewWaves) + i;
             const int r = c * RC + lane / (D / 8), row = r < rows ? r : 0;
-            const int off = (row / a.G) * (int)a.q_nb_t + (row % a.G) * (int)a.q_nb_h;
+            const int rt = div_g(a, row), off = rt * (int)a.q_nb_t + (row - rt * a.G) * (int)a.q_nb_h;
             dma16<false>(qb, off + (((lane % (D / 8)) ^ k_swz<D>(r)) << 4), qs + c * 1024);
         }
     }
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
     QF qf[DS];
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) qf[ds] = as_vec<QF>(lds_read((qs + k_off) ^ (ds << 5)));
-    const int lim = l32 < rows ? min(L - 1, past + l32 / a.G) : -1;   // the last key the lane's row sees
+    const int lim = l32 < rows ? min(L - 1, past + div_g(a, l32)) : -1;   // the last key the lane's row sees
     const float sl2 = a.scale * kLog2e;
     float m = -INFINITY, lsum = 0.0f;
     f32x16 o[DT];
@@ -464,7 +464,8 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
         const float inv = den > 0.0f ? 1.0f / den : 0.0f;
         uint2 y = {pack2<KT>(num.x * inv, num.y * inv), pack2<KT>(num.z * inv, num.w * inv)};
         if (any_bad) y.x = y.y = 0x7fff7fffu;
-        *(uint2*)(a.out + (int64_t)(it.q.q0 + row / a.G) * a.o_nb_t + (int64_t)(kvh * a.G + row % a.G) * a.o_nb_h + 8 * c) = y;
+        const int rt = div_g(a, row);
+        *(uint2*)(a.out + (int64_t)(it.q.q0 + rt) * a.o_nb_t + (int64_t)(kvh * a.G + row - rt * a.G) * a.o_nb_h + 8 * c) = y;
     }
     if (it.parts == 1) return;
     // ---- the last of the sequence's pieces adds their partials, in order:
@@ -528,7 +529,8 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
         const float inv = den > 0.0f ? 1.0f / den : 0.0f;
         uint2 y = {pack2<KT>(num.x * inv, num.y * inv), pack2<KT>(num.z * inv, num.w * inv)};
         if (nan) y.x = y.y = 0x7fff7fffu;
-        *(uint2*)(a.out + (int64_t)(it.q.q0 + row / a.G) * a.o_nb_t + (int64_t)(kvh * a.G + row % a.G) * a.o_nb_h + 8 * c) = y;
+        const int rt = div_g(a, row);
+        *(uint2*)(a.out + (int64_t)(it.q.q0 + rt) * a.o_nb_t + (int64_t)(kvh * a.G + row - rt * a.G) * a.o_nb_h + 8 * c) = y;
     }
 }
 
@@ -553,7 +555,7 @@ __device__ __forceinline__ int many_row_tiles(const PagedArgs& a, const Seq& q) 
 __device__ __forceinline__ int many_key_tiles(const PagedArgs& a, const Seq& q, int rt) {
     const int n = min(q.n, a.max_new);
     const int t_hi = min(n * a.G, (rt + 1) * kRowsWG) - 1;
-    return (max(0, min(q.L, q.L - q.n + t_hi / a.G + 1)) + kBN - 1) / kBN;
+    return (max(0, min(q.L, q.L - q.n + div_g(a, t_hi) + 1)) + kBN - 1) / kBN;
 }
 
 // The call's work on one axis: kv heads, in them the sequences, in them the
@@ -574,6 +576,13 @@ __device__ __forceinline__ ManyWeight many_weight(const PagedArgs& a, const Seq&
     w.slope = slope >> shift;
     return w;
 }
+// p / n for a uniform p >= 0 whose quotient a float holds
+__device__ __forceinline__ int part_of(int p, int n) {
+    int k = uni((int)((float)p * __builtin_amdgcn_rcpf((float)n))), r = p - k * n;   // within one or two of it
+    while (r < 0) --k, r += n;
+    while (r >= n) ++k, r -= n;
+    return k;
+}
 struct ManyAxis {
     int slope;              // of a row tile, in sixteenths
     int shift;              // the unit's power of two above a sixteenth
@@ -583,7 +592,7 @@ struct ManyAxis {
 __device__ __forceinline__ ManyAxis many_axis(const PagedArgs& a, const Seq& mine) {
     const int lane = threadIdx.x & 63;
     ManyAxis x;
-    x.slope = uni(kRowsWG * 16 / kBN / a.G);
+    x.slope = div_g(a, kRowsWG * 16 / kBN);
     float all = 0.0f;
     for (int s = lane; s < a.n_seq; s += 64) {
         const ManyWeight w = many_weight(a, s == lane ? mine : seq_of(a, s), x.slope, 0);
@@ -632,6 +641,15 @@ __device__ __forceinline__ ManySeq many_seq(const PagedArgs& a, const ManyAxis& 
     return r;
 }
 
+// The kernel's arguments, read again from their segment: each phase loads the
+// few that it needs (they hit the scalar cache), so that not all of them are
+// held, and spilled, through the key tiles.
+__device__ __forceinline__ const PagedArgs& fresh_args() {
+    uint64_t p = (uint64_t)(uintptr_t)(const char*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const PagedArgs*)(const __attribute__((address_space(4))) PagedArgs*)(uintptr_t)p;
+}
+
 // One workgroup per share of the work: 8 waves x 32 rows that share every K / V
 // tile.  A row tile that lies in one share is written at once; of one that
 // several workgroups share, each leaves its rows' sums in the workspace, wave
@@ -661,7 +679,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     ManySeq sq{};                                  // the sequence at hand, and its end on the axis
     int sq_kvh = 0, sq_end = -1;
     int head, axis_shift, axis_slope;
-    int g, wgs, share, more;
+    int g, wgs, share, total;
     {
     const Seq mine = seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1));
     const ManyAxis axis = many_axis(a, mine);
@@ -669,26 +687,22 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     axis_shift = axis.shift;
     axis_slope = axis.slope;
     if (head <= 0) return;
-    const int total = head * a.Hkv;
-    wgs = uni(min((int)gridDim.x, max(1, total / max((16 * kMinShare) >> axis_shift, 1))));
+    total = head * a.Hkv;
+    const float unit = (float)max((16 * kMinShare) >> axis.shift, 1);
+    wgs = uni(max(1, min((int)gridDim.x, (int)((float)total * __builtin_amdgcn_rcpf(unit)))));
     if ((int)blockIdx.x >= wgs) return;
     // neighbouring shares on one XCD (workgroups go round its 8): they read the same keys
     g = wgs % 8 == 0 ? (int)(blockIdx.x % 8) * (wgs / 8) + (int)(blockIdx.x / 8) : (int)blockIdx.x;
-    share = uni(total / wgs);
-    more = uni(total - share * wgs);
-    const int p = g * share + min(g, more);
-    sq_kvh = uni(p / head);
+    share = uni((int)((float)total * 1.000001f * __builtin_amdgcn_rcpf((float)wgs)) + 1);      // share * wgs >= total
+    const int p = min(g * share, total - 1);
+    sq_kvh = part_of(p, head);
     sq = many_seq(a, axis, mine, p - sq_kvh * head);
     sq_end = sq_kvh * head + sq.end;
     }
     // the workgroup whose share holds place p
-    auto owner = [&](int p) {
-        const int cut = more * (share + 1);
-        return uni(min(wgs - 1, p < cut ? p / (share + 1) : more + (p - cut) / max(share, 1)));
-    };
-    const int p_end = (g + 1) * share + min(g + 1, more);
-    const int G = a.G;
-    const float inv_g = uni(1.0f / (float)G);
+    auto owner = [&](int p) { return min(wgs - 1, part_of(p, share)); };
+    const int p_end = min(total, (g + 1) * share);
+    const float inv_g = uni(1.0f / (float)a.G);
 
     // ---- the row tile at place p of the axis, and this workgroup's keys of it
     struct Cut {
@@ -699,9 +713,11 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         int next;                                  // the place after this part
     };
     auto find = [&](int p) {
+        const PagedArgs& a = fresh_args();
+        const int G = a.G;
         Cut c;
         if (p >= sq_end) {
-            sq_kvh = uni(p / head);
+            sq_kvh = part_of(p, head);
             sq = many_seq(a, ManyAxis{axis_slope, axis_shift, head}, seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1)), p - sq_kvh * head);
             sq_end = sq.end > sq.start ? sq_kvh * head + sq.end : p_end;   // no sequence: a batch that changed meanwhile
         }
@@ -709,7 +725,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         wt.r = uni(wt.r);
         const int ps = p - sq_kvh * head - sq.start;           // place in the sequence
         const float s2 = 0.5f * (float)wt.slope, f1 = (float)wt.first + s2;
-        int rt = (int)(wt.slope > 0 ? (sqrtf(f1 * f1 + 4.0f * s2 * (float)ps) - f1) * __builtin_amdgcn_rcpf(2.0f * s2)
+        int rt = (int)(wt.slope > 0 ? (__builtin_amdgcn_sqrtf(f1 * f1 + 4.0f * s2 * (float)ps) - f1) * __builtin_amdgcn_rcpf(2.0f * s2)
                                     : (float)ps * __builtin_amdgcn_rcpf((float)wt.first));
         rt = uni(max(0, min(rt, wt.r - 1)));
         while (rt > 0 && wt.before(rt) > ps) --rt;
@@ -745,26 +761,37 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     const float sl2 = uni(a.scale * kLog2e);
     bool bad = false;
     int ids[NI];
-    auto fetch = [&](const Cut& c, int j, int (&id)[NI]) {
-        const ConstInts table = (ConstInts)(uintptr_t)(a.table + (int64_t)c.s * a.table_stride);
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-            id[i] = table[min((c.kb0 + j * kBN + i * kWaves * RC + r0w) >> a.page_shift, max(0, (c.L - 1) >> a.page_shift))];
+    // where a part's K and V come from
+    struct Source {
+        uint64_t k, v;                             // the pools' kv head
+        int64_t k_page, v_page;
+        int k_slot, v_slot, n_pages, shift, last;  // last: the sequence's last page
+        ConstInts table;
     };
-    // the loads of tile j (K, then V); past the last tile further ones of the
-    // sequence, to a stage that nobody reads any more, so that every tile
-    // counts the same
-    auto issue = [&](const Cut& c, int j, const int (&id)[NI]) {
+    auto source = [&](const Cut& c) {
+        const PagedArgs& a = fresh_args();
+        return Source{uniform64((uint64_t)(uintptr_t)a.k + c.kvh * a.k_nb_head), uniform64((uint64_t)(uintptr_t)a.v + c.kvh * a.v_nb_head),
+                      a.k_nb_page, a.v_nb_page, (int)a.k_nb_slot, (int)a.v_nb_slot, a.n_pages, a.page_shift,
+                      max(0, (c.L - 1) >> a.page_shift), (ConstInts)(uintptr_t)(a.table + (int64_t)c.s * a.table_stride)};
+    };
+    auto fetch = [&](const Source& t, int key, int (&id)[NI]) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) id[i] = t.table[min((key + i * kWaves * RC + r0w) >> t.shift, t.last)];
+    };
+    // the loads of tile j, from key `key` on (K, then V); past the last tile
+    // further ones of the sequence, to a stage that nobody reads any more, so
+    // that every tile counts the same
+    auto issue = [&](const Source& t, int j, int key, const int (&id)[NI]) {
         const uint32_t st = lds0 + (j % kStages) * STAGE + w * 1024;
         uint64_t kb[NI], vb[NI];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const bool ok = (uint32_t)id[i] < (uint32_t)a.n_pages;
+            const bool ok = (uint32_t)id[i] < (uint32_t)t.n_pages;
             bad = bad || !ok;
             const int64_t page = ok ? id[i] : 0;
-            const int64_t slot = (c.kb0 + j * kBN + i * kWaves * RC + r0w) & ((1 << a.page_shift) - 1);
-            kb[i] = uniform64((uint64_t)(uintptr_t)a.k + page * a.k_nb_page + c.kvh * a.k_nb_head + slot * a.k_nb_slot);
-            vb[i] = uniform64((uint64_t)(uintptr_t)a.v + page * a.v_nb_page + c.kvh * a.v_nb_head + slot * a.v_nb_slot);
+            const int slot = (key + i * kWaves * RC + r0w) & ((1 << t.shift) - 1);
+            kb[i] = uniform64(t.k + page * t.k_page + slot * t.k_slot);
+            vb[i] = uniform64(t.v + page * t.v_page + slot * t.v_slot);
         }
 #pragma unroll
         for (int i = 0; i < NI; ++i) dma16<false>(kb[i], koff, st + i * kWaves * 1024);
@@ -772,39 +799,42 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         for (int i = 0; i < NI; ++i) dma16<false>(vb[i], voff, st + TB + i * kWaves * 1024);
     };
     // x = t * G + h for small x (below G + 32): one product
-    auto small_divide = [&](int x, int& t, int& h) {
+    auto small_divide = [&](int x, int G, int& t, int& h) {
         t = (int)(((float)x + 0.5f) * inv_g);
         h = x - t * G;
     };
     // a part's first loads: the wave's rows of Q (laid out as K is, in the
     // stages of tiles 2 and 3; rows past the last: one that is there), two tiles
-    auto start = [&](const Cut& c) {
+    auto start = [&](const Cut& c, const Source& src) {
+        const PagedArgs& a = fresh_args();
+        const int G = a.G;
         bad = false;
         const int ln = lane_id();                  // offsets made here, not held from one part to the next
         int id0[NI], id1[NI];
-        fetch(c, 0, id0);
-        fetch(c, 1, id1);
-        fetch(c, 2, ids);
+        fetch(src, c.kb0, id0);
+        fetch(src, c.kb0 + kBN, id1);
+        fetch(src, c.kb0 + 2 * kBN, ids);
         const int wr0 = min(c.rt * kRowsWG + w * kRowsWave, c.rows - 1), live = min(kRowsWave, c.rows - wr0);
-        const int t0 = wr0 / G, h0 = wr0 - t0 * G;
+        const int t0 = div_g(a, wr0), h0 = wr0 - t0 * G;
         const uint64_t qb = uniform64((uint64_t)(uintptr_t)a.q + (int64_t)(c.q0 + t0) * a.q_nb_t + (int64_t)c.kvh * G * a.q_nb_h);
 #pragma unroll
         for (int i = 0; i < kRowsWave / RC; ++i) {
             const int r = i * RC + ln / (D / 8);
             int t, h;
-            small_divide(h0 + (r < live ? r : 0), t, h);
+            small_divide(h0 + (r < live ? r : 0), G, t, h);
             dma16<false>(qb, t * (int)a.q_nb_t + h * (int)a.q_nb_h + (((ln % (D / 8)) ^ k_swz<D>(r)) << 4),
                          lds0 + 2 * STAGE + w * kRowsWave * ROW + i * 1024);
         }
-        issue(c, 0, id0);
-        issue(c, 1, id1);
+        issue(src, 0, c.kb0, id0);
+        issue(src, 1, c.kb0 + kBN, id1);
     };
 
     int fix_id = 0;
-    for (int p = g * share + min(g, more), seg = 0, p_next; p < p_end; p = p_next, ++seg) {
+    for (int p = g * share, seg = 0, p_next; p < p_end; p = p_next, ++seg) {
     const Cut c = find(p);
     p_next = c.next;
-    if (c.n_tiles > 0) start(c);
+    const Source src = source(c);
+    if (c.n_tiles > 0) start(c, src);
     const int L = c.L, past = c.past, kb0 = c.kb0, n_tiles = c.n_tiles, rows = c.rows;
     const int wr0 = c.rt * kRowsWG + w * kRowsWave;
     const bool wave_live = wr0 < rows;
@@ -813,13 +843,15 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
     if (n_tiles > 0) {                                        // uniform
+        const PagedArgs& a = fresh_args();
+        const int G = a.G;
         // keys [0, kend_w) are seen by some row of the wave, keys up to lim_w by every row
-        const int kend_w = uni(wave_live ? max(0, min(L, past + (min(wr0 + kRowsWave, rows) - 1) / G + 1)) : 0);
-        const int lim_w = uni(min(L - 1, past + min(wr0, rows - 1) / G));
+        const int kend_w = uni(wave_live ? max(0, min(L, past + div_g(a, min(wr0 + kRowsWave, rows) - 1) + 1)) : 0);
+        const int lim_w = uni(min(L - 1, past + div_g(a, min(wr0, rows - 1))));
         int lim, hcol;                                        // the last key the lane's row sees
-        const int wr = min(wr0, rows - 1), t0 = wr / G;
+        const int wr = min(wr0, rows - 1), t0 = div_g(a, wr);
         const int l32 = lane_id() & 31;
-        small_divide(wr - t0 * G + (wr0 + l32 < rows ? l32 : 0), lim, hcol);
+        small_divide(wr - t0 * G + (wr0 + l32 < rows ? l32 : 0), G, lim, hcol);
         lim = min(L - 1, past + t0 + lim);
         wait_vm<2 * NLD>();                                   // Q has landed
         QF qf[DS];
@@ -830,8 +862,8 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         }
         // K of tile 0 has landed (its V and tile 1 may still fly), and every wave has its Q
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(NI + NLD) : "memory");
-        issue(c, 2, ids);
-        fetch(c, 3, ids);
+        issue(src, 2, kb0 + 2 * kBN, ids);
+        fetch(src, kb0 + 3 * kBN, ids);
         auto stage = [&](int j) { return lds0 + (j % kStages) * STAGE; };
         auto read_k = [&](uint32_t ka, int ds, int kt) { return lds_read((ka ^ (ds << 5)) + kt * 32 * ROW); };
         auto apply_mask = [&](f32x16 (&s)[2], int k0) {
@@ -921,7 +953,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         // looks at its share of V, and where a value is not finite every row adds
         // the ones that it sees and the tile goes on with zeros in their places
         // (the order of the barriers is the workgroup's; seen by no other tile).
-        const int lim_wg = uni(min(L - 1, past + min(c.rt * kRowsWG, rows - 1) / G));
+        const int lim_wg = uni(min(L - 1, past + div_g(a, min(c.rt * kRowsWG, rows - 1))));
         auto fix_tile = [&](int j) {
             const int lane = lane_id();
             const uint32_t vs = stage(j) + TB;
@@ -959,8 +991,8 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
             // K of tile j + 1 and V of tile j have landed, and every wave is done
             // with tile j - 1, whose stage tile j + 3 now takes
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(NI + NLD) : "memory");
-            issue(c, j + 3, ids);
-            fetch(c, j + 4, ids);
+            issue(src, j + 3, kb0 + (j + 3) * kBN, ids);
+            fetch(src, kb0 + (j + 4) * kBN, ids);
             if (j < n_live) rescale(mx);                      // wave-uniform
             if (kb0 + j * kBN + kBN - 1 > lim_wg) fix_tile(j);
             if (j < n_live) {
@@ -984,6 +1016,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     // ---- this workgroup's sums of the wave's rows (lanes l and l ^ 32 summed
     // different keys); with the other pieces' where the row tile has several
     const int ln = lane_id();
+    const PagedArgs& args = fresh_args();
     float lt = add_swap32(lsum);
     bool nan = c.n_tiles > 0 && *(volatile __attribute__((address_space(3))) int*)&bad_seg == seg;
     bool done = true;
@@ -1068,12 +1101,12 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         }
     }
     if (done) {
-        const int t0 = wr0 / G;
+        const int G = args.G, t0 = div_g(args, wr0);
         int t, h;
-        small_divide(wr0 - t0 * G + (ln & 31), t, h);
+        small_divide(wr0 - t0 * G + (ln & 31), G, t, h);
         // lanes l and l + 32 have 4 dims each of 8: they trade halves of pairs
         // of such groups, so that each stores 16 bytes
-        char* const op = a.out + (int64_t)(c.q0 + t0 + t) * a.o_nb_t + (int64_t)(c.kvh * G + h) * a.o_nb_h + 16 * (ln >> 5);
+        char* const op = args.out + (int64_t)(c.q0 + t0 + t) * args.o_nb_t + (int64_t)(c.kvh * G + h) * args.o_nb_h + 16 * (ln >> 5);
         const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
 #pragma unroll
         for (int i = 0; i < DT * 2; ++i) {

@@ -50,3 +50,7 @@ __device__ __forceinline__ int wave_total(int x) {
     const auto b = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
     return __builtin_amdgcn_readfirstlane((int)(b[0] + b[1]));
 }
+// x / G for 0 <= x < 2^31, by the call's multiplier
+__device__ __forceinline__ int div_g(const PagedArgs& a, int x) {
+    return a.g_mul ? (int)(__umulhi((uint32_t)x, a.g_mul) >> a.g_shift) : x;
+}

@@ -1539,6 +1539,11 @@ vva_status fill_paged(vva_context* ctx, const char* what, const vva_tensor* kp, 
     p.max_new = (int)std::min<int64_t>(b->max_new, N);
     p.page_shift = __builtin_ctz((unsigned)ps);
     p.d = (int)d; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv);
+    // 2^(31 + l) / G rounded up, 2^(l - 1) < G <= 2^l: exact quotients below 2^31
+    int l = 0;
+    while ((1 << l) < p.G) ++l;
+    p.g_mul = l > 0 ? (uint32_t)(((uint64_t)1 << (31 + l)) / p.G + 1) : 0;
+    p.g_shift = l - 1;
     p.k = (char*)kp->data; p.v = (char*)vp->data; p.type = kp->type;
     p.k_nb_slot = kp->nb[1]; p.k_nb_head = kp->nb[2]; p.k_nb_page = kp->nb[3];
     p.v_nb_slot = vp->nb[1]; p.v_nb_head = vp->nb[2]; p.v_nb_page = vp->nb[3];

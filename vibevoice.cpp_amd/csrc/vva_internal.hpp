@@ -202,6 +202,7 @@ struct PagedArgs {
     int n_seq, n_tok, n_pages, max_pages, max_new;
     int page_shift;                                // page size = 1 << page_shift
     int d, Hq, Hkv, G;                             // G = Hq / Hkv
+    uint32_t g_mul; int g_shift;                   // x / G = high word of x * g_mul >> g_shift; g_mul = 0: G = 1
     char* k; char* v; int type;
     int64_t k_nb_slot, k_nb_head, k_nb_page, v_nb_slot, v_nb_head, v_nb_page;
     const char* q; int64_t q_nb_h, q_nb_t;
