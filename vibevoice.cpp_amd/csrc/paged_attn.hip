@@ -201,6 +201,15 @@ __device__ __forceinline__ void add_not_finite(uint32_t v_lds, int k0, int lim, 
     }
 }
 
+// The kernel's arguments, read again from their segment: each phase loads the
+// few that it needs (they hit the scalar cache), so that not all of them are
+// held, and spilled, through the key tiles.
+__device__ __forceinline__ const PagedArgs& fresh_args() {
+    uint64_t p = (uint64_t)(uintptr_t)(const char*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const PagedArgs*)(const __attribute__((address_space(4))) PagedArgs*)(uintptr_t)p;
+}
+
 // ------------------------------------------------------------ few rows
 
 // Workgroups per kv head that paged_few_kernel's work is cut into, and the
@@ -262,6 +271,7 @@ __device__ __forceinline__ FewItem few_item(const PagedArgs& a, int item, int sl
 }
 
 constexpr int kSc1 = 16;           // cache policy of the partials: agent scope
+constexpr int kFewTickets = kMaxPagedSeqHeads; // a ticket per sequence and kv head; then one per piece and kv head
 // pieces whose partials are loaded together (16: 8 x 1024 keys 9.4 -> 10.0 us, two
 // streams of 1k keys 6.8 -> 7.3, 1 x 32768 keys 23.2 -> 22.2)
 constexpr int kMergeBatch = 8;
@@ -423,114 +433,137 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
     __syncthreads();
     float* const ow = (float*)lds;
     float* const ml = ow + kFewWaves * kFewRows * OP;
+    if (l32 < rows) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4)
-            *(float4*)(ow + (w * kFewRows + l32) * OP + dt * 32 + 8 * q4 + 4 * half) =
-                make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
-    if (half == 0) *(float2*)(ml + (w * kFewRows + l32) * 2) = make_float2(m, lt);
-    const bool any_bad = __syncthreads_or(bad);
+            for (int q4 = 0; q4 < 4; ++q4)
+                *(float4*)(ow + (w * kFewRows + l32) * OP + dt * 32 + 8 * q4 + 4 * half) =
+                    make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
+        if (half == 0) *(float2*)(ml + (w * kFewRows + l32) * 2) = make_float2(m, lt);
+    }
+    bool nan = __syncthreads_or(bad);
+    const PagedArgs& args = fresh_args();
+    // thread i's part of the sums: 4 dims of a row
+    struct Sum {
+        float4 num;
+        float M, den;
+    };
+    auto write = [&](int row, int c, const Sum& x) {
+        const float inv = x.den > 0.0f ? 1.0f / x.den : 0.0f;
+        uint2 y = {pack2<KT>(x.num.x * inv, x.num.y * inv), pack2<KT>(x.num.z * inv, x.num.w * inv)};
+        if (nan) y.x = y.y = 0x7fff7fffu;
+        const int rt = div_g(args, row);
+        *(uint2*)(args.out + (int64_t)(it.q.q0 + rt) * args.o_nb_t + (int64_t)(kvh * args.G + row - rt * args.G) * args.o_nb_h + 8 * c) = y;
+    };
     auto piece_rsrc = [&](int part) {
         const uint32_t bytes = cap * (D + 2) * sizeof(float);
-        return make_rsrc((const char*)ws + ((int64_t)(it.first + part) * a.Hkv + kvh) * bytes, bytes);
+        return make_rsrc((const char*)ws + ((int64_t)(it.first + part) * args.Hkv + kvh) * bytes, bytes);
+    };
+    // agent-scope stores: coherent across the XCDs' L2 caches
+    auto store = [&](int part, int row, int c, const Sum& x) {
+        const BufRsrc rs = piece_rsrc(part);
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(x.num.x), __float_as_uint(x.num.y), __float_as_uint(x.num.z), __float_as_uint(x.num.w)},
+                                               rs, (row * D + 4 * c) * 4, 0, kSc1);
+        if (c == 0)
+            __builtin_amdgcn_raw_buffer_store_b64(u32x2{nan ? kNanBits : __float_as_uint(x.M), __float_as_uint(x.den)}, rs,
+                                                  (cap * D + row * 2) * 4, 0, kSc1);
     };
     for (int i = tid; i < rows * (D / 4); i += kFewWaves * 64) {
         const int row = i / (D / 4), c = i % (D / 4);
-        float M = -INFINITY;
+        Sum x{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
 #pragma unroll
-        for (int k = 0; k < kFewWaves; ++k) M = fmaxf(M, ml[(k * kFewRows + row) * 2]);
-        const float base = M == -INFINITY ? 0.0f : M;
-        float den = 0.0f;
-        float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = 0; k < kFewWaves; ++k) x.M = fmaxf(x.M, ml[(k * kFewRows + row) * 2]);
+        const float base = x.M == -INFINITY ? 0.0f : x.M;
 #pragma unroll
         for (int k = 0; k < kFewWaves; ++k) {
             const float f = __builtin_amdgcn_exp2f(ml[(k * kFewRows + row) * 2] - base);   // 0 for a wave without keys
             const float4 v = *(const float4*)(ow + (k * kFewRows + row) * OP + 4 * c);
-            den = fmaf(f, ml[(k * kFewRows + row) * 2 + 1], den);
-            num.x = fmaf(f, v.x, num.x); num.y = fmaf(f, v.y, num.y);
-            num.z = fmaf(f, v.z, num.z); num.w = fmaf(f, v.w, num.w);
+            x.den = fmaf(f, ml[(k * kFewRows + row) * 2 + 1], x.den);
+            x.num.x = fmaf(f, v.x, x.num.x); x.num.y = fmaf(f, v.y, x.num.y);
+            x.num.z = fmaf(f, v.z, x.num.z); x.num.w = fmaf(f, v.w, x.num.w);
         }
-        if (it.parts > 1) {
-            // agent-scope stores: coherent across the XCDs' L2 caches
-            __builtin_amdgcn_raw_buffer_store_b128(
-                u32x4{__float_as_uint(num.x), __float_as_uint(num.y), __float_as_uint(num.z), __float_as_uint(num.w)},
-                piece_rsrc(it.part), (row * D + 4 * c) * 4, 0, kSc1);
-            if (c == 0)
-                __builtin_amdgcn_raw_buffer_store_b64(u32x2{any_bad ? kNanBits : __float_as_uint(M), __float_as_uint(den)},
-                                                      piece_rsrc(it.part), (cap * D + row * 2) * 4, 0, kSc1);
-            continue;
-        }
-        const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-        uint2 y = {pack2<KT>(num.x * inv, num.y * inv), pack2<KT>(num.z * inv, num.w * inv)};
-        if (any_bad) y.x = y.y = 0x7fff7fffu;
-        const int rt = div_g(a, row);
-        *(uint2*)(a.out + (int64_t)(it.q.q0 + rt) * a.o_nb_t + (int64_t)(kvh * a.G + row - rt * a.G) * a.o_nb_h + 8 * c) = y;
+        if (it.parts > 1) store(it.part, row, c, x);
+        else write(row, c, x);
     }
     if (it.parts == 1) return;
-    // ---- the last of the sequence's pieces adds their partials, in order:
-    // every store of this workgroup is done before its ticket
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    int* const last = (int*)lds;
-    if (tid == 0) {
-        unsigned* tk = tickets + it.s * a.Hkv + kvh;
-        const unsigned old = __hip_atomic_fetch_add(tk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *last = old == (unsigned)(it.parts - 1);
-        if (*last) __hip_atomic_store(tk, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!*last) return;
-    for (int i = tid; i < rows * (D / 4); i += kFewWaves * 64) {
-        const int row = i / (D / 4), c = i % (D / 4);
-        float M = -INFINITY, den = 0.0f;
-        float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        bool nan = false;
-        for (int p0 = 0; p0 < it.parts; p0 += kMergeBatch) {
-            // a batch's loads go out together, one round trip each; those past
-            // the last piece lie outside their buffer and read nothing
-            u32x2 e[kMergeBatch];
-            u32x4 v[kMergeBatch];
-#pragma unroll
-            for (int u = 0; u < kMergeBatch; ++u) {
-                const bool in = p0 + u < it.parts;
-                const BufRsrc rs = piece_rsrc(in ? p0 + u : 0);
-                e[u] = __builtin_amdgcn_raw_buffer_load_b64(rs, in ? (cap * D + row * 2) * 4 : 0x7ffffff0, 0, kSc1);
-                v[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, in ? (row * D + 4 * c) * 4 : 0x7ffffff0, 0, kSc1);
+    // ---- the last of a group of pieces adds their partials, in order, and the
+    // last of more groups adds the groups (one group of up to 16 pieces, more
+    // of 8: two batches of loads in a row cost less than a second ticket).
+    // The group's sums take the place of its first piece's, which a thread
+    // overwrites where it alone has read them (a row's exponent: its wave).
+    const int size = it.parts <= 2 * kMergeBatch ? 2 * kMergeBatch : kMergeBatch, grp = it.part / size;
+    const int groups = (it.parts + size - 1) / size;
+    unsigned* tk = tickets + kFewTickets + (it.first + grp * size) * args.Hkv + kvh;
+    int first = grp * size, by = 1, n_add = min(size, it.parts - first);
+#pragma unroll 1
+    for (int level = 0; level < 2; ++level) {
+        const bool final = level > 0 || groups == 1;
+        if (n_add > 1) {
+            __builtin_amdgcn_s_waitcnt(0);             // every store of this workgroup is done before its ticket
+            __syncthreads();
+            int* const last = (int*)lds;
+            if (tid == 0) {
+                const unsigned old = __hip_atomic_fetch_add(tk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                *last = old == (unsigned)(n_add - 1);
+                if (*last) __hip_atomic_store(tk, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
+            __syncthreads();
+            if (!*last) return;
+#pragma unroll 1
+            for (int i = tid; i < rows * (D / 4); i += kFewWaves * 64) {
+                const int row = i / (D / 4), c = i % (D / 4);
+                Sum x{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+#pragma unroll 1
+                for (int p0 = 0; p0 < n_add; p0 += kMergeBatch) {
+                    // a batch's loads go out together, one round trip each; those
+                    // past the last piece lie outside their buffer and read nothing
+                    u32x2 e[kMergeBatch];
+                    u32x4 v[kMergeBatch];
 #pragma unroll
-            for (int u = 0; u < kMergeBatch; ++u) asm volatile("" : "+v"(e[u]), "+v"(v[u]));
-            float mb = M;
+                    for (int u = 0; u < kMergeBatch; ++u) {
+                        const bool in = p0 + u < n_add;
+                        const BufRsrc rs = piece_rsrc(first + (in ? p0 + u : 0) * by);
+                        e[u] = __builtin_amdgcn_raw_buffer_load_b64(rs, in ? (cap * D + row * 2) * 4 : 0x7ffffff0, 0, kSc1);
+                        v[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, in ? (row * D + 4 * c) * 4 : 0x7ffffff0, 0, kSc1);
+                    }
 #pragma unroll
-            for (int u = 0; u < kMergeBatch; ++u) {
-                const bool hit = e[u].x == kNanBits;
-                nan = nan || hit;
-                if (hit || p0 + u >= it.parts) {              // nothing to add
-                    e[u] = u32x2{0xff800000u, 0u};
-                    v[u] = u32x4{0u, 0u, 0u, 0u};
+                    for (int u = 0; u < kMergeBatch; ++u) asm volatile("" : "+v"(e[u]), "+v"(v[u]));
+                    float mb = x.M;
+#pragma unroll
+                    for (int u = 0; u < kMergeBatch; ++u) {
+                        const bool hit = e[u].x == kNanBits;
+                        nan = nan || hit;
+                        if (hit || p0 + u >= n_add) {          // nothing to add
+                            e[u] = u32x2{0xff800000u, 0u};
+                            v[u] = u32x4{0u, 0u, 0u, 0u};
+                        }
+                        mb = fmaxf(mb, __uint_as_float(e[u].x));
+                    }
+                    const float base = mb == -INFINITY ? 0.0f : mb;
+                    const float f0 = __builtin_amdgcn_exp2f(x.M - base);
+                    x.M = mb;
+                    x.den *= f0;
+                    x.num.x *= f0; x.num.y *= f0; x.num.z *= f0; x.num.w *= f0;
+#pragma unroll
+                    for (int u = 0; u < kMergeBatch; ++u) {
+                        const float f = __builtin_amdgcn_exp2f(__uint_as_float(e[u].x) - base);
+                        x.den = fmaf(f, __uint_as_float(e[u].y), x.den);
+                        x.num.x = fmaf(f, __uint_as_float(v[u].x), x.num.x);
+                        x.num.y = fmaf(f, __uint_as_float(v[u].y), x.num.y);
+                        x.num.z = fmaf(f, __uint_as_float(v[u].z), x.num.z);
+                        x.num.w = fmaf(f, __uint_as_float(v[u].w), x.num.w);
+                    }
                 }
-                mb = fmaxf(mb, __uint_as_float(e[u].x));
-            }
-            const float base = mb == -INFINITY ? 0.0f : mb;
-            const float f0 = __builtin_amdgcn_exp2f(M - base);
-            M = mb;
-            den *= f0;
-            num.x *= f0; num.y *= f0; num.z *= f0; num.w *= f0;
-#pragma unroll
-            for (int u = 0; u < kMergeBatch; ++u) {
-                const float f = __builtin_amdgcn_exp2f(__uint_as_float(e[u].x) - base);
-                den = fmaf(f, __uint_as_float(e[u].y), den);
-                num.x = fmaf(f, __uint_as_float(v[u].x), num.x);
-                num.y = fmaf(f, __uint_as_float(v[u].y), num.y);
-                num.z = fmaf(f, __uint_as_float(v[u].z), num.z);
-                num.w = fmaf(f, __uint_as_float(v[u].w), num.w);
+                if (final) write(row, c, x);
+                else store(first, row, c, x);
             }
         }
-        const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-        uint2 y = {pack2<KT>(num.x * inv, num.y * inv), pack2<KT>(num.z * inv, num.w * inv)};
-        if (nan) y.x = y.y = 0x7fff7fffu;
-        const int rt = div_g(a, row);
-        *(uint2*)(a.out + (int64_t)(it.q.q0 + rt) * a.o_nb_t + (int64_t)(kvh * a.G + row - rt * a.G) * a.o_nb_h + 8 * c) = y;
+        if (final) return;
+        tk = tickets + it.s * args.Hkv + kvh;
+        first = 0;
+        by = size;
+        n_add = groups;
     }
 }
 
@@ -639,15 +672,6 @@ __device__ __forceinline__ ManySeq many_seq(const PagedArgs& a, const ManyAxis& 
         base = lane_of(end, 63);
     }
     return r;
-}
-
-// The kernel's arguments, read again from their segment: each phase loads the
-// few that it needs (they hit the scalar cache), so that not all of them are
-// held, and spilled, through the key tiles.
-__device__ __forceinline__ const PagedArgs& fresh_args() {
-    uint64_t p = (uint64_t)(uintptr_t)(const char*)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(p));
-    return *(const PagedArgs*)(const __attribute__((address_space(4))) PagedArgs*)(uintptr_t)p;
 }
 
 // One workgroup per share of the work: 8 waves x 32 rows that share every K / V
@@ -1140,7 +1164,8 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, float* ws, unsig
     return e;
 }
 
-static_assert(kManyTickets <= kMaxPagedTickets, "the context holds the tickets");
+// (n_seq + 1) * Hkv <= kFewTickets (the caller); pieces * Hkv: at most that and the workgroups at once
+static_assert(kManyTickets <= kMaxPagedTickets && 2 * kFewTickets + 4 * kMaxWgs <= kMaxPagedTickets, "the context holds the tickets");
 
 }  // namespace
 
@@ -1160,7 +1185,7 @@ PagedPlan paged_plan(const PagedArgs& a, int n_cu) {
         // no CU's share of the bytes is less (1 x 32768 keys 29.3 -> 22.3 us, 64 x 4096
         // 88.8 -> 83.8); all of them where the sequences are too many to be cut evenly
         // into that few (48 of 500 to 8000 keys: 94.2 -> 79.3)
-        const int slots = n_cu * (a.d == 64 ? 2 : 1);
+        const int slots = std::min(n_cu, kMaxWgs) * (a.d == 64 ? 2 : 1);
         p.few_slots = std::max(1, (2 * a.n_seq * a.Hkv > slots ? 2 : 1) * slots / a.Hkv);
         const int64_t seq_tiles = (max_keys + kFewTile - 1) / kFewTile;
         p.few_split = seq_tiles > kFewMin;

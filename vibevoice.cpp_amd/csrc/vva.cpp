@@ -1611,8 +1611,9 @@ extern "C" vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, cons
     a.out = (char*)out->data; a.o_nb_h = out->nb[1]; a.o_nb_t = out->nb[2];
     a.scale = scale;
     DeviceGuard g(ctx->device);
-    if ((int64_t)a.n_seq * a.Hkv > kMaxPagedTickets)
-        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "paged_attn: %d sequences x %d kv heads, at most %d", a.n_seq, a.Hkv, kMaxPagedTickets);
+    if (((int64_t)a.n_seq + 1) * a.Hkv > kMaxPagedSeqHeads)
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "paged_attn: %d sequences x %d kv heads, their product at most %d", a.n_seq, a.Hkv,
+                    kMaxPagedSeqHeads - a.Hkv);
     const PagedPlan plan = paged_plan(a, ctx->n_cu);
     if ((st = ensure_ws(ctx, paged_ws_bytes(a, plan))) != VVA_OK) return st;
     const hipError_t e = launch_paged_attn(a, plan, ctx->ws, ctx->tickets + kMaxStepTickets + kMaxPrefillTickets + kMaxProjTickets,

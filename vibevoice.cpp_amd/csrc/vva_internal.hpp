@@ -241,8 +241,9 @@ struct PagedPlan {
 };
 PagedPlan paged_plan(const PagedArgs& a, int n_cu);
 size_t paged_ws_bytes(const PagedArgs& a, const PagedPlan& p);
-// tickets: [kMaxPagedTickets], zero between launches; n_seq * Hkv of them at most are used for sequences
-constexpr int kMaxPagedTickets = 67584;
+// tickets: [kMaxPagedTickets], zero between launches; n_seq * Hkv <= kMaxPagedSeqHeads
+constexpr int kMaxPagedSeqHeads = 65536;
+constexpr int kMaxPagedTickets = 2 * kMaxPagedSeqHeads + 1024;
 hipError_t launch_paged_attn(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s);
 hipError_t launch_norm(const NormArgs& a, hipStream_t s);
 
