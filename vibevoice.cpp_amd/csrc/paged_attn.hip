@@ -574,8 +574,8 @@ constexpr int kRowsWave = 32;
 constexpr int kWaves = 8;          // two per SIMD
 constexpr int kRowsWG = kRowsWave * kWaves;
 constexpr int kStages = 4;         // LDS ring: tile j + 3 loads while tile j is computed
-constexpr int kMinShare = 4;       // key tiles of a workgroup's share at least
 constexpr int kRowTileCost = 4;    // what a row tile costs beside its keys, in key tiles
+constexpr int kSnap = 3;           // cuts this near an end of a row tile, in key tiles, are moved there
 constexpr int kMaxWgs = 256;       // workgroups of a call at most
 constexpr int kGroup = 8;          // pieces whose partials are added at once
 constexpr int kManyTickets = kMaxWgs * kWaves * (1 + kMaxWgs / kGroup);
@@ -620,6 +620,7 @@ struct ManyAxis {
     int slope;              // of a row tile, in sixteenths
     int shift;              // the unit's power of two above a sixteenth
     int head;               // length of a kv head's part (0: no work)
+    int row_tiles;          // in it
 };
 // `mine`: the lane's own of the first 64 sequences.  By whole waves.
 __device__ __forceinline__ ManyAxis many_axis(const PagedArgs& a, const Seq& mine) {
@@ -635,12 +636,14 @@ __device__ __forceinline__ ManyAxis many_axis(const PagedArgs& a, const Seq& min
     int shift = 0;
     for (; all > 1.0e9f; all *= 0.5f) ++shift;
     x.shift = uni(shift);
-    int total = 0;
+    int total = 0, r = 0;
     for (int s = lane; s < a.n_seq; s += 64) {
         const ManyWeight w = many_weight(a, s == lane ? mine : seq_of(a, s), x.slope, x.shift);
         total += w.before(w.r);
+        r += w.r;
     }
     x.head = wave_total(total);
+    x.row_tiles = wave_total(r);
     return x;
 }
 // The sequence at place p of a kv head's part, and where it starts and ends
@@ -712,8 +715,14 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     axis_slope = axis.slope;
     if (head <= 0) return;
     total = head * a.Hkv;
-    const float unit = (float)max((16 * kMinShare) >> axis.shift, 1);
-    wgs = uni(max(1, min((int)gridDim.x, (int)((float)total * __builtin_amdgcn_rcpf(unit)))));
+    // A row tile of t key tiles cut into n parts takes about t / n of them, and
+    // a part of one more per piece to add: shares are not below 0.6 times the
+    // square root of the average t and what a row tile costs (256 tokens behind
+    // 4096 keys, 28 row tiles: 51.6 us with shares of 4 tiles, 47.8 with 8).
+    const float tile = 16.0f * __builtin_amdgcn_rcpf((float)(1 << axis.shift));
+    const float mean = fmaxf((float)head * __builtin_amdgcn_rcpf((float)axis.row_tiles * tile) - (float)kRowTileCost, 1.0f);
+    const float least = ((float)kRowTileCost + 0.6f * __builtin_amdgcn_sqrtf(mean)) * tile;
+    wgs = uni(max(1, min((int)gridDim.x, (int)((float)total * __builtin_amdgcn_rcpf(least)))));
     if ((int)blockIdx.x >= wgs) return;
     // neighbouring shares on one XCD (workgroups go round its 8): they read the same keys
     g = wgs % 8 == 0 ? (int)(blockIdx.x % 8) * (wgs / 8) + (int)(blockIdx.x / 8) : (int)blockIdx.x;
@@ -723,8 +732,22 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     sq = many_seq(a, axis, mine, p - sq_kvh * head);
     sq_end = sq_kvh * head + sq.end;
     }
-    // the workgroup whose share holds place p
-    auto owner = [&](int p) { return min(wgs - 1, part_of(p, share)); };
+    // Where the cut at place b, inside the row tile [x, x + len), falls: a cut
+    // near one of its ends is moved there.
+    const int snap = max(1, min(share / 2, (16 * kSnap) >> axis_shift));
+    auto cut = [&](int b, int x, int len) {
+        const int l = b - x, r = x + len - b;
+        return l < snap && l <= r ? x : (r < snap ? x + len : b);
+    };
+    // the first and the last workgroup of the row tile [x, x + len)
+    auto first_of = [&](int x, int len) {
+        const int k = part_of(x, share), b = (k + 1) * share;
+        return min(wgs - 1, b < x + len && cut(b, x, len) == x ? k + 1 : k);
+    };
+    auto final_of = [&](int x, int len) {
+        const int k = part_of(x + len - 1, share), b = k * share;
+        return min(wgs - 1, b > x && cut(b, x, len) == x + len ? k - 1 : k);
+    };
     const int p_end = min(total, (g + 1) * share);
     const float inv_g = uni(1.0f / (float)a.G);
 
@@ -733,10 +756,10 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         int s, kvh, q0, rows, L, past;             // the sequence; rows of its kv group
         int rt, n_tiles, kb0;                      // row tile, key tiles from key kb0 on
         int place, len;                            // the row tile on the axis
-        bool whole;
+        bool whole, empty;
         int next;                                  // the place after this part
     };
-    auto find = [&](int p) {
+    auto find = [&](int p, bool begin) {           // begin: p is the share's own, yet to be moved
         const PagedArgs& a = fresh_args();
         const int G = a.G;
         Cut c;
@@ -762,10 +785,12 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         c.L = sq.q.L;
         c.past = sq.q.L - sq.q.n;
         c.len = wt.of(rt);
-        const int off = ps - wt.before(rt), off_end = min(c.len, off + p_end - p);
-        c.place = p - off;
+        c.place = p - (ps - wt.before(rt));
+        const int off = (begin ? cut(p, c.place, c.len) : p) - c.place;
+        const int off_end = (p_end < c.place + c.len ? cut(p_end, c.place, c.len) : c.place + c.len) - c.place;
         c.whole = off <= 0 && off_end == c.len;
-        c.next = p + max(1, off_end - off);
+        c.empty = off_end <= off;                  // the share begins with the next row tile, or ended with the last
+        c.next = c.place + max(c.empty ? off : off_end, 1);
         // keys in proportion: a function of the place alone, so that a part ends where the next begins
         const int tiles = uni(many_key_tiles(a, sq.q, rt));
         const float r = (float)tiles * __builtin_amdgcn_rcpf((float)c.len);
@@ -855,8 +880,13 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
 
     int fix_id = 0;
     for (int p = g * share, seg = 0, p_next; p < p_end; p = p_next, ++seg) {
-    const Cut c = find(p);
+    const Cut c = find(p, seg == 0);
     p_next = c.next;
+    if (c.empty) {
+        if (p_next >= p_end || seg > 0) break;     // moved past its end, or its end to here
+        if (p_next <= p) break;
+        continue;
+    }
     const Source src = source(c);
     if (c.n_tiles > 0) start(c, src);
     const int L = c.L, past = c.past, kb0 = c.kb0, n_tiles = c.n_tiles, rows = c.rows;
@@ -1045,7 +1075,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     bool nan = c.n_tiles > 0 && *(volatile __attribute__((address_space(3))) int*)&bad_seg == seg;
     bool done = true;
     if (!c.whole) {
-        const int g0 = owner(c.place), pieces = owner(c.place + c.len - 1) - g0 + 1;
+        const int g0 = first_of(c.place, c.len), pieces = final_of(c.place, c.len) - g0 + 1;
         // piece k's slot: workgroup g0's second, the others' first
         auto piece_rsrc = [&](int k) {
             const int slot = k == 0 ? 2 * g0 + 1 : 2 * min(g0 + k, wgs - 1);
