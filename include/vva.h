@@ -336,8 +336,11 @@ typedef struct {
  * for V: ne = [head_dim, page_size, n_kv_heads, n_pages], F16 or BF16, rows
  * contiguous, any other strides (of 16 bytes' multiples; the memory order
  * [page][head][slot][dim] of a contiguous tensor streams best).  head_dim is 64
- * or 128, page_size a power of two from 16 to 1024 (otherwise
- * VVA_ERR_NOT_IMPLEMENTED).  Sequences may share pages they only read. */
+ * or 128, page_size a power of two from 16 to 1024.  Sequences may share pages
+ * they only read.
+ * Beyond that the calls take at most 2^22 token rows, 256 query heads per kv
+ * head, (n_seq + 1) * n_kv_heads <= 65536, and a table of at most 2^30 keys per
+ * sequence and 2^34 in all; larger ones get VVA_ERR_NOT_IMPLEMENTED. */
 
 /* RoPE of packed rows and their append into the pages: vva_rope_append for
  * the tokens of a batch.
@@ -353,7 +356,8 @@ typedef struct {
  * Writes RoPE(k) and v, rounded to the pages' type, to the tokens' slots.
  * A token whose page id is outside the pool, or which belongs to no sequence,
  * or lies before key 0, is not appended; a position outside the table gives
- * NaN.  q_out rows of no sequence are left as they were. */
+ * NaN.  q_out rows of no sequence are left as they were.  The pages lie apart
+ * from every input, K's from V's (they may interleave). */
 VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, const vva_tensor* k,
                                          const vva_tensor* v, const vva_tensor* rope, const vva_tensor* pos,
                                          const vva_batch* batch, const vva_tensor* k_pages,
@@ -363,15 +367,20 @@ VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, 
  * vva_attn for packed sequences, each with any number of new tokens behind any
  * number of keys (whole prompts, chunks and single tokens in one call).
  *   q:   ne = [d, Hq, N], already RoPE'd, in the pages' type;
- *   out: ne = [d, Hq, N], in that type too, apart from q's memory;
+ *   out: ne = [d, Hq, N], in that type too, apart from the memory of every
+ *        input; rows of q less than 4 MiB apart;
  *   scale: a finite number above 0.
  * Token t of sequence s sees keys 0 .. kv_len[s] - n_s + t; one that sees none
  * gets zeros.  Rows of no sequence are left as they were; rows that see a key
- * whose page id is outside the pool get NaN (other rows of that sequence may).  What is stored behind the
- * keys of a sequence (NaN included) does not matter.  The products run on the
- * matrix cores in the pages' type with F32 sums, the probabilities rounded to
- * that type; the softmax is F32.
- * Every row of q and out and every page row starts on 16 bytes. */
+ * whose page id is outside the pool get NaN (other rows of that sequence may).
+ * What is stored behind the keys of a sequence (NaN included) does not matter.
+ * The products run on the matrix cores in the pages' type with F32 sums, the
+ * probabilities rounded to that type; the softmax is F32.
+ * Every row of q and out and every page row starts on 16 bytes.
+ * Partial sums go through the context's workspace, as those of the other
+ * calls: under stream capture a call larger than any before it is refused
+ * (VVA_ERR_INVALID_ARG), and graphs captured from one context are replayed one
+ * after the other. */
 VVA_API vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, const vva_tensor* k_pages,
                                   const vva_tensor* v_pages, const vva_batch* batch, float scale,
                                   const vva_tensor* out);
@@ -387,7 +396,8 @@ VVA_API vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, const v
  *        (then hidden is a multiple of 32; scale amax / 127, codes
  *        round(y * 127 / amax), as in the Q8_0 caches); may be x or add itself
  *        where the types match.
- * Everything is computed in F32 from the unrounded h.  hidden <= 16384, rows
+ * Outputs otherwise lie apart from each other and the inputs (rows may
+ * interleave).  Everything is computed in F32 from the unrounded h.  hidden <= 16384, rows
  * contiguous, any strides between them; eps >= 0. */
 VVA_API vva_status vva_add_rms_norm(vva_context* ctx, const vva_tensor* x, const vva_tensor* add, const vva_tensor* w,
                                     float eps, const vva_tensor* sum, const vva_tensor* y);

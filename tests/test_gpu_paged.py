@@ -184,6 +184,42 @@ def test_batches_that_point_outside_are_cut(ctx, torch_gpu):
         assert bool((out[2 + m:] == 5.0).all())
 
 
+@pytest.mark.parametrize("lens,max_new,pad", [([(1, 100), (40, 300)], 40, 39), ([(0, 0), (3, 70), (64, 64)], 64, 125),
+                                              ([(2, 33), (0, 9), (1, 1)], 2, 3), ([(4, 900)], 80, 76)])
+@pytest.mark.parametrize("heads", [H7, H05])
+def test_batch_padded_to_its_rows(ctx, torch_gpu, lens, max_new, pad, heads):
+    """n_seq * max_new rows, of which the sequences fill some: short ones are computed, the rows behind them kept."""
+    P = Pages(torch_gpu, lens, *heads, vva.F16, 16, seed=6, extra_rows=pad)
+    assert P.rows == len(lens) * max_new
+    run_attn(ctx, P, max_new=max_new)
+
+
+@pytest.mark.parametrize("heads,t", [(H7, vva.F16), (H05, vva.BF16)])
+def test_parts_of_one_projections_rows(ctx, torch_gpu, heads, t):
+    """q, k and v as the parts of packed rows, q rotated in place; K and V pages by turns in one pool."""
+    torch = torch_gpu
+    Hq, Hkv, d = heads
+    lens = [(1, 40), (50, 90), (2, 7)]
+    P, R = [Pages(torch, lens, *heads, t, 16, seed=8) for _ in range(2)]
+    both = torch.stack([P.k, P.v], 1)
+    P.k, P.v = both[:, 0], both[:, 1]
+    y = torch.randn(P.rows, Hq + 2 * Hkv, d, generator=P.gen, device="cuda").to(dtype(torch, t))
+    q, k, v = y.split([Hq, Hkv, Hkv], 1)
+    rope = rope_table(ctx, torch, 100, d)
+    plain = torch.empty(P.rows, Hq, d, dtype=y.dtype, device="cuda")
+    ctx.paged_rope_append(q.contiguous(), k.contiguous(), v.contiguous(), rope, R.batch(), R.k, R.v, plain)
+    keep = y[:, Hq:].clone()
+    ctx.paged_rope_append(q, k, v, rope, P.batch(), P.k, P.v, q)
+    torch.cuda.synchronize()
+    assert torch.equal(q, plain) and torch.equal(y[:, Hq:], keep)
+    for a, b in ((P.k, R.k), (P.v, R.v)):
+        assert bool(((a == b) | (a.isnan() & b.isnan())).all())
+    wide = torch.full((P.rows, 2 * Hq, d), 77.0, dtype=y.dtype, device="cuda")
+    wide[:, :Hq] = q
+    P.q = wide[:, :Hq]
+    run_attn(ctx, P, out=wide[:, Hq:])
+
+
 def test_pool_beyond_32_bit_offsets(ctx, torch_gpu):
     """Pools of 5 GiB: the pages at their far end."""
     torch = torch_gpu

@@ -580,10 +580,11 @@ constexpr int kMaxWgs = 256;       // workgroups of a call at most
 constexpr int kGroup = 8;          // pieces whose partials are added at once
 constexpr int kManyTickets = kMaxWgs * kWaves * (1 + kMaxWgs / kGroup);
 
-// Row tiles of a sequence, and the key tiles that one sees
+// Row tiles of a sequence (few_rows: what paged_few_kernel takes, 0 where it is
+// not launched), and the key tiles that one sees
 __device__ __forceinline__ int many_row_tiles(const PagedArgs& a, const Seq& q) {
     const int n = min(q.n, a.max_new);
-    return n * a.G > kFewRows ? (n * a.G + kRowsWG - 1) / kRowsWG : 0;
+    return n * a.G > a.few_rows ? (n * a.G + kRowsWG - 1) / kRowsWG : 0;
 }
 __device__ __forceinline__ int many_key_tiles(const PagedArgs& a, const Seq& q, int rt) {
     const int n = min(q.n, a.max_new);
@@ -1206,7 +1207,9 @@ PagedPlan paged_plan(const PagedArgs& a, int n_cu) {
     PagedPlan p{};
     const int64_t rows = (int64_t)a.max_new * a.G;
     const int64_t max_keys = (int64_t)a.max_pages << a.page_shift;
-    // every sequence brings max_new tokens where their number says so
+    // Every sequence brings max_new tokens where their number says so: one
+    // kernel is launched, which takes any others as well (a batch padded to its
+    // token rows).
     const bool even = (int64_t)a.n_seq * a.max_new == a.n_tok;
     if (rows > kFewRows) p.many_wgs = std::min(n_cu, kMaxWgs);
     if (rows <= kFewRows || !even) {
@@ -1229,7 +1232,8 @@ size_t paged_ws_bytes(const PagedArgs& a, const PagedPlan& p) {
     return std::max(many, few);                    // one after the other on the stream
 }
 
-hipError_t launch_paged_attn(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s) {
+hipError_t launch_paged_attn(PagedArgs a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s) {
+    a.few_rows = p.few_pieces > 0 ? kFewRows : 0;
     if (a.d == 64)
         return a.type == VVA_TYPE_F16 ? launch_paged<64, VVA_TYPE_F16>(a, p, ws, tickets, s) : launch_paged<64, VVA_TYPE_BF16>(a, p, ws, tickets, s);
     return a.type == VVA_TYPE_F16 ? launch_paged<128, VVA_TYPE_F16>(a, p, ws, tickets, s) : launch_paged<128, VVA_TYPE_BF16>(a, p, ws, tickets, s);

@@ -15,17 +15,6 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int s) {
     return r;
 }
 
-// The sequence whose rows hold token row n, or n_seq.  Called by whole waves.
-__device__ __forceinline__ int seq_of_token(const PagedArgs& a, int n) {
-    const int lane = threadIdx.x & 63;
-    for (int i = 0; i < a.n_seq; i += 64) {
-        const int s = min(i + lane, a.n_seq - 1);
-        const uint64_t hit = __ballot(a.q_start[s] <= n && n < a.q_start[s + 1]);
-        if (hit) return min(i + __ffsll((unsigned long long)hit) - 1, a.n_seq - 1);
-    }
-    return a.n_seq;
-}
-
 __device__ __forceinline__ int lane_of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
 // Sum of x over the lanes up to and with this one (DPP: shifts within rows of
 // 16 lanes, then the rows' totals broadcast upwards)

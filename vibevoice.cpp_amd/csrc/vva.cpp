@@ -1501,6 +1501,26 @@ vva_status fill_paged(vva_context* ctx, const char* what, const vva_tensor* kp, 
     if (kp->type != vp->type || (kp->type != VVA_TYPE_F16 && kp->type != VVA_TYPE_BF16))
         return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: pages must be F16 or BF16, K and V alike", what);
     for (int i = 0; i < 4; ++i)
+// Whether two tensors of token rows (dims [0, dim) of a row) share memory.
+// Rows may interleave, as the parts of one projection's rows do: all row
+// strides are then multiples of one period, in which the rows lie apart.
+bool rows_overlap(const vva_tensor* a, const vva_tensor* b, int dim) {
+    if (!overlaps(a, b)) return false;
+    uint64_t period = ~(uint64_t)0;
+    for (int i = dim; i < 4; ++i) {
+        if (a->ne[i] > 1) period = std::min(period, (uint64_t)a->nb[i]);
+        if (b->ne[i] > 1) period = std::min(period, (uint64_t)b->nb[i]);
+    }
+    if (period == 0 || period == ~(uint64_t)0) return true;
+    for (int i = dim; i < 4; ++i)
+        if ((a->ne[i] > 1 && a->nb[i] % period) || (b->ne[i] > 1 && b->nb[i] % period)) return true;
+    vva_tensor ra = *a, rb = *b;
+    for (int i = dim; i < 4; ++i) ra.ne[i] = rb.ne[i] = 1;
+    const uint64_t sa = tensor_span(&ra), sb = tensor_span(&rb), da = (uint64_t)a->data % period, db = (uint64_t)b->data % period;
+    const uint64_t at = (db + period - da) % period;              // b's row in a's period
+    return sa > period || sb > period || at < sa || at + sb > period;
+}
+
         if (kp->ne[i] != vp->ne[i]) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: k_pages and v_pages differ in ne[%d]", what, i);
     if (kp->nb[0] != 2 || vp->nb[0] != 2 || !al16(kp, 3) || !al16(vp, 3))
         return fail(ctx, VVA_ERR_INVALID_ARG, "%s: page rows must be contiguous and 16-byte aligned", what);
@@ -1512,7 +1532,7 @@ vva_status fill_paged(vva_context* ctx, const char* what, const vva_tensor* kp, 
     if ((uint64_t)kp->nb[1] * ps >= ((uint64_t)1 << 31) || (uint64_t)vp->nb[1] * ps >= ((uint64_t)1 << 31) ||
         n_pages > 0x7fffffff)
         return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: pages too large", what);
-    if (Hq / Hkv > 256 || Hkv > 65535 || N > (1 << 22))
+    if (Hq / Hkv > 256 || N > (1 << 22))
         return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: %lld tokens, %lld / %lld heads: at most 2^22 tokens and 256 query heads per kv head",
                     what, (long long)N, (long long)Hq, (long long)Hkv);
     if (!b) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: batch is null", what);
@@ -1554,6 +1574,9 @@ vva_status fill_paged(vva_context* ctx, const char* what, const vva_tensor* kp, 
 
 extern "C" vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, const vva_tensor* k,
                                             const vva_tensor* v, const vva_tensor* rope, const vva_tensor* pos,
+    if (Hkv > kMaxPagedSeqHeads / (n_seq + 1))
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: %lld sequences x %lld kv heads: (n_seq + 1) * n_kv_heads is at most %d", what,
+                    (long long)n_seq, (long long)Hkv, kMaxPagedSeqHeads);
                                             const vva_batch* batch, const vva_tensor* k_pages,
                                             const vva_tensor* v_pages, const vva_tensor* q_out) {
     if (!ctx) return VVA_ERR_INVALID_ARG;
@@ -1572,10 +1595,16 @@ extern "C" vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* 
         !al16(rope, 1) || rope->ne[1] > 0x7fffffff)
         return fail(ctx, VVA_ERR_INVALID_ARG, "rope must be F32 ne=[%lld,n_pos] with 16-byte aligned rows", (long long)d);
     if (pos && (st = check_ints(ctx, pos, "pos", N)) != VVA_OK) return st;
-    // q_out: q itself, row for row, or memory of its own
+    // what one workgroup reads no other may write: the pages apart from the
+    // inputs (interleaved pools overlap as ranges, so K and V are told apart by
+    // their first rows), q_out q itself, row for row, or memory of its own
+    for (const vva_tensor* t : {q, k, v, rope, pos, &batch->q_start, &batch->kv_len, &batch->table})
+        if (t && (overlaps(k_pages, t) || overlaps(v_pages, t) || (t != q && rows_overlap(q_out, t, 2))))
+            return fail(ctx, VVA_ERR_INVALID_ARG, "paged_rope_append: the pages or q_out overlap an input (only q_out == q may alias)");
+    if (k_pages->data == v_pages->data)
+        return fail(ctx, VVA_ERR_INVALID_ARG, "paged_rope_append: k_pages and v_pages are the same memory");
     const bool same = q_out->data == q->data && q_out->type == q->type && q_out->nb[1] == q->nb[1] && q_out->nb[2] == q->nb[2];
-    if ((!same && overlaps(q_out, q)) || overlaps(q_out, k) || overlaps(q_out, v) || overlaps(q_out, k_pages) ||
-        overlaps(q_out, v_pages) || overlaps(q_out, rope))
+    if ((!same && rows_overlap(q_out, q, 2)) || overlaps(q_out, k_pages) || overlaps(q_out, v_pages))
         return fail(ctx, VVA_ERR_INVALID_ARG, "paged_rope_append: q_out overlaps another tensor (only q_out == q may alias)");
     a.p.q = (const char*)q->data; a.q_type = q->type; a.p.q_nb_h = q->nb[1]; a.p.q_nb_t = q->nb[2];
     a.k_new = (const char*)k->data; a.k_type = k->type; a.k_nb_h = k->nb[1]; a.k_nb_t = k->nb[2];
@@ -1605,15 +1634,12 @@ extern "C" vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, cons
     if (q->type != a.type || out->type != a.type)
         return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: q and out must have the pages' type (%d)", a.type);
     if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: scale must be finite and > 0");
-    if (overlaps(out, q) || overlaps(out, k_pages) || overlaps(out, v_pages))
-        return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: out overlaps q or the pages");
+    for (const vva_tensor* t : {q, k_pages, v_pages, &batch->q_start, &batch->kv_len, &batch->table})
+        if (rows_overlap(out, t, 2)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: out overlaps q, the pages or the batch");
     a.q = (const char*)q->data; a.q_nb_h = q->nb[1]; a.q_nb_t = q->nb[2];
     a.out = (char*)out->data; a.o_nb_h = out->nb[1]; a.o_nb_t = out->nb[2];
     a.scale = scale;
     DeviceGuard g(ctx->device);
-    if (((int64_t)a.n_seq + 1) * a.Hkv > kMaxPagedSeqHeads)
-        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "paged_attn: %d sequences x %d kv heads, their product at most %d", a.n_seq, a.Hkv,
-                    kMaxPagedSeqHeads - a.Hkv);
     const PagedPlan plan = paged_plan(a, ctx->n_cu);
     if ((st = ensure_ws(ctx, paged_ws_bytes(a, plan))) != VVA_OK) return st;
     const hipError_t e = launch_paged_attn(a, plan, ctx->ws, ctx->tickets + kMaxStepTickets + kMaxPrefillTickets + kMaxProjTickets,
@@ -1651,9 +1677,9 @@ extern "C" vva_status vva_add_rms_norm(vva_context* ctx, const vva_tensor* x, co
     auto same = [](const vva_tensor* o, const vva_tensor* i) {
         return o->data == i->data && o->type == i->type && (o->ne[1] == 1 || o->nb[1] == i->nb[1]) && (o->ne[2] == 1 || o->nb[2] == i->nb[2]);
     };
-    auto clash = [&](const vva_tensor* o, const vva_tensor* i) { return o && i && !same(o, i) && overlaps(o, i); };
+    auto clash = [&](const vva_tensor* o, const vva_tensor* i) { return o && i && !same(o, i) && rows_overlap(o, i, 1); };
     if (clash(y, x) || clash(y, add) || clash(sum, x) || clash(sum, add) || overlaps(y, w) || (sum && overlaps(sum, w)) ||
-        (sum && overlaps(sum, y)))
+        (sum && rows_overlap(sum, y, 1)))
         return fail(ctx, VVA_ERR_INVALID_ARG, "add_rms_norm: outputs overlap each other or an input (only an input itself may alias)");
     NormArgs a{};
     a.x = (const char*)x->data; a.x_type = x->type; a.x_nb_t = x->nb[1]; a.x_nb_b = x->nb[2];

@@ -137,7 +137,7 @@ hipError_t launch_decode_attn(const StepArgs& a, int n_splits, hipStream_t s);
 // its epilogue (F32 / F16 / BF16 caches)
 enum { kProjQKV = 0, kProjResidual = 1, kProjQKVRope = 2 };
 struct ProjPrepArgs {
-    const char* x; int x_type; int64_t x_nb_t, x_nb_b;   // rows of K elements (F32 / F16 / BF16)
+    const char* x; int x_type; int64_t x_nb_t, x_nb_b;   // rows of K elements (F32 / F16 / BF16, with Q8_0 weights Q8_0)
     int K, T, N;
     int q8;                                              // Q8_0 round trip (Q8_0 weights)
     uint16_t* xh;                                        // out: f16 [N][K]
@@ -208,6 +208,7 @@ struct PagedArgs {
     const char* q; int64_t q_nb_h, q_nb_t;
     char* out; int64_t o_nb_h, o_nb_t;
     float scale;
+    int few_rows;                                  // rows of a sequence and kv head that the few-row kernel takes (launch_paged_attn)
 };
 // RoPE + append: q, k, v rows in, q_out = PagedArgs::out
 struct PagedAppendArgs {
@@ -244,7 +245,7 @@ size_t paged_ws_bytes(const PagedArgs& a, const PagedPlan& p);
 // tickets: [kMaxPagedTickets], zero between launches; n_seq * Hkv <= kMaxPagedSeqHeads
 constexpr int kMaxPagedSeqHeads = 65536;
 constexpr int kMaxPagedTickets = 2 * kMaxPagedSeqHeads + 1024;
-hipError_t launch_paged_attn(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s);
+hipError_t launch_paged_attn(PagedArgs a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s);
 hipError_t launch_norm(const NormArgs& a, hipStream_t s);
 
 hipError_t launch_rope_append(const RopeAppendArgs& a, hipStream_t s);
