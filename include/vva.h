@@ -4,8 +4,9 @@
  * Scope: NeoX RoPE, KV-cache append, causal grouped-query attention for
  * prefill and single-token decode — the attention section of
  * vibevoice.cpp's Qwen2 layer builders (src/qwen2.cpp:101-185 classic,
- * src/qwen2.cpp:278-347 resident).  Everything else in the layer
- * (projections, norms, FFN) stays in the caller.
+ * src/qwen2.cpp:278-347 resident) — with the projections on either side and
+ * the norm before them, over a resident cache or, for many requests at once,
+ * over a cache in pages.  The FFN stays in the caller.
  *
  * Conventions (mirroring include/vibevoice.h:23-33 and src/vibevoice_capi.cpp):
  *   - every entry point returns vva_status: 0 = OK, negative = error, with
@@ -261,6 +262,9 @@ VVA_API vva_status vva_flash_attn_ext(vva_context* ctx, const vva_tensor* q, con
  * and everything vva_rope_append does (src/qwen2.cpp:282-306), in one GEMM
  * whose epilogue rotates and stores:
  *   x:  ne = [hidden, T, B] (F32 / F16 / BF16), the normed layer input xn;
+ *       with Q8_0 weights also Q8_0 rows, as vva_add_rms_norm writes them
+ *       (2-byte aligned; the results are those of F32 rows of the blocks'
+ *       values, scale times code);
  *   wq: ne = [hidden, Hq*d], wk, wv: ne = [hidden, Hkv*d], all F16 or all
  *       Q8_0 (GGUF blocks along hidden), rows contiguous (F16: 16-byte
  *       aligned rows, Q8_0: 4-byte aligned);

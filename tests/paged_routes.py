@@ -212,7 +212,113 @@ def norm():
     refused(INV, x, w, y, a, T(vva.F32, [64, 5, 2], data=x.data + 4))
 
 
-SCENARIOS = [refusals, overlaps, accepted, norm]
+def limits():
+    """The largest calls, and those past them."""
+    for kw, ok in ((dict(Hq=256, Hkv=1, N=1), True), (dict(Hq=257, Hkv=1, N=1), False), (dict(Hq=512, Hkv=2, N=1), True),
+                   (dict(Hq=1, Hkv=1, N=1 << 22), True), (dict(Hq=1, Hkv=1, N=(1 << 22) + 1), False),
+                   (dict(Hq=63, Hkv=63, N=1, n_seq=1024), True), (dict(Hq=64, Hkv=64, N=1, n_seq=1024), False),
+                   (dict(n_seq=16, max_pages=(1 << 30) // 16), True), (dict(n_seq=17, max_pages=(1 << 30) // 16), False),
+                   (dict(n_seq=1, max_pages=(1 << 30) // 16 + 1), False)):
+        for name in ("append", "attn"):
+            c = Call(**kw)
+            if ok:
+                assert getattr(c, name)() == vva.OK, (name, kw, LIB.vva_last_error(c.c.h))
+            else:
+                c.refused(getattr(c, name), NOT, (name, kw))
+    c = Call()
+    change(c, "k_pages", nb={1: 1 << 27})
+    c.refused(c.attn, NOT, "a page of 2 GiB")
+    for i in (1, 2):                                        # rows of q 4 MiB apart
+        c = Call()
+        change(c, "qa", nb={i: 1 << 22, 2: 1 << 26} if i == 1 else {2: 1 << 22})
+        c.refused(c.attn, NOT, i)
+    c = Call(max_pages=500)                                 # keys enough for partial sums
+    log()
+    FAKE.fake_set(1, NO_LIMIT)                              # under capture, before the workspace has grown
+    c.refused(c.attn, INV, "capture")
+    assert c.append() == vva.OK
+    FAKE.fake_set(0, 0)                                     # on a full device
+    c.refused(c.attn, -5, "no memory")
+    FAKE.fake_set(0, NO_LIMIT)
+    assert c.attn() == vva.OK
+
+
+def interleaved_rows():
+    """The parts of one projection's rows, q in place or out beside it; pages of K and V by turns."""
+    for io in (vva.F32, vva.F16):
+        c = Call(io=io, t=vva.F16)
+        es, whole = (4 if io == vva.F32 else 2), 14 + 4
+        y = c.make(io, [64, whole, 5])
+        for name, h, at in (("q", 14, 0), ("k", 2, 14), ("v", 2, 16)):
+            change(c, name, data=y.data + at * 64 * es, ne={1: h}, nb={2: 64 * es * whole, 3: 64 * es * whole * 5})
+        c.a["q_out"] = c.a["q"]
+        assert c.append() == vva.OK, LIB.vva_last_error(c.c.h)
+        change(c, "q_out", shift=64 * es)
+        c.refused(c.append, INV, "a head further: k's first")
+    c = Call()                                             # out between q's rows
+    change(c, "qa", nb={2: 2 * 14 * 128, 3: 2 * 14 * 128 * 5})
+    change(c, "out", data=c.a["qa"].data + 14 * 128, nb={2: 2 * 14 * 128, 3: 2 * 14 * 128 * 5})
+    assert c.attn() == vva.OK, LIB.vva_last_error(c.c.h)
+    change(c, "out", shift=-16)
+    c.refused(c.attn, INV, "16 bytes of each row")
+    change(c, "out", shift=16, nb={2: 3 * 14 * 128, 3: 3 * 14 * 128 * 5})
+    c.refused(c.attn, INV, "rows of another pitch")
+    c = Call()
+    p = c.a["k_pages"]
+    two = {3: 2 * p.nb[3]}
+    change(c, "v_pages", data=p.data + p.nb[3], nb=two)
+    change(c, "k_pages", nb=two)
+    assert c.append() == vva.OK and c.attn() == vva.OK, LIB.vva_last_error(c.c.h)
+    change(c, "v_pages", data=c.a["k_pages"].data)
+    c.refused(c.append, INV, "K and V in the same rows")
+    for name in ("q", "k", "v", "rope", "pos", "q_start", "kv_len", "table"):
+        c = Call()
+        c.a["pos"] = c.make(INT, [5])
+        change(c, name, data=c.a["v_pages"].data + 4096)
+        c.refused(c.append, INV, name)
+    for name in ("q_start", "kv_len", "table"):
+        c = Call()
+        change(c, "out", data=c.a[name].data - c.a[name].data % 16)
+        c.refused(c.attn, INV, name)
+
+
+def blocks_to_projections():
+    """Q8_0 rows as x of the projections, beside Q8_0 weights."""
+    h = Host()
+    T = h.tensor
+    w = lambda t, K=896: [T(t, [K, m]) for m in (896, 128, 128)]  # noqa: E731
+
+    def proj(x, ws, N, expect, kernels=None, **kw):
+        y = T(vva.F32, [1152, N])
+        st, names, _ = h.call("vva_qkv_proj", ref(x), *map(ref, ws), None, None, None, ref(y), **kw)
+        assert st == expect, (st, h.err())
+        assert [n.split("<")[0] for n in names] == (kernels or []), names
+
+    def fused(x, ws, N, expect, **kw):
+        kv = h.kv(2, 64, 64, 1, vva.F16, [0])
+        q, pos = T(vva.F32, [64, 14, N]), T(INT, [N])
+        st, names, _ = h.call("vva_qkv_rope_append", kv, 0, ref(x), *map(ref, ws), None, None, None, ref(pos), None, 1e6, ref(q), **kw)
+        assert st == expect, (st, h.err())
+        return [n.split("<")[0] for n in names]
+
+    wq8, wf16 = w(vva.Q8_0), w(vva.F16)
+    x = T(vva.Q8_0, [896, 3])
+    proj(x, wq8, 3, INV, capturing=True)                   # the F32 rows' workspace is not there yet
+    proj(x, wq8, 3, vva.OK, ["proj_rows_from_q8_kernel", "proj_gemv_q8_kernel"])
+    proj(x, wq8, 3, vva.OK, ["proj_rows_from_q8_kernel", "proj_gemv_q8_kernel"], capturing=True)
+    proj(T(vva.F32, [896, 3]), wq8, 3, vva.OK, ["proj_gemv_q8_kernel"])
+    assert fused(x, wq8, 3, vva.OK)[0] == "proj_rows_from_q8_kernel"
+    assert "proj_rows_from_q8_kernel" not in fused(T(vva.Q8_0, [896, 40]), wq8, 40, vva.OK)
+    bad = [(x, wf16, INV), (T(vva.Q8_0, [896, 3], off=1), wq8, INV), (T(vva.Q8_0, [896, 3], nb=[34, 953, 2859, 2859]), wq8, INV),
+           (T(vva.Q8_0, [896, 3], nb=[68, 1904, 5712, 5712]), wq8, INV), (T(vva.Q8_0, [896, 3, 1, 2]), wq8, INV),
+           (T(vva.Q8_0, [832, 3]), wq8, INV)]
+    for b, ws, st in bad:
+        proj(b, ws, 3, st)
+        assert fused(b, ws, 3, st) == []
+    proj(T(vva.Q8_0, [896, 9]), wq8, 9, NOT)
+
+
+SCENARIOS = [refusals, overlaps, accepted, norm, limits, interleaved_rows, blocks_to_projections]
 
 if __name__ == "__main__":
     FAKE.fake_set(0, NO_LIMIT)

@@ -10,7 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 DRIVER = os.path.join(HERE, "paged_routes.py")
 
 
-@pytest.mark.parametrize("name", ["refusals", "overlaps", "accepted", "norm"])
+@pytest.mark.parametrize("name", ["refusals", "overlaps", "accepted", "norm", "limits", "interleaved_rows", "blocks_to_projections"])
 def test_route(name):
     assert os.path.exists(os.path.join(HERE, "cpp", "bin", "libfakehip.so")), "run __graft_entry__.build()"
     r = subprocess.run([sys.executable, DRIVER, name], capture_output=True, text=True, timeout=120)

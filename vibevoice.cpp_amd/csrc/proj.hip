@@ -8,7 +8,8 @@
 //
 // Numerics follow ggml's CPU mul_mat: x is first converted to the weight's
 // vec-dot type by proj_prep_kernel (F16 weights: x rounded to f16; Q8_0
-// weights: x quantized to Q8_0 blocks, kept as f16 d_x * q values), then
+// weights: x quantized to Q8_0 blocks, or given in them, kept as f16 d_x * q
+// values), then
 // every product of f16 operands is exact in the fp32 MFMA accumulators.
 // Q8_0 weight blocks are dequantized to f16 d_w * q values while the tile is
 // staged in LDS.  (The two f16 roundings of d * q are the only departure from
@@ -256,6 +257,31 @@ __device__ __forceinline__ void splitk_sum(const char* piece0, int ksplit, float
 
 // ------------------------------------------------------------ prep
 
+// Elements k .. k + 7 (k a multiple of 8) of a row of Q8_0 blocks
+__device__ __forceinline__ void q8_load8(const char* row, int k, float (&x)[8]) {
+    const uint16_t* blk = (const uint16_t*)(row + (int64_t)(k / kQK8) * kQ8Bytes);
+    const float d = f16_to_f32(blk[0]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint16_t c = blk[1 + (k % kQK8) / 2 + e];
+        x[2 * e] = d * (float)(int8_t)(c & 0xffu);
+        x[2 * e + 1] = d * (float)(int8_t)(c >> 8);
+    }
+}
+
+// Rows of Q8_0 blocks as F32 [N][K], for the few-row kernels, which quantize
+// rows themselves: a block's values give the same scale and codes again.
+__global__ void __launch_bounds__(256) proj_rows_from_q8_kernel(ProjPrepArgs a, float* __restrict__ dst) {
+    const int n = blockIdx.y, b = n / a.T, t = n - b * a.T;
+    const int k = (blockIdx.x * 256 + threadIdx.x) * 8;
+    if (k >= a.K) return;
+    float x[8];
+    q8_load8(a.x + b * a.x_nb_b + t * a.x_nb_t, k, x);
+    float4* p = (float4*)(dst + (int64_t)n * a.K + k);
+    p[0] = make_float4(x[0], x[1], x[2], x[3]);
+    p[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+
 // One workgroup per token row n = b * T + t: the row in the weights'
 // vec-dot type, as f16 (F16 weights: x rounded; Q8_0 weights: the Q8_0
 // round trip, d * q with the fp16 d), and, for the q/k/v projections, the
@@ -271,7 +297,9 @@ __global__ void __launch_bounds__(256) proj_prep_kernel(ProjPrepArgs a) {
     // 16-byte aligned row is read with vector loads, two passes' loads out
     // together (K <= 4096); otherwise element by element.
     const bool f32 = a.x_type == VVA_TYPE_F32, bf = a.x_type == VVA_TYPE_BF16;
-    const bool vec = ((uintptr_t)src & 15) == 0;
+    // Q8_0 rows (a norm's output) hold their round trip already: code times scale
+    const bool blocks = a.x_type == VVA_TYPE_Q8_0;
+    const bool vec = !blocks && ((uintptr_t)src & 15) == 0;
     u32x4 raw[2][2];
     if (vec) {
 #pragma unroll
@@ -290,12 +318,14 @@ __global__ void __launch_bounds__(256) proj_prep_kernel(ProjPrepArgs a) {
                 const uint16_t v16 = (uint16_t)(e & 1 ? wd >> 16 : wd & 0xffffu);
                 x[e] = f32 ? __uint_as_float(raw[u][e / 4][e % 4]) : (bf ? bf16_to_f32(v16) : f16_to_f32(v16));
             }
+        } else if (blocks) {
+            q8_load8(src, k0, x);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = load_elem(src + (k0 + e) * es, a.x_type);
         }
         uint16_t h[8];
-        if (a.q8) {
+        if (a.q8 && !blocks) {
             float am = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(x[e]));
@@ -2592,6 +2622,10 @@ __global__ void __launch_bounds__(kDqThreads) proj_dequant_q8_kernel(ProjArgs a,
     }
 }
 
+hipError_t launch_proj_rows_from_q8(const ProjPrepArgs& p, float* dst, hipStream_t s) {
+    hipLaunchKernelGGL(proj_rows_from_q8_kernel, dim3((p.K / 8 + 255) / 256, p.N), dim3(256), 0, s, p, dst);
+    return hipGetLastError();
+}
 hipError_t launch_proj_dequant_q8(const ProjArgs& a, uint16_t* dst, hipStream_t s) {
     hipLaunchKernelGGL(proj_dequant_q8_kernel, dim3((unsigned)a.M), dim3(kDqThreads), 0, s, a, dst);
     return hipGetLastError();

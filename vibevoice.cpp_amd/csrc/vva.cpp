@@ -1045,11 +1045,20 @@ vva_status check_act(vva_context* ctx, const vva_tensor* x, const char* name, in
     return VVA_OK;
 }
 
+// x of a projection: as check_act, and Q8_0 rows (vva_add_rms_norm's) beside
+// Q8_0 weights.
+vva_status check_proj_x(vva_context* ctx, const vva_tensor* x, int64_t K, int64_t T, int64_t B, int w_type) {
+    if (x->type != VVA_TYPE_Q8_0 || w_type != VVA_TYPE_Q8_0) return check_act(ctx, x, "x", K, T, B);
+    if (x->ne[3] != 1 || x->nb[0] != kQ8Bytes)
+        return fail(ctx, VVA_ERR_INVALID_ARG, "x: Q8_0 rows ne=[%lld,%lld,%lld,1] of whole blocks", (long long)K, (long long)T, (long long)B);
+    if ((uintptr_t)x->data % 2 || x->nb[1] % 2 || x->nb[2] % 2)
+        return fail(ctx, VVA_ERR_INVALID_ARG, "x: Q8_0 rows must be 2-byte aligned");
+    return VVA_OK;
+}
+
 // Rows that start on 16-byte boundaries (the few-row projection reads them
 // 16 bytes at a time).
-bool rows16(const vva_tensor* x) {
-    return (uintptr_t)x->data % 16 == 0 && x->nb[1] % 16 == 0 && x->nb[2] % 16 == 0;
-}
+bool rows16(const ProjArgs& a) { return (uintptr_t)a.x % 16 == 0 && a.x_nb_t % 16 == 0 && a.x_nb_b % 16 == 0; }
 
 }  // namespace
 
@@ -1069,11 +1078,26 @@ static ProjGemm plan_proj_gemm(vva_context* ctx, ProjArgs& a, int P) {
     g.total = g.base + g.wbytes + proj_part_bytes(a, g.plan);
     return g;
 }
+// Q8_0 token rows as F32 rows at `off` of the workspace, for the few-row
+// kernels, which quantize F32 rows themselves (to the same codes).  p's rows
+// become those.
+static vva_status f32_rows(vva_context* ctx, ProjPrepArgs& p, size_t off) {
+    const vva_status st = ensure_ws(ctx, off + (size_t)p.N * p.K * sizeof(float));
+    if (st != VVA_OK) return st;
+    float* rows = (float*)((char*)ctx->ws + off);
+    const hipError_t e = launch_proj_rows_from_q8(p, rows, ctx->stream);
+    if (e != hipSuccess) return hip_fail(ctx, e, "projection rows launch");
+    p.x = (const char*)rows;
+    p.x_type = VVA_TYPE_F32;
+    p.x_nb_t = (int64_t)p.K * 4;
+    p.x_nb_b = p.x_nb_t * p.T;
+    return VVA_OK;
+}
 // Whether a call takes the GEMV: few token rows, 16-byte aligned, and the GEMM
 // is not the faster one (or its workspace cannot be had: under capture, or on
 // a full device).  Otherwise *g is the GEMM's plan.
-static bool takes_gemv(vva_context* ctx, const vva_tensor* x, ProjArgs& a, int P, ProjGemm* g) {
-    const bool can = proj_gemv_supported(a.N, a.K, a.M) && rows16(x);
+static bool takes_gemv(vva_context* ctx, ProjArgs& a, int P, ProjGemm* g) {
+    const bool can = proj_gemv_supported(a.N, a.K, a.M) && rows16(a);
     if (can && !proj_few_rows_gemm(a)) return true;
     *g = plan_proj_gemm(ctx, a, P);
     return can && !try_ws(ctx, g->total);
@@ -1121,7 +1145,7 @@ extern "C" vva_status vva_qkv_rope_append(vva_context* ctx, vva_kv* kv, int laye
     if (K % 64 || (Hq * d) % 128 || (Hkv * d) % 128 || (d != 64 && d != 128))
         return fail(ctx, VVA_ERR_NOT_IMPLEMENTED,
                     "qkv_rope_append: needs hidden %% 64 == 0, Hq*d and Hkv*d multiples of 128, head_dim 64 or 128");
-    if ((st = check_act(ctx, x, "x", K, T, B)) != VVA_OK) return st;
+    if ((st = check_proj_x(ctx, x, K, T, B, wt)) != VVA_OK) return st;
     if ((st = check_weight(ctx, wq, "wq", K, Hq * d, wt)) != VVA_OK) return st;
     if ((st = check_weight(ctx, wk, "wk", K, Hkv * d, wt)) != VVA_OK) return st;
     if ((st = check_weight(ctx, wv, "wv", K, Hkv * d, wt)) != VVA_OK) return st;
@@ -1191,9 +1215,14 @@ extern "C" vva_status vva_qkv_rope_append(vva_context* ctx, vva_kv* kv, int laye
     p.P = (int)(d / 2);
     p.theta_scale = powf(freq_base, -2.0f / (float)d);
     DeviceGuard dev(ctx->device);
+    if (x->type == VVA_TYPE_Q8_0 && proj_gemv_supported(a.N, a.K, a.M)) {
+        // the few-row kernels read F32 rows; their projections go before the rows
+        const size_t y = ((size_t)N * a.M * sizeof(float) + 255) / 256 * 256;
+        if ((st = f32_rows(ctx, p, y)) != VVA_OK) return st;
+    }
     a.x = p.x; a.x_type = p.x_type; a.x_nb_t = p.x_nb_t; a.x_nb_b = p.x_nb_b;
     ProjGemm g;
-    if (takes_gemv(ctx, x, a, p.P, &g)) {
+    if (takes_gemv(ctx, a, p.P, &g)) {
         // a decode step: the weight-streaming GEMV.  F32 / F16 / BF16 caches:
         // it rotates q and k and stores q_out and the cache rows itself (each
         // wave computes two whole rotation pairs), one launch.  Q8_0 caches
@@ -1241,7 +1270,7 @@ extern "C" vva_status vva_qkv_proj(vva_context* ctx, const vva_tensor* x, const 
     if (B < 1 || B > VVA_MAX_BATCH) return fail(ctx, VVA_ERR_INVALID_ARG, "qkv_proj: B must be 1..%d", VVA_MAX_BATCH);
     if (K % 64 || Mq % 64 || Mk % 64 || Mv % 64 || Mq < 64 || Mk < 64 || Mv < 64)
         return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "qkv_proj: needs hidden and the weights' output rows multiples of 64");
-    if ((st = check_act(ctx, x, "x", K, T, B)) != VVA_OK) return st;
+    if ((st = check_proj_x(ctx, x, K, T, B, wt)) != VVA_OK) return st;
     if ((st = check_weight(ctx, wq, "wq", K, Mq, wt)) != VVA_OK) return st;
     if ((st = check_weight(ctx, wk, "wk", K, Mk, wt)) != VVA_OK) return st;
     if ((st = check_weight(ctx, wv, "wv", K, Mv, wt)) != VVA_OK) return st;
@@ -1253,11 +1282,17 @@ extern "C" vva_status vva_qkv_proj(vva_context* ctx, const vva_tensor* x, const 
         return fail(ctx, VVA_ERR_INVALID_ARG, "qkv_proj: y must be F32 ne=[%lld,%lld,%lld,1], contiguous", (long long)M,
                     (long long)T, (long long)B);
     const int64_t N = T * B;
-    if (!proj_gemv_supported((int)N, (int)K, (int)M) || !rows16(x))
+    ProjPrepArgs p{};
+    p.x = (const char*)x->data; p.x_type = x->type;
+    p.x_nb_t = (int64_t)x->nb[1]; p.x_nb_b = (int64_t)x->nb[2];
+    p.K = (int)K; p.T = (int)T; p.N = (int)N;
+    ProjArgs a{};
+    a.x = p.x; a.x_nb_t = p.x_nb_t; a.x_nb_b = p.x_nb_b;
+    const bool q8_rows = x->type == VVA_TYPE_Q8_0;
+    if (!proj_gemv_supported((int)N, (int)K, (int)M) || !(q8_rows || rows16(a)))
         return fail(ctx, VVA_ERR_NOT_IMPLEMENTED,
                     "qkv_proj: decode-sized calls only (at most 8 token rows of 16-byte aligned x; hidden <= 4096); "
                     "prefill chunks take vva_qkv_rope_append");
-    ProjArgs a{};
     const vva_tensor* ws_[3] = {wq, wk, wv};
     const vva_tensor* bs_[3] = {bq, bk, bv};
     const int64_t rows[3] = {Mq, Mk, Mv};
@@ -1272,9 +1307,9 @@ extern "C" vva_status vva_qkv_proj(vva_context* ctx, const vva_tensor* x, const 
     a.w_type = wt;
     a.N = (int)N; a.K = (int)K; a.M = (int)M; a.T = (int)T;
     a.mode = kProjQKV;
-    a.x = (const char*)x->data; a.x_type = x->type;
-    a.x_nb_t = (int64_t)x->nb[1]; a.x_nb_b = (int64_t)x->nb[2];
     DeviceGuard g(ctx->device);
+    if (q8_rows && (st = f32_rows(ctx, p, 0)) != VVA_OK) return st;
+    a.x = p.x; a.x_type = p.x_type; a.x_nb_t = p.x_nb_t; a.x_nb_b = p.x_nb_b;
     const hipError_t e = launch_proj_gemv(a, (float*)y->data, ctx->n_cu, ctx->stream);
     return e == hipSuccess ? VVA_OK : hip_fail(ctx, e, "qkv_proj launch");
 }
@@ -1330,7 +1365,7 @@ extern "C" vva_status vva_out_proj_residual(vva_context* ctx, const vva_tensor* 
     DeviceGuard g(ctx->device);
     a.x = p.x; a.x_type = p.x_type; a.x_nb_t = p.x_nb_t; a.x_nb_b = p.x_nb_b;
     ProjGemm pg;
-    if (takes_gemv(ctx, o, a, 0, &pg)) {
+    if (takes_gemv(ctx, a, 0, &pg)) {
         const hipError_t e = launch_proj_gemv(a, nullptr, ctx->n_cu, ctx->stream);
         return e == hipSuccess ? VVA_OK : hip_fail(ctx, e, "out_proj_residual launch");
     }
@@ -1466,6 +1501,26 @@ extern "C" vva_status vva_decode_step(vva_context* ctx, vva_kv* kv, int layer, c
 
 namespace {
 
+// Whether two tensors of token rows (dims [0, dim) of a row) share memory.
+// Rows may interleave, as the parts of one projection's rows do: all row
+// strides are then multiples of one period, in which the rows lie apart.
+bool rows_overlap(const vva_tensor* a, const vva_tensor* b, int dim) {
+    if (!overlaps(a, b)) return false;
+    uint64_t period = ~(uint64_t)0;
+    for (int i = dim; i < 4; ++i) {
+        if (a->ne[i] > 1) period = std::min(period, (uint64_t)a->nb[i]);
+        if (b->ne[i] > 1) period = std::min(period, (uint64_t)b->nb[i]);
+    }
+    if (period == 0 || period == ~(uint64_t)0) return true;
+    for (int i = dim; i < 4; ++i)
+        if ((a->ne[i] > 1 && a->nb[i] % period) || (b->ne[i] > 1 && b->nb[i] % period)) return true;
+    vva_tensor ra = *a, rb = *b;
+    for (int i = dim; i < 4; ++i) ra.ne[i] = rb.ne[i] = 1;
+    const uint64_t sa = tensor_span(&ra), sb = tensor_span(&rb), da = (uint64_t)a->data % period, db = (uint64_t)b->data % period;
+    const uint64_t at = (db + period - da) % period;              // b's row in a's period
+    return sa > period || sb > period || at < sa || at + sb > period;
+}
+
 bool al16(const vva_tensor* t, int dims) {
     bool ok = (uintptr_t)t->data % 16 == 0;
     for (int i = 1; i <= dims; ++i) ok = ok && (t->ne[i] == 1 || t->nb[i] % 16 == 0);
@@ -1501,26 +1556,6 @@ vva_status fill_paged(vva_context* ctx, const char* what, const vva_tensor* kp, 
     if (kp->type != vp->type || (kp->type != VVA_TYPE_F16 && kp->type != VVA_TYPE_BF16))
         return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: pages must be F16 or BF16, K and V alike", what);
     for (int i = 0; i < 4; ++i)
-// Whether two tensors of token rows (dims [0, dim) of a row) share memory.
-// Rows may interleave, as the parts of one projection's rows do: all row
-// strides are then multiples of one period, in which the rows lie apart.
-bool rows_overlap(const vva_tensor* a, const vva_tensor* b, int dim) {
-    if (!overlaps(a, b)) return false;
-    uint64_t period = ~(uint64_t)0;
-    for (int i = dim; i < 4; ++i) {
-        if (a->ne[i] > 1) period = std::min(period, (uint64_t)a->nb[i]);
-        if (b->ne[i] > 1) period = std::min(period, (uint64_t)b->nb[i]);
-    }
-    if (period == 0 || period == ~(uint64_t)0) return true;
-    for (int i = dim; i < 4; ++i)
-        if ((a->ne[i] > 1 && a->nb[i] % period) || (b->ne[i] > 1 && b->nb[i] % period)) return true;
-    vva_tensor ra = *a, rb = *b;
-    for (int i = dim; i < 4; ++i) ra.ne[i] = rb.ne[i] = 1;
-    const uint64_t sa = tensor_span(&ra), sb = tensor_span(&rb), da = (uint64_t)a->data % period, db = (uint64_t)b->data % period;
-    const uint64_t at = (db + period - da) % period;              // b's row in a's period
-    return sa > period || sb > period || at < sa || at + sb > period;
-}
-
         if (kp->ne[i] != vp->ne[i]) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: k_pages and v_pages differ in ne[%d]", what, i);
     if (kp->nb[0] != 2 || vp->nb[0] != 2 || !al16(kp, 3) || !al16(vp, 3))
         return fail(ctx, VVA_ERR_INVALID_ARG, "%s: page rows must be contiguous and 16-byte aligned", what);
@@ -1539,6 +1574,9 @@ bool rows_overlap(const vva_tensor* a, const vva_tensor* b, int dim) {
     const int64_t n_seq = b->kv_len.ne[0];
     if (n_seq < 1 || n_seq > VVA_MAX_BATCH_SEQ)
         return fail(ctx, VVA_ERR_INVALID_ARG, "%s: %lld sequences, at most %d", what, (long long)n_seq, VVA_MAX_BATCH_SEQ);
+    if (Hkv > kMaxPagedSeqHeads / (n_seq + 1))
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: %lld sequences x %lld kv heads: (n_seq + 1) * n_kv_heads is at most %d", what,
+                    (long long)n_seq, (long long)Hkv, kMaxPagedSeqHeads);
     if ((st = check_ints(ctx, &b->kv_len, "kv_len", n_seq)) != VVA_OK) return st;
     if ((st = check_ints(ctx, &b->q_start, "q_start", n_seq + 1)) != VVA_OK) return st;
     const vva_tensor* t = &b->table;
@@ -1574,9 +1612,6 @@ bool rows_overlap(const vva_tensor* a, const vva_tensor* b, int dim) {
 
 extern "C" vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, const vva_tensor* k,
                                             const vva_tensor* v, const vva_tensor* rope, const vva_tensor* pos,
-    if (Hkv > kMaxPagedSeqHeads / (n_seq + 1))
-        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: %lld sequences x %lld kv heads: (n_seq + 1) * n_kv_heads is at most %d", what,
-                    (long long)n_seq, (long long)Hkv, kMaxPagedSeqHeads);
                                             const vva_batch* batch, const vva_tensor* k_pages,
                                             const vva_tensor* v_pages, const vva_tensor* q_out) {
     if (!ctx) return VVA_ERR_INVALID_ARG;

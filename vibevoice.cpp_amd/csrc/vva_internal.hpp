@@ -315,6 +315,8 @@ size_t prefill_ws_bytes(const AttnArgs& a, const PrefillPlan& p);
 // a.part proj_part_bytes.
 size_t proj_ws_bytes(int N, int K, int P);
 hipError_t launch_proj_dequant_q8(const ProjArgs& a, uint16_t* dst, hipStream_t s);
+// Q8_0 token rows (p.x) as F32 [N][K]
+hipError_t launch_proj_rows_from_q8(const ProjPrepArgs& p, float* dst, hipStream_t s);
 hipError_t launch_proj(ProjPrepArgs& p, ProjArgs& a, const ProjPlan& plan, void* ws, hipStream_t s);
 // Few token rows (decode steps): one weight-streaming GEMV launch that
 // converts the rows itself.  kProjQKV writes y = x w^T + bias (F32 [N][M],

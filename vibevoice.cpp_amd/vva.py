@@ -185,6 +185,11 @@ def q8_view(raw) -> Tensor:
                 ggml_nb=[Q8_BLOCK_BYTES, raw.stride(1), raw.stride(0), raw.stride(0) * B], type_=Q8_0)
 
 
+def _rows_view(x) -> Tensor:
+    """Token rows: a torch tensor, or a view made already (q8_view)."""
+    return x if isinstance(x, Tensor) else view(x)
+
+
 class Batch:
     """vva_batch: the sequences of a call over a paged cache.  q_start int32 [n_seq + 1], kv_len int32 [n_seq], table
     int32 [n_seq, max_pages], all on the device; max_new: the most new tokens a sequence brings."""
@@ -305,17 +310,19 @@ class Context:
 
     def qkv_rope_append(self, kv: "KVCache", layer: int, x, wq: "Weight", wk: "Weight", wv: "Weight", pos,
                         q_out, bq=None, bk=None, bv=None, seq_ids=None, freq_base: float = 1.0e6):
-        """x: [B, T, hidden]; weights: Weight; biases f32 [rows] or None; q_out [B, T, Hq, d]."""
+        """x: [B, T, hidden], or q8_view(...) of its blocks; weights: Weight; biases f32 [rows] or None; q_out
+        [B, T, Hq, d]."""
         ids = _ids(seq_ids)
         bref = [ctypes.byref(view(t)) if t is not None else None for t in (bq, bk, bv)]
-        self.check(self.lib.vva_qkv_rope_append(self.h, kv.h, layer, ctypes.byref(view(x)), ctypes.byref(wq.t),
+        self.check(self.lib.vva_qkv_rope_append(self.h, kv.h, layer, ctypes.byref(_rows_view(x)), ctypes.byref(wq.t),
                                                 ctypes.byref(wk.t), ctypes.byref(wv.t), bref[0], bref[1], bref[2],
                                                 ctypes.byref(view(pos)), ids, freq_base, ctypes.byref(view(q_out))))
 
     def qkv_proj(self, x, wq: "Weight", wk: "Weight", wv: "Weight", y, bq=None, bk=None, bv=None):
-        """x: [B, T, hidden]; weights: Weight; biases f32 [rows] or None; y f32 [B, T, Mq + Mk + Mv]."""
+        """x: [B, T, hidden], or q8_view(...) of its blocks; weights: Weight; biases f32 [rows] or None; y f32
+        [B, T, Mq + Mk + Mv]."""
         bref = [ctypes.byref(view(t)) if t is not None else None for t in (bq, bk, bv)]
-        self.check(self.lib.vva_qkv_proj(self.h, ctypes.byref(view(x)), ctypes.byref(wq.t), ctypes.byref(wk.t),
+        self.check(self.lib.vva_qkv_proj(self.h, ctypes.byref(_rows_view(x)), ctypes.byref(wq.t), ctypes.byref(wk.t),
                                          ctypes.byref(wv.t), bref[0], bref[1], bref[2], ctypes.byref(view(y))))
 
     def out_proj_residual(self, o, w_o: "Weight", x, h):
@@ -361,7 +368,7 @@ class Context:
         blocks.  Returns the call."""
         return self._bound(self.lib.vva_add_rms_norm, (x, w, y, add, total), view(x),
                            view(add) if add is not None else None, view(w), eps,
-                           view(total) if total is not None else None, y if isinstance(y, Tensor) else view(y))
+                           view(total) if total is not None else None, _rows_view(y))
 
     def add_rms_norm(self, *args, **kw):
         """bind_add_rms_norm's call, once."""
