@@ -194,6 +194,58 @@ def test_batch_padded_to_its_rows(ctx, torch_gpu, lens, max_new, pad, heads):
     run_attn(ctx, P, max_new=max_new)
 
 
+RAGGED = [(1, (97 * i) % 401) for i in range(100)] + [(90, 500), (0, 9), (40, 77)]
+
+
+@pytest.mark.parametrize("lens,heads,max_new", [
+    (RAGGED, H7, 0), (RAGGED, H05, 0), ([(1, 20000), (2, 7000), (200, 300)], H7, 0), ([(1, 40), (300, 6000), (1, 1)], H05, 0),
+    ([(1, 9000), (1, 3), (2, 70)], H7, 40), ([(1, 64 * i + 1) for i in range(30)], H15, 64),
+    ([(1, 300), (1, 70), (50, 80), (4, 4)], (300, 300, 64), 0), ([(1, 5000), (40, 900)], (8, 8, 128), 0),
+    ([(1, 32 * i) for i in range(1, 9)] + [(33, 33)], H05, 0),
+])
+def test_few_rows_beside_many(ctx, torch_gpu, lens, heads, max_new):
+    print(lens[:3], heads, max_new, flush=True)
+    P = Pages(torch_gpu, lens, *heads, vva.BF16, 16, seed=len(lens), extra_rows=1)
+    out = run_attn(ctx, P, max_new=max_new)
+    again = torch_gpu.full_like(P.q, 77.0)
+    ctx.paged_attn(P.q, P.k, P.v, P.batch(max_new), P.d ** -0.5, again)
+    torch_gpu.cuda.synchronize()
+    assert torch_gpu.equal(out, again)
+
+
+def test_one_captured_call_for_every_kind_of_batch(ctx, torch_gpu):
+    """128 token rows for 8 sequences, captured once: prompts, single tokens, both, nothing, whatever the batch says."""
+    torch = torch_gpu
+    P = Pages(torch, [(0, 1200)] * 8, *H7, vva.F16, 16, seed=12, extra_rows=128)
+    batch = vva.Batch(P.q_start, P.kv_len, P.table, 100)
+    out = torch.zeros_like(P.q)
+    ctx.paged_attn(P.q, P.k, P.v, batch, 0.09, out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    default = torch.cuda.current_stream()
+    try:
+        with torch.cuda.graph(g):
+            ctx.set_stream(torch.cuda.current_stream())
+            ctx.paged_attn(P.q, P.k, P.v, batch, 0.09, out)
+    finally:
+        ctx.set_stream(default)
+    ones = [(1, L) for L in (1200, 1, 64, 700, 33, 1199, 5, 90)]
+    for lens in (ones, [(100, 1100)] + ones[:5], [(50, 50), (28, 900)] + [(0, 0)] * 6, [(0, 3)] * 8, ones[:7] + [(0, 0)],
+                 [(4, 1000)] * 8, [(5, 600)] * 8, [(99, 99)] + [(1, 1000), (2, 1000)] + [(0, 0)] * 5, ones):
+        P.lens = lens + [(0, 0)] * (8 - len(lens))
+        P.starts = np.concatenate([[0], np.cumsum([n for n, _ in P.lens])]).astype(np.int32)
+        P.n_tok = int(P.starts[-1])
+        P.q_start.copy_(torch.from_numpy(P.starts))
+        P.kv_len.copy_(torch.tensor([L for _, L in P.lens], dtype=torch.int32))
+        out.fill_(77.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        ref, tol = attention(P, 0.09)
+        check_rows(out[:P.n_tok], ref[:P.n_tok], tol[:P.n_tok], f"{lens}")
+        assert bool((out[P.n_tok:] == 77.0).all())
+
+
 @pytest.mark.parametrize("heads,t", [(H7, vva.F16), (H05, vva.BF16)])
 def test_parts_of_one_projections_rows(ctx, torch_gpu, heads, t):
     """q, k and v as the parts of packed rows, q rotated in place; K and V pages by turns in one pool."""

@@ -9,8 +9,15 @@
 // Query rows are the (token, head) pairs of one kv group, r = t * G + head, so
 // the G heads of a group share every K / V row that is read.  Sequences whose
 // rows fit one 32-wide matrix operand (n_s * G <= 32: single tokens, a few
-// proposed ones) take paged_few_kernel, which is bound by the cache's bytes;
-// the others paged_many_kernel, which is bound by the matrix cores.
+// proposed ones) go through few_piece, which is bound by the cache's bytes, the
+// others through many_share, which is bound by the matrix cores.  A call whose
+// max_new tokens are few rows is paged_few_kernel; one of n_seq * max_new tokens
+// paged_many_kernel, which then takes short sequences too; any other may bring
+// both kinds and is paged_mixed_kernel, which runs them side by side.
+//
+// Reached, of a copy's 4.9 TB/s and a large product's 1175 TFLOP/s: single
+// tokens 5.6 TB/s (48 sequences of 500 to 8000 keys, 405 MB, 72 us); 2048 tokens
+// behind 28672 keys 990 TFLOP/s (880 us), 512 behind 15872 860 (138 us).
 //
 // Both compute, per 32 rows and a tile of keys, with
 // v_mfma_f32_32x32x16_{f16,bf16} (layouts in mfma_ops.hpp):
@@ -212,36 +219,80 @@ __device__ __forceinline__ const PagedArgs& fresh_args() {
 
 // ------------------------------------------------------------ few rows
 
-// Workgroups per kv head that paged_few_kernel's work is cut into, and the
-// least tiles (32 keys) of one: a tile per wave.
-constexpr int kFewWaves = 4;
+constexpr int kFewWaves = 4;       // of a workgroup of paged_few_kernel
 constexpr int kFewTile = 32;
-constexpr int kFewMin = kFewWaves;
+constexpr int kMaxWgs = 256;       // workgroups of the many rows at most
+constexpr int kFewCost = 4;        // what a piece costs beside its keys, in tiles
+constexpr int kFewSnap = 8;        // cuts this near an end of a sequence, in tiles, are moved there
 
-// A piece of a sequence's keys: piece `part` of `parts`; n = 0: none
-struct FewItem {
-    Seq q;
-    int s, part, parts, first;      // first: the sequence's piece 0
-};
-// Tiles of sequence q that paged_few_kernel works on
+// Tiles of sequence q that few_piece works on
 __device__ __forceinline__ int few_tiles(const PagedArgs& a, const Seq& q) {
     const int n = min(q.n, a.max_new);
     return n > 0 && n * a.G <= kFewRows ? max(1, (q.L + kFewTile - 1) / kFewTile) : 0;
 }
-// Piece `item` of the call.  All sequences are cut into pieces of at most
-// `chunk` tiles, the least for which the pieces are no more than `slots` (the
-// workgroups that run at once, per kv head), so a long sequence among short
-// ones gets its share of the chip and no piece waits for a second round: tried
-// from the even share up in steps of an eighth, for up to 64 sequences; more
-// of them leave many pieces, whose rounds even out.  By whole waves.
-__device__ __forceinline__ FewItem few_item(const PagedArgs& a, int item, int slots) {
+__device__ __forceinline__ int few_weight(const PagedArgs& a, const Seq& q) {
+    const int t = few_tiles(a, q);
+    return t > 0 ? t + kFewCost : 0;
+}
+// Length of the axis on which a kv head's sequences lie one after the other,
+// each as long as its tiles and what a piece costs beside them.  `mine`: the
+// lane's own of the first 64.  By whole waves.
+__device__ __forceinline__ int few_axis(const PagedArgs& a, const Seq& mine) {
+    const int lane = threadIdx.x & 63;
+    int total = lane < a.n_seq ? few_weight(a, mine) : 0;
+    for (int s = lane + 64; s < a.n_seq; s += 64) total += few_weight(a, seq_of(a, s));
+    return wave_total(total);
+}
+
+// x / n for a uniform p >= 0 whose quotient a float holds
+__device__ __forceinline__ int part_of(int p, int n) {
+    int k = uni((int)((float)p * __builtin_amdgcn_rcpf((float)n))), r = p - k * n;   // within one or two of it
+    while (r < 0) --k, r += n;
+    while (r >= n) ++k, r -= n;
+    return k;
+}
+// An axis cut into n equal shares, a workgroup's each.  A cut at place b inside
+// the item [x, x + len) that is near one of its ends is moved there.
+struct Shares {
+    int share, n, snap;
+    __device__ __forceinline__ int cut(int b, int x, int len) const {
+        const int l = b - x, r = x + len - b;
+        return l < snap && l <= r ? x : (r < snap ? x + len : b);
+    }
+    // the first and the last workgroup of the item [x, x + len)
+    __device__ __forceinline__ int first_of(int x, int len) const {
+        const int k = part_of(x, share), b = (k + 1) * share;
+        return min(n - 1, b < x + len && cut(b, x, len) == x ? k + 1 : k);
+    }
+    __device__ __forceinline__ int final_of(int x, int len) const {
+        const int k = part_of(x + len - 1, share), b = k * share;
+        return min(n - 1, b > x && cut(b, x, len) == x + len ? k - 1 : k);
+    }
+};
+
+// A piece of a sequence's keys: piece `part` of `parts`, tiles [t0, t1)
+struct FewItem {
+    Seq q;
+    int part, parts, t0, t1;
+    int first;                      // piece 0's number, or workgroup
+};
+// Piece `item` of a call of few rows alone.  All sequences are cut into pieces
+// of at most `chunk` tiles, the least for which the pieces are no more than
+// `slots` (the workgroups that run at once, per kv head), so a long sequence
+// among short ones gets its share of the chip and no piece waits for a second
+// round: tried from the even share up in steps of an eighth, for up to 64
+// sequences; more of them leave many pieces, whose rounds even out.  Against
+// equal shares of the axis, which cross the sequences' ends, the workgroups find
+// their work sooner (8 x 1024 keys 8.4 us against 11.4, 64 x 4096 88 against 89).
+// By whole waves.
+__device__ __forceinline__ FewItem few_item(const PagedArgs& a, int item, int slots, int least) {
     const int lane = threadIdx.x & 63;
     Seq q = seq_of(a, min(lane, a.n_seq - 1));
     int t = lane < a.n_seq ? few_tiles(a, q) : 0;
     int total = t;
     for (int s = lane + 64; s < a.n_seq; s += 64) total += few_tiles(a, seq_of(a, s));
     total = wave_total(total);
-    int chunk = max(kFewMin, (total + slots - 1) / slots);
+    int chunk = max(least, (total + slots - 1) / slots);
     if (a.n_seq <= 64)
         for (int i = 0; i < 12 && wave_total((t + chunk - 1) / chunk) > slots; ++i) chunk += (chunk + 7) / 8;
     FewItem r{};
@@ -259,54 +310,59 @@ __device__ __forceinline__ FewItem few_item(const PagedArgs& a, int item, int sl
             r.q.q0 = lane_of(q.q0, l);
             r.q.n = lane_of(q.n, l);
             r.q.L = lane_of(q.L, l);
-            r.s = i + l;
+            r.q.s = i + l;
             r.parts = lane_of(c, l);
             r.first = base + lane_of(end - c, l);
             r.part = item - r.first;
+            const int tiles = (r.q.L + kFewTile - 1) / kFewTile;
+            r.t0 = (int)((int64_t)r.part * tiles / r.parts);
+            r.t1 = (int)((int64_t)(r.part + 1) * tiles / r.parts);
             return r;
         }
         base += lane_of(end, 63);
     }
     return r;
 }
-
 constexpr int kSc1 = 16;           // cache policy of the partials: agent scope
-constexpr int kFewTickets = kMaxPagedSeqHeads; // a ticket per sequence and kv head; then one per piece and kv head
+// a ticket per piece (or partial's place) and kv head, and one per sequence's
+// first; pieces are at most n_seq and the workgroups at once, per kv head
+constexpr int kFewTickets = kMaxPagedSeqHeads + 4 * kMaxWgs;
 // pieces whose partials are loaded together (16: 8 x 1024 keys 9.4 -> 10.0 us, two
 // streams of 1k keys 6.8 -> 7.3, 1 x 32768 keys 23.2 -> 22.2)
 constexpr int kMergeBatch = 8;
 
-// One workgroup per (piece of a sequence's keys, kv head), two of them (D = 64:
-// four) on a CU.  Each wave streams every fourth tile of the piece through LDS of its
-// own, without a barrier: the next K goes out when K is read, the next V when V
-// is, so 16 KB of the wave's loads fly while it waits and 8 while it computes.
-// The waves' sums meet at the end.  Partials in the workspace, per
-// piece and kv head: [cap rows][D] sums, then [cap] (exponent base, row sum).
-template <int D, int KT>
-__global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets, int slots, int cap) {
-    prefetch_kernargs<sizeof(PagedArgs)>();
+// LDS of few_piece: a K and a V tile per wave and the rows of Q, then the
+// waves' sums
+template <int D, int WAVES>
+struct FewLds {
+    static constexpr int TB = kFewTile * 2 * D;    // bytes of a K (V) tile, and of the rows of Q
+    static constexpr int OP = D + 4;               // pitch of a row of sums
+    static constexpr int SUMS = WAVES * kFewRows * (OP + 2) * (int)sizeof(float), RING = (WAVES * 2 + 1) * TB;
+    static constexpr int BYTES = RING > SUMS ? RING : SUMS;
+};
+
+// A workgroup's piece of a sequence's keys, for one kv head: each wave streams
+// every WAVES-th tile of the piece through LDS of its own, without a barrier:
+// the next K goes out when K is read, the next V when V is, so 16 KB of the
+// wave's loads fly while it waits and 8 while it computes.  The waves' sums
+// meet at the end.  Partials in the workspace, per piece and kv head: [cap
+// rows][D] sums, then [cap] (exponent base, row sum).
+template <int D, int KT, int WAVES, bool SHARES>
+__device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, int cap, const FewItem& it, int kvh, char* lds) {
     using F = Frag<KT>;
     using QF = typename F::type;
     constexpr int DS = D / 16, DT = D / 32;
     constexpr int NC = kFewTile * 2 * D / 1024;    // loads of a K (V) tile
     constexpr int RC = 1024 / (2 * D);             // rows of a load
-    constexpr int TB = kFewTile * 2 * D;           // bytes of a K (V) tile, and of the rows of Q
-    constexpr int OP = D + 4;                      // pitch of a row of sums
-    constexpr int SUMS = kFewWaves * kFewRows * (OP + 2) * (int)sizeof(float);
-    constexpr int RING = (kFewWaves * 2 + 1) * TB;
-    __shared__ __attribute__((aligned(1024))) char lds[RING > SUMS ? RING : SUMS];
+    constexpr int TB = FewLds<D, WAVES>::TB, OP = FewLds<D, WAVES>::OP;
 
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kvh = blockIdx.x % a.Hkv, piece = blockIdx.x / a.Hkv;
-    const FewItem it = few_item(a, piece, slots);
-    if (it.parts == 0) return;
     const int n = min(it.q.n, a.max_new), L = it.q.L, rows = n * a.G, past = L - it.q.n;
-    const int tiles = (L + kFewTile - 1) / kFewTile;
-    const int t0 = (int)((int64_t)it.part * tiles / it.parts), t1 = (int)((int64_t)(it.part + 1) * tiles / it.parts);
+    const int t0 = it.t0, t1 = it.t1;
 
     // ---- this wave's tiles: t0 + w, + 4, ...
-    const ConstInts table = (ConstInts)(uintptr_t)(a.table + (int64_t)it.s * a.table_stride);
+    const ConstInts table = (ConstInts)(uintptr_t)(a.table + (int64_t)it.q.s * a.table_stride);
     const int last_page = (L - 1) >> a.page_shift;
     const uint32_t qs = (uint32_t)(uintptr_t)(lds_char*)lds, ks = qs + (1 + 2 * w) * TB, vs = ks + TB;
     int koff[4], voff[4];                          // by row group: the swizzles repeat every 16 rows
@@ -341,13 +397,14 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
     auto issue_v = [&](int t) { issue(t, vs, a.v, a.v_nb_page, a.v_nb_head, a.v_nb_slot, voff); };
     int t = t0 + w;
     if (t < t1) fetch(t);
-    // the rows of Q, a quarter by each wave, laid out as K is; rows that are
+    // the rows of Q, a part by each wave, laid out as K is; rows that are
     // not there are row 0 again (no one reads their results)
     {
         const uint64_t qb = uniform64((uint64_t)(uintptr_t)a.q + (int64_t)it.q.q0 * a.q_nb_t + (int64_t)kvh * a.G * a.q_nb_h);
 #pragma unroll
-        for (int i = 0; i < NC / kFewWaves; ++i) {
-            const int c = w * (NC / kFewWaves) + i;
+        for (int i = 0; i < (NC + WAVES - 1) / WAVES; ++i) {
+            const int c = w + i * WAVES;
+            if (NC % WAVES && c >= NC) break;
             const int r = c * RC + lane / (D / 8), row = r < rows ? r : 0;
             const int rt = div_g(a, row), off = rt * (int)a.q_nb_t + (row - rt * a.G) * (int)a.q_nb_h;
             dma16<false>(qb, off + (((lane % (D / 8)) ^ k_swz<D>(r)) << 4), qs + c * 1024);
@@ -371,16 +428,16 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
-    for (; t < t1; t += kFewWaves) {
-        const bool more = t + kFewWaves < t1;
-        if (more) fetch(t + kFewWaves);
+    for (; t < t1; t += WAVES) {
+        const bool more = t + WAVES < t1;
+        if (more) fetch(t + WAVES);
         wait_vm<NC>();                             // K; V may still fly
         f32x16 s{};
 #pragma unroll
         for (int ds = 0; ds < DS; ++ds) s = F::mma(as_vec<QF>(lds_read((ks + k_off) ^ (ds << 5))), qf[ds], s);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // K is read
-            issue_k(t + kFewWaves);
+            issue_k(t + WAVES);
         }
         const int k0 = t * kFewTile;
         const bool masked = k0 + kFewTile - 1 > min(L - 1, past);      // some row must not see some key
@@ -425,14 +482,14 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
         if (fix) add_not_finite<D, KT, kFewTile>(vs, k0, lim, half, o);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // V is read
-            issue_v(t + kFewWaves);
+            issue_v(t + WAVES);
         }
     }
     // ---- the waves' sums, in LDS, added in wave order
     const float lt = add_swap32(lsum);
     __syncthreads();
     float* const ow = (float*)lds;
-    float* const ml = ow + kFewWaves * kFewRows * OP;
+    float* const ml = ow + WAVES * kFewRows * OP;
     if (l32 < rows) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -456,9 +513,13 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
         const int rt = div_g(args, row);
         *(uint2*)(args.out + (int64_t)(it.q.q0 + rt) * args.o_nb_t + (int64_t)(kvh * args.G + row - rt * args.G) * args.o_nb_h + 8 * c) = y;
     };
+    // A piece's place for its partial, by its number; in shares, where a
+    // workgroup may end one sequence and begin another, the workgroup's first, for
+    // a sequence's first piece its second
+    auto place = [&](int part) { return (SHARES ? 2 * (it.first + part) + (part == 0) : it.first + part) * args.Hkv + kvh; };
     auto piece_rsrc = [&](int part) {
         const uint32_t bytes = cap * (D + 2) * sizeof(float);
-        return make_rsrc((const char*)ws + ((int64_t)(it.first + part) * args.Hkv + kvh) * bytes, bytes);
+        return make_rsrc((const char*)ws + (int64_t)place(part) * bytes, bytes);
     };
     // agent-scope stores: coherent across the XCDs' L2 caches
     auto store = [&](int part, int row, int c, const Sum& x) {
@@ -469,14 +530,14 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
             __builtin_amdgcn_raw_buffer_store_b64(u32x2{nan ? kNanBits : __float_as_uint(x.M), __float_as_uint(x.den)}, rs,
                                                   (cap * D + row * 2) * 4, 0, kSc1);
     };
-    for (int i = tid; i < rows * (D / 4); i += kFewWaves * 64) {
+    for (int i = tid; i < rows * (D / 4); i += WAVES * 64) {
         const int row = i / (D / 4), c = i % (D / 4);
         Sum x{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
 #pragma unroll
-        for (int k = 0; k < kFewWaves; ++k) x.M = fmaxf(x.M, ml[(k * kFewRows + row) * 2]);
+        for (int k = 0; k < WAVES; ++k) x.M = fmaxf(x.M, ml[(k * kFewRows + row) * 2]);
         const float base = x.M == -INFINITY ? 0.0f : x.M;
 #pragma unroll
-        for (int k = 0; k < kFewWaves; ++k) {
+        for (int k = 0; k < WAVES; ++k) {
             const float f = __builtin_amdgcn_exp2f(ml[(k * kFewRows + row) * 2] - base);   // 0 for a wave without keys
             const float4 v = *(const float4*)(ow + (k * kFewRows + row) * OP + 4 * c);
             x.den = fmaf(f, ml[(k * kFewRows + row) * 2 + 1], x.den);
@@ -494,7 +555,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
     // overwrites where it alone has read them (a row's exponent: its wave).
     const int size = it.parts <= 2 * kMergeBatch ? 2 * kMergeBatch : kMergeBatch, grp = it.part / size;
     const int groups = (it.parts + size - 1) / size;
-    unsigned* tk = tickets + kFewTickets + (it.first + grp * size) * args.Hkv + kvh;
+    unsigned* tk = tickets + kFewTickets + place(grp * size);
     int first = grp * size, by = 1, n_add = min(size, it.parts - first);
 #pragma unroll 1
     for (int level = 0; level < 2; ++level) {
@@ -511,7 +572,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
             __syncthreads();
             if (!*last) return;
 #pragma unroll 1
-            for (int i = tid; i < rows * (D / 4); i += kFewWaves * 64) {
+            for (int i = tid; i < rows * (D / 4); i += WAVES * 64) {
                 const int row = i / (D / 4), c = i % (D / 4);
                 Sum x{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
 #pragma unroll 1
@@ -560,11 +621,20 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs 
             }
         }
         if (final) return;
-        tk = tickets + it.s * args.Hkv + kvh;
+        tk = tickets + place(0);
         first = 0;
         by = size;
         n_add = groups;
     }
+}
+
+// One workgroup per (piece, kv head), two of them (D = 64: four) on a CU.
+template <int D, int KT>
+__global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets, int slots, int cap) {
+    prefetch_kernargs<sizeof(PagedArgs)>();
+    __shared__ __attribute__((aligned(1024))) char lds[FewLds<D, kFewWaves>::BYTES];
+    const FewItem it = few_item(a, blockIdx.x / a.Hkv, slots, kFewWaves);
+    if (it.parts > 0) few_piece<D, KT, kFewWaves, false>(a, ws, tickets, cap, it, blockIdx.x % a.Hkv, lds);
 }
 
 // ----------------------------------------------------------- many rows
@@ -576,7 +646,6 @@ constexpr int kRowsWG = kRowsWave * kWaves;
 constexpr int kStages = 4;         // LDS ring: tile j + 3 loads while tile j is computed
 constexpr int kRowTileCost = 4;    // what a row tile costs beside its keys, in key tiles
 constexpr int kSnap = 3;           // cuts this near an end of a row tile, in key tiles, are moved there
-constexpr int kMaxWgs = 256;       // workgroups of a call at most
 constexpr int kGroup = 8;          // pieces whose partials are added at once
 constexpr int kManyTickets = kMaxWgs * kWaves * (1 + kMaxWgs / kGroup);
 
@@ -609,13 +678,6 @@ __device__ __forceinline__ ManyWeight many_weight(const PagedArgs& a, const Seq&
     w.first = max((max(q.L - q.n, 0) / (kBN / 16) + 16 * kRowTileCost) >> shift, 1);
     w.slope = slope >> shift;
     return w;
-}
-// p / n for a uniform p >= 0 whose quotient a float holds
-__device__ __forceinline__ int part_of(int p, int n) {
-    int k = uni((int)((float)p * __builtin_amdgcn_rcpf((float)n))), r = p - k * n;   // within one or two of it
-    while (r < 0) --k, r += n;
-    while (r >= n) ++k, r -= n;
-    return k;
 }
 struct ManyAxis {
     int slope;              // of a row tile, in sixteenths
@@ -678,16 +740,31 @@ __device__ __forceinline__ ManySeq many_seq(const PagedArgs& a, const ManyAxis& 
     return r;
 }
 
-// One workgroup per share of the work: 8 waves x 32 rows that share every K / V
-// tile.  A row tile that lies in one share is written at once; of one that
+// The shares of the work, n at most.  A row tile of t key tiles cut into n
+// parts takes about t / n of them, and a part of one more per piece to add:
+// shares are not below 0.6 times the square root of the average t and what a
+// row tile costs (256 tokens behind 4096 keys, 28 row tiles: 51.6 us with
+// shares of 4 tiles, 47.8 with 8).
+__device__ __forceinline__ int many_shares(const PagedArgs& a, const ManyAxis& axis, int n) {
+    const float tile = 16.0f * __builtin_amdgcn_rcpf((float)(1 << axis.shift));
+    const float mean = fmaxf((float)axis.head * __builtin_amdgcn_rcpf((float)axis.row_tiles * tile) - (float)kRowTileCost, 1.0f);
+    const float least = ((float)kRowTileCost + 0.6f * __builtin_amdgcn_sqrtf(mean)) * tile;
+    return uni(max(1, min(n, (int)((float)(axis.head * a.Hkv) * __builtin_amdgcn_rcpf(least)))));
+}
+
+// Share `block` of `wgs`, by one workgroup: 8 waves x 32 rows that share every
+// K / V tile.  A row tile that lies in one share is written at once; of one that
 // several workgroups share, each leaves its rows' sums in the workspace, wave
 // by wave ([wave][16-byte group][lane], then (exponent base, row sum)), and
 // takes the wave's ticket: the last of up to kGroup pieces adds them, and of
 // more groups the last adds the groups, in the order of the keys whoever it is
 // (its own sums are read back too, so that they need no registers meanwhile).
+template <int D>
+struct ManyLds {
+    static constexpr int BYTES = kStages * 2 * kBN * 2 * D;
+};
 template <int D, int KT>
-__global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets) {
-    prefetch_kernargs<sizeof(PagedArgs)>();
+__device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, const ManyAxis& axis, const Seq& mine, int block, int wgs, char* lds, int* marks) {
     using F = Frag<KT>;
     using QF = typename F::type;
     constexpr int DS = D / 16, DT = D / 32;
@@ -699,56 +776,24 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     constexpr int NLD = 2 * NI;
     constexpr int WAVE_O = DT * 16 * 64 * 4;       // bytes of a wave's sums
     constexpr int WAVE = WAVE_O + 64 * 8;
-    __shared__ __attribute__((aligned(1024))) char lds[kStages * STAGE];
-    __shared__ int fix, bad_seg;                   // the last tile with a V that is not finite, the last share with a bad page
+    int& fix = marks[0];                           // the last tile with a V that is not finite
+    int& bad_seg = marks[1];                       // the last share with a bad page
 
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (threadIdx.x == 0) fix = bad_seg = -1;      // before the first tile's barrier
     ManySeq sq{};                                  // the sequence at hand, and its end on the axis
     int sq_kvh = 0, sq_end = -1;
-    int head, axis_shift, axis_slope;
-    int g, wgs, share, total;
-    {
-    const Seq mine = seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1));
-    const ManyAxis axis = many_axis(a, mine);
-    head = axis.head;
-    axis_shift = axis.shift;
-    axis_slope = axis.slope;
-    if (head <= 0) return;
-    total = head * a.Hkv;
-    // A row tile of t key tiles cut into n parts takes about t / n of them, and
-    // a part of one more per piece to add: shares are not below 0.6 times the
-    // square root of the average t and what a row tile costs (256 tokens behind
-    // 4096 keys, 28 row tiles: 51.6 us with shares of 4 tiles, 47.8 with 8).
-    const float tile = 16.0f * __builtin_amdgcn_rcpf((float)(1 << axis.shift));
-    const float mean = fmaxf((float)head * __builtin_amdgcn_rcpf((float)axis.row_tiles * tile) - (float)kRowTileCost, 1.0f);
-    const float least = ((float)kRowTileCost + 0.6f * __builtin_amdgcn_sqrtf(mean)) * tile;
-    wgs = uni(max(1, min((int)gridDim.x, (int)((float)total * __builtin_amdgcn_rcpf(least)))));
-    if ((int)blockIdx.x >= wgs) return;
+    const int head = axis.head, axis_shift = axis.shift, axis_slope = axis.slope, total = head * a.Hkv;
     // neighbouring shares on one XCD (workgroups go round its 8): they read the same keys
-    g = wgs % 8 == 0 ? (int)(blockIdx.x % 8) * (wgs / 8) + (int)(blockIdx.x / 8) : (int)blockIdx.x;
-    share = uni((int)((float)total * 1.000001f * __builtin_amdgcn_rcpf((float)wgs)) + 1);      // share * wgs >= total
+    const int g = wgs % 8 == 0 ? (block % 8) * (wgs / 8) + block / 8 : block;
+    const int share = uni((int)((float)total * 1.000001f * __builtin_amdgcn_rcpf((float)wgs)) + 1);      // share * wgs >= total
+    {
     const int p = min(g * share, total - 1);
     sq_kvh = part_of(p, head);
     sq = many_seq(a, axis, mine, p - sq_kvh * head);
     sq_end = sq_kvh * head + sq.end;
     }
-    // Where the cut at place b, inside the row tile [x, x + len), falls: a cut
-    // near one of its ends is moved there.
-    const int snap = max(1, min(share / 2, (16 * kSnap) >> axis_shift));
-    auto cut = [&](int b, int x, int len) {
-        const int l = b - x, r = x + len - b;
-        return l < snap && l <= r ? x : (r < snap ? x + len : b);
-    };
-    // the first and the last workgroup of the row tile [x, x + len)
-    auto first_of = [&](int x, int len) {
-        const int k = part_of(x, share), b = (k + 1) * share;
-        return min(wgs - 1, b < x + len && cut(b, x, len) == x ? k + 1 : k);
-    };
-    auto final_of = [&](int x, int len) {
-        const int k = part_of(x + len - 1, share), b = k * share;
-        return min(wgs - 1, b > x && cut(b, x, len) == x + len ? k - 1 : k);
-    };
+    const Shares cuts{share, wgs, max(1, min(share / 2, (16 * kSnap) >> axis_shift))};
     const int p_end = min(total, (g + 1) * share);
     const float inv_g = uni(1.0f / (float)a.G);
 
@@ -787,8 +832,8 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
         c.past = sq.q.L - sq.q.n;
         c.len = wt.of(rt);
         c.place = p - (ps - wt.before(rt));
-        const int off = (begin ? cut(p, c.place, c.len) : p) - c.place;
-        const int off_end = (p_end < c.place + c.len ? cut(p_end, c.place, c.len) : c.place + c.len) - c.place;
+        const int off = (begin ? cuts.cut(p, c.place, c.len) : p) - c.place;
+        const int off_end = (p_end < c.place + c.len ? cuts.cut(p_end, c.place, c.len) : c.place + c.len) - c.place;
         c.whole = off <= 0 && off_end == c.len;
         c.empty = off_end <= off;                  // the share begins with the next row tile, or ended with the last
         c.next = c.place + max(c.empty ? off : off_end, 1);
@@ -1076,7 +1121,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     bool nan = c.n_tiles > 0 && *(volatile __attribute__((address_space(3))) int*)&bad_seg == seg;
     bool done = true;
     if (!c.whole) {
-        const int g0 = first_of(c.place, c.len), pieces = final_of(c.place, c.len) - g0 + 1;
+        const int g0 = cuts.first_of(c.place, c.len), pieces = cuts.final_of(c.place, c.len) - g0 + 1;
         // piece k's slot: workgroup g0's second, the others' first
         auto piece_rsrc = [&](int k) {
             const int slot = k == 0 ? 2 * g0 + 1 : 2 * min(g0 + k, wgs - 1);
@@ -1182,21 +1227,120 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
 }
 
 template <int D, int KT>
-hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s) {
-    hipError_t e = hipSuccess;
-    if (p.many_wgs > 0) {
-        hipLaunchKernelGGL((paged_many_kernel<D, KT>), dim3(p.many_wgs), dim3(kWaves * 64), 0, s, a, ws, tickets);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
-    if (p.few_pieces > 0) {
-        hipLaunchKernelGGL((paged_few_kernel<D, KT>), dim3(p.few_pieces * a.Hkv), dim3(kFewWaves * 64), 0, s, a, ws, tickets, p.few_slots, p.few_cap);
-        e = hipGetLastError();
-    }
-    return e;
+__global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets) {
+    prefetch_kernargs<sizeof(PagedArgs)>();
+    __shared__ __attribute__((aligned(1024))) char lds[ManyLds<D>::BYTES];
+    __shared__ int marks[2];
+    const Seq mine = seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1));
+    const ManyAxis axis = many_axis(a, mine);
+    if (axis.head <= 0) return;
+    const int wgs = many_shares(a, axis, gridDim.x);
+    if ((int)blockIdx.x < wgs) many_share<D, KT>(a, ws, tickets, axis, mine, blockIdx.x, wgs, lds, marks);
 }
 
-// (n_seq + 1) * Hkv <= kFewTickets (the caller); pieces * Hkv: at most that and the workgroups at once
-static_assert(kManyTickets <= kMaxPagedTickets && 2 * kFewTickets + 4 * kMaxWgs <= kMaxPagedTickets, "the context holds the tickets");
+// Few rows beside many: share `item / Hkv` of kv head item % Hkv, the axis cut
+// into at most `slots` equal shares, of a tile per wave and a piece's cost at
+// least.  The workgroups are fewer than the pieces here, so that even work
+// counts for more than what a cut costs (60 sequences of up to 8000 keys beside
+// 700 tokens: 159 us with whole pieces by turns, 97 so).  False: no share.
+template <int D, int KT>
+__device__ __forceinline__ bool few_share(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, int cap, int item, int slots, int axis, const Seq& mine, char* lds) {
+    const int n = max(1, min(slots, axis / (kWaves + kFewCost)));
+    const Shares cuts{(axis + n - 1) / n, n, max(kFewCost + 1, min(kFewSnap, (axis + n - 1) / n / 2))};
+    const int g = item / a.Hkv, kvh = item - g * a.Hkv;
+    const int p_end = min(axis, (g + 1) * cuts.share);
+    if (g >= n) return false;
+    const int lane = threadIdx.x & 63;
+    bool begin = true;
+    int base = 0, block = -64, end = 0, len = 0;   // 64 sequences from `block` on: where each ends
+    Seq q{};
+    for (int p = g * cuts.share; p < p_end;) {
+        uint64_t hit;
+        while (!(hit = __ballot(p >= end - len && p < end))) {
+            block += 64;
+            if (block >= a.n_seq) return true;     // a batch that changed meanwhile
+            if (block > 0) base = lane_of(end, 63);
+            q = block > 0 ? seq_of(a, min(block + lane, a.n_seq - 1)) : mine;
+            len = block + lane < a.n_seq ? few_weight(a, q) : 0;
+            end = base + wave_scan(len);
+        }
+        const int l = __ffsll((unsigned long long)hit) - 1;
+        const int size = lane_of(len, l), x = lane_of(end, l) - size;
+        FewItem it;
+        it.q.q0 = lane_of(q.q0, l);
+        it.q.n = lane_of(q.n, l);
+        it.q.L = lane_of(q.L, l);
+        it.q.s = block + l;
+        const int off = (begin ? cuts.cut(p, x, size) : p) - x;
+        const int off_end = (p_end < x + size ? cuts.cut(p_end, x, size) : x + size) - x;
+        begin = false;
+        p = x + size;
+        if (off_end <= off) continue;              // moved past its end, or its end to here
+        it.first = off > 0 || off_end < size ? cuts.first_of(x, size) : g;
+        it.parts = off > 0 || off_end < size ? cuts.final_of(x, size) - it.first + 1 : 1;
+        it.part = g - it.first;
+        it.t0 = max(0, off - kFewCost);            // a cut is more than kFewCost from the ends, or at one
+        it.t1 = min(off_end - kFewCost, (it.q.L + kFewTile - 1) / kFewTile);   // no keys: none
+        few_piece<D, KT, kWaves, true>(a, ws, tickets, cap, it, kvh, lds);
+        __syncthreads();                           // the next piece's rows of Q go where this one's sums are
+    }
+    return true;
+}
+
+// Sequences of both kinds in one launch of a workgroup per CU: the first take
+// shares of the many rows' work, the others of the few rows', as many as the
+// times of both kinds say (on the device, from the batch).  So the bytes of the
+// one come while the matrix cores work on the other, and no launch waits.
+// Against the two kernels one after the other: 64 x 4096 keys and 512 tokens
+// behind 4096 142 -> 109 us, 23 x 2000 and 512 tokens 50 -> 35, prompts of 40 to
+// 1100 tokens (no few rows) 40 -> 38; 8 x 1024 alone in a call that could have
+// brought more 10 -> 13, 64 x 4096 alone 90 -> 85.
+// Time of a few-row tile to that of a key tile of a row tile (0.16 and 0.22: D =
+// 64, 64 x 2000 keys and 512 tokens 21.9 and 25.4 us; D = 128, 60 sequences of up
+// to 8000 and 700 behind 2000 105 and 97):
+template <int D>
+constexpr float kFewTime = D == 64 ? 0.16f : 0.22f;
+template <int D, int KT>
+__global__ void __launch_bounds__(kWaves * 64) paged_mixed_kernel(PagedArgs a, float* __restrict__ ws, float* __restrict__ few_ws, unsigned* tickets, int cap) {
+    prefetch_kernargs<sizeof(PagedArgs)>();
+    constexpr int FEW = FewLds<D, kWaves>::BYTES;
+    __shared__ __attribute__((aligned(1024))) char lds[ManyLds<D>::BYTES > FEW ? ManyLds<D>::BYTES : FEW];
+    __shared__ int marks[2];
+    const Seq mine = seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1));
+    const ManyAxis axis = many_axis(a, mine);
+    const int few = few_axis(a, mine);
+    int wgs = 0;
+    if (axis.head > 0) {
+        const float many = (float)(axis.head * a.Hkv) * (float)(1 << axis.shift) * (1.0f / 16), rest = kFewTime<D> * (float)few * (float)a.Hkv;
+        const int n = (int)((float)gridDim.x * many * __builtin_amdgcn_rcpf(many + rest) * (1.0f / 8) + 0.5f) * 8;
+        wgs = many_shares(a, axis, max(min(8, (int)gridDim.x - 1), min(n, (int)gridDim.x - (few > 0 ? 8 : 0))));
+        if ((int)blockIdx.x < wgs) {
+            many_share<D, KT>(a, ws, tickets, axis, mine, blockIdx.x, wgs, lds, marks);
+            return;
+        }
+    }
+    if (few == 0) return;
+    const int slots = max(1, ((int)gridDim.x - wgs) / a.Hkv);
+    for (int i = blockIdx.x - wgs; few_share<D, KT>(a, few_ws, tickets + kManyTickets, cap, i, slots, few, mine, lds);) i += gridDim.x - wgs;
+}
+
+size_t many_ws_bytes(const PagedArgs& a, const PagedPlan& p) {
+    return (size_t)p.many_wgs * 2 * kWaves * (a.d * kRowsWave * sizeof(float) + 64 * 8);
+}
+
+template <int D, int KT>
+hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s) {
+    if (p.many_wgs > 0 && p.few_pieces > 0) {
+        hipLaunchKernelGGL((paged_mixed_kernel<D, KT>), dim3(p.many_wgs), dim3(kWaves * 64), 0, s, a, ws, (float*)((char*)ws + many_ws_bytes(a, p)), tickets, p.few_cap);
+    } else if (p.many_wgs > 0) {
+        hipLaunchKernelGGL((paged_many_kernel<D, KT>), dim3(p.many_wgs), dim3(kWaves * 64), 0, s, a, ws, tickets);
+    } else {
+        hipLaunchKernelGGL((paged_few_kernel<D, KT>), dim3(p.few_pieces * a.Hkv), dim3(kFewWaves * 64), 0, s, a, ws, tickets, p.few_slots, p.few_cap);
+    }
+    return hipGetLastError();
+}
+
+static_assert(kManyTickets + 2 * kFewTickets <= kMaxPagedTickets, "the context holds the tickets");
 
 }  // namespace
 
@@ -1211,7 +1355,7 @@ PagedPlan paged_plan(const PagedArgs& a, int n_cu) {
     // kernel is launched, which takes any others as well (a batch padded to its
     // token rows).
     const bool even = (int64_t)a.n_seq * a.max_new == a.n_tok;
-    if (rows > kFewRows) p.many_wgs = std::min(n_cu, kMaxWgs);
+    if (rows > kFewRows) p.many_wgs = std::max(16, std::min(n_cu, kMaxWgs));   // 8 for each kind at least
     if (rows <= kFewRows || !even) {
         p.few_cap = (int)std::min<int64_t>(rows, kFewRows);
         // Half the workgroups that fit a CU, so that fewer partials are added and
@@ -1221,15 +1365,15 @@ PagedPlan paged_plan(const PagedArgs& a, int n_cu) {
         const int slots = std::min(n_cu, kMaxWgs) * (a.d == 64 ? 2 : 1);
         p.few_slots = std::max(1, (2 * a.n_seq * a.Hkv > slots ? 2 : 1) * slots / a.Hkv);
         const int64_t seq_tiles = (max_keys + kFewTile - 1) / kFewTile;
-        p.few_split = seq_tiles > kFewMin;
-        p.few_pieces = (int)std::min<int64_t>(p.few_slots + (int64_t)a.n_seq, a.n_seq * ((seq_tiles + kFewMin - 1) / kFewMin));
+        p.few_split = seq_tiles > kFewWaves;
+        p.few_pieces = (int)std::min<int64_t>(p.few_slots + (int64_t)a.n_seq, a.n_seq * ((seq_tiles + kFewWaves - 1) / kFewWaves));
     }
     return p;
 }
 size_t paged_ws_bytes(const PagedArgs& a, const PagedPlan& p) {
-    const size_t many = (size_t)p.many_wgs * 2 * kWaves * (a.d * kRowsWave * sizeof(float) + 64 * 8);
-    const size_t few = p.few_split ? (size_t)p.few_pieces * a.Hkv * p.few_cap * (a.d + 2) * sizeof(float) : 0;
-    return std::max(many, few);                    // one after the other on the stream
+    // beside many rows: two places per share
+    const size_t places = p.many_wgs > 0 ? (size_t)2 * std::max(p.many_wgs, a.Hkv) : (size_t)p.few_pieces * a.Hkv;
+    return many_ws_bytes(a, p) + (p.few_split ? places * p.few_cap * (a.d + 2) * sizeof(float) : 0);
 }
 
 hipError_t launch_paged_attn(PagedArgs a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s) {

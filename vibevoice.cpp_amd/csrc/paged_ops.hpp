@@ -6,9 +6,11 @@
 struct Seq {
     int q0, n;          // first token row, new tokens
     int L;              // keys
+    int s;              // its index
 };
 __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int s) {
     Seq r;
+    r.s = s;
     r.q0 = min(max(a.q_start[s], 0), a.n_tok);
     r.n = min(max(a.q_start[s + 1], r.q0), a.n_tok) - r.q0;
     r.L = min(max(a.kv_len[s], 0), a.max_pages << a.page_shift);

@@ -237,14 +237,14 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s);
 // (upper bounds; paged_attn.hip)
 struct PagedPlan {
     int many_wgs;                              // workgroups of paged_many_kernel (0: no launch)
-    int few_pieces, few_slots, few_cap;        // pieces per kv head (0: no launch), how many run at once, rows of a partial
+    int few_pieces, few_slots, few_cap;        // few rows: pieces per kv head (0: none), how many run at once, rows of a partial
     bool few_split;                            // whether pieces may leave partials
 };
 PagedPlan paged_plan(const PagedArgs& a, int n_cu);
 size_t paged_ws_bytes(const PagedArgs& a, const PagedPlan& p);
-// tickets: [kMaxPagedTickets], zero between launches; n_seq * Hkv <= kMaxPagedSeqHeads
+// tickets: [kMaxPagedTickets], zero between launches; (n_seq + 1) * Hkv <= kMaxPagedSeqHeads
 constexpr int kMaxPagedSeqHeads = 65536;
-constexpr int kMaxPagedTickets = 2 * kMaxPagedSeqHeads + 1024;
+constexpr int kMaxPagedTickets = 256 * 8 * 33 + 2 * (kMaxPagedSeqHeads + 1024);
 hipError_t launch_paged_attn(PagedArgs a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s);
 hipError_t launch_norm(const NormArgs& a, hipStream_t s);
 
