@@ -327,7 +327,8 @@ VVA_API vva_status vva_out_proj_residual(vva_context* ctx, const vva_tensor* o, 
  *            i % page_size.  Entries past a sequence's keys are not read.
  *   max_new: no sequence of the call brings more new tokens (the rows of one
  *            that does are computed up to here).
- * n_seq <= VVA_MAX_BATCH_SEQ.  Values that point outside are kept inside:
+ * n_seq <= VVA_MAX_BATCH_SEQ.  The tensors must not change while a call runs
+ * (write them in stream order).  Values that point outside are kept inside:
  * q_start is cut to the token rows there are, kv_len to the table's row. */
 typedef struct {
     vva_tensor q_start;
