@@ -201,7 +201,8 @@ RAGGED = [(1, (97 * i) % 401) for i in range(100)] + [(90, 500), (0, 9), (40, 77
     (RAGGED, H7, 0), (RAGGED, H05, 0), ([(1, 20000), (2, 7000), (200, 300)], H7, 0), ([(1, 40), (300, 6000), (1, 1)], H05, 0),
     ([(1, 9000), (1, 3), (2, 70)], H7, 40), ([(1, 64 * i + 1) for i in range(30)], H15, 64),
     ([(1, 300), (1, 70), (50, 80), (4, 4)], (300, 300, 64), 0), ([(1, 5000), (40, 900)], (8, 8, 128), 0),
-    ([(1, 32 * i) for i in range(1, 9)] + [(33, 33)], H05, 0),
+    ([(1, 32 * i) for i in range(1, 9)] + [(33, 33)], H05, 0), ([(2500, 2500)], H05, 0), ([(700, 900), (800, 800), (90, 90)], (32, 1, 64), 0),
+    ([(9, 2683)] * 3, H7, 0), ([(64, 4160)], H7, 0), ([(40, 40), (7, 7), (300, 310), (0, 8), (33, 1000)], H15, 0), ([(60, 0), (50, 20)], H7, 0),
 ])
 def test_few_rows_beside_many(ctx, torch_gpu, lens, heads, max_new):
     print(lens[:3], heads, max_new, flush=True)

@@ -712,7 +712,7 @@ __device__ __forceinline__ ManyAxis many_axis(const PagedArgs& a, const Seq& min
 // The sequence at place p of a kv head's part, and where it starts and ends
 struct ManySeq {
     Seq q;
-    int s, start, end;
+    int start, end;
 };
 __device__ __forceinline__ ManySeq many_seq(const PagedArgs& a, const ManyAxis& x, const Seq& mine, int p) {
     const int lane = threadIdx.x & 63;
@@ -730,7 +730,7 @@ __device__ __forceinline__ ManySeq many_seq(const PagedArgs& a, const ManyAxis& 
             r.q.q0 = lane_of(q.q0, l);
             r.q.n = lane_of(q.n, l);
             r.q.L = lane_of(q.L, l);
-            r.s = i + l;
+            r.q.s = i + l;
             r.end = lane_of(end, l);
             r.start = r.end - lane_of(len, l);
             return r;
@@ -752,7 +752,117 @@ __device__ __forceinline__ int many_shares(const PagedArgs& a, const ManyAxis& a
     return uni(max(1, min(n, (int)((float)(axis.head * a.Hkv) * __builtin_amdgcn_rcpf(least)))));
 }
 
-// Share `block` of `wgs`, by one workgroup: 8 waves x 32 rows that share every
+// The share of a workgroup: neighbouring shares on one XCD (workgroups go round
+// its 8), since they read the same keys (252 shares of 256 tokens behind 4096
+// keys 44 us by turns, 38 so).
+__device__ __forceinline__ int on_xcds(int block, int wgs) {
+    const int x = block % 8;
+    return x * (wgs / 8) + min(x, wgs % 8) + block / 8;
+}
+
+// The other way to cut, for calls of few row tiles: each into equal parts of at
+// most S key tiles, a part per workgroup.
+struct ManyPieces {
+    int head;               // parts of a kv head, 0: equal shares
+    Seq q;                  // the workgroup's row tile
+    int rt, kvh, first, parts;  // its parts are `first` .. of all; how many
+};
+// Where the row tiles are no more than the workgroups (n), S is the least for
+// which the parts are not either: tried up in steps of an eighth from the even
+// length or, where that is longer, what a cut is worth (kPieceLeast, and
+// kPieceRoot times the root of the longest row tile, as each part is one more to
+// add).  A share that crosses a row tile's end costs its workgroup a second
+// opening and more sums, about kPieceGain key tiles of time; against it stand
+// the workgroups that parts of one length leave idle, so that parts longer by
+// more than that are left to the shares.  Shares against parts, us: 1.5B heads,
+// a prompt of 700 tokens 29.6 and 22.4; 7B, 4 prompts of up to 1000 38.3 and 33.9, 64
+// tokens behind 4096 keys 42 and 34, 128 behind 8192 51 and 40; 0.5B, 4096 tokens
+// (28 key tiles a share) 51.1 and 52.6.  By whole waves.
+constexpr int kPieceGain = 9;
+constexpr int kPieceMost = 16;     // shares longer than this, in key tiles, are not worth the look
+constexpr float kPieceLeast = 4.0f, kPieceRoot = 1.1f;
+__device__ __forceinline__ ManyPieces many_pieces(const PagedArgs& a, const ManyAxis& axis, const Seq& mine, int n, int block) {
+    constexpr int CH = 4;   // row tiles of a lane
+    const int lane = threadIdx.x & 63;
+    const int slots = part_of(n, a.Hkv);
+    ManyPieces m{};
+    // (key tiles of a share)
+    const float mean = (float)axis.head * (float)(1 << axis.shift) * (1.0f / 16) - (float)kRowTileCost * (float)axis.row_tiles;
+    if (a.n_seq > 64 || axis.row_tiles > min(slots, 64 * CH) || mean > (float)kPieceMost * (float)slots) return m;
+    const int r = lane < a.n_seq ? many_row_tiles(a, mine) : 0;
+    const int end = wave_scan(r);
+    int tiles[CH] = {}, total = 0;
+    for (uint64_t left = __ballot(r > 0); left; left &= left - 1) {
+        const int l = __ffsll((unsigned long long)left) - 1;
+        const Seq q{lane_of(mine.q0, l), lane_of(mine.n, l), lane_of(mine.L, l), l};
+        const int e = lane_of(end, l), b = e - lane_of(r, l);
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+            if (64 * k >= e || 64 * (k + 1) <= b) continue;
+            const int i = 64 * k + lane;
+            if (i >= b && i < e) tiles[k] = max(1, many_key_tiles(a, q, i - b));
+        }
+    }
+    float most = 0.0f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+        total += tiles[k];
+        most = fmaxf(most, (float)tiles[k]);
+    }
+    total = wave_total(total);
+    most = fmaxf(most, dpp<kDppXor1>(most));
+    most = fmaxf(most, dpp<kDppXor2>(most));
+    most = fmaxf(most, dpp<kDppHalfMirror>(most));
+    most = fmaxf(most, dpp<kDppMirror>(most));
+    most = uni(max_swap32(max_swap16(most)));
+    const int even = part_of(total + slots - 1, slots);
+    const int floor = uni((int)fmaxf(kPieceLeast, kPieceRoot * __builtin_amdgcn_sqrtf(most)));
+    int S = max(even, floor);
+    int parts[CH];
+    auto count = [&] {
+        const float inv = __builtin_amdgcn_rcpf((float)S);
+        int c = 0;
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+            parts[k] = 0;
+            if (k > 0 && axis.row_tiles <= 64 * k) continue;
+            parts[k] = tiles[k] > 0 ? max(1, (int)__builtin_ceilf((float)tiles[k] * inv - 0.01f)) : 0;
+            c += parts[k];
+        }
+        return wave_total(c);
+    };
+    int c = count();
+    for (const int limit = S + kPieceGain; c > slots;) {
+        S += (S + 7) / 8;
+        if (S > limit) return m;
+        c = count();
+    }
+    m.head = c;
+    const int wgs = c * a.Hkv;
+    if (block >= wgs) return m;
+    const int g = on_xcds(block, wgs);
+    m.kvh = part_of(g, c);
+    const int p = g - m.kvh * c;
+    int base = 0, i = 0;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+        const int to = base + wave_scan(parts[k]);
+        const uint64_t hit = __ballot(p >= to - parts[k] && p < to);
+        if (hit) {
+            const int l = __ffsll((unsigned long long)hit) - 1;
+            m.parts = lane_of(parts[k], l);
+            m.first = m.kvh * c + lane_of(to, l) - m.parts;
+            i = 64 * k + l;
+        }
+        base = lane_of(to, 63);
+    }
+    const int l = __ffsll((unsigned long long)__ballot(r > 0 && i < end && i >= end - r)) - 1;
+    m.q = Seq{lane_of(mine.q0, l), lane_of(mine.n, l), lane_of(mine.L, l), l};
+    m.rt = i - lane_of(end - r, l);
+    return m;
+}
+
+// Share `block` of `wgs`, or a part (parts.head > 0), by one workgroup: 8 waves x 32 rows that share every
 // K / V tile.  A row tile that lies in one share is written at once; of one that
 // several workgroups share, each leaves its rows' sums in the workspace, wave
 // by wave ([wave][16-byte group][lane], then (exponent base, row sum)), and
@@ -764,7 +874,7 @@ struct ManyLds {
     static constexpr int BYTES = kStages * 2 * kBN * 2 * D;
 };
 template <int D, int KT>
-__device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, const ManyAxis& axis, const Seq& mine, int block, int wgs, char* lds, int* marks) {
+__device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, const ManyAxis& axis, const ManyPieces& pc, const Seq& mine, int block, int wgs, char* lds, int* marks) {
     using F = Frag<KT>;
     using QF = typename F::type;
     constexpr int DS = D / 16, DT = D / 32;
@@ -783,17 +893,22 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
     if (threadIdx.x == 0) fix = bad_seg = -1;      // before the first tile's barrier
     ManySeq sq{};                                  // the sequence at hand, and its end on the axis
     int sq_kvh = 0, sq_end = -1;
-    const int head = axis.head, axis_shift = axis.shift, axis_slope = axis.slope, total = head * a.Hkv;
-    // neighbouring shares on one XCD (workgroups go round its 8): they read the same keys
-    const int g = wgs % 8 == 0 ? (block % 8) * (wgs / 8) + block / 8 : block;
-    const int share = uni((int)((float)total * 1.000001f * __builtin_amdgcn_rcpf((float)wgs)) + 1);      // share * wgs >= total
-    {
-    const int p = min(g * share, total - 1);
-    sq_kvh = part_of(p, head);
-    sq = many_seq(a, axis, mine, p - sq_kvh * head);
-    sq_end = sq_kvh * head + sq.end;
+    // parts lie on an axis of their own, a unit each, in shares of one
+    const bool whole_parts = pc.head > 0;
+    const int head = whole_parts ? pc.head : axis.head, axis_shift = axis.shift, axis_slope = axis.slope, total = head * a.Hkv;
+    const int g = on_xcds(block, wgs);
+    const int share = whole_parts ? 1 : uni((int)((float)total * 1.000001f * __builtin_amdgcn_rcpf((float)wgs)) + 1);      // share * wgs >= total
+    if (whole_parts) {
+        sq.q = pc.q;
+        sq_kvh = pc.kvh;
+        sq_end = total;
+    } else {
+        const int p = min(g * share, total - 1);
+        sq_kvh = part_of(p, head);
+        sq = many_seq(a, axis, mine, p - sq_kvh * head);
+        sq_end = sq_kvh * head + sq.end;
     }
-    const Shares cuts{share, wgs, max(1, min(share / 2, (16 * kSnap) >> axis_shift))};
+    const Shares cuts{share, wgs, whole_parts ? 0 : max(1, min(share / 2, (16 * kSnap) >> axis_shift))};
     const int p_end = min(total, (g + 1) * share);
     const float inv_g = uni(1.0f / (float)a.G);
 
@@ -814,24 +929,29 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
             sq = many_seq(a, ManyAxis{axis_slope, axis_shift, head}, seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1)), p - sq_kvh * head);
             sq_end = sq.end > sq.start ? sq_kvh * head + sq.end : p_end;   // no sequence: a batch that changed meanwhile
         }
+        int rt = pc.rt;
+        c.len = pc.parts;
+        c.place = pc.first;
+        if (!whole_parts) {
         ManyWeight wt = many_weight(a, sq.q, axis_slope, axis_shift);
         wt.r = uni(wt.r);
         const int ps = p - sq_kvh * head - sq.start;           // place in the sequence
         const float s2 = 0.5f * (float)wt.slope, f1 = (float)wt.first + s2;
-        int rt = (int)(wt.slope > 0 ? (__builtin_amdgcn_sqrtf(f1 * f1 + 4.0f * s2 * (float)ps) - f1) * __builtin_amdgcn_rcpf(2.0f * s2)
+        rt = (int)(wt.slope > 0 ? (__builtin_amdgcn_sqrtf(f1 * f1 + 4.0f * s2 * (float)ps) - f1) * __builtin_amdgcn_rcpf(2.0f * s2)
                                     : (float)ps * __builtin_amdgcn_rcpf((float)wt.first));
         rt = uni(max(0, min(rt, wt.r - 1)));
         while (rt > 0 && wt.before(rt) > ps) --rt;
         while (rt + 1 < wt.r && wt.before(rt + 1) <= ps) ++rt;
+        c.len = wt.of(rt);
+        c.place = p - (ps - wt.before(rt));
+        }
         c.rt = rt;
-        c.s = sq.s;
+        c.s = sq.q.s;
         c.kvh = sq_kvh;
         c.q0 = sq.q.q0;
         c.rows = min(sq.q.n, a.max_new) * G;
         c.L = sq.q.L;
         c.past = sq.q.L - sq.q.n;
-        c.len = wt.of(rt);
-        c.place = p - (ps - wt.before(rt));
         const int off = (begin ? cuts.cut(p, c.place, c.len) : p) - c.place;
         const int off_end = (p_end < c.place + c.len ? cuts.cut(p_end, c.place, c.len) : c.place + c.len) - c.place;
         c.whole = off <= 0 && off_end == c.len;
@@ -1234,8 +1354,9 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     const Seq mine = seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1));
     const ManyAxis axis = many_axis(a, mine);
     if (axis.head <= 0) return;
-    const int wgs = many_shares(a, axis, gridDim.x);
-    if ((int)blockIdx.x < wgs) many_share<D, KT>(a, ws, tickets, axis, mine, blockIdx.x, wgs, lds, marks);
+    const ManyPieces pc = many_pieces(a, axis, mine, gridDim.x, blockIdx.x);
+    const int wgs = pc.head > 0 ? pc.head * a.Hkv : many_shares(a, axis, gridDim.x);
+    if ((int)blockIdx.x < wgs) many_share<D, KT>(a, ws, tickets, axis, pc, mine, blockIdx.x, wgs, lds, marks);
 }
 
 // Few rows beside many: share `item / Hkv` of kv head item % Hkv, the axis cut
@@ -1313,9 +1434,11 @@ __global__ void __launch_bounds__(kWaves * 64) paged_mixed_kernel(PagedArgs a, f
     if (axis.head > 0) {
         const float many = (float)(axis.head * a.Hkv) * (float)(1 << axis.shift) * (1.0f / 16), rest = kFewTime<D> * (float)few * (float)a.Hkv;
         const int n = (int)((float)gridDim.x * many * __builtin_amdgcn_rcpf(many + rest) * (1.0f / 8) + 0.5f) * 8;
-        wgs = many_shares(a, axis, max(min(8, (int)gridDim.x - 1), min(n, (int)gridDim.x - (few > 0 ? 8 : 0))));
+        const int most = max(8, min(n, (int)gridDim.x - (few > 0 ? 8 : 0)));
+        const ManyPieces pc = many_pieces(a, axis, mine, most, blockIdx.x);
+        wgs = pc.head > 0 ? pc.head * a.Hkv : many_shares(a, axis, most);
         if ((int)blockIdx.x < wgs) {
-            many_share<D, KT>(a, ws, tickets, axis, mine, blockIdx.x, wgs, lds, marks);
+            many_share<D, KT>(a, ws, tickets, axis, pc, mine, blockIdx.x, wgs, lds, marks);
             return;
         }
     }
