@@ -17,7 +17,7 @@
 //
 // Reached, of a copy's 4.9 TB/s and a large product's 1175 TFLOP/s: single
 // tokens 5.6 TB/s (48 sequences of 500 to 8000 keys, 405 MB, 72 us); 2048 tokens
-// behind 28672 keys 990 TFLOP/s (880 us), 512 behind 15872 860 (138 us).
+// behind 28672 keys 1000 TFLOP/s (872 us), 512 behind 15872 874 (135 us).
 //
 // Both compute, per 32 rows and a tile of keys, with
 // v_mfma_f32_32x32x16_{f16,bf16} (layouts in mfma_ops.hpp):
