@@ -1413,9 +1413,9 @@ __device__ __forceinline__ bool few_share(const PagedArgs& a, float* __restrict_
 // times of both kinds say (on the device, from the batch).  So the bytes of the
 // one come while the matrix cores work on the other, and no launch waits.
 // Against the two kernels one after the other: 64 x 4096 keys and 512 tokens
-// behind 4096 142 -> 109 us, 23 x 2000 and 512 tokens 50 -> 35, prompts of 40 to
-// 1100 tokens (no few rows) 40 -> 38; 8 x 1024 alone in a call that could have
-// brought more 10 -> 13, 64 x 4096 alone 90 -> 85.
+// behind 4096 142 -> 109 us, 23 x 2000 and 512 tokens 50 -> 29, 1.5B prompts of
+// 40 to 1100 tokens (no few rows) 35 -> 27; 8 x 1024 alone in a call that could
+// have brought more 10 -> 13, 64 x 4096 alone 90 -> 85.
 // Time of a few-row tile to that of a key tile of a row tile (0.16 and 0.22: D =
 // 64, 64 x 2000 keys and 512 tokens 21.9 and 25.4 us; D = 128, 60 sequences of up
 // to 8000 and 700 behind 2000 105 and 97):
