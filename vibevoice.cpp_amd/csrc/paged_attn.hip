@@ -24,13 +24,17 @@
 //   S^T[key][row] = K . Q^T    Q^T in registers; a lane owns one query row
 //   softmax                    fp32, exp2 domain, scale folded into the exp's
 //                              fma; the running max of a row is raised only
-//                              when a tile's max passes it by more than 2^8,
-//                              so p <= 256 fits f16 and rescales are rare
+//                              when a tile's max passes it by more than 2^8
+//                              (rescales are rare), so p <= 2^8
 //   O^T[dim][row] += V^T . P^T P converted in place from the accumulators: the
 //                              key order of a step is the one they have
-// P is rounded to the pages' type, a relative 2^-11 (F16) or 2^-8 (BF16) at
-// most, as the output itself is; the row sum adds the rounded values, so the
-// weights of a row sum to one.
+// P is rounded to the pages' type, as the output itself is: a relative 2^-8 at
+// most in BF16.  F16 has fewer exponents than a long row has sizes of weights,
+// so its P carry a factor of 2^7 (p <= 2^15), which leaves with the row sum:
+// weights down to 2^-21 of the row's largest are rounded by a relative 2^-11,
+// smaller ones by 2^-32 of it (without the factor a weight of e^-17 is 44 % off,
+// and a long cache has many).  The row sum adds the rounded values, so the weights
+// of a row sum to one.
 //
 // K and V rows go from the pages straight into LDS (global_load_lds, 1 KB =
 // 4 rows of 128 dims an instruction, no registers), 16-byte chunk c of row r
@@ -56,6 +60,8 @@ namespace {
 #include "paged_ops.hpp"
 
 constexpr float kLazy = 8.0f;      // running-max slack in log2 units
+// log2 of the factor that P carries
+template <int KT> constexpr float kLift = KT == VVA_TYPE_F16 ? 7.0f : 0.0f;
 constexpr int kFewRows = 32;       // rows of a sequence and kv head that paged_few_kernel takes
 // exponent base of a partial whose keys lie in a page outside the pool; handled as
 // bits, since this file is compiled for numbers alone
@@ -458,7 +464,7 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
                 m = mx;
             }
         }
-        const float nb = m == -INFINITY ? 0.0f : -m;
+        const float nb = kLift<KT> - (m == -INFINITY ? 0.0f : m);
         uint32_t p[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
@@ -1123,7 +1129,7 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
         auto block = [&](const f32x16 (&cur)[2], f32x16 (&nxt)[2], uint32_t ka, uint32_t va) {
             constexpr int NQ = 2 * DS, NP = 4 * DT, NS = NQ + NP;
             constexpr int KAHEAD = 2, VAHEAD = 2;             // operand reads ahead of their slot
-            const float nb = m == -INFINITY ? 0.0f : -m;      // no visible key yet: every s is -inf
+            const float nb = kLift<KT> - (m == -INFINITY ? 0.0f : m);   // no visible key yet: every s is -inf
             u32x4 kf[NQ], vf[NP];
             float pe[32];
             uint32_t pp[16];
