@@ -40,3 +40,52 @@ def test_tail_of_small_weights(ctx, torch_gpu, monkeypatch, lens, heads, gap):
     ref, tol = attention(P, 1.0)
     # and half a step of the output, 2^-25 below 2^-14
     check_rows(out, ref, tol + 2.0 ** -25, f"{lens} {gap}")
+
+
+def call(ctx, P, out=None):
+    out = P.torch.full_like(P.q, 77.0) if out is None else out
+    ctx.paged_attn(P.q, P.k, P.v, P.batch(), P.d ** -0.5, out)
+    P.torch.cuda.synchronize()
+    return out
+
+
+# few rows in one piece and in many (two levels of sums too), many rows in one share and in many, both kinds in a launch
+NAN_SETS = [([(4, 40)], H7), ([(4, 3000), (3, 700)], H7), ([(2, 40000)], H05), ([(3, 65)] * 70, H05), ([(90, 90)], H05),
+            ([(300, 2500)], H7), ([(256, 9000)], H7), ([(4, 2000), (70, 1500), (1, 900)], H05), ([(2, 9), (33, 64)], H7)]
+
+
+@pytest.mark.parametrize("t", [vva.F16, vva.BF16])
+@pytest.mark.parametrize("lens,heads", NAN_SETS)
+def test_nan_in_a_query_row(ctx, torch_gpu, lens, heads, t):
+    """One head of some tokens with a NaN in its q answers NaN; every other row keeps its bits."""
+    torch = torch_gpu
+    print(lens[:3], heads, t, flush=True)
+    P = Pages(torch, lens, *heads, t, 16, seed=3)
+    ref = call(ctx, P)
+    own = torch.zeros(ref.shape[:2], dtype=torch.bool, device="cuda")
+    for n, h in [(int(P.starts[0]), heads[0] - 1), (int(P.starts[0]) + lens[0][0] // 2, 0), (P.n_tok - 1, 3)]:
+        P.q[n, h, 7] = float("nan")
+        own[n, h] = True
+    out = call(ctx, P)
+    assert bool(out[own].isnan().all())
+    assert torch.equal(out[~own], ref[~own])
+
+
+@pytest.mark.parametrize("t", [vva.F16, vva.BF16])
+@pytest.mark.parametrize("lens,heads", NAN_SETS)
+@pytest.mark.parametrize("back", [1, 2])
+def test_nan_in_a_row_of_k(ctx, torch_gpu, lens, heads, t, back):
+    """A NaN in the K of a sequence's newest key, or of the one before, for one kv head: that head's rows that see it answer
+    NaN, every other row keeps its bits."""
+    torch = torch_gpu
+    print(lens[:3], heads, t, back, flush=True)
+    P = Pages(torch, lens, *heads, t, 16, seed=4)
+    ref = call(ctx, P)
+    n, L = lens[0]
+    j, kvh, G = L - back, heads[1] - 1, heads[0] // heads[1]
+    P.k[int(P.table_host[0, j // 16]), kvh, j % 16, 5] = float("nan")
+    out = call(ctx, P)
+    sees = torch.zeros(out.shape[:2], dtype=torch.bool, device="cuda")
+    sees[max(0, n - back):n, kvh * G:] = True
+    assert bool(out[sees].isnan().all())
+    assert torch.equal(out[~sees], ref[~sees])

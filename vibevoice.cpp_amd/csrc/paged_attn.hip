@@ -63,8 +63,9 @@ constexpr float kLazy = 8.0f;      // running-max slack in log2 units
 // log2 of the factor that P carries
 template <int KT> constexpr float kLift = KT == VVA_TYPE_F16 ? 7.0f : 0.0f;
 constexpr int kFewRows = 32;       // rows of a sequence and kv head that paged_few_kernel takes
-// exponent base of a partial whose keys lie in a page outside the pool; handled as
-// bits, since this file is compiled for numbers alone
+// Exponent base of a partial whose keys lie in a page outside the pool, compared as
+// bits.  No sums' own base is one: a running max is raised only where a score is
+// greater, which none is to or from a NaN.
 constexpr uint32_t kNanBits = 0x7fc00000u;
 
 typedef const __attribute__((address_space(4))) int32_t* ConstInts;
@@ -505,14 +506,15 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
                     make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
         if (half == 0) *(float2*)(ml + (w * kFewRows + l32) * 2) = make_float2(m, lt);
     }
-    bool nan = __syncthreads_or(bad);
+    const bool bad_page = __syncthreads_or(bad);
     const PagedArgs& args = fresh_args();
     // thread i's part of the sums: 4 dims of a row
     struct Sum {
         float4 num;
         float M, den;
     };
-    auto write = [&](int row, int c, const Sum& x) {
+    // nan: the row is to answer NaN
+    auto write = [&](int row, int c, const Sum& x, bool nan) {
         const float inv = x.den > 0.0f ? 1.0f / x.den : 0.0f;
         uint2 y = {pack2<KT>(x.num.x * inv, x.num.y * inv), pack2<KT>(x.num.z * inv, x.num.w * inv)};
         if (nan) y.x = y.y = 0x7fff7fffu;
@@ -528,7 +530,7 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
         return make_rsrc((const char*)ws + (int64_t)place(part) * bytes, bytes);
     };
     // agent-scope stores: coherent across the XCDs' L2 caches
-    auto store = [&](int part, int row, int c, const Sum& x) {
+    auto store = [&](int part, int row, int c, const Sum& x, bool nan) {
         const BufRsrc rs = piece_rsrc(part);
         __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(x.num.x), __float_as_uint(x.num.y), __float_as_uint(x.num.z), __float_as_uint(x.num.w)},
                                                rs, (row * D + 4 * c) * 4, 0, kSc1);
@@ -550,8 +552,8 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
             x.num.x = fmaf(f, v.x, x.num.x); x.num.y = fmaf(f, v.y, x.num.y);
             x.num.z = fmaf(f, v.z, x.num.z); x.num.w = fmaf(f, v.w, x.num.w);
         }
-        if (it.parts > 1) store(it.part, row, c, x);
-        else write(row, c, x);
+        if (it.parts > 1) store(it.part, row, c, x, bad_page);
+        else write(row, c, x, bad_page);
     }
     if (it.parts == 1) return;
     // ---- the last of a group of pieces adds their partials, in order, and the
@@ -581,6 +583,7 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
             for (int i = tid; i < rows * (D / 4); i += WAVES * 64) {
                 const int row = i / (D / 4), c = i % (D / 4);
                 Sum x{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+                bool nan = false;
 #pragma unroll 1
                 for (int p0 = 0; p0 < n_add; p0 += kMergeBatch) {
                     // a batch's loads go out together, one round trip each; those
@@ -622,8 +625,8 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
                         x.num.w = fmaf(f, __uint_as_float(v[u].w), x.num.w);
                     }
                 }
-                if (final) write(row, c, x);
-                else store(first, row, c, x);
+                if (final) write(row, c, x, nan);
+                else store(first, row, c, x, nan);
             }
         }
         if (final) return;
