@@ -379,6 +379,9 @@ VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, 
  * gets zeros.  Rows of no sequence are left as they were; rows that see a key
  * whose page id is outside the pool get NaN (other rows of that sequence may).
  * What is stored behind the keys of a sequence (NaN included) does not matter.
+ * Infinities and NaN in what a row sees go by the softmax's definition: scores
+ * of +inf or NaN, or of -inf alone, give NaN; keys of -inf beside others are
+ * left out.
  * The products run on the matrix cores in the pages' type with F32 sums, the
  * probabilities rounded to that type; the softmax is F32.
  * Every row of q and out and every page row starts on 16 bytes.

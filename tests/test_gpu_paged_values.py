@@ -89,3 +89,67 @@ def test_nan_in_a_row_of_k(ctx, torch_gpu, lens, heads, t, back):
     sees[max(0, n - back):n, kvh * G:] = True
     assert bool(out[sees].isnan().all())
     assert torch.equal(out[~sees], ref[~sees])
+
+
+@pytest.mark.parametrize("t", [vva.F16, vva.BF16])
+@pytest.mark.parametrize("lens,heads", NAN_SETS)
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf")])
+def test_infinity_in_a_query_row(ctx, torch_gpu, lens, heads, t, bad):
+    """Scores of one sign's infinity by K's: the softmax of such a row is NaN where one is +inf, and where all are -inf, as a
+    prompt's first token's only one may be.  Rows whose scores are -inf in part are not made here (no K is 0)."""
+    torch = torch_gpu
+    print(lens[:3], heads, t, bad, flush=True)
+    P = Pages(torch, lens, *heads, t, 16, seed=3)
+    ref = call(ctx, P)
+    own = torch.zeros(ref.shape[:2], dtype=torch.bool, device="cuda")
+    for n, h in [(int(P.starts[0]), heads[0] - 1), (P.n_tok - 1, 3)]:
+        P.q[n, h, 7] = bad
+        own[n, h] = True
+    out = call(ctx, P)
+    assert bool(out[own].isnan().all())
+    assert torch.equal(out[~own], ref[~own])
+
+
+@pytest.mark.parametrize("t", [vva.F16, vva.BF16])
+@pytest.mark.parametrize("lens,heads", [([(1, 1)], H7), ([(4, 30)], H7), ([(2, 5000)], H05), ([(60, 90)], H05), ([(300, 2500)], H7),
+                                        ([(3, 2), (70, 1500), (1, 900)], H05)])
+def test_rows_whose_scores_are_all_minus_infinity(ctx, torch_gpu, lens, heads, t):
+    """K of -inf times a q above 0 for every key: NaN, but zeros still where a token sees no key."""
+    torch = torch_gpu
+    print(lens, heads, t, flush=True)
+    P = Pages(torch, lens, *heads, t, 16, seed=5)
+    P.q[:, :, 9] = 0.5
+    n, L = lens[0]
+    for j in range(L):
+        P.k[int(P.table_host[0, j // 16]), :, j % 16, 9] = -float("inf")
+    out = call(ctx, P)
+    none = max(0, n - L)                                    # tokens before key 0
+    assert bool((out[:none] == 0).all()) and bool(out[none:n].isnan().all())
+    ref, tol = attention(P, P.d ** -0.5)
+    check_rows(out[n:P.n_tok], ref[n:P.n_tok], tol[n:P.n_tok])
+
+
+@pytest.mark.parametrize("lens,heads", [([(4, 3000), (1, 9)], H7), ([(70, 300)], H05)])
+def test_keys_of_minus_infinity_are_left_out(ctx, torch_gpu, lens, heads):
+    """Some keys' scores -inf, whole tiles of them and the first ones among them: the others' softmax."""
+    torch = torch_gpu
+    P = Pages(torch, lens, *heads, vva.BF16, 16, seed=5)
+    P.q[:, :, 9] = 0.5
+    n, L = lens[0]
+    gone = list(range(0, 70)) + list(range(128, 192)) + [200, 201]
+    for j in gone:
+        P.k[int(P.table_host[0, j // 16]), :, j % 16, 9] = -float("inf")
+    out = call(ctx, P)
+    G, scale = heads[0] // heads[1], P.d ** -0.5
+    for h in range(heads[0]):
+        k, v = P.keys(0, P.k, h // G), P.keys(0, P.v, h // G)
+        q = P.q[:n, h].double()
+        sc = (q @ k.t().contiguous()) * scale
+        seen = torch.arange(L, device="cuda")[None] <= (L - n + torch.arange(n, device="cuda"))[:, None]
+        w = torch.softmax(sc.masked_fill(~seen, -float("inf")), -1)
+        mag = (q.abs() @ k.abs().nan_to_num(posinf=0.0).t().contiguous()) * scale
+        # as in attention(): half a step of each weight, its score's error, twice for the row sum, and the output's half step
+        e = w * (2.0 ** -8 + 2.0 ** -23 * (8 + (P.d + 2) * mag + (sc - sc.amax(-1, keepdim=True)).abs().nan_to_num(posinf=0.0)))
+        ref = w @ v
+        tol = 1.01 * (e @ v.abs() + e.sum(-1, keepdim=True) * ref.abs()) + 2.0 ** -8 * ref.abs()
+        check_rows(out[:n, h], ref, tol)

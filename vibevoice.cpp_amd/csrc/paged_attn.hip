@@ -515,10 +515,11 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
     };
     // nan: the row is to answer NaN
     auto write = [&](int row, int c, const Sum& x, bool nan) {
-        const float inv = x.den > 0.0f ? 1.0f / x.den : 0.0f;
+        const int rt = div_g(args, row);
+        // zeros where the row sees no key; all scores -inf: 0 * (1 / 0), the softmax's NaN
+        const float inv = min(it.q.L - 1, it.q.L - it.q.n + rt) >= 0 ? 1.0f / x.den : 0.0f;
         uint2 y = {pack2<KT>(x.num.x * inv, x.num.y * inv), pack2<KT>(x.num.z * inv, x.num.w * inv)};
         if (nan) y.x = y.y = 0x7fff7fffu;
-        const int rt = div_g(args, row);
         *(uint2*)(args.out + (int64_t)(it.q.q0 + rt) * args.o_nb_t + (int64_t)(kvh * args.G + row - rt * args.G) * args.o_nb_h + 8 * c) = y;
     };
     // A piece's place for its partial, by its number; in shares, where a
@@ -1336,7 +1337,8 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
         // lanes l and l + 32 have 4 dims each of 8: they trade halves of pairs
         // of such groups, so that each stores 16 bytes
         char* const op = args.out + (int64_t)(c.q0 + t0 + t) * args.o_nb_t + (int64_t)(c.kvh * G + h) * args.o_nb_h + 16 * (ln >> 5);
-        const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
+        // zeros where the row sees no key; all scores -inf: 0 * (1 / 0), the softmax's NaN
+        const float inv = min(c.L - 1, c.past + t0 + t) >= 0 ? 1.0f / lt : 0.0f;
 #pragma unroll
         for (int i = 0; i < DT * 2; ++i) {
             uint32_t y[2][2];
