@@ -153,3 +153,26 @@ def test_keys_of_minus_infinity_are_left_out(ctx, torch_gpu, lens, heads):
         ref = w @ v
         tol = 1.01 * (e @ v.abs() + e.sum(-1, keepdim=True) * ref.abs()) + 2.0 ** -8 * ref.abs()
         check_rows(out[:n, h], ref, tol)
+
+
+@pytest.mark.parametrize("t,digits", [(vva.F16, 2.0 ** -22), (vva.BF16, 2.0 ** -16)])
+@pytest.mark.parametrize("lens,heads,scale", [([(1, 130), (2, 40)], H7, 1.0), ([(4, 3001)], H7, 0.5), ([(1, 20000), (3, 77)], H05, 0.2),
+                                              ([(2, 700), (90, 200)], H05, 0.3), ([(1, 5)] * 80, H05, 1.0)])
+def test_few_rows_keep_the_digits_of_their_probabilities(ctx, torch_gpu, monkeypatch, t, digits, lens, heads, scale):
+    """Sequences of at most 32 rows of a kv group: probabilities in two parts of the pages' type, each within half a step of
+    what it stands for (F16: of 2^7 times the share of the largest, down to its smallest step)."""
+    torch = torch_gpu
+    print(lens[:3], heads, t, scale, flush=True)
+    P = Pages(torch, lens, *heads, t, 16, seed=17)
+    out = torch.empty_like(P.q)
+    ctx.paged_attn(P.q, P.k, P.v, P.batch(), scale, out)
+    torch.cuda.synchronize()
+    last = paged_util.HALF[t], paged_util.TINY[t]
+    monkeypatch.setitem(paged_util.HALF, t, digits)
+    monkeypatch.setitem(paged_util.TINY, t, 2.0 ** -32 if t == vva.F16 else 0.0)
+    ref, tol = attention(P, scale)
+    for s, (n, _) in enumerate(lens):
+        if n * (heads[0] // heads[1]) <= 32:
+            r = slice(int(P.starts[s]), int(P.starts[s]) + n)
+            # and the output's one rounding
+            check_rows(out[r], ref[r], tol[r] + last[0] * (ref[r].abs() + tol[r]) + last[1], f"sequence {s}")
