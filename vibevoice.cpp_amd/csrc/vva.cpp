@@ -1501,26 +1501,33 @@ extern "C" vva_status vva_decode_step(vva_context* ctx, vva_kv* kv, int layer, c
 
 namespace {
 
-// Whether two tensors of token rows (dims [0, dim) of a row) share memory.
-// Rows may interleave, as the parts of one projection's rows do: all row
-// strides are then multiples of one period, in which the rows lie apart.
-bool rows_overlap(const vva_tensor* a, const vva_tensor* b, int dim) {
+// Whether two tensors share memory.  Their rows may interleave, as the parts of
+// one projection's rows or K and V pages of one pool do: they lie apart if for
+// some stride, a period, all strides from it on are its multiples and what the
+// smaller ones reach lies apart within it.
+bool meets(const vva_tensor* a, const vva_tensor* b) {
     if (!overlaps(a, b)) return false;
-    uint64_t period = ~(uint64_t)0;
-    for (int i = dim; i < 4; ++i) {
-        if (a->ne[i] > 1) period = std::min(period, (uint64_t)a->nb[i]);
-        if (b->ne[i] > 1) period = std::min(period, (uint64_t)b->nb[i]);
+    const vva_tensor* t[2] = {a, b};
+    for (int k = 0; k < 6; ++k) {
+        if (t[k / 3]->ne[k % 3 + 1] == 1) continue;
+        const uint64_t period = t[k / 3]->nb[k % 3 + 1];
+        bool fits = period > 0;
+        uint64_t span[2] = {0, 0};                                // of the dims below the period
+        for (int x = 0; x < 2 && fits; ++x) {
+            vva_tensor in = *t[x];
+            for (int i = 1; i < 4; ++i) {
+                if (in.ne[i] == 1 || in.nb[i] < period) continue;
+                fits = fits && in.nb[i] % period == 0;
+                in.ne[i] = 1;
+            }
+            span[x] = tensor_span(&in);
+        }
+        if (!fits) continue;
+        const uint64_t at = ((uint64_t)b->data % period + period - (uint64_t)a->data % period) % period;   // b in a's period
+        if (span[0] <= at && at <= period && span[1] <= period - at) return false;
     }
-    if (period == 0 || period == ~(uint64_t)0) return true;
-    for (int i = dim; i < 4; ++i)
-        if ((a->ne[i] > 1 && a->nb[i] % period) || (b->ne[i] > 1 && b->nb[i] % period)) return true;
-    vva_tensor ra = *a, rb = *b;
-    for (int i = dim; i < 4; ++i) ra.ne[i] = rb.ne[i] = 1;
-    const uint64_t sa = tensor_span(&ra), sb = tensor_span(&rb), da = (uint64_t)a->data % period, db = (uint64_t)b->data % period;
-    const uint64_t at = (db + period - da) % period;              // b's row in a's period
-    return sa > period || sb > period || at < sa || at + sb > period;
+    return true;
 }
-
 bool al16(const vva_tensor* t, int dims) {
     bool ok = (uintptr_t)t->data % 16 == 0;
     for (int i = 1; i <= dims; ++i) ok = ok && (t->ne[i] == 1 || t->nb[i] % 16 == 0);
@@ -1630,16 +1637,14 @@ extern "C" vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* 
         !al16(rope, 1) || rope->ne[1] > 0x7fffffff)
         return fail(ctx, VVA_ERR_INVALID_ARG, "rope must be F32 ne=[%lld,n_pos] with 16-byte aligned rows", (long long)d);
     if (pos && (st = check_ints(ctx, pos, "pos", N)) != VVA_OK) return st;
-    // what one workgroup reads no other may write: the pages apart from the
-    // inputs (interleaved pools overlap as ranges, so K and V are told apart by
-    // their first rows), q_out q itself, row for row, or memory of its own
+    // what one workgroup reads or writes no other may write: the pages apart from
+    // the inputs and each other, q_out q itself, row for row, or memory of its own
     for (const vva_tensor* t : {q, k, v, rope, pos, &batch->q_start, &batch->kv_len, &batch->table})
-        if (t && (overlaps(k_pages, t) || overlaps(v_pages, t) || (t != q && rows_overlap(q_out, t, 2))))
+        if (t && (overlaps(k_pages, t) || overlaps(v_pages, t) || (t != q && meets(q_out, t))))
             return fail(ctx, VVA_ERR_INVALID_ARG, "paged_rope_append: the pages or q_out overlap an input (only q_out == q may alias)");
-    if (k_pages->data == v_pages->data)
-        return fail(ctx, VVA_ERR_INVALID_ARG, "paged_rope_append: k_pages and v_pages are the same memory");
+    if (meets(k_pages, v_pages)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_rope_append: k_pages and v_pages overlap");
     const bool same = q_out->data == q->data && q_out->type == q->type && q_out->nb[1] == q->nb[1] && q_out->nb[2] == q->nb[2];
-    if ((!same && rows_overlap(q_out, q, 2)) || overlaps(q_out, k_pages) || overlaps(q_out, v_pages))
+    if ((!same && meets(q_out, q)) || overlaps(q_out, k_pages) || overlaps(q_out, v_pages))
         return fail(ctx, VVA_ERR_INVALID_ARG, "paged_rope_append: q_out overlaps another tensor (only q_out == q may alias)");
     a.p.q = (const char*)q->data; a.q_type = q->type; a.p.q_nb_h = q->nb[1]; a.p.q_nb_t = q->nb[2];
     a.k_new = (const char*)k->data; a.k_type = k->type; a.k_nb_h = k->nb[1]; a.k_nb_t = k->nb[2];
@@ -1670,7 +1675,7 @@ extern "C" vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, cons
         return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: q and out must have the pages' type (%d)", a.type);
     if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: scale must be finite and > 0");
     for (const vva_tensor* t : {q, k_pages, v_pages, &batch->q_start, &batch->kv_len, &batch->table})
-        if (rows_overlap(out, t, 2)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: out overlaps q, the pages or the batch");
+        if (meets(out, t)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: out overlaps q, the pages or the batch");
     a.q = (const char*)q->data; a.q_nb_h = q->nb[1]; a.q_nb_t = q->nb[2];
     a.out = (char*)out->data; a.o_nb_h = out->nb[1]; a.o_nb_t = out->nb[2];
     a.scale = scale;
@@ -1712,9 +1717,9 @@ extern "C" vva_status vva_add_rms_norm(vva_context* ctx, const vva_tensor* x, co
     auto same = [](const vva_tensor* o, const vva_tensor* i) {
         return o->data == i->data && o->type == i->type && (o->ne[1] == 1 || o->nb[1] == i->nb[1]) && (o->ne[2] == 1 || o->nb[2] == i->nb[2]);
     };
-    auto clash = [&](const vva_tensor* o, const vva_tensor* i) { return o && i && !same(o, i) && rows_overlap(o, i, 1); };
+    auto clash = [&](const vva_tensor* o, const vva_tensor* i) { return o && i && !same(o, i) && meets(o, i); };
     if (clash(y, x) || clash(y, add) || clash(sum, x) || clash(sum, add) || overlaps(y, w) || (sum && overlaps(sum, w)) ||
-        (sum && rows_overlap(sum, y, 1)))
+        (sum && meets(sum, y)))
         return fail(ctx, VVA_ERR_INVALID_ARG, "add_rms_norm: outputs overlap each other or an input (only an input itself may alias)");
     NormArgs a{};
     a.x = (const char*)x->data; a.x_type = x->type; a.x_nb_t = x->nb[1]; a.x_nb_b = x->nb[2];
