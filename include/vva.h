@@ -362,7 +362,8 @@ typedef struct {
  * A token whose page id is outside the pool, or which belongs to no sequence,
  * or lies before key 0, is not appended; a position outside the table gives
  * NaN.  q_out rows of no sequence are left as they were.  The pages lie apart
- * from every input, K's from V's (they may interleave). */
+ * from every input, K's from V's (they may interleave), and the rows of each
+ * output from one another. */
 VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, const vva_tensor* k,
                                          const vva_tensor* v, const vva_tensor* rope, const vva_tensor* pos,
                                          const vva_batch* batch, const vva_tensor* k_pages,
@@ -372,8 +373,8 @@ VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, 
  * vva_attn for packed sequences, each with any number of new tokens behind any
  * number of keys (whole prompts, chunks and single tokens in one call).
  *   q:   ne = [d, Hq, N], already RoPE'd, in the pages' type;
- *   out: ne = [d, Hq, N], in that type too, apart from the memory of every
- *        input; rows of q less than 4 MiB apart;
+ *   out: ne = [d, Hq, N], in that type too, its rows apart from one another and
+ *        from the memory of every input; rows of q less than 4 MiB apart;
  *   scale: a finite number above 0.
  * Token t of sequence s sees keys 0 .. kv_len[s] - n_s + t; one that sees none
  * gets zeros.  Rows of no sequence are left as they were; rows that see a key
@@ -409,7 +410,8 @@ VVA_API vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, const v
  *        round(y * 127 / amax), as in the Q8_0 caches); may be x or add itself
  *        where the types match.
  * Outputs otherwise lie apart from each other and the inputs (rows may
- * interleave).  Everything is computed in F32 from the unrounded h.  hidden <= 16384, rows
+ * interleave), and their rows from one another: an add whose rows are one
+ * (stride 0) cannot be an output too.  Everything is computed in F32 from the unrounded h.  hidden <= 16384, rows
  * contiguous, any strides between them; eps >= 0. */
 VVA_API vva_status vva_add_rms_norm(vva_context* ctx, const vva_tensor* x, const vva_tensor* add, const vva_tensor* w,
                                     float eps, const vva_tensor* sum, const vva_tensor* y);

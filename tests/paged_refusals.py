@@ -2,7 +2,7 @@
 a test module), over the stand-in of the HIP runtime that host_routes.py loads.  `python paged_refusals.py NAME` runs one."""
 import sys
 
-from host_routes import FAKE, LIB, NO_LIMIT, ref, vva
+from host_routes import FAKE, LIB, NO_LIMIT, Host, ref, vva
 from paged_routes import INV, Call, change
 
 
@@ -43,7 +43,60 @@ def pages_that_meet():
         assert c.attn() == vva.OK, (off, LIB.vva_last_error(c.c.h))     # reads them only
 
 
-SCENARIOS = [pages_that_meet]
+def rows_that_meet_their_own():
+    """Outputs whose rows share memory: refused; inputs may (broadcast)."""
+    for name, fn in (("q_out", "append"), ("out", "attn")):
+        row = 64 * 2
+        for nb in ([0, 14 * row], [row, 0], [row, 13 * row], [row - 16, 14 * row], [4 * row, row], [row, row]):
+            c = Call()
+            layout(c, name, c.a[name].data, nb)
+            c.refused(getattr(c, fn), INV, (name, nb))
+        for nb in ([row, 14 * row], [row + 16, 16 * row], [5 * row, row]):        # the last: the tokens of a head together
+            c = Call()
+            layout(c, name, c.a[name].data, nb)
+            assert getattr(c, fn)() == vva.OK, (name, nb, LIB.vva_last_error(c.c.h))
+    for name in ("k_pages", "v_pages"):
+        row, page = 128, 16 * 128
+        for nb in ([0, page, 2 * page], [row, 0, 2 * page], [row, page, 0], [row, page, page], [row - 16, page, 2 * page]):
+            c = Call()
+            layout(c, name, c.a[name].data, nb)
+            c.refused(c.append, INV, (name, nb))
+            assert c.attn() == vva.OK, (name, nb, LIB.vva_last_error(c.c.h))
+    c = Call(N=1, n_seq=1, n_pages=1)                      # strides of dims of one element do not count
+    layout(c, "q_out", c.a["q_out"].data, [128, 0])
+    layout(c, "k_pages", c.a["k_pages"].data, [128, 16 * 128, 0])
+    assert c.append() == vva.OK, LIB.vva_last_error(c.c.h)
+    for name in ("q", "k", "v", "rope"):                   # the same rows for every token, or every position
+        c = Call()
+        change(c, name, nb={1 if name == "rope" else 2: 0})
+        assert c.append() == vva.OK, (name, LIB.vva_last_error(c.c.h))
+
+
+def norm_rows_that_meet_their_own():
+    h = Host()
+    T = h.tensor
+
+    def norm(x, y, add=None, total=None):
+        return LIB.vva_add_rms_norm(h.h, ref(x), ref(add) if add else None, ref(w), 1e-6, ref(total) if total else None, ref(y))
+
+    w = T(vva.F32, [64])
+    dense = [T(vva.F32, [64, 5, 2]) for _ in range(3)]
+    once = [T(vva.F32, [64, 5, 2], nb=[4, 0, 0, 0]), T(vva.F32, [64, 5, 2], nb=[4, 256, 0, 0]), T(vva.F32, [64, 5, 2], nb=[4, 0, 256, 0]),
+            T(vva.F32, [64, 5, 2], nb=[4, 252, 1280, 2560]), T(vva.F32, [64, 5, 2], nb=[4, 256, 1024, 2048])]
+    for o in once:
+        FAKE.fake_take_log()
+        for x, y, add, total in ((dense[0], o, None, None), (dense[0], dense[1], dense[2], o), (dense[0], dense[1], o, o), (o, o, None, None)):
+            assert norm(x, y, add, total) == INV, list(o.nb)
+        assert not FAKE.fake_take_log()
+        assert norm(o, dense[1], dense[0]) == vva.OK and norm(dense[0], dense[1], o, dense[2]) == vva.OK
+    q8 = T(vva.Q8_0, [64, 5, 2], nb=[34, 34, 340, 680])
+    assert norm(dense[0], q8) == INV
+    assert norm(dense[0], T(vva.Q8_0, [64, 5, 2])) == vva.OK
+    # rows of the batches by turns
+    assert norm(dense[0], T(vva.F32, [64, 5, 2], nb=[4, 512, 256, 4096])) == vva.OK
+
+
+SCENARIOS = [pages_that_meet, rows_that_meet_their_own, norm_rows_that_meet_their_own]
 
 if __name__ == "__main__":
     FAKE.fake_set(0, NO_LIMIT)

@@ -10,7 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 DRIVER = os.path.join(HERE, "paged_refusals.py")
 
 
-@pytest.mark.parametrize("name", ["pages_that_meet"])
+@pytest.mark.parametrize("name", ["pages_that_meet", "rows_that_meet_their_own", "norm_rows_that_meet_their_own"])
 def test_layouts(name):
     assert os.path.exists(os.path.join(HERE, "cpp", "bin", "libfakehip.so")), "run __graft_entry__.build()"
     r = subprocess.run([sys.executable, DRIVER, name], capture_output=True, text=True, timeout=120)

@@ -1528,6 +1528,21 @@ bool meets(const vva_tensor* a, const vva_tensor* b) {
     }
     return true;
 }
+// Whether rows of one tensor may share memory: some dim's stride is less than
+// what the dims of smaller strides reach.
+bool meets_itself(const vva_tensor* t) {
+    vva_tensor in = *t;
+    for (int i = 1; i < 4; ++i) in.ne[i] = 1;
+    for (;;) {
+        int next = 0;
+        for (int i = 1; i < 4; ++i)
+            if (in.ne[i] < t->ne[i] && (next == 0 || t->nb[i] < t->nb[next])) next = i;
+        if (next == 0) return false;
+        if (t->nb[next] < tensor_span(&in)) return true;
+        in.ne[next] = t->ne[next];
+    }
+}
+
 bool al16(const vva_tensor* t, int dims) {
     bool ok = (uintptr_t)t->data % 16 == 0;
     for (int i = 1; i <= dims; ++i) ok = ok && (t->ne[i] == 1 || t->nb[i] % 16 == 0);
@@ -1639,6 +1654,8 @@ extern "C" vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* 
     if (pos && (st = check_ints(ctx, pos, "pos", N)) != VVA_OK) return st;
     // what one workgroup reads or writes no other may write: the pages apart from
     // the inputs and each other, q_out q itself, row for row, or memory of its own
+    for (const vva_tensor* t : {k_pages, v_pages, q_out})
+        if (meets_itself(t)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_rope_append: rows of the pages or of q_out overlap each other");
     for (const vva_tensor* t : {q, k, v, rope, pos, &batch->q_start, &batch->kv_len, &batch->table})
         if (t && (overlaps(k_pages, t) || overlaps(v_pages, t) || (t != q && meets(q_out, t))))
             return fail(ctx, VVA_ERR_INVALID_ARG, "paged_rope_append: the pages or q_out overlap an input (only q_out == q may alias)");
@@ -1676,6 +1693,7 @@ extern "C" vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, cons
     if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: scale must be finite and > 0");
     for (const vva_tensor* t : {q, k_pages, v_pages, &batch->q_start, &batch->kv_len, &batch->table})
         if (meets(out, t)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: out overlaps q, the pages or the batch");
+    if (meets_itself(out)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: rows of out overlap each other");
     a.q = (const char*)q->data; a.q_nb_h = q->nb[1]; a.q_nb_t = q->nb[2];
     a.out = (char*)out->data; a.o_nb_h = out->nb[1]; a.o_nb_t = out->nb[2];
     a.scale = scale;
@@ -1721,6 +1739,8 @@ extern "C" vva_status vva_add_rms_norm(vva_context* ctx, const vva_tensor* x, co
     if (clash(y, x) || clash(y, add) || clash(sum, x) || clash(sum, add) || overlaps(y, w) || (sum && overlaps(sum, w)) ||
         (sum && meets(sum, y)))
         return fail(ctx, VVA_ERR_INVALID_ARG, "add_rms_norm: outputs overlap each other or an input (only an input itself may alias)");
+    if (meets_itself(y) || (sum && meets_itself(sum)))
+        return fail(ctx, VVA_ERR_INVALID_ARG, "add_rms_norm: rows of an output overlap each other (an input whose rows are one cannot be it)");
     NormArgs a{};
     a.x = (const char*)x->data; a.x_type = x->type; a.x_nb_t = x->nb[1]; a.x_nb_b = x->nb[2];
     if (add) { a.add = (const char*)add->data; a.add_type = add->type; a.add_nb_t = add->nb[1]; a.add_nb_b = add->nb[2]; }
