@@ -407,8 +407,9 @@ VVA_API vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, const v
  *        may be x or add itself where the types match;
  *   y:   ne = [hidden, T, B], F32 / F16 / BF16, or Q8_0 blocks along hidden
  *        (then hidden is a multiple of 32; scale amax / 127, codes
- *        round(y * 127 / amax), as in the Q8_0 caches); may be x or add itself
- *        where the types match.
+ *        round(y * 127 / amax), as in the Q8_0 caches; a block with an infinity
+ *        or a NaN has a NaN scale and codes of 1); may be x or add itself where
+ *        the types match.
  * Outputs otherwise lie apart from each other and the inputs (rows may
  * interleave), and their rows from one another: an add whose rows are one
  * (stride 0) cannot be an output too.  Everything is computed in F32 from the unrounded h.  hidden <= 16384, rows

@@ -1,0 +1,58 @@
+"""Q8_0 rows between the norm and the projections: values that are not finite, blocks whose largest code is not 127."""
+import numpy as np
+import pytest
+
+import vva
+import vvo
+
+pytestmark = pytest.mark.gpu
+
+
+def values(torch, raw):
+    """Scale times code of uint8 blocks [..., 34], [..., 32] in 32 bits (exact)."""
+    return raw[..., :2].contiguous().view(torch.float16).float() * raw[..., 2:].contiguous().view(torch.int8).float()
+
+
+def norm(ctx, torch, x, w, add=None, eps=1e-6):
+    raw = torch.full((*x.shape[:-1], x.shape[-1] // 32, 34), 201, dtype=torch.uint8, device="cuda")
+    ctx.add_rms_norm(x, w, vva.q8_view(raw), add=add, eps=eps)
+    torch.cuda.synchronize()
+    return raw
+
+
+@pytest.mark.parametrize("K", [32, 512, 3584])
+@pytest.mark.parametrize("dt", ["float32", "bfloat16"])
+def test_norm_blocks_that_are_not_finite(ctx, torch_gpu, K, dt):
+    """What the F32 output gives as NaN or infinity the blocks give as NaN, 32 values at a time, and the others as ever."""
+    torch = torch_gpu
+    x = torch.randn(1, 7, K, device="cuda", generator=torch.Generator(device="cuda").manual_seed(K)).to(getattr(torch, dt))
+    w = torch.ones(K, device="cuda")
+    clean = norm(ctx, torch, x, w)
+    x[0, 1, K // 2], x[0, 3, 5], x[0, 4, K - 1] = float("nan"), float("inf"), -float("inf")
+    w2 = w.clone()
+    raw = norm(ctx, torch, x, w)
+    y = torch.empty(1, 7, K, device="cuda")
+    ctx.add_rms_norm(x, w, y)
+    torch.cuda.synchronize()
+    bad = ~torch.isfinite(y.unflatten(-1, (-1, 32))).all(-1)
+    assert bool(bad[0, 1].all()) and int(bad[0, 3].sum()) == int(bad[0, 4].sum()) == 1      # inf: 0 times the others
+    got = values(torch, raw)
+    assert bool(got[bad].isnan().all()) and bool(torch.isfinite(got[~bad]).all())
+    assert bool((raw[..., 2:][bad] == 1).all())
+    assert torch.equal(raw[0, [0, 2, 5, 6]], clean[0, [0, 2, 5, 6]])
+    # a weight that is not finite: its block alone
+    w2[K - 1] = float("inf")
+    raw = norm(ctx, torch, torch.ones(1, 2, K, device="cuda"), w2)
+    got = values(torch, raw)
+    assert bool(got[:, :, -1].isnan().all()) and bool(torch.isfinite(got[:, :, :-1]).all())
+
+
+def test_norm_blocks_of_a_zero_row_without_eps(ctx, torch_gpu):
+    """0 / 0: NaN, as in the other types."""
+    torch = torch_gpu
+    x = torch.zeros(1, 2, 96, device="cuda")
+    x[0, 1] = 1.0
+    got = values(torch, norm(ctx, torch, x, torch.ones(96, device="cuda"), eps=0.0))
+    assert bool(got[0, 0].isnan().all()) and bool((got[0, 1] - 1.0).abs().max() <= 2.0 ** -11)
+    got = values(torch, norm(ctx, torch, x, torch.ones(96, device="cuda"), eps=1e-6))
+    assert bool((got[0, 0] == 0).all())
