@@ -179,10 +179,17 @@ def view(t, ggml_ne=None, ggml_nb=None, type_=None) -> Tensor:
 
 
 def q8_view(raw) -> Tensor:
-    """View of uint8 blocks [B, T, hidden / 32, 34] (rows contiguous) as Q8_0 rows ne = [hidden, T, B]."""
+    """View of uint8 blocks [B, T, hidden / 32, 34] (rows contiguous) as Q8_0 rows ne = [hidden, T, B]; it keeps them alive."""
+    torch = _torch()
+    if (raw.dtype != torch.uint8 or raw.dim() != 4 or raw.shape[3] != Q8_BLOCK_BYTES or raw.stride(3) != 1 or
+            (raw.shape[2] > 1 and raw.stride(2) != Q8_BLOCK_BYTES)):
+        raise ValueError(f"q8_view: uint8 [B, T, hidden / 32, {Q8_BLOCK_BYTES}] with contiguous rows, not {raw.dtype} "
+                         f"{tuple(raw.shape)} of strides {raw.stride()}")
     B, T, n, _ = raw.shape
-    return view(raw, ggml_ne=[n * 32, T, B, 1],
-                ggml_nb=[Q8_BLOCK_BYTES, raw.stride(1), raw.stride(0), raw.stride(0) * B], type_=Q8_0)
+    v = view(raw, ggml_ne=[n * 32, T, B, 1],
+             ggml_nb=[Q8_BLOCK_BYTES, raw.stride(1), raw.stride(0), raw.stride(0) * B], type_=Q8_0)
+    v.raw = raw
+    return v
 
 
 def _rows_view(x) -> Tensor:
