@@ -56,3 +56,45 @@ def test_norm_blocks_of_a_zero_row_without_eps(ctx, torch_gpu):
     assert bool(got[0, 0].isnan().all()) and bool((got[0, 1] - 1.0).abs().max() <= 2.0 ** -11)
     got = values(torch, norm(ctx, torch, x, torch.ones(96, device="cuda"), eps=1e-6))
     assert bool((got[0, 0] == 0).all())
+
+
+def weights(torch, rng, K, rows):
+    return [vva.Weight(torch.from_numpy(vvo.from_f32((rng.standard_normal((m, K)) * K ** -0.5).astype(np.float32), vva.Q8_0)).cuda(),
+                       vva.Q8_0, K, m) for m in rows]
+
+
+def project(ctx, torch, x, ws, T, Hq, Hkv, d, ct):
+    """q and the cache rows of vva_qkv_rope_append, as arrays."""
+    kv = vva.KVCache(ctx, 1, Hkv, d, T, 1, ct)
+    q = torch.empty(1, T, Hq, d, device="cuda")
+    ctx.qkv_rope_append(kv, 0, x, *ws, torch.arange(T, dtype=torch.int32, device="cuda"), q)
+    torch.cuda.synchronize()
+    got = [q[0].cpu().numpy()] + [np.asarray(r).reshape(T, -1).copy() for r in kv.download(0, 0, T)]
+    kv.free()
+    return got
+
+
+@pytest.mark.parametrize("hidden", [896, 4480])
+@pytest.mark.parametrize("T", [1, 3, 8, 9, 40, 1100])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+def test_projections_of_blocks_that_are_not_finite(ctx, torch_gpu, hidden, T, bad):
+    """A NaN in a row of the hidden state: the row's q, k and v are NaN, the other rows' the bits they were."""
+    torch = torch_gpu
+    Hq, Hkv, d = 14, 2, 64
+    ws = weights(torch, np.random.default_rng(hidden), hidden, (Hq * d, Hkv * d, Hkv * d))
+    x = torch.randn(1, T, hidden, device="cuda", generator=torch.Generator(device="cuda").manual_seed(T))
+    w = torch.ones(hidden, device="cuda")
+    ref = project(ctx, torch, vva.q8_view(norm(ctx, torch, x, w)), ws, T, Hq, Hkv, d, vva.F32)
+    x[0, T // 2, 77] = float(bad)
+    raw = norm(ctx, torch, x, w)
+    got = project(ctx, torch, vva.q8_view(raw), ws, T, Hq, Hkv, d, vva.F32)
+    keep = [t for t in range(T) if t != T // 2]
+    for a, b in zip(got, ref):
+        a, b = (v.view(np.float32).reshape(T, -1) for v in (a, b))
+        assert np.isnan(a[T // 2]).all()
+        assert a[keep].tobytes() == b[keep].tobytes()
+    if hidden <= 4096 and T <= 8:
+        y = torch.empty(1, T, (Hq + 2 * Hkv) * d, device="cuda")
+        ctx.qkv_proj(vva.q8_view(raw), *ws, y)
+        torch.cuda.synchronize()
+        assert bool(y[0, T // 2].isnan().all()) and bool(torch.isfinite(y[0, keep]).all())

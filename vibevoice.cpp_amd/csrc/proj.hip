@@ -270,13 +270,20 @@ __device__ __forceinline__ void q8_load8(const char* row, int k, float (&x)[8]) 
 }
 
 // Rows of Q8_0 blocks as F32 [N][K], for the few-row kernels, which quantize
-// rows themselves: a block's values give the same scale and codes again.
+// rows themselves: a block's values give the same scale and codes again.  A block
+// whose scale is not finite goes as infinities: the largest magnitude that those
+// kernels look for passes over a NaN, but of an infinity their products are NaN.
 __global__ void __launch_bounds__(256) proj_rows_from_q8_kernel(ProjPrepArgs a, float* __restrict__ dst) {
     const int n = blockIdx.y, b = n / a.T, t = n - b * a.T;
     const int k = (blockIdx.x * 256 + threadIdx.x) * 8;
     if (k >= a.K) return;
     float x[8];
     q8_load8(a.x + b * a.x_nb_b + t * a.x_nb_t, k, x);
+    const uint16_t d = *(const uint16_t*)(a.x + b * a.x_nb_b + t * a.x_nb_t + (int64_t)(k / kQK8) * kQ8Bytes);
+    if ((d & 0x7c00u) == 0x7c00u) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = INFINITY;
+    }
     float4* p = (float4*)(dst + (int64_t)n * a.K + k);
     p[0] = make_float4(x[0], x[1], x[2], x[3]);
     p[1] = make_float4(x[4], x[5], x[6], x[7]);
