@@ -264,7 +264,10 @@ VVA_API vva_status vva_flash_attn_ext(vva_context* ctx, const vva_tensor* q, con
  *   x:  ne = [hidden, T, B] (F32 / F16 / BF16), the normed layer input xn;
  *       with Q8_0 weights also Q8_0 rows, as vva_add_rms_norm writes them
  *       (2-byte aligned; the results are those of F32 rows of the blocks'
- *       values, scale times code);
+ *       values, scale times code: blocks whose largest code is not 127, which
+ *       no rounding to Q8_0 makes, are rounded once more; a scale that is NaN
+ *       or infinite gives NaN.  Up to 8 rows are made F32 rows first, by a
+ *       launch of their own: there F32 rows of the norm are the shorter way);
  *   wq: ne = [hidden, Hq*d], wk, wv: ne = [hidden, Hkv*d], all F16 or all
  *       Q8_0 (GGUF blocks along hidden), rows contiguous (F16: 16-byte
  *       aligned rows, Q8_0: 4-byte aligned);

@@ -92,9 +92,36 @@ def test_projections_of_blocks_that_are_not_finite(ctx, torch_gpu, hidden, T, ba
     for a, b in zip(got, ref):
         a, b = (v.view(np.float32).reshape(T, -1) for v in (a, b))
         assert np.isnan(a[T // 2]).all()
-        assert a[keep].tobytes() == b[keep].tobytes()
+        assert (a[keep].view(np.uint32) == b[keep].view(np.uint32)).all()
     if hidden <= 4096 and T <= 8:
         y = torch.empty(1, T, (Hq + 2 * Hkv) * d, device="cuda")
         ctx.qkv_proj(vva.q8_view(raw), *ws, y)
         torch.cuda.synchronize()
         assert bool(y[0, T // 2].isnan().all()) and bool(torch.isfinite(y[0, keep]).all())
+
+
+@pytest.mark.parametrize("hidden,T", [(896, 1), (896, 8), (896, 9), (896, 130), (896, 1100), (4480, 3), (3584, 60)])
+@pytest.mark.parametrize("kind", ["small", "-128", "random", "tiny"])
+def test_projections_of_blocks_no_rounding_made(ctx, torch_gpu, hidden, T, kind):
+    """Blocks whose largest code is below 127 or is -128: the bits of F32 rows of their values, at every count of rows."""
+    torch = torch_gpu
+    Hq, Hkv, d = 14, 2, 64
+    rng = np.random.default_rng(T)
+    ws = weights(torch, rng, hidden, (Hq * d, Hkv * d, Hkv * d))
+    lo, hi = {"small": (-77, 78), "-128": (-128, -127), "random": (-128, 128), "tiny": (-1, 2)}[kind]
+    codes = rng.integers(lo, hi, (1, T, hidden // 32, 32)).astype(np.int8)
+    if kind == "-128":
+        codes[..., 3:9], codes[..., 9] = 50, 100
+    scales = (rng.random((1, T, hidden // 32, 1)) * 0.05 + 1e-4).astype(np.float16)
+    scales[0, 0, 0] = 0.0
+    raw = torch.from_numpy(np.concatenate([scales.view(np.uint8), codes.view(np.uint8)], -1)).cuda()
+    rows = values(torch, raw).flatten(2)
+    a, b = (project(ctx, torch, x, ws, T, Hq, Hkv, d, vva.F32) for x in (vva.q8_view(raw), rows))
+    for x, y in zip(a, b):
+        assert (x.view(np.uint8) == y.view(np.uint8)).all()
+    if hidden <= 4096 and T <= 8:
+        ys = [torch.empty(1, T, (Hq + 2 * Hkv) * d, device="cuda") for _ in range(2)]
+        for x, y in zip((vva.q8_view(raw), rows), ys):
+            ctx.qkv_proj(x, *ws, y)
+        torch.cuda.synchronize()
+        assert torch.equal(*ys)

@@ -8,8 +8,8 @@
 //
 // Numerics follow ggml's CPU mul_mat: x is first converted to the weight's
 // vec-dot type by proj_prep_kernel (F16 weights: x rounded to f16; Q8_0
-// weights: x quantized to Q8_0 blocks, or given in them, kept as f16 d_x * q
-// values), then
+// weights: x, or the values of its Q8_0 blocks, quantized to Q8_0 blocks, kept as
+// f16 d_x * q values), then
 // every product of f16 operands is exact in the fp32 MFMA accumulators.
 // Q8_0 weight blocks are dequantized to f16 d_w * q values while the tile is
 // staged in LDS.  (The two f16 roundings of d * q are the only departure from
@@ -270,9 +270,10 @@ __device__ __forceinline__ void q8_load8(const char* row, int k, float (&x)[8]) 
 }
 
 // Rows of Q8_0 blocks as F32 [N][K], for the few-row kernels, which quantize
-// rows themselves: a block's values give the same scale and codes again.  A block
-// whose scale is not finite goes as infinities: the largest magnitude that those
-// kernels look for passes over a NaN, but of an infinity their products are NaN.
+// rows themselves (a block's values give the same scale and codes again, if its
+// largest code is 127).  A block whose scale is not finite goes as infinities:
+// the largest magnitude that those kernels look for passes over a NaN, but of an
+// infinity their products are NaN.
 __global__ void __launch_bounds__(256) proj_rows_from_q8_kernel(ProjPrepArgs a, float* __restrict__ dst) {
     const int n = blockIdx.y, b = n / a.T, t = n - b * a.T;
     const int k = (blockIdx.x * 256 + threadIdx.x) * 8;
@@ -304,7 +305,9 @@ __global__ void __launch_bounds__(256) proj_prep_kernel(ProjPrepArgs a) {
     // 16-byte aligned row is read with vector loads, two passes' loads out
     // together (K <= 4096); otherwise element by element.
     const bool f32 = a.x_type == VVA_TYPE_F32, bf = a.x_type == VVA_TYPE_BF16;
-    // Q8_0 rows (a norm's output) hold their round trip already: code times scale
+    // Q8_0 rows (a norm's output): their values, quantized as F32 rows of them are.
+    // Blocks whose largest code is 127, as every rounding makes them, stay what
+    // they are; any others change alike at every count of rows.
     const bool blocks = a.x_type == VVA_TYPE_Q8_0;
     const bool vec = !blocks && ((uintptr_t)src & 15) == 0;
     u32x4 raw[2][2];
@@ -332,7 +335,7 @@ __global__ void __launch_bounds__(256) proj_prep_kernel(ProjPrepArgs a) {
             for (int e = 0; e < 8; ++e) x[e] = load_elem(src + (k0 + e) * es, a.x_type);
         }
         uint16_t h[8];
-        if (a.q8 && !blocks) {
+        if (a.q8) {
             float am = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(x[e]));
