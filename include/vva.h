@@ -328,8 +328,9 @@ VVA_API vva_status vva_out_proj_residual(vva_context* ctx, const vva_tensor* o, 
  *   table:   I32 ne = [max_pages, n_seq], contiguous rows of any stride: page
  *            table[s][i / page_size] of the pool holds key i in its slot
  *            i % page_size.  Entries past a sequence's keys are not read.
- *   max_new: no sequence of the call brings more new tokens (the rows of one
- *            that does are computed up to here).
+ *   max_new: no sequence of the call brings more new tokens.  The attention
+ *            picks its kernels by it and computes the rows of a sequence that
+ *            does up to here; the append takes all of its tokens.
  * n_seq <= VVA_MAX_BATCH_SEQ.  The tensors must not change while a call runs
  * (write them in stream order).  Values that point outside are kept inside:
  * q_start is cut to the token rows there are, kv_len to the table's row. */

@@ -1,9 +1,10 @@
-"""Batches of more than 64 sequences (the kernels look 64 of them up at a time)."""
+"""Batches of more than 64 sequences (the kernels look 64 of them up at a time), and tokens beyond
+max_new."""
 import numpy as np
 import pytest
 
 import vva
-from paged_util import Pages
+from paged_util import Pages, attention, check_rows
 from test_gpu_paged import append, run_attn
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +73,20 @@ def test_few_beside_many_of_many_sequences(ctx, torch_gpu):
     for s in (3, 63, 64, 100, 149):
         lens[s] = (40 + s, 900 + s)
     run_attn(ctx, Pages(torch_gpu, lens, *H7, vva.F16, 64, seed=5, extra_rows=3))
+
+
+@pytest.mark.parametrize("max_new", [1, 2, 40])
+def test_tokens_beyond_max_new(ctx, torch_gpu, max_new):
+    """The attention computes a sequence's first max_new tokens; the append takes all of them."""
+    torch = torch_gpu
+    P = Pages(torch, [(2, 40), (50, 60)], *H05, vva.F16, 16, seed=15, extra_rows=1)
+    P.max_new = max_new
+    append(ctx, P, vva.F16)
+    out = torch.full_like(P.q, 5.0)
+    ctx.paged_attn(P.q, P.k, P.v, P.batch(), 0.125, out)
+    torch.cuda.synchronize()
+    ref, tol = attention(P, 0.125)
+    a, b = min(max_new, 2), 2 + max_new
+    check_rows(out[:a], ref[:a], tol[:a])
+    check_rows(out[2:b], ref[2:b], tol[2:b])
+    assert bool((out[a:2] == 5.0).all()) and bool((out[b:] == 5.0).all())
