@@ -388,11 +388,11 @@ VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, 
  * of +inf or NaN, or of -inf alone, give NaN; keys of -inf beside others are
  * left out.
  * The products run on the matrix cores in the pages' type with F32 sums; the
- * softmax is F32.  Its probabilities go into them in two parts of that type
- * where a sequence's new tokens times Hq / Hkv are at most 32 (within 2^-16 of
- * themselves in BF16, 2^-22 in F16), else, and in calls of n_seq * max_new
- * tokens where max_new * Hq / Hkv is above 32, rounded to it (2^-8, 2^-11; in
- * F16 by up to 2^-32 of a row's largest where that is more).
+ * softmax is F32.  Its probabilities are rounded to that type (F16: 2^-11, or
+ * 2^-32 of the row's largest where that is more; BF16: 2^-8), but for BF16 go
+ * into the products in two parts (2^-15) where a sequence's new tokens times
+ * Hq / Hkv are at most 32 (not in calls of n_seq * max_new tokens whose max_new
+ * times that is more).
  * Every row of q and out and every page row starts on 16 bytes.
  * Partial sums go through the context's workspace, as those of the other
  * calls: under stream capture a call larger than any before it is refused

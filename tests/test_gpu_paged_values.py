@@ -155,24 +155,41 @@ def test_keys_of_minus_infinity_are_left_out(ctx, torch_gpu, lens, heads):
         check_rows(out[:n, h], ref, tol)
 
 
-@pytest.mark.parametrize("t,digits", [(vva.F16, 2.0 ** -22), (vva.BF16, 2.0 ** -16)])
 @pytest.mark.parametrize("lens,heads,scale", [([(1, 130), (2, 40)], H7, 1.0), ([(4, 3001)], H7, 0.5), ([(1, 20000), (3, 77)], H05, 0.2),
                                               ([(2, 700), (90, 200)], H05, 0.3), ([(1, 5)] * 80, H05, 1.0)])
-def test_few_rows_keep_the_digits_of_their_probabilities(ctx, torch_gpu, monkeypatch, t, digits, lens, heads, scale):
-    """Sequences of at most 32 rows of a kv group: probabilities in two parts of the pages' type, each within half a step of
-    what it stands for (F16: of 2^7 times the share of the largest, down to its smallest step)."""
+def test_few_rows_keep_the_digits_of_bf16_probabilities(ctx, torch_gpu, monkeypatch, lens, heads, scale):
+    """Sequences of at most 32 rows of a kv group: probabilities p in two BF16 parts.  The first is p cut to 8 digits, which
+    leaves less than 2^-7 p (and 2^-23 p that is added); the second is that, rounded by 2^-8 of it: together 2^-15 p."""
     torch = torch_gpu
-    print(lens[:3], heads, t, scale, flush=True)
-    P = Pages(torch, lens, *heads, t, 16, seed=17)
+    print(lens[:3], heads, scale, flush=True)
+    P = Pages(torch, lens, *heads, vva.BF16, 16, seed=17)
     out = torch.empty_like(P.q)
     ctx.paged_attn(P.q, P.k, P.v, P.batch(), scale, out)
     torch.cuda.synchronize()
-    last = paged_util.HALF[t], paged_util.TINY[t]
-    monkeypatch.setitem(paged_util.HALF, t, digits)
-    monkeypatch.setitem(paged_util.TINY, t, 2.0 ** -32 if t == vva.F16 else 0.0)
+    last = paged_util.HALF[vva.BF16]
+    monkeypatch.setitem(paged_util.HALF, vva.BF16, 2.0 ** -15 * (1 + 2.0 ** -6))
     ref, tol = attention(P, scale)
     for s, (n, _) in enumerate(lens):
         if n * (heads[0] // heads[1]) <= 32:
             r = slice(int(P.starts[s]), int(P.starts[s]) + n)
             # and the output's one rounding
-            check_rows(out[r], ref[r], tol[r] + last[0] * (ref[r].abs() + tol[r]) + last[1], f"sequence {s}")
+            check_rows(out[r], ref[r], tol[r] + last * (ref[r].abs() + tol[r]), f"sequence {s}")
+
+
+@pytest.mark.parametrize("t", [vva.F16, vva.BF16])
+@pytest.mark.parametrize("lens,heads", NAN_SETS)
+def test_infinite_value_gives_its_infinity(ctx, torch_gpu, lens, heads, t):
+    """V infinite at a key that every token sees, +inf in some dims and -inf in others: those dims answer with its sign, the
+    others keep their bits."""
+    torch = torch_gpu
+    print(lens[:3], heads, t, flush=True)
+    P = Pages(torch, lens, *heads, t, 16, seed=6, scale=0.3)
+    ref = call(ctx, P)
+    n, L = lens[0]
+    for j in {0, (L - n) // 2, max(0, L - n - 1)}:
+        row = P.v[int(P.table_host[0, j // 16]), :, j % 16]
+        row[:, 3], row[:, 40] = float("inf"), -float("inf")
+    out = call(ctx, P)
+    assert bool((out[:n, :, 3] == float("inf")).all()) and bool((out[:n, :, 40] == -float("inf")).all())
+    keep = [i for i in range(P.d) if i not in (3, 40)]
+    assert torch.equal(out[:n][..., keep], ref[:n][..., keep]) and torch.equal(out[n:], ref[n:])

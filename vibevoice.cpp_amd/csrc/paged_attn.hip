@@ -34,11 +34,11 @@
 // weights down to 2^-21 of the row's largest are rounded by a relative 2^-11,
 // smaller ones by 2^-32 of it (without the factor a weight of e^-17 is 44 % off,
 // and a long cache has many).  The row sum adds the rounded values, so the weights
-// of a row sum to one.  Few rows, which wait for the cache's bytes, multiply what
-// the rounding left as well, in a second product with the same V: their P have
-// twice the digits (2^-16 in BF16, 2^-22 in F16) for 1 to 3 % of the time (48
-// sequences of 500 to 8000 keys 73.2 -> 74.0 us).  Beside the many rows' scores it
-// would be a half more matrix work where that is the bound: there one rounding stays.
+// of a row sum to one.  Few rows of BF16 pages, which wait for the cache's bytes,
+// multiply what the rounding leaves as well, in a second product with the same V:
+// their P are within 2^-15 (48 sequences of 500 to 8000 keys 72.7 -> 72.9 us).  Beside the
+// many rows' scores it would be a half more matrix work where that is the bound:
+// there one rounding stays.
 //
 // K and V rows go from the pages straight into LDS (global_load_lds, 1 KB =
 // 4 rows of 128 dims an instruction, no registers), 16-byte chunk c of row r
@@ -143,16 +143,15 @@ template <int KT>
 __device__ __forceinline__ float sum2(uint32_t p, float acc) {
     return KT == VVA_TYPE_BF16 ? dot2_bf16(p, 0x3f803f80u, acc) : dot2_f16(p, 0x3c003c00u, acc);
 }
-// x, y less the pair that pack2 made of them, packed: what the rounding left
-template <int KT>
-__device__ __forceinline__ uint32_t rest2(float x, float y, uint32_t p) {
-    if constexpr (KT == VVA_TYPE_BF16) {
-        return pack2<KT>(x - __uint_as_float(p << 16), y - __uint_as_float(p & 0xffff0000u));
-    } else {
-        h2 v;
-        __builtin_memcpy(&v, &p, 4);
-        return pack2<KT>(x - (float)v.x, y - (float)v.y);
-    }
+// Two probabilities x, y >= 0 in two BF16 parts each: the upper half of the
+// float's bits, and the rest.  The rest is above 0 wherever x is (x goes into it
+// a step of 2^-23 larger, as into the row sum), so that the products with an
+// infinite V have its sign alone.
+__device__ __forceinline__ void split2_bf16(float x, float y, uint32_t& p, uint32_t& rest) {
+    const uint32_t hx = __float_as_uint(x) & 0xffff0000u, hy = __float_as_uint(y) & 0xffff0000u;
+    constexpr float up = 1.0f + 0x1p-23f;
+    p = (hx >> 16) | hy;
+    rest = pack2<VVA_TYPE_BF16>(fmaf(x, up, -__uint_as_float(hx)), fmaf(y, up, -__uint_as_float(hy)));
 }
 // whether either half of x is infinite or NaN, and x with such halves zeroed
 template <int KT>
@@ -481,13 +480,18 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
             }
         }
         const float nb = kLift<KT> - (m == -INFINITY ? 0.0f : m);
-        uint32_t p[8], rest[8];
+        uint32_t p[8];
+        [[maybe_unused]] uint32_t rest[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
             const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * r], sl2, nb)), y = __builtin_amdgcn_exp2f(fmaf(s[2 * r + 1], sl2, nb));
-            p[r] = pack2<KT>(x, y);
-            rest[r] = rest2<KT>(x, y, p[r]);
-            lsum = sum2<KT>(rest[r], sum2<KT>(p[r], lsum));
+            if constexpr (KT == VVA_TYPE_BF16) {
+                split2_bf16(x, y, p[r], rest[r]);
+                lsum = sum2<KT>(rest[r], lsum);
+            } else {
+                p[r] = pack2<KT>(x, y);
+            }
+            lsum = sum2<KT>(p[r], lsum);
         }
         if (more) wait_vm<NC>();                   // V; the next K may still fly
         else wait_vm<0>();
@@ -495,13 +499,14 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             const QF pf = as_vec<QF>(u32x4{p[4 * kk], p[4 * kk + 1], p[4 * kk + 2], p[4 * kk + 3]});
-            const QF rf = as_vec<QF>(u32x4{rest[4 * kk], rest[4 * kk + 1], rest[4 * kk + 2], rest[4 * kk + 3]});
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 const uint32_t v = ((vs + v_off) ^ (dt << 6)) + kk * 16 * 2 * D;
                 u32x4 vf = v_bits<KT>(lds_at(v), lds_at(v + 8 * 2 * D));
                 if (fix) vf = u32x4{finite2<KT>(vf.x), finite2<KT>(vf.y), finite2<KT>(vf.z), finite2<KT>(vf.w)};
-                o[dt] = F::mma(as_vec<QF>(vf), rf, F::mma(as_vec<QF>(vf), pf, o[dt]));
+                o[dt] = F::mma(as_vec<QF>(vf), pf, o[dt]);
+                if constexpr (KT == VVA_TYPE_BF16)
+                    o[dt] = F::mma(as_vec<QF>(vf), as_vec<QF>(u32x4{rest[4 * kk], rest[4 * kk + 1], rest[4 * kk + 2], rest[4 * kk + 3]}), o[dt]);
             }
         }
         if (fix) add_not_finite<D, KT, kFewTile>(vs, k0, lim, half, o);
