@@ -16,8 +16,8 @@
 // both kinds and is paged_mixed_kernel, which runs them side by side.
 //
 // Reached, of a copy's 4.9 TB/s and a large product's 1175 TFLOP/s: single
-// tokens 5.6 TB/s (48 sequences of 500 to 8000 keys, 405 MB, 72 us); 2048 tokens
-// behind 28672 keys 1000 TFLOP/s (872 us), 512 behind 15872 874 (135 us).
+// tokens 5.5 TB/s (48 sequences of 500 to 8000 keys, 405 MB, 73 us); 2048 tokens
+// behind 28672 keys 991 TFLOP/s (880 us), 512 behind 15872 858 (138 us).
 //
 // Both compute, per 32 rows and a tile of keys, with
 // v_mfma_f32_32x32x16_{f16,bf16} (layouts in mfma_ops.hpp):
@@ -36,9 +36,9 @@
 // and a long cache has many).  The row sum adds the rounded values, so the weights
 // of a row sum to one.  Few rows of BF16 pages, which wait for the cache's bytes,
 // multiply what the rounding leaves as well, in a second product with the same V:
-// their P are within 2^-15 (48 sequences of 500 to 8000 keys 72.7 -> 72.9 us).  Beside the
-// many rows' scores it would be a half more matrix work where that is the bound:
-// there one rounding stays.
+// their P are within 2^-15 (48 sequences of 500 to 8000 keys 72.1 -> 72.9 us).
+// Many rows, with 250 of 256 registers in use and the arithmetic their bound,
+// round once.
 //
 // K and V rows go from the pages straight into LDS (global_load_lds, 1 KB =
 // 4 rows of 128 dims an instruction, no registers), 16-byte chunk c of row r
