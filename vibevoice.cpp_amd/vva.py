@@ -349,9 +349,17 @@ class Context:
         call.keep = (keep, args)
         return call
 
+    def _here(self, *tensors):
+        """Refuses what does not lie on the context's device: tensors, a batch's, the blocks of a q8_view."""
+        for t in tensors:
+            for x in t.tensors if isinstance(t, Batch) else (getattr(t, "raw", None) if isinstance(t, Tensor) else t,):
+                if x is not None and (x.device.type, x.device.index) != ("cuda", self.device):
+                    raise ValueError(f"a tensor on {x.device}, where the context is on cuda:{self.device}")
+
     def bind_paged_rope_append(self, q, k, v, rope, batch: Batch, k_pages, v_pages, q_out, pos=None):
         """q, q_out: [N, Hq, d]; k, v: [N, Hkv, d] packed tokens; rope f32 [n_pos, d] (cos, then sin); pos int32 [N] or
         None; k_pages, v_pages: [n_pages, Hkv, page_size, d].  Returns the call."""
+        self._here(q, k, v, rope, pos, batch, k_pages, v_pages, q_out)
         return self._bound(self.lib.vva_paged_rope_append, (q, k, v, rope, pos, batch, k_pages, v_pages, q_out), view(q),
                            view(k), view(v), view(rope), view(pos) if pos is not None else None, batch.c, view(k_pages),
                            view(v_pages), view(q_out))
@@ -363,6 +371,7 @@ class Context:
     def bind_paged_attn(self, q, k_pages, v_pages, batch: Batch, scale: float, out):
         """q, out: [N, Hq, d] packed tokens in the pages' dtype; k_pages, v_pages: [n_pages, Hkv, page_size, d].  Returns
         the call."""
+        self._here(q, k_pages, v_pages, batch, out)
         return self._bound(self.lib.vva_paged_attn, (q, k_pages, v_pages, batch, out), view(q), view(k_pages),
                            view(v_pages), batch.c, scale, view(out))
 
@@ -373,6 +382,7 @@ class Context:
     def bind_add_rms_norm(self, x, w, y, add=None, total=None, eps: float = 1.0e-6):
         """x, add, total (receives x + add): [B, T, hidden]; w f32 [hidden]; y: a tensor like x or q8_view(...) of Q8_0
         blocks.  Returns the call."""
+        self._here(x, w, y, add, total)
         return self._bound(self.lib.vva_add_rms_norm, (x, w, y, add, total), view(x),
                            view(add) if add is not None else None, view(w), eps,
                            view(total) if total is not None else None, _rows_view(y))
