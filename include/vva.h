@@ -264,9 +264,9 @@ VVA_API vva_status vva_flash_attn_ext(vva_context* ctx, const vva_tensor* q, con
  *   x:  ne = [hidden, T, B] (F32 / F16 / BF16), the normed layer input xn;
  *       with Q8_0 weights also Q8_0 rows, as vva_add_rms_norm writes them
  *       (2-byte aligned; the results are those of F32 rows of the blocks'
- *       values, scale times code: blocks whose largest code is not 127, which
- *       no rounding to Q8_0 makes, are rounded once more; a scale that is NaN
- *       or infinite gives NaN.  Up to 8 rows are made F32 rows first, by a
+ *       values, scale times code: blocks whose largest code is not 127 or
+ *       -127, which no rounding to Q8_0 makes, are rounded once more; a scale
+ *       that is NaN or infinite gives NaN.  Up to 8 rows are made F32 rows first, by a
  *       launch of their own: there F32 rows of the norm are the shorter way);
  *   wq: ne = [hidden, Hq*d], wk, wv: ne = [hidden, Hkv*d], all F16 or all
  *       Q8_0 (GGUF blocks along hidden), rows contiguous (F16: 16-byte
@@ -416,8 +416,9 @@ VVA_API vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, const v
  *        the types match.
  * Outputs otherwise lie apart from each other and the inputs (rows may
  * interleave), and their rows from one another: an add whose rows are one
- * (stride 0) cannot be an output too.  Everything is computed in F32 from the unrounded h.  hidden <= 16384, rows
- * contiguous, any strides between them; eps >= 0. */
+ * (stride 0) cannot be an output too.  Everything is computed in F32 from the
+ * unrounded h.  hidden <= 16384, rows contiguous, any strides between them;
+ * eps >= 0. */
 VVA_API vva_status vva_add_rms_norm(vva_context* ctx, const vva_tensor* x, const vva_tensor* add, const vva_tensor* w,
                                     float eps, const vva_tensor* sum, const vva_tensor* y);
 

@@ -271,7 +271,7 @@ __device__ __forceinline__ void q8_load8(const char* row, int k, float (&x)[8]) 
 
 // Rows of Q8_0 blocks as F32 [N][K], for the few-row kernels, which quantize
 // rows themselves (a block's values give the same scale and codes again, if its
-// largest code is 127).  A block whose scale is not finite goes as infinities:
+// largest code is 127 or -127).  A block whose scale is not finite goes as infinities:
 // the largest magnitude that those kernels look for passes over a NaN, but of an
 // infinity their products are NaN.
 __global__ void __launch_bounds__(256) proj_rows_from_q8_kernel(ProjPrepArgs a, float* __restrict__ dst) {
@@ -306,8 +306,8 @@ __global__ void __launch_bounds__(256) proj_prep_kernel(ProjPrepArgs a) {
     // together (K <= 4096); otherwise element by element.
     const bool f32 = a.x_type == VVA_TYPE_F32, bf = a.x_type == VVA_TYPE_BF16;
     // Q8_0 rows (a norm's output): their values, quantized as F32 rows of them are.
-    // Blocks whose largest code is 127, as every rounding makes them, stay what
-    // they are; any others change alike at every count of rows.
+    // Blocks whose largest code is 127 or -127, as every rounding makes them, stay
+    // what they are; any others change alike at every count of rows.
     const bool blocks = a.x_type == VVA_TYPE_Q8_0;
     const bool vec = !blocks && ((uintptr_t)src & 15) == 0;
     u32x4 raw[2][2];
