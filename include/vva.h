@@ -342,11 +342,17 @@ typedef struct {
 } vva_batch;
 
 /* A layer's cache in pages is two tensors of the caller's, one for K and one
- * for V: ne = [head_dim, page_size, n_kv_heads, n_pages], F16 or BF16, rows
- * contiguous, any other strides (of 16 bytes' multiples; the memory order
- * [page][head][slot][dim] of a contiguous tensor streams best).  head_dim is 64
- * or 128, page_size a power of two from 16 to 1024.  Sequences may share pages
- * they only read.
+ * for V: ne = [head_dim, page_size, n_kv_heads, n_pages], F16, BF16 or Q8_0
+ * (both alike), rows contiguous, any other strides (of 16 bytes' multiples; the
+ * memory order [page][head][slot][dim] of a contiguous tensor streams best).
+ * head_dim is 64 or 128, page_size a power of two from 16 to 1024.  Sequences
+ * may share pages they only read.
+ * Q8_0 pages hold the values of Q8_0 blocks (32 dims: codes times their F16
+ * scale) in an order of their own: a page of a head is one run of page_size *
+ * head_dim / 32 * 34 bytes, first page_size rows of head_dim codes (int8), then
+ * head_dim / 32 rows of page_size scales, row b those of dims 32 b .. 32 b + 31.
+ * nb[0] is 34, nb[1] head_dim / 32 * 34 (a row's share of the run), data, nb[2]
+ * and nb[3] multiples of 16.
  * Beyond that the calls take at most 2^22 token rows, 256 query heads per kv
  * head, (n_seq + 1) * n_kv_heads <= 65536, and a table of at most 2^30 keys per
  * sequence and 2^34 in all; larger ones get VVA_ERR_NOT_IMPLEMENTED. */
@@ -362,7 +368,9 @@ typedef struct {
  *   pos: I32 ne = [N], or NULL: each token's index in its sequence;
  *   q_out: ne = [d, Hq, N], F32 / F16 / BF16 (may be q itself where the types
  *      match), receives RoPE(q).
- * Writes RoPE(k) and v, rounded to the pages' type, to the tokens' slots.
+ * Writes RoPE(k) and v, rounded to the pages' type, to the tokens' slots (Q8_0:
+ * scale amax / 127, codes round(y * 127 / amax), as in the Q8_0 caches; a block
+ * with an infinity or a NaN has a NaN scale and codes of 1).
  * A token whose page id is outside the pool, or which belongs to no sequence,
  * or lies before key 0, is not appended; a position outside the table gives
  * NaN.  q_out rows of no sequence are left as they were.  The pages lie apart
@@ -376,8 +384,9 @@ VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, 
 /* Causal grouped-query attention of a batch's new tokens over the pages:
  * vva_attn for packed sequences, each with any number of new tokens behind any
  * number of keys (whole prompts, chunks and single tokens in one call).
- *   q:   ne = [d, Hq, N], already RoPE'd, in the pages' type;
- *   out: ne = [d, Hq, N], in that type too, its rows apart from one another and
+ *   q:   ne = [d, Hq, N], already RoPE'd, in the pages' type (over Q8_0 pages
+ *        F16 or BF16);
+ *   out: ne = [d, Hq, N], in q's type, its rows apart from one another and
  *        from the memory of every input; rows of q less than 4 MiB apart;
  *   scale: a finite number above 0.
  * Token t of sequence s sees keys 0 .. kv_len[s] - n_s + t; one that sees none
@@ -393,6 +402,9 @@ VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, 
  * into the products in two parts (2^-15) where a sequence's new tokens times
  * Hq / Hkv are at most 32 (not in calls of n_seq * max_new tokens whose max_new
  * times that is more).
+ * Over Q8_0 pages the products and probabilities are those of F16 pages that
+ * hold scale times code rounded to F16 (infinite beyond 65504), and BF16 q are
+ * taken as F16 too (their 8 bits are kept from 2^-17 to 65504).
  * Every row of q and out and every page row starts on 16 bytes.
  * Partial sums go through the context's workspace, as those of the other
  * calls: under stream capture a call larger than any before it is refused
@@ -401,6 +413,19 @@ VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, 
 VVA_API vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, const vva_tensor* k_pages,
                                   const vva_tensor* v_pages, const vva_batch* batch, float scale,
                                   const vva_tensor* out);
+
+/* Keys and values of a batch's tokens read back out of the pages, to keep or
+ * move a sequence's cache (a voice prompt, a parked request, vva_kv_upload):
+ *   k, v: ne = [d, Hkv, N], F32 / F16 / BF16, 16-byte aligned rows, either NULL
+ *         (not read).
+ * Row q_start[s] + t receives key kv_len[s] - n_s + t of sequence s, as the pages
+ * hold it (Q8_0: scale times code), rounded to the row's type: with n_s =
+ * kv_len[s] the whole sequence.  Rows whose page id is outside the pool, and
+ * those of keys before key 0, get NaN; rows of no sequence are left as they were.
+ * All tokens of a sequence are read, whatever max_new is.  The outputs lie apart
+ * from the pages, the batch and each other (k and v may interleave). */
+VVA_API vva_status vva_paged_read(vva_context* ctx, const vva_batch* batch, const vva_tensor* k_pages,
+                                  const vva_tensor* v_pages, const vva_tensor* k, const vva_tensor* v);
 
 /* Residual addition and root-mean-square norm, the ggml_add and the
  * ggml_rms_norm + ggml_mul before the projections (src/qwen2.cpp:250-275):

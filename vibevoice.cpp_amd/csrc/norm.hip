@@ -132,26 +132,13 @@ __global__ void __launch_bounds__(256) norm_kernel(NormArgs a) {
             store8<VEC>(y + (int64_t)k * (a.y_type == VVA_TYPE_F32 ? 4 : 2), a.y_type, left, z);
             continue;
         }
-        // the 4 lanes of a block (K is a multiple of 32: a block's lanes are all
-        // here), the rule of the Q8_0 caches.  The largest magnitude as bits, among
-        // which an infinity or a NaN is above every number: a block that has one
-        // gets a NaN scale and codes of 1, so that it reads as NaN throughout.
-        uint32_t ab = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ab = max(ab, __float_as_uint(z[e]) & 0x7fffffffu);
-        ab = max(ab, __float_as_uint(dpp<kDppXor1>(__uint_as_float(ab))));
-        ab = max(ab, __float_as_uint(dpp<kDppXor2>(__uint_as_float(ab))));
-        const bool finite = ab < 0x7f800000u;
-        const float d = __uint_as_float(ab) / 127.0f, id = d != 0.0f ? 1.0f / d : 0.0f;
+        // the 4 lanes of a block (K is a multiple of 32: a block's lanes are all here)
+        const Q8Block q8 = q8_block(z);
         uint16_t* blk = (uint16_t*)(y + (int64_t)(k / kQK8) * kQ8Bytes);
         const int q = (k % kQK8) / 2;
-        if (q == 0) blk[0] = finite ? f32_to_f16(d) : (uint16_t)0x7e00u;
+        if (q == 0) blk[0] = q8.scale;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float z0 = finite ? z[2 * e] * id : 1.0f, z1 = finite ? z[2 * e + 1] * id : 1.0f;
-            const uint8_t lo = (uint8_t)(int8_t)roundf(z0), hi = (uint8_t)(int8_t)roundf(z1);
-            blk[1 + q + e] = (uint16_t)(lo | (hi << 8));
-        }
+        for (int e = 0; e < 4; ++e) blk[1 + q + e] = (uint16_t)(q8.code(z[2 * e]) | (q8.code(z[2 * e + 1]) << 8));
     }
 }
 

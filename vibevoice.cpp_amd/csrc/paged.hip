@@ -1,5 +1,5 @@
 // paged.hip — RoPE + append of packed tokens of many sequences into a cache in
-// pages.
+// pages, of 16 bits or quantised to Q8_0, and rows read back out of it.
 //
 // What a call covers is on the device (vva_batch): the kernel finds its
 // sequence in q_start, its keys in kv_len and their places in the page table,
@@ -12,7 +12,7 @@ namespace vva {
 
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+#include "wave_ops.hpp"
 #include "paged_ops.hpp"
 
 // 8 elements, 16-byte aligned: as loaded, as fp32, and stored
@@ -49,11 +49,26 @@ __device__ __forceinline__ void store8(char* p, int type, const float (&y)[8]) {
     *(u32x4*)p = w;
 }
 
+// 8 elements from i on of a Q8_0 page's row, by 4 lanes per block: the codes are
+// d bytes a slot, the scales of a block `page` F16 behind all of them
+__device__ __forceinline__ void store8_q8(char* tile, int d, int page_shift, int slot, int i, const float (&y)[8]) {
+    const Q8Block b = q8_block(y);
+    uint2 c = {0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        c.x |= (uint32_t)b.code(y[e]) << (8 * e);
+        c.y |= (uint32_t)b.code(y[e + 4]) << (8 * e);
+    }
+    *(uint2*)(tile + slot * d + i) = c;
+    if (i % kQK8 == 0) *(uint16_t*)(tile + (d << page_shift) + (((i / kQK8) << page_shift) + slot) * 2) = b.scale;
+}
+
 // One workgroup per token row, a thread per 8 rotation pairs (elements i ..
 // i + 7 and i + P .. of a head); no head's item crosses a wave's table lookup.
 // HBM-bound (4k tokens 78 -> 33 us against one pair per thread); a short call
 // is a chain of two round trips: the batch, with the token's own rows under
 // way, then the page id and the row of the rope table.
+template <bool Q8>
 __global__ void __launch_bounds__(512) paged_append_kernel(PagedAppendArgs a) {
     prefetch_kernargs<sizeof(PagedAppendArgs)>();
     const PagedArgs& p = a.p;
@@ -145,9 +160,16 @@ __global__ void __launch_bounds__(512) paged_append_kernel(PagedAppendArgs a) {
         } else if (!live) {
             continue;
         } else if (t.h < p.Hq + p.Hkv) {
-            dst = p.k + page * p.k_nb_page + (t.h - p.Hq) * p.k_nb_head + slot * p.k_nb_slot;
+            dst = p.k + page * p.k_nb_page + (t.h - p.Hq) * p.k_nb_head + (Q8 ? 0 : slot * p.k_nb_slot);
         } else {
-            dst = p.v + page * p.v_nb_page + (t.h - p.Hq - p.Hkv) * p.v_nb_head + slot * p.v_nb_slot;
+            dst = p.v + page * p.v_nb_page + (t.h - p.Hq - p.Hkv) * p.v_nb_head + (Q8 ? 0 : slot * p.v_nb_slot);
+        }
+        if constexpr (Q8) {
+            if (t.h >= p.Hq) {                     // the same for the 4 lanes of a block
+                store8_q8(dst, p.d, p.page_shift, slot, t.e, y0);
+                store8_q8(dst, p.d, p.page_shift, slot, t.e + P, y1);
+                continue;
+            }
         }
         const int es = type == VVA_TYPE_F32 ? 4 : 2;
         store8(dst + t.e * es, type, y0);
@@ -155,11 +177,89 @@ __global__ void __launch_bounds__(512) paged_append_kernel(PagedAppendArgs a) {
     }
 }
 
+// Rows read back: one workgroup per kReadTokens token rows, a wave for every
+// fourth of them; a lane takes 8 elements of a K or V row at a time.
+constexpr int kReadTokens = 16, kReadWaves = 4;
+
+template <bool Q8>
+__global__ void __launch_bounds__(kReadWaves * 64) paged_read_kernel(PagedReadArgs a) {
+    prefetch_kernargs<sizeof(PagedReadArgs)>();
+    constexpr int NT = kReadTokens / kReadWaves;
+    const PagedArgs& p = a.p;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n0 = blockIdx.x * kReadTokens + w;
+    int page[NT], slot[NT];                        // page: -1: NaN, -2: no row
+    for (int i = 0; i < NT; ++i) page[i] = -2, slot[i] = 0;
+    for (int base = 0; base < p.n_seq; base += 64) {
+        const Seq q = seq_of(p, min(base + lane, p.n_seq - 1));
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int n = n0 + i * kReadWaves;
+            const uint64_t hit = __ballot(n < p.n_tok && n >= q.q0 && n < q.q0 + q.n);
+            if (!hit || page[i] != -2) continue;
+            const int l = __ffsll((unsigned long long)hit) - 1;
+            const int at = lane_of(q.L, l) - lane_of(q.n, l) + (n - lane_of(q.q0, l));
+            const int id = at >= 0 ? p.table[min(base + l, p.n_seq - 1) * p.table_stride + (at >> p.page_shift)] : -1;
+            page[i] = id >= 0 && id < p.n_pages ? id : -1;
+            slot[i] = at & ((1 << p.page_shift) - 1);
+        }
+    }
+    const int ph = p.d == 128 ? 16 : 8, each = p.Hkv * ph;   // 8-element parts of a head, of K's row
+    for (int k = lane; k < 2 * each; k += 64) {
+        const bool v = k >= each;
+        char* const out = v ? a.v_out : a.k_out;
+        if (!out) continue;
+        const int kk = v ? k - each : k, h = p.d == 128 ? kk >> 4 : kk >> 3, e = (kk & (ph - 1)) * 8;
+        const char* const pool = (v ? p.v + h * p.v_nb_head : p.k + h * p.k_nb_head);
+        const int64_t nb_page = v ? p.v_nb_page : p.k_nb_page, nb_slot = v ? p.v_nb_slot : p.k_nb_slot;
+        const int type = v ? a.v_type : a.k_type;
+        char* const dst = out + (v ? h * a.v_nb_h : h * a.k_nb_h) + e * (type == VVA_TYPE_F32 ? 4 : 2);
+        const int64_t nb_t = v ? a.v_nb_t : a.k_nb_t;
+        u32x4 raw[NT];
+        uint16_t scale[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const char* tile = pool + max(page[i], 0) * nb_page;
+            if constexpr (Q8) {
+                const uint2 c = *(const uint2*)(tile + slot[i] * p.d + e);
+                raw[i] = u32x4{c.x, c.y, 0u, 0u};
+                scale[i] = *(const uint16_t*)(tile + (p.d << p.page_shift) + (((e / kQK8) << p.page_shift) + slot[i]) * 2);
+            } else {
+                raw[i] = *(const u32x4*)(tile + slot[i] * nb_slot + e * 2);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            if (page[i] == -2) continue;
+            float x[8];
+            if constexpr (Q8) {
+                const float s = f16_to_f32(scale[i]);
+#pragma unroll
+                for (int b = 0; b < 8; ++b) x[b] = s * (float)(int8_t)(raw[i][b / 4] >> (8 * (b % 4)));
+            } else {
+                raw8_to_f32(Raw8{raw[i], raw[i]}, p.type, x);
+            }
+            if (page[i] == -1)
+#pragma unroll
+                for (int b = 0; b < 8; ++b) x[b] = __builtin_nanf("");
+            store8(dst + (n0 + i * kReadWaves) * nb_t, type, x);
+        }
+    }
+}
+
 }  // namespace
 
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
     const int items = (a.p.Hq + 2 * a.p.Hkv) * (a.p.d / 16);
-    hipLaunchKernelGGL(paged_append_kernel, dim3(a.p.n_tok), dim3(std::min(512, (items + 63) / 64 * 64)), 0, s, a);
+    const dim3 g(a.p.n_tok), b(std::min(512, (items + 63) / 64 * 64));
+    if (a.p.type == VVA_TYPE_Q8_0) hipLaunchKernelGGL(paged_append_kernel<true>, g, b, 0, s, a);
+    else hipLaunchKernelGGL(paged_append_kernel<false>, g, b, 0, s, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_paged_read(const PagedReadArgs& a, hipStream_t s) {
+    const dim3 g((a.p.n_tok + kReadTokens - 1) / kReadTokens), b(kReadWaves * 64);
+    if (a.p.type == VVA_TYPE_Q8_0) hipLaunchKernelGGL(paged_read_kernel<true>, g, b, 0, s, a);
+    else hipLaunchKernelGGL(paged_read_kernel<false>, g, b, 0, s, a);
     return hipGetLastError();
 }
 

@@ -54,6 +54,7 @@
 #include "vva_internal.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace vva {
 
@@ -64,6 +65,8 @@ namespace {
 #include "paged_ops.hpp"
 
 constexpr float kLazy = 8.0f;      // running-max slack in log2 units
+// The type that the products take: the pages' own, F16 for Q8_0
+template <int KT> constexpr int kComp = KT == VVA_TYPE_Q8_0 ? VVA_TYPE_F16 : KT;
 // log2 of the factor that P carries
 template <int KT> constexpr float kLift = KT == VVA_TYPE_F16 ? 7.0f : 0.0f;
 constexpr int kFewRows = 32;       // rows of a sequence and kv head that paged_few_kernel takes
@@ -229,6 +232,48 @@ __device__ __forceinline__ void add_not_finite(uint32_t v_lds, int k0, int lim, 
     }
 }
 
+// Q fragment as the products take it, from the 16 bytes of a row
+template <int KT, int OT>
+__device__ __forceinline__ typename Frag<KT>::type q_frag(u32x4 x) {
+    if constexpr (OT != KT) {                      // BF16 rows over Q8_0 pages: F16 holds their 8 bits
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = pack2<KT>(__uint_as_float(x[e] << 16), __uint_as_float(x[e] & 0xffff0000u));
+    }
+    return as_vec<typename Frag<KT>::type>(x);
+}
+// 4 codes of a Q8_0 page times their scale, as F16: 1024 + (code + 128) has the
+// code's byte as its last bits, so a byte permutation and an exact subtraction
+// make a pair; the product with the scale is rounded (2^-11 at most).
+__device__ __forceinline__ u32x2 q8_values(uint32_t codes, h2 scale) {
+    const uint32_t x = codes ^ 0x80808080u;
+    const uint32_t p[2] = {__builtin_amdgcn_perm(0x64646464u, x, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)};
+    u32x2 r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        h2 v;
+        __builtin_memcpy(&v, &p[i], 4);
+        v = (v - h2{(_Float16)1152.0f, (_Float16)1152.0f}) * scale;
+        uint32_t u;
+        __builtin_memcpy(&u, &v, 4);
+        r[i] = u;
+    }
+    return r;
+}
+__device__ __forceinline__ h2 q8_scale(uint16_t bits) {
+    _Float16 s;
+    __builtin_memcpy(&s, &bits, 2);
+    return h2{s, s};
+}
+// Row r, chunk c (16 dims) of a 16-bit tile from the codes of those dims
+template <int D, bool V>
+__device__ __forceinline__ void q8_store(uint32_t tile, int r, int c, u32x4 codes, uint16_t scale) {
+    const h2 sc = q8_scale(scale);
+    const u32x2 a = q8_values(codes.x, sc), b = q8_values(codes.y, sc), e = q8_values(codes.z, sc), f = q8_values(codes.w, sc);
+    const int z = V ? v_swz<D>(r) : k_swz<D>(r);
+    *lds_vec(tile + r * 2 * D + (((2 * c) ^ z) << 4)) = u32x4{a.x, a.y, b.x, b.y};
+    *lds_vec(tile + r * 2 * D + (((2 * c + 1) ^ z) << 4)) = u32x4{e.x, e.y, f.x, f.y};
+}
+
 // The kernel's arguments, read again from their segment: each phase loads the
 // few that it needs (they hit the scalar cache), so that not all of them are
 // held, and spilled, through the key tiles.
@@ -368,8 +413,10 @@ struct FewLds {
 // wave's loads fly while it waits and 8 while it computes.  The waves' sums
 // meet at the end.  Partials in the workspace, per piece and kv head: [cap
 // rows][D] sums, then [cap] (exponent base, row sum).
-template <int D, int KT, int WAVES, bool SHARES>
+template <int D, int PT, int OT, int WAVES, bool SHARES>
 __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, int cap, const FewItem& it, int kvh, char* lds) {
+    constexpr int KT = kComp<PT>;
+    constexpr bool Q8 = PT == VVA_TYPE_Q8_0;
     using F = Frag<KT>;
     using QF = typename F::type;
     constexpr int DS = D / 16, DT = D / 32;
@@ -414,8 +461,32 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
             dma16<true>(base[r / 16] + (uint64_t)(r % 16) * nb_slot, off[c % 4], dst + c * 1024);
         }
     };
-    auto issue_k = [&](int t) { issue(t, ks, a.k, a.k_nb_page, a.k_nb_head, a.k_nb_slot, koff); };
-    auto issue_v = [&](int t) { issue(t, vs, a.v, a.v_nb_page, a.v_nb_head, a.v_nb_slot, voff); };
+    auto issue_q8 = [&](int t, uint32_t dst, const char* pool, int64_t nb_page, int64_t nb_head, auto is_v) {
+        constexpr int C = D / 16, N = kFewTile * C / 64;
+        const int page = 1 << a.page_shift;
+        u32x4 codes[N];
+        uint16_t scale[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = i * (64 / C) + lane / C, c = lane % C, hf = i * (64 / C) / 16;
+            const bool ok = (uint32_t)ids[hf] < (uint32_t)a.n_pages;
+            bad = bad || !ok;
+            const char* p = pool + (int64_t)(ok ? ids[hf] : 0) * nb_page + kvh * nb_head;
+            const int slot = ((t * kFewTile + 16 * hf) & (page - 1)) + r % 16;
+            codes[i] = *(const u32x4*)(p + slot * D + c * 16);
+            scale[i] = *(const uint16_t*)(p + page * D + ((c >> 1) * page + slot) * 2);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) q8_store<D, decltype(is_v)::value>(dst, i * (64 / C) + lane / C, lane % C, codes[i], scale[i]);
+    };
+    auto issue_k = [&](int t) {
+        if constexpr (Q8) issue_q8(t, ks, a.k, a.k_nb_page, a.k_nb_head, std::false_type{});
+        else issue(t, ks, a.k, a.k_nb_page, a.k_nb_head, a.k_nb_slot, koff);
+    };
+    auto issue_v = [&](int t) {
+        if constexpr (Q8) issue_q8(t, vs, a.v, a.v_nb_page, a.v_nb_head, std::true_type{});
+        else issue(t, vs, a.v, a.v_nb_page, a.v_nb_head, a.v_nb_slot, voff);
+    };
     int t = t0 + w;
     if (t < t1) fetch(t);
     // the rows of Q, a part by each wave, laid out as K is; rows that are
@@ -434,7 +505,7 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
     if (t < t1) {
         issue_k(t);
         issue_v(t);
-        wait_vm<2 * NC>();                         // Q
+        wait_vm<Q8 ? 0 : 2 * NC>();                // Q
     } else {
         wait_vm<0>();
     }
@@ -442,7 +513,7 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
     const int k_off = k_lane_off<D>(lane), v_off = v_lane_off<D>(lane);
     QF qf[DS];
 #pragma unroll
-    for (int ds = 0; ds < DS; ++ds) qf[ds] = as_vec<QF>(lds_read((qs + k_off) ^ (ds << 5)));
+    for (int ds = 0; ds < DS; ++ds) qf[ds] = q_frag<KT, OT>(lds_read((qs + k_off) ^ (ds << 5)));
     const int lim = l32 < rows ? min(L - 1, past + div_g(a, l32)) : -1;   // the last key the lane's row sees
     const float sl2 = a.scale * kLog2e;
     float m = -INFINITY, lsum = 0.0f;
@@ -452,7 +523,7 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
     for (; t < t1; t += WAVES) {
         const bool more = t + WAVES < t1;
         if (more) fetch(t + WAVES);
-        wait_vm<NC>();                             // K; V may still fly
+        wait_vm<Q8 ? 0 : NC>();                    // K; V may still fly
         f32x16 s{};
 #pragma unroll
         for (int ds = 0; ds < DS; ++ds) s = F::mma(as_vec<QF>(lds_read((ks + k_off) ^ (ds << 5))), qf[ds], s);
@@ -493,7 +564,7 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
             }
             lsum = sum2<KT>(p[r], lsum);
         }
-        if (more) wait_vm<NC>();                   // V; the next K may still fly
+        if (more) wait_vm<Q8 ? 0 : NC>();          // V; the next K may still fly
         else wait_vm<0>();
         const bool fix = masked && tile_not_finite<D, KT, kFewTile>(vs, lane);
 #pragma unroll
@@ -541,7 +612,7 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
         const int rt = div_g(args, row);
         // zeros where the row sees no key; all scores -inf: 0 * (1 / 0), the softmax's NaN
         const float inv = min(it.q.L - 1, it.q.L - it.q.n + rt) >= 0 ? 1.0f / x.den : 0.0f;
-        uint2 y = {pack2<KT>(x.num.x * inv, x.num.y * inv), pack2<KT>(x.num.z * inv, x.num.w * inv)};
+        uint2 y = {pack2<OT>(x.num.x * inv, x.num.y * inv), pack2<OT>(x.num.z * inv, x.num.w * inv)};
         if (nan) y.x = y.y = 0x7fff7fffu;
         *(uint2*)(args.out + (int64_t)(it.q.q0 + rt) * args.o_nb_t + (int64_t)(kvh * args.G + row - rt * args.G) * args.o_nb_h + 8 * c) = y;
     };
@@ -662,12 +733,12 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
 }
 
 // One workgroup per (piece, kv head), two of them (D = 64: four) on a CU.
-template <int D, int KT>
+template <int D, int PT, int OT>
 __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets, int slots, int cap) {
     prefetch_kernargs<sizeof(PagedArgs)>();
     __shared__ __attribute__((aligned(1024))) char lds[FewLds<D, kFewWaves>::BYTES];
     const FewItem it = few_item(a, blockIdx.x / a.Hkv, slots, kFewWaves);
-    if (it.parts > 0) few_piece<D, KT, kFewWaves, false>(a, ws, tickets, cap, it, blockIdx.x % a.Hkv, lds);
+    if (it.parts > 0) few_piece<D, PT, OT, kFewWaves, false>(a, ws, tickets, cap, it, blockIdx.x % a.Hkv, lds);
 }
 
 // ----------------------------------------------------------- many rows
@@ -906,8 +977,10 @@ template <int D>
 struct ManyLds {
     static constexpr int BYTES = kStages * 2 * kBN * 2 * D;
 };
-template <int D, int KT>
+template <int D, int PT, int OT>
 __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, const ManyAxis& axis, const ManyPieces& pc, const Seq& mine, int block, int wgs, char* lds, int* marks) {
+    constexpr int KT = kComp<PT>;
+    constexpr bool Q8 = PT == VVA_TYPE_Q8_0;
     using F = Frag<KT>;
     using QF = typename F::type;
     constexpr int DS = D / 16, DT = D / 32;
@@ -917,6 +990,7 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
     constexpr int RC = 1024 / ROW;                 // rows of a load
     constexpr int STAGE = 2 * TB;
     constexpr int NLD = 2 * NI;
+    constexpr int NID = Q8 ? 1 : NI;               // page ids of a wave's loads of a tile
     constexpr int WAVE_O = DT * 16 * 64 * 4;       // bytes of a wave's sums
     constexpr int WAVE = WAVE_O + 64 * 8;
     int& fix = marks[0];                           // the last tile with a V that is not finite
@@ -1008,7 +1082,7 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)lds;
     const float sl2 = uni(a.scale * kLog2e);
     bool bad = false;
-    int ids[NI];
+    int ids[NID];
     // where a part's K and V come from
     struct Source {
         uint64_t k, v;                             // the pools' kv head
@@ -1022,14 +1096,44 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
                       a.k_nb_page, a.v_nb_page, (int)a.k_nb_slot, (int)a.v_nb_slot, a.n_pages, a.page_shift,
                       max(0, (c.L - 1) >> a.page_shift), (ConstInts)(uintptr_t)(a.table + (int64_t)c.s * a.table_stride)};
     };
-    auto fetch = [&](const Source& t, int key, int (&id)[NI]) {
+    auto fetch = [&](const Source& t, int key, int (&id)[NID]) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) id[i] = t.table[min((key + i * kWaves * RC + r0w) >> t.shift, t.last)];
+        for (int i = 0; i < NID; ++i) id[i] = t.table[min((key + (Q8 ? 8 * w : i * kWaves * RC + r0w)) >> t.shift, t.last)];
     };
     // the loads of tile j, from key `key` on (K, then V); past the last tile
     // further ones of the sequence, to a stage that nobody reads any more, so
     // that every tile counts the same
-    auto issue = [&](const Source& t, int j, int key, const int (&id)[NI]) {
+    auto issue = [&](const Source& t, int j, int key, const int (&id)[NID]) {
+        if constexpr (Q8) {
+            // 8 rows a wave: K, then V (D = 64: K by the lower lanes, V by the upper)
+            const int ln = lane_id(), page = 1 << t.shift;
+            constexpr int C = D / 16;
+            const int r = 8 * w + (ln / C) % 8, c = ln % C;
+            const bool ok = (uint32_t)id[0] < (uint32_t)t.n_pages;
+            bad = bad || !ok;
+            const int64_t at = ok ? id[0] : 0;
+            const int slot = ((key + 8 * w) & (page - 1)) + r % 8;
+            const uint32_t st = lds0 + (j % kStages) * STAGE;
+            const char* kp = (const char*)(uintptr_t)(t.k + at * t.k_page);
+            const char* vp = (const char*)(uintptr_t)(t.v + at * t.v_page);
+            auto load = [&](const char* p, u32x4& codes, uint16_t& scale) {
+                codes = *(const u32x4*)(p + slot * D + c * 16);
+                scale = *(const uint16_t*)(p + page * D + ((c >> 1) * page + slot) * 2);
+            };
+            u32x4 x, y;
+            uint16_t sx, sy;
+            if constexpr (D == 128) {
+                load(kp, x, sx);
+                load(vp, y, sy);
+                q8_store<D, false>(st, r, c, x, sx);
+                q8_store<D, true>(st + TB, r, c, y, sy);
+            } else {
+                load(ln < 32 ? kp : vp, x, sx);
+                if (ln < 32) q8_store<D, false>(st, r, c, x, sx);
+                else q8_store<D, true>(st + TB, r, c, x, sx);
+            }
+            return;
+        } else {
         const uint32_t st = lds0 + (j % kStages) * STAGE + w * 1024;
         uint64_t kb[NI], vb[NI];
 #pragma unroll
@@ -1045,6 +1149,7 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
         for (int i = 0; i < NI; ++i) dma16<false>(kb[i], koff, st + i * kWaves * 1024);
 #pragma unroll
         for (int i = 0; i < NI; ++i) dma16<false>(vb[i], voff, st + TB + i * kWaves * 1024);
+        }
     };
     // x = t * G + h for small x (below G + 32): one product
     auto small_divide = [&](int x, int G, int& t, int& h) {
@@ -1058,7 +1163,7 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
         const int G = a.G;
         bad = false;
         const int ln = lane_id();                  // offsets made here, not held from one part to the next
-        int id0[NI], id1[NI];
+        int id0[NID], id1[NID];
         fetch(src, c.kb0, id0);
         fetch(src, c.kb0 + kBN, id1);
         fetch(src, c.kb0 + 2 * kBN, ids);
@@ -1106,15 +1211,15 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
         const int l32 = lane_id() & 31;
         small_divide(wr - t0 * G + (wr0 + l32 < rows ? l32 : 0), G, lim, hcol);
         lim = min(L - 1, past + t0 + lim);
-        wait_vm<2 * NLD>();                                   // Q has landed
+        wait_vm<Q8 ? 0 : 2 * NLD>();                          // Q has landed
         QF qf[DS];
         {
             const uint32_t qa = lds0 + 2 * STAGE + w * kRowsWave * ROW + k_lane_off<D>(lane_id());
 #pragma unroll
-            for (int ds = 0; ds < DS; ++ds) qf[ds] = as_vec<QF>(lds_read(qa ^ (ds << 5)));
+            for (int ds = 0; ds < DS; ++ds) qf[ds] = q_frag<KT, OT>(lds_read(qa ^ (ds << 5)));
         }
         // K of tile 0 has landed (its V and tile 1 may still fly), and every wave has its Q
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(NI + NLD) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(Q8 ? 0 : NI + NLD) : "memory");
         issue(src, 2, kb0 + 2 * kBN, ids);
         fetch(src, kb0 + 3 * kBN, ids);
         auto stage = [&](int j) { return lds0 + (j % kStages) * STAGE; };
@@ -1243,7 +1348,7 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
         auto step = [&](int j, const f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
             // K of tile j + 1 and V of tile j have landed, and every wave is done
             // with tile j - 1, whose stage tile j + 3 now takes
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(NI + NLD) : "memory");
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(Q8 ? 0 : NI + NLD) : "memory");
             issue(src, j + 3, kb0 + (j + 3) * kBN, ids);
             fetch(src, kb0 + (j + 4) * kBN, ids);
             if (j < n_live) rescale(mx);                      // wave-uniform
@@ -1368,7 +1473,7 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int q4 = 2 * (i % 2) + x / 2, r = 4 * q4 + 2 * (x % 2);
-                y[x / 2][x % 2] = pack2<KT>(o[i / 2][r] * inv, o[i / 2][r + 1] * inv);
+                y[x / 2][x % 2] = pack2<OT>(o[i / 2][r] * inv, o[i / 2][r + 1] * inv);
             }
             const auto s0 = __builtin_amdgcn_permlane32_swap(y[0][0], y[1][0], false, false);
             const auto s1 = __builtin_amdgcn_permlane32_swap(y[0][1], y[1][1], false, false);
@@ -1380,7 +1485,7 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
     }
 }
 
-template <int D, int KT>
+template <int D, int PT, int OT>
 __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets) {
     prefetch_kernargs<sizeof(PagedArgs)>();
     __shared__ __attribute__((aligned(1024))) char lds[ManyLds<D>::BYTES];
@@ -1390,7 +1495,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
     if (axis.head <= 0) return;
     const ManyPieces pc = many_pieces(a, axis, mine, gridDim.x, blockIdx.x);
     const int wgs = pc.head > 0 ? pc.head * a.Hkv : many_shares(a, axis, gridDim.x);
-    if ((int)blockIdx.x < wgs) many_share<D, KT>(a, ws, tickets, axis, pc, mine, blockIdx.x, wgs, lds, marks);
+    if ((int)blockIdx.x < wgs) many_share<D, PT, OT>(a, ws, tickets, axis, pc, mine, blockIdx.x, wgs, lds, marks);
 }
 
 // Few rows beside many: share `item / Hkv` of kv head item % Hkv, the axis cut
@@ -1398,7 +1503,7 @@ __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, fl
 // least.  The workgroups are fewer than the pieces here, so that even work
 // counts for more than what a cut costs (60 sequences of up to 8000 keys beside
 // 700 tokens: 159 us with whole pieces by turns, 97 so).  False: no share.
-template <int D, int KT>
+template <int D, int PT, int OT>
 __device__ __forceinline__ bool few_share(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, int cap, int item, int slots, int axis, const Seq& mine, char* lds) {
     const int n = max(1, min(slots, axis / (kWaves + kFewCost)));
     const Shares cuts{(axis + n - 1) / n, n, max(kFewCost + 1, min(kFewSnap, (axis + n - 1) / n / 2))};
@@ -1436,7 +1541,7 @@ __device__ __forceinline__ bool few_share(const PagedArgs& a, float* __restrict_
         it.part = g - it.first;
         it.t0 = max(0, off - kFewCost);            // a cut is more than kFewCost from the ends, or at one
         it.t1 = min(off_end - kFewCost, (it.q.L + kFewTile - 1) / kFewTile);   // no keys: none
-        few_piece<D, KT, kWaves, true>(a, ws, tickets, cap, it, kvh, lds);
+        few_piece<D, PT, OT, kWaves, true>(a, ws, tickets, cap, it, kvh, lds);
         __syncthreads();                           // the next piece's rows of Q go where this one's sums are
     }
     return true;
@@ -1455,7 +1560,7 @@ __device__ __forceinline__ bool few_share(const PagedArgs& a, float* __restrict_
 // to 8000 and 700 behind 2000 105 and 97):
 template <int D>
 constexpr float kFewTime = D == 64 ? 0.16f : 0.22f;
-template <int D, int KT>
+template <int D, int PT, int OT>
 __global__ void __launch_bounds__(kWaves * 64) paged_mixed_kernel(PagedArgs a, float* __restrict__ ws, float* __restrict__ few_ws, unsigned* tickets, int cap) {
     prefetch_kernargs<sizeof(PagedArgs)>();
     constexpr int FEW = FewLds<D, kWaves>::BYTES;
@@ -1472,29 +1577,38 @@ __global__ void __launch_bounds__(kWaves * 64) paged_mixed_kernel(PagedArgs a, f
         const ManyPieces pc = many_pieces(a, axis, mine, most, blockIdx.x);
         wgs = pc.head > 0 ? pc.head * a.Hkv : many_shares(a, axis, most);
         if ((int)blockIdx.x < wgs) {
-            many_share<D, KT>(a, ws, tickets, axis, pc, mine, blockIdx.x, wgs, lds, marks);
+            many_share<D, PT, OT>(a, ws, tickets, axis, pc, mine, blockIdx.x, wgs, lds, marks);
             return;
         }
     }
     if (few == 0) return;
     const int slots = max(1, ((int)gridDim.x - wgs) / a.Hkv);
-    for (int i = blockIdx.x - wgs; few_share<D, KT>(a, few_ws, tickets + kManyTickets, cap, i, slots, few, mine, lds);) i += gridDim.x - wgs;
+    for (int i = blockIdx.x - wgs; few_share<D, PT, OT>(a, few_ws, tickets + kManyTickets, cap, i, slots, few, mine, lds);) i += gridDim.x - wgs;
 }
 
 size_t many_ws_bytes(const PagedArgs& a, const PagedPlan& p) {
     return (size_t)p.many_wgs * 2 * kWaves * (a.d * kRowsWave * sizeof(float) + 64 * 8);
 }
 
-template <int D, int KT>
+template <int D, int PT, int OT>
 hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s) {
     if (p.many_wgs > 0 && p.few_pieces > 0) {
-        hipLaunchKernelGGL((paged_mixed_kernel<D, KT>), dim3(p.many_wgs), dim3(kWaves * 64), 0, s, a, ws, (float*)((char*)ws + many_ws_bytes(a, p)), tickets, p.few_cap);
+        hipLaunchKernelGGL((paged_mixed_kernel<D, PT, OT>), dim3(p.many_wgs), dim3(kWaves * 64), 0, s, a, ws, (float*)((char*)ws + many_ws_bytes(a, p)), tickets, p.few_cap);
     } else if (p.many_wgs > 0) {
-        hipLaunchKernelGGL((paged_many_kernel<D, KT>), dim3(p.many_wgs), dim3(kWaves * 64), 0, s, a, ws, tickets);
+        hipLaunchKernelGGL((paged_many_kernel<D, PT, OT>), dim3(p.many_wgs), dim3(kWaves * 64), 0, s, a, ws, tickets);
     } else {
-        hipLaunchKernelGGL((paged_few_kernel<D, KT>), dim3(p.few_pieces * a.Hkv), dim3(kFewWaves * 64), 0, s, a, ws, tickets, p.few_slots, p.few_cap);
+        hipLaunchKernelGGL((paged_few_kernel<D, PT, OT>), dim3(p.few_pieces * a.Hkv), dim3(kFewWaves * 64), 0, s, a, ws, tickets, p.few_slots, p.few_cap);
     }
     return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_typed(const PagedArgs& a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s) {
+    if (a.type == VVA_TYPE_Q8_0)
+        return a.io_type == VVA_TYPE_F16 ? launch_paged<D, VVA_TYPE_Q8_0, VVA_TYPE_F16>(a, p, ws, tickets, s)
+                                         : launch_paged<D, VVA_TYPE_Q8_0, VVA_TYPE_BF16>(a, p, ws, tickets, s);
+    return a.type == VVA_TYPE_F16 ? launch_paged<D, VVA_TYPE_F16, VVA_TYPE_F16>(a, p, ws, tickets, s)
+                                  : launch_paged<D, VVA_TYPE_BF16, VVA_TYPE_BF16>(a, p, ws, tickets, s);
 }
 
 static_assert(kManyTickets + 2 * kFewTickets <= kMaxPagedTickets, "the context holds the tickets");
@@ -1535,9 +1649,7 @@ size_t paged_ws_bytes(const PagedArgs& a, const PagedPlan& p) {
 
 hipError_t launch_paged_attn(PagedArgs a, const PagedPlan& p, float* ws, unsigned* tickets, hipStream_t s) {
     a.few_rows = p.few_pieces > 0 ? kFewRows : 0;
-    if (a.d == 64)
-        return a.type == VVA_TYPE_F16 ? launch_paged<64, VVA_TYPE_F16>(a, p, ws, tickets, s) : launch_paged<64, VVA_TYPE_BF16>(a, p, ws, tickets, s);
-    return a.type == VVA_TYPE_F16 ? launch_paged<128, VVA_TYPE_F16>(a, p, ws, tickets, s) : launch_paged<128, VVA_TYPE_BF16>(a, p, ws, tickets, s);
+    return a.d == 64 ? launch_typed<64>(a, p, ws, tickets, s) : launch_typed<128>(a, p, ws, tickets, s);
 }
 
 }  // namespace vva

@@ -1575,12 +1575,19 @@ vva_status fill_paged(vva_context* ctx, const char* what, const vva_tensor* kp, 
     if ((st = check_tensor(ctx, kp, "k_pages")) != VVA_OK) return st;
     if ((st = check_tensor(ctx, vp, "v_pages")) != VVA_OK) return st;
     const int64_t d = kp->ne[0], ps = kp->ne[1], Hkv = kp->ne[2], n_pages = kp->ne[3];
-    if (kp->type != vp->type || (kp->type != VVA_TYPE_F16 && kp->type != VVA_TYPE_BF16))
-        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: pages must be F16 or BF16, K and V alike", what);
+    const bool q8 = kp->type == VVA_TYPE_Q8_0;
+    if (kp->type != vp->type || (!q8 && kp->type != VVA_TYPE_F16 && kp->type != VVA_TYPE_BF16))
+        return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: pages must be F16, BF16 or Q8_0, K and V alike", what);
     for (int i = 0; i < 4; ++i)
         if (kp->ne[i] != vp->ne[i]) return fail(ctx, VVA_ERR_INVALID_ARG, "%s: k_pages and v_pages differ in ne[%d]", what, i);
-    if (kp->nb[0] != 2 || vp->nb[0] != 2 || !al16(kp, 3) || !al16(vp, 3))
+    if (!q8 && (kp->nb[0] != 2 || vp->nb[0] != 2 || !al16(kp, 3) || !al16(vp, 3)))
         return fail(ctx, VVA_ERR_INVALID_ARG, "%s: page rows must be contiguous and 16-byte aligned", what);
+    for (const vva_tensor* t : {kp, vp})
+        // the rows of a page of a head are one run
+        if (q8 && (d % kQK8 || t->nb[0] != (size_t)kQ8Bytes || (int64_t)t->nb[1] != type_row_bytes(VVA_TYPE_Q8_0, d) ||
+                   (uintptr_t)t->data % 16 || (Hkv > 1 && t->nb[2] % 16) || (n_pages > 1 && t->nb[3] % 16)))
+            return fail(ctx, VVA_ERR_INVALID_ARG, "%s: Q8_0 pages need nb = [34, %lld, ...], each page of a head in one 16-byte aligned run",
+                        what, (long long)type_row_bytes(VVA_TYPE_Q8_0, d));
     if (d != 64 && d != 128) return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: head_dim %lld, needs 64 or 128", what, (long long)d);
     if (ps < 16 || ps > 1024 || (ps & (ps - 1)))
         return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "%s: page_size %lld, needs a power of two from 16 to 1024", what, (long long)ps);
@@ -1624,7 +1631,7 @@ vva_status fill_paged(vva_context* ctx, const char* what, const vva_tensor* kp, 
     while ((1 << l) < p.G) ++l;
     p.g_mul = l > 0 ? (uint32_t)(((uint64_t)1 << (31 + l)) / p.G + 1) : 0;
     p.g_shift = l - 1;
-    p.k = (char*)kp->data; p.v = (char*)vp->data; p.type = kp->type;
+    p.k = (char*)kp->data; p.v = (char*)vp->data; p.type = p.io_type = kp->type;
     p.k_nb_slot = kp->nb[1]; p.k_nb_head = kp->nb[2]; p.k_nb_page = kp->nb[3];
     p.v_nb_slot = vp->nb[1]; p.v_nb_head = vp->nb[2]; p.v_nb_page = vp->nb[3];
     return VVA_OK;
@@ -1688,8 +1695,13 @@ extern "C" vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, cons
     // 32 tokens' rows of up to 256 heads in 32-bit offsets
     if ((Hq > 1 && q->nb[1] >= ((size_t)1 << 22)) || (N > 1 && q->nb[2] >= ((size_t)1 << 22)))
         return fail(ctx, VVA_ERR_NOT_IMPLEMENTED, "paged_attn: rows of q 4 MiB apart");
-    if (q->type != a.type || out->type != a.type)
+    if (a.type == VVA_TYPE_Q8_0) {
+        if (out->type != q->type || (q->type != VVA_TYPE_F16 && q->type != VVA_TYPE_BF16))
+            return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: q and out must be F16 or BF16, both alike, over Q8_0 pages");
+        a.io_type = q->type;
+    } else if (q->type != a.type || out->type != a.type) {
         return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: q and out must have the pages' type (%d)", a.type);
+    }
     if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: scale must be finite and > 0");
     for (const vva_tensor* t : {q, k_pages, v_pages, &batch->q_start, &batch->kv_len, &batch->table})
         if (meets(out, t)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_attn: out overlaps q, the pages or the batch");
@@ -1703,6 +1715,33 @@ extern "C" vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, cons
     const hipError_t e = launch_paged_attn(a, plan, ctx->ws, ctx->tickets + kMaxStepTickets + kMaxPrefillTickets + kMaxProjTickets,
                                            ctx->stream);
     return e == hipSuccess ? VVA_OK : hip_fail(ctx, e, "paged_attn launch");
+}
+
+extern "C" vva_status vva_paged_read(vva_context* ctx, const vva_batch* batch, const vva_tensor* k_pages,
+                                     const vva_tensor* v_pages, const vva_tensor* k, const vva_tensor* v) {
+    if (!ctx) return VVA_ERR_INVALID_ARG;
+    if (!k && !v) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_read: neither k nor v");
+    vva_status st;
+    const vva_tensor* one = k ? k : v;
+    if ((st = check_tensor(ctx, one, k ? "k" : "v")) != VVA_OK) return st;
+    if ((st = check_tensor(ctx, k_pages, "k_pages")) != VVA_OK) return st;
+    const int64_t N = one->ne[2], Hkv = k_pages->ne[2];
+    PagedReadArgs a{};
+    if ((st = fill_paged(ctx, "paged_read", k_pages, v_pages, batch, Hkv, N, a.p)) != VVA_OK) return st;
+    if (k && (st = check_packed(ctx, k, "k", a.p.d, Hkv, N)) != VVA_OK) return st;
+    if (v && (st = check_packed(ctx, v, "v", a.p.d, Hkv, N)) != VVA_OK) return st;
+    for (const vva_tensor* out : {k, v}) {
+        if (!out) continue;
+        if (meets_itself(out)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_read: rows of an output overlap each other");
+        for (const vva_tensor* t : {k_pages, v_pages, &batch->q_start, &batch->kv_len, &batch->table})
+            if (overlaps(out, t)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_read: an output overlaps the pages or the batch");
+    }
+    if (k && v && meets(k, v)) return fail(ctx, VVA_ERR_INVALID_ARG, "paged_read: k and v overlap");
+    if (k) a.k_out = (char*)k->data, a.k_type = k->type, a.k_nb_h = k->nb[1], a.k_nb_t = k->nb[2];
+    if (v) a.v_out = (char*)v->data, a.v_type = v->type, a.v_nb_h = v->nb[1], a.v_nb_t = v->nb[2];
+    DeviceGuard g(ctx->device);
+    const hipError_t e = launch_paged_read(a, ctx->stream);
+    return e == hipSuccess ? VVA_OK : hip_fail(ctx, e, "paged_read launch");
 }
 
 extern "C" vva_status vva_add_rms_norm(vva_context* ctx, const vva_tensor* x, const vva_tensor* add, const vva_tensor* w,

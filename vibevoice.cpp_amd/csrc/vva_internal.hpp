@@ -195,7 +195,9 @@ size_t proj_part_bytes(const ProjArgs& a, const ProjPlan& p);
 
 // Packed tokens of many sequences over a cache in pages (paged.hip).  Row
 // (slot, head, page) of K at k + page * k_nb_page + head * k_nb_head + slot *
-// k_nb_slot; token rows n of q, out at base + n * nb_t + h * nb_h.
+// k_nb_slot; token rows n of q, out at base + n * nb_t + h * nb_h.  Q8_0: a
+// page of a head is page_size rows of d codes, then d / 32 rows of page_size F16
+// scales (k_nb_slot is not used).
 struct PagedArgs {
     const int32_t* q_start; const int32_t* kv_len; const int32_t* table;
     int64_t table_stride;                          // in elements
@@ -204,6 +206,7 @@ struct PagedArgs {
     int d, Hq, Hkv, G;                             // G = Hq / Hkv
     uint32_t g_mul; int g_shift;                   // x / G = high word of x * g_mul >> g_shift; g_mul = 0: G = 1
     char* k; char* v; int type;
+    int io_type;                                   // of q and out (attention): type, or F16 / BF16 over Q8_0 pages
     int64_t k_nb_slot, k_nb_head, k_nb_page, v_nb_slot, v_nb_head, v_nb_page;
     const char* q; int64_t q_nb_h, q_nb_t;
     char* out; int64_t o_nb_h, o_nb_t;
@@ -219,6 +222,13 @@ struct PagedAppendArgs {
     const char* rope; int64_t rope_nb; int n_pos;  // rows of d floats, cos then sin
     const int32_t* pos;                            // [n_tok] or null
 };
+// Reading back: PagedArgs' q and out unused, Hq = Hkv
+struct PagedReadArgs {
+    PagedArgs p;
+    char* k_out; char* v_out;                      // either may be null
+    int k_type, v_type;
+    int64_t k_nb_h, k_nb_t, v_nb_h, v_nb_t;
+};
 // Residual addition + RMS norm (norm.hip)
 struct NormArgs {
     const char* x; int x_type; int64_t x_nb_t, x_nb_b;
@@ -233,6 +243,7 @@ struct NormArgs {
 // --------------------------------------------------------- host launchers
 
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s);
+hipError_t launch_paged_read(const PagedReadArgs& a, hipStream_t s);
 // Launches of a paged_attn call of these shapes, whatever its lengths are
 // (upper bounds; paged_attn.hip)
 struct PagedPlan {

@@ -116,6 +116,30 @@ __device__ __forceinline__ float wave_sum(float x) {
     return add_swap32(x);
 }
 
+// A Q8_0 block held by 4 lanes (an aligned group) of 8 values each: the rule of
+// the Q8_0 caches.  The largest magnitude is found as bits, among which an
+// infinity or a NaN is above every number: a block that has one gets a NaN scale
+// and codes of 1, so that it reads as NaN throughout.
+struct Q8Block {
+    float inv;
+    bool finite;
+    uint16_t scale;                                    // F16 bits
+    __device__ __forceinline__ uint8_t code(float z) const { return (uint8_t)(int8_t)roundf(finite ? z * inv : 1.0f); }
+};
+__device__ __forceinline__ Q8Block q8_block(const float (&z)[8]) {
+    uint32_t ab = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ab = max(ab, __float_as_uint(z[e]) & 0x7fffffffu);
+    ab = max(ab, __float_as_uint(dpp<kDppXor1>(__uint_as_float(ab))));
+    ab = max(ab, __float_as_uint(dpp<kDppXor2>(__uint_as_float(ab))));
+    Q8Block b;
+    b.finite = ab < 0x7f800000u;
+    const float d = __uint_as_float(ab) / 127.0f;
+    b.inv = d != 0.0f ? 1.0f / d : 0.0f;
+    b.scale = b.finite ? f32_to_f16(d) : (uint16_t)0x7e00u;
+    return b;
+}
+
 // First dot of a chain: the VOP3P form with an inline 0 accumulator (the
 // accumulate-in-place form would need the zero moved in first).
 __device__ __forceinline__ int sdot4_first(uint32_t a, uint32_t b) {

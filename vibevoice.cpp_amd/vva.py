@@ -33,7 +33,7 @@ EXPORTS = [
     "vva_flash_attn_ext", "vva_supports", "vva_set_attn_path", "vva_last_decode_splits",
     "vva_set_schedule", "vva_attn_noalloc", "vva_qkv_rope_append", "vva_out_proj_residual",
     "vva_set_flash_attn", "vva_decode_step", "vva_qkv_proj", "vva_set_log_callback",
-    "vva_paged_rope_append", "vva_paged_attn", "vva_add_rms_norm",
+    "vva_paged_rope_append", "vva_paged_attn", "vva_paged_read", "vva_add_rms_norm",
 ]
 
 LOG_ERROR, LOG_WARN, LOG_INFO, LOG_DEBUG = 0, 1, 2, 3
@@ -119,6 +119,7 @@ def load_library(path: str = LIB_PATH):
         "vva_set_log_callback": (None, [LOG_CB, P, I]),
         "vva_paged_rope_append": (I, [P, TP, TP, TP, TP, TP, ctypes.POINTER(BatchDesc), TP, TP, TP]),
         "vva_paged_attn": (I, [P, TP, TP, TP, ctypes.POINTER(BatchDesc), F, TP]),
+        "vva_paged_read": (I, [P, ctypes.POINTER(BatchDesc), TP, TP, TP, TP]),
         "vva_add_rms_norm": (I, [P, TP, TP, TP, F, TP, TP]),
     }
     for name, (res, args) in sig.items():
@@ -192,8 +193,22 @@ def q8_view(raw) -> Tensor:
     return v
 
 
+def q8_pages(raw, d: int) -> Tensor:
+    """View of uint8 [n_pages, Hkv, page_size * d / 32 * 34], each [page, head] one run, as Q8_0 pages ne = [d, page_size,
+    Hkv, n_pages]; it keeps them alive.  A run is page_size rows of d codes, then d / 32 rows of page_size F16 scales."""
+    torch = _torch()
+    row = d // 32 * Q8_BLOCK_BYTES
+    if raw.dtype != torch.uint8 or raw.dim() != 3 or raw.stride(2) != 1 or d % 32 or d < 32 or raw.shape[2] % row:
+        raise ValueError(f"q8_pages: uint8 [n_pages, Hkv, page_size * {row}] of whole runs, not {raw.dtype} "
+                         f"{tuple(raw.shape)} of strides {raw.stride()}")
+    n, h, size = raw.shape
+    v = view(raw, ggml_ne=[d, size // row, h, n], ggml_nb=[Q8_BLOCK_BYTES, row, raw.stride(1), raw.stride(0)], type_=Q8_0)
+    v.raw = raw
+    return v
+
+
 def _rows_view(x) -> Tensor:
-    """Token rows: a torch tensor, or a view made already (q8_view)."""
+    """Token rows or pages: a torch tensor, or a view made already (q8_view, q8_pages)."""
     return x if isinstance(x, Tensor) else view(x)
 
 
@@ -358,26 +373,37 @@ class Context:
 
     def bind_paged_rope_append(self, q, k, v, rope, batch: Batch, k_pages, v_pages, q_out, pos=None):
         """q, q_out: [N, Hq, d]; k, v: [N, Hkv, d] packed tokens; rope f32 [n_pos, d] (cos, then sin); pos int32 [N] or
-        None; k_pages, v_pages: [n_pages, Hkv, page_size, d].  Returns the call."""
+        None; k_pages, v_pages: [n_pages, Hkv, page_size, d], or q8_pages(...) of Q8_0 ones.  Returns the call."""
         self._here(q, k, v, rope, pos, batch, k_pages, v_pages, q_out)
         return self._bound(self.lib.vva_paged_rope_append, (q, k, v, rope, pos, batch, k_pages, v_pages, q_out), view(q),
-                           view(k), view(v), view(rope), view(pos) if pos is not None else None, batch.c, view(k_pages),
-                           view(v_pages), view(q_out))
+                           view(k), view(v), view(rope), view(pos) if pos is not None else None, batch.c,
+                           _rows_view(k_pages), _rows_view(v_pages), view(q_out))
 
     def paged_rope_append(self, *args, **kw):
         """bind_paged_rope_append's call, once."""
         self.bind_paged_rope_append(*args, **kw)()
 
     def bind_paged_attn(self, q, k_pages, v_pages, batch: Batch, scale: float, out):
-        """q, out: [N, Hq, d] packed tokens in the pages' dtype; k_pages, v_pages: [n_pages, Hkv, page_size, d].  Returns
-        the call."""
+        """q, out: [N, Hq, d] packed tokens in the pages' dtype (over q8_pages(...) f16 or bf16); k_pages, v_pages:
+        [n_pages, Hkv, page_size, d].  Returns the call."""
         self._here(q, k_pages, v_pages, batch, out)
-        return self._bound(self.lib.vva_paged_attn, (q, k_pages, v_pages, batch, out), view(q), view(k_pages),
-                           view(v_pages), batch.c, scale, view(out))
+        return self._bound(self.lib.vva_paged_attn, (q, k_pages, v_pages, batch, out), view(q), _rows_view(k_pages),
+                           _rows_view(v_pages), batch.c, scale, view(out))
 
     def paged_attn(self, *args, **kw):
         """bind_paged_attn's call, once."""
         self.bind_paged_attn(*args, **kw)()
+
+    def bind_paged_read(self, batch: Batch, k_pages, v_pages, k=None, v=None):
+        """k, v: [N, Hkv, d], receive the keys and values of the batch's tokens (either None); k_pages, v_pages:
+        [n_pages, Hkv, page_size, d], or q8_pages(...).  Returns the call."""
+        self._here(batch, k_pages, v_pages, k, v)
+        return self._bound(self.lib.vva_paged_read, (batch, k_pages, v_pages, k, v), batch.c, _rows_view(k_pages),
+                           _rows_view(v_pages), view(k) if k is not None else None, view(v) if v is not None else None)
+
+    def paged_read(self, *args, **kw):
+        """bind_paged_read's call, once."""
+        self.bind_paged_read(*args, **kw)()
 
     def bind_add_rms_norm(self, x, w, y, add=None, total=None, eps: float = 1.0e-6):
         """x, add, total (receives x + add): [B, T, hidden]; w f32 [hidden]; y: a tensor like x or q8_view(...) of Q8_0
