@@ -54,7 +54,6 @@
 #include "vva_internal.hpp"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace vva {
 
@@ -241,39 +240,6 @@ __device__ __forceinline__ typename Frag<KT>::type q_frag(u32x4 x) {
     }
     return as_vec<typename Frag<KT>::type>(x);
 }
-// 4 codes of a Q8_0 page times their scale, as F16: 1024 + (code + 128) has the
-// code's byte as its last bits, so a byte permutation and an exact subtraction
-// make a pair; the product with the scale is rounded (2^-11 at most).
-__device__ __forceinline__ u32x2 q8_values(uint32_t codes, h2 scale) {
-    const uint32_t x = codes ^ 0x80808080u;
-    const uint32_t p[2] = {__builtin_amdgcn_perm(0x64646464u, x, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)};
-    u32x2 r;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        h2 v;
-        __builtin_memcpy(&v, &p[i], 4);
-        v = (v - h2{(_Float16)1152.0f, (_Float16)1152.0f}) * scale;
-        uint32_t u;
-        __builtin_memcpy(&u, &v, 4);
-        r[i] = u;
-    }
-    return r;
-}
-__device__ __forceinline__ h2 q8_scale(uint16_t bits) {
-    _Float16 s;
-    __builtin_memcpy(&s, &bits, 2);
-    return h2{s, s};
-}
-// Row r, chunk c (16 dims) of a 16-bit tile from the codes of those dims
-template <int D, bool V>
-__device__ __forceinline__ void q8_store(uint32_t tile, int r, int c, u32x4 codes, uint16_t scale) {
-    const h2 sc = q8_scale(scale);
-    const u32x2 a = q8_values(codes.x, sc), b = q8_values(codes.y, sc), e = q8_values(codes.z, sc), f = q8_values(codes.w, sc);
-    const int z = V ? v_swz<D>(r) : k_swz<D>(r);
-    *lds_vec(tile + r * 2 * D + (((2 * c) ^ z) << 4)) = u32x4{a.x, a.y, b.x, b.y};
-    *lds_vec(tile + r * 2 * D + (((2 * c + 1) ^ z) << 4)) = u32x4{e.x, e.y, f.x, f.y};
-}
-
 // The kernel's arguments, read again from their segment: each phase loads the
 // few that it needs (they hit the scalar cache), so that not all of them are
 // held, and spilled, through the key tiles.
@@ -397,35 +363,85 @@ constexpr int kFewTickets = kMaxPagedSeqHeads + 4 * kMaxWgs;
 // streams of 1k keys 6.8 -> 7.3, 1 x 32768 keys 23.2 -> 22.2)
 constexpr int kMergeBatch = 8;
 
-// LDS of few_piece: a K and a V tile per wave and the rows of Q, then the
-// waves' sums
-template <int D, int WAVES>
+// LDS of few_piece: the rows of Q and a wave's tiles (16-bit pages: a K and a V
+// tile, Q8_0: two of each, codes and scales), then the waves' sums
+template <int D, int PT, int WAVES>
 struct FewLds {
-    static constexpr int TB = kFewTile * 2 * D;    // bytes of a K (V) tile, and of the rows of Q
+    static constexpr int TB = kFewTile * 2 * D;    // bytes of a 16-bit K (V) tile, and of the rows of Q
     static constexpr int OP = D + 4;               // pitch of a row of sums
-    static constexpr int SUMS = WAVES * kFewRows * (OP + 2) * (int)sizeof(float), RING = (WAVES * 2 + 1) * TB;
+    static constexpr int SUMS = WAVES * kFewRows * (OP + 2) * (int)sizeof(float);
+    static constexpr int RING = PT == VVA_TYPE_Q8_0 ? TB + WAVES * 4 * (kFewTile * D + kFewTile * (D / 32) * 2) : (WAVES * 2 + 1) * TB;
     static constexpr int BYTES = RING > SUMS ? RING : SUMS;
 };
 
-// A workgroup's piece of a sequence's keys, for one kv head: each wave streams
-// every WAVES-th tile of the piece through LDS of its own, without a barrier:
-// the next K goes out when K is read, the next V when V is, so 16 KB of the
-// wave's loads fly while it waits and 8 while it computes.  The waves' sums
-// meet at the end.  Partials in the workspace, per piece and kv head: [cap
-// rows][D] sums, then [cap] (exponent base, row sum).
-template <int D, int PT, int OT, int WAVES, bool SHARES>
-__device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, int cap, const FewItem& it, int kvh, char* lds) {
-    constexpr int KT = kComp<PT>;
-    constexpr bool Q8 = PT == VVA_TYPE_Q8_0;
+// What a wave's walk over the tiles of a piece leaves
+template <int D>
+struct FewSums {
+    f32x16 o[D / 32];
+    float m, lsum;
+    bool bad;                       // a page outside the pool
+};
+// The rows of Q into LDS, a part by each wave, laid out as 16-bit K is; rows that
+// are not there are row 0 again (no one reads their results)
+template <int D, int WAVES>
+__device__ __forceinline__ void few_load_q(const PagedArgs& a, const FewItem& it, int kvh, int rows, uint32_t qs) {
+    constexpr int NC = kFewRows * 2 * D / 1024, RC = 1024 / (2 * D);
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t qb = uniform64((uint64_t)(uintptr_t)a.q + (int64_t)it.q.q0 * a.q_nb_t + (int64_t)kvh * a.G * a.q_nb_h);
+#pragma unroll
+    for (int i = 0; i < (NC + WAVES - 1) / WAVES; ++i) {
+        const int c = w + i * WAVES;
+        if (NC % WAVES && c >= NC) break;
+        const int r = c * RC + lane / (D / 8), row = r < rows ? r : 0;
+        const int rt = div_g(a, row), off = rt * (int)a.q_nb_t + (row - rt * a.G) * (int)a.q_nb_h;
+        dma16<false>(qb, off + (((lane % (D / 8)) ^ k_swz<D>(r)) << 4), qs + c * 1024);
+    }
+}
+// The softmax of a tile's scores: the running max and the sums raised to it, the
+// probabilities packed (BF16: with what their rounding leaves), their sum
+template <int D, int KT>
+__device__ __forceinline__ void few_probs(const f32x16& s, float sl2, FewSums<D>& f, uint32_t (&p)[8], uint32_t (&rest)[8]) {
+    float mx = fmaxf(s[0], s[1]);
+#pragma unroll
+    for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
+    mx = max_swap32(mx) * sl2;
+    if (__any(mx > f.m + kLazy)) {
+        if (mx > f.m + kLazy) {
+            const float alpha = __builtin_amdgcn_exp2f(f.m - mx);  // 0 while m = -inf
+            f.lsum *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt) f.o[dt] *= alpha;
+            f.m = mx;
+        }
+    }
+    const float nb = kLift<KT> - (f.m == -INFINITY ? 0.0f : f.m);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * r], sl2, nb)), y = __builtin_amdgcn_exp2f(fmaf(s[2 * r + 1], sl2, nb));
+        if constexpr (KT == VVA_TYPE_BF16) {
+            split2_bf16(x, y, p[r], rest[r]);
+            f.lsum = sum2<KT>(rest[r], f.lsum);
+        } else {
+            p[r] = pack2<KT>(x, y);
+        }
+        f.lsum = sum2<KT>(p[r], f.lsum);
+    }
+}
+
+// Each wave streams every WAVES-th tile of a piece through LDS of its own, without
+// a barrier: the next K goes out when K is read, the next V when V is, so 16 KB of
+// the wave's loads fly while it waits and 8 while it computes.
+template <int D, int KT, int WAVES>
+__device__ __forceinline__ void few_stream(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D>& f) {
     using F = Frag<KT>;
     using QF = typename F::type;
     constexpr int DS = D / 16, DT = D / 32;
     constexpr int NC = kFewTile * 2 * D / 1024;    // loads of a K (V) tile
     constexpr int RC = 1024 / (2 * D);             // rows of a load
-    constexpr int TB = FewLds<D, WAVES>::TB, OP = FewLds<D, WAVES>::OP;
+    constexpr int TB = FewLds<D, KT, WAVES>::TB;
 
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = min(it.q.n, a.max_new), L = it.q.L, rows = n * a.G, past = L - it.q.n;
     const int t0 = it.t0, t1 = it.t1;
 
@@ -439,7 +455,6 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
         koff[i] = dma_off<D, false>(lane, i * RC, (int)a.k_nb_slot);
         voff[i] = dma_off<D, true>(lane, i * RC, (int)a.v_nb_slot);
     }
-    bool bad = false;
     int ids[2];                                    // pages of the two 16-key halves of the next tile to load
     auto fetch = [&](int t) {
 #pragma unroll
@@ -450,7 +465,7 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const bool ok = (uint32_t)ids[i] < (uint32_t)a.n_pages;
-            bad = bad || !ok;
+            f.bad = f.bad || !ok;
             const int64_t id = ok ? ids[i] : 0;
             const int64_t slot = (t * kFewTile + 16 * i) & ((1 << a.page_shift) - 1);
             base[i] = uniform64((uint64_t)(uintptr_t)pool + id * nb_page + kvh * nb_head + slot * nb_slot);
@@ -461,51 +476,15 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
             dma16<true>(base[r / 16] + (uint64_t)(r % 16) * nb_slot, off[c % 4], dst + c * 1024);
         }
     };
-    auto issue_q8 = [&](int t, uint32_t dst, const char* pool, int64_t nb_page, int64_t nb_head, auto is_v) {
-        constexpr int C = D / 16, N = kFewTile * C / 64;
-        const int page = 1 << a.page_shift;
-        u32x4 codes[N];
-        uint16_t scale[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int r = i * (64 / C) + lane / C, c = lane % C, hf = i * (64 / C) / 16;
-            const bool ok = (uint32_t)ids[hf] < (uint32_t)a.n_pages;
-            bad = bad || !ok;
-            const char* p = pool + (int64_t)(ok ? ids[hf] : 0) * nb_page + kvh * nb_head;
-            const int slot = ((t * kFewTile + 16 * hf) & (page - 1)) + r % 16;
-            codes[i] = *(const u32x4*)(p + slot * D + c * 16);
-            scale[i] = *(const uint16_t*)(p + page * D + ((c >> 1) * page + slot) * 2);
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) q8_store<D, decltype(is_v)::value>(dst, i * (64 / C) + lane / C, lane % C, codes[i], scale[i]);
-    };
-    auto issue_k = [&](int t) {
-        if constexpr (Q8) issue_q8(t, ks, a.k, a.k_nb_page, a.k_nb_head, std::false_type{});
-        else issue(t, ks, a.k, a.k_nb_page, a.k_nb_head, a.k_nb_slot, koff);
-    };
-    auto issue_v = [&](int t) {
-        if constexpr (Q8) issue_q8(t, vs, a.v, a.v_nb_page, a.v_nb_head, std::true_type{});
-        else issue(t, vs, a.v, a.v_nb_page, a.v_nb_head, a.v_nb_slot, voff);
-    };
+    auto issue_k = [&](int t) { issue(t, ks, a.k, a.k_nb_page, a.k_nb_head, a.k_nb_slot, koff); };
+    auto issue_v = [&](int t) { issue(t, vs, a.v, a.v_nb_page, a.v_nb_head, a.v_nb_slot, voff); };
     int t = t0 + w;
     if (t < t1) fetch(t);
-    // the rows of Q, a part by each wave, laid out as K is; rows that are
-    // not there are row 0 again (no one reads their results)
-    {
-        const uint64_t qb = uniform64((uint64_t)(uintptr_t)a.q + (int64_t)it.q.q0 * a.q_nb_t + (int64_t)kvh * a.G * a.q_nb_h);
-#pragma unroll
-        for (int i = 0; i < (NC + WAVES - 1) / WAVES; ++i) {
-            const int c = w + i * WAVES;
-            if (NC % WAVES && c >= NC) break;
-            const int r = c * RC + lane / (D / 8), row = r < rows ? r : 0;
-            const int rt = div_g(a, row), off = rt * (int)a.q_nb_t + (row - rt * a.G) * (int)a.q_nb_h;
-            dma16<false>(qb, off + (((lane % (D / 8)) ^ k_swz<D>(r)) << 4), qs + c * 1024);
-        }
-    }
+    few_load_q<D, WAVES>(a, it, kvh, rows, qs);
     if (t < t1) {
         issue_k(t);
         issue_v(t);
-        wait_vm<Q8 ? 0 : 2 * NC>();                // Q
+        wait_vm<2 * NC>();                         // Q
     } else {
         wait_vm<0>();
     }
@@ -513,17 +492,13 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
     const int k_off = k_lane_off<D>(lane), v_off = v_lane_off<D>(lane);
     QF qf[DS];
 #pragma unroll
-    for (int ds = 0; ds < DS; ++ds) qf[ds] = q_frag<KT, OT>(lds_read((qs + k_off) ^ (ds << 5)));
+    for (int ds = 0; ds < DS; ++ds) qf[ds] = as_vec<QF>(lds_read((qs + k_off) ^ (ds << 5)));
     const int lim = l32 < rows ? min(L - 1, past + div_g(a, l32)) : -1;   // the last key the lane's row sees
     const float sl2 = a.scale * kLog2e;
-    float m = -INFINITY, lsum = 0.0f;
-    f32x16 o[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
     for (; t < t1; t += WAVES) {
         const bool more = t + WAVES < t1;
         if (more) fetch(t + WAVES);
-        wait_vm<Q8 ? 0 : NC>();                    // K; V may still fly
+        wait_vm<NC>();                             // K; V may still fly
         f32x16 s{};
 #pragma unroll
         for (int ds = 0; ds < DS; ++ds) s = F::mma(as_vec<QF>(lds_read((ks + k_off) ^ (ds << 5))), qf[ds], s);
@@ -537,34 +512,10 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + r % 4 > lim - k0 - 4 * half ? -INFINITY : s[r];
         }
-        float mx = fmaxf(s[0], s[1]);
-#pragma unroll
-        for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
-        mx = max_swap32(mx) * sl2;
-        if (__any(mx > m + kLazy)) {
-            if (mx > m + kLazy) {
-                const float alpha = __builtin_amdgcn_exp2f(m - mx);    // 0 while m = -inf
-                lsum *= alpha;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-                m = mx;
-            }
-        }
-        const float nb = kLift<KT> - (m == -INFINITY ? 0.0f : m);
         uint32_t p[8];
         [[maybe_unused]] uint32_t rest[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * r], sl2, nb)), y = __builtin_amdgcn_exp2f(fmaf(s[2 * r + 1], sl2, nb));
-            if constexpr (KT == VVA_TYPE_BF16) {
-                split2_bf16(x, y, p[r], rest[r]);
-                lsum = sum2<KT>(rest[r], lsum);
-            } else {
-                p[r] = pack2<KT>(x, y);
-            }
-            lsum = sum2<KT>(p[r], lsum);
-        }
-        if (more) wait_vm<Q8 ? 0 : NC>();          // V; the next K may still fly
+        few_probs<D, KT>(s, sl2, f, p, rest);
+        if (more) wait_vm<NC>();                   // V; the next K may still fly
         else wait_vm<0>();
         const bool fix = masked && tile_not_finite<D, KT, kFewTile>(vs, lane);
 #pragma unroll
@@ -575,19 +526,40 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
                 const uint32_t v = ((vs + v_off) ^ (dt << 6)) + kk * 16 * 2 * D;
                 u32x4 vf = v_bits<KT>(lds_at(v), lds_at(v + 8 * 2 * D));
                 if (fix) vf = u32x4{finite2<KT>(vf.x), finite2<KT>(vf.y), finite2<KT>(vf.z), finite2<KT>(vf.w)};
-                o[dt] = F::mma(as_vec<QF>(vf), pf, o[dt]);
+                f.o[dt] = F::mma(as_vec<QF>(vf), pf, f.o[dt]);
                 if constexpr (KT == VVA_TYPE_BF16)
-                    o[dt] = F::mma(as_vec<QF>(vf), as_vec<QF>(u32x4{rest[4 * kk], rest[4 * kk + 1], rest[4 * kk + 2], rest[4 * kk + 3]}), o[dt]);
+                    f.o[dt] = F::mma(as_vec<QF>(vf), as_vec<QF>(u32x4{rest[4 * kk], rest[4 * kk + 1], rest[4 * kk + 2], rest[4 * kk + 3]}), f.o[dt]);
             }
         }
-        if (fix) add_not_finite<D, KT, kFewTile>(vs, k0, lim, half, o);
+        if (fix) add_not_finite<D, KT, kFewTile>(vs, k0, lim, half, f.o);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // V is read
             issue_v(t + WAVES);
         }
     }
+}
+
+#include "paged_q8.hpp"
+
+// A workgroup's piece of a sequence's keys, for one kv head.  The waves' sums
+// meet at the end.  Partials in the workspace, per piece and kv head: [cap
+// rows][D] sums, then [cap] (exponent base, row sum).
+template <int D, int PT, int OT, int WAVES, bool SHARES>
+__device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, int cap, const FewItem& it, int kvh, char* lds) {
+    constexpr int DT = D / 32, OP = FewLds<D, PT, WAVES>::OP;
+    const int tid = threadIdx.x, half = (tid & 63) >> 5, l32 = tid & 31;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rows = min(it.q.n, a.max_new) * a.G;
+    FewSums<D> f;
+    f.m = -INFINITY;
+    f.lsum = 0.0f;
+    f.bad = false;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) f.o[dt] = f32x16{};
+    if constexpr (PT == VVA_TYPE_Q8_0) few_stream_q8<D, OT, WAVES>(a, it, kvh, lds, f);
+    else few_stream<D, PT, WAVES>(a, it, kvh, lds, f);
     // ---- the waves' sums, in LDS, added in wave order
-    const float lt = add_swap32(lsum);
+    const float lt = add_swap32(f.lsum);
     __syncthreads();
     float* const ow = (float*)lds;
     float* const ml = ow + WAVES * kFewRows * OP;
@@ -597,10 +569,10 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
                 *(float4*)(ow + (w * kFewRows + l32) * OP + dt * 32 + 8 * q4 + 4 * half) =
-                    make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
-        if (half == 0) *(float2*)(ml + (w * kFewRows + l32) * 2) = make_float2(m, lt);
+                    make_float4(f.o[dt][4 * q4], f.o[dt][4 * q4 + 1], f.o[dt][4 * q4 + 2], f.o[dt][4 * q4 + 3]);
+        if (half == 0) *(float2*)(ml + (w * kFewRows + l32) * 2) = make_float2(f.m, lt);
     }
-    const bool bad_page = __syncthreads_or(bad);
+    const bool bad_page = __syncthreads_or(f.bad);
     const PagedArgs& args = fresh_args();
     // thread i's part of the sums: 4 dims of a row
     struct Sum {
@@ -641,11 +613,11 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
         const float base = x.M == -INFINITY ? 0.0f : x.M;
 #pragma unroll
         for (int k = 0; k < WAVES; ++k) {
-            const float f = __builtin_amdgcn_exp2f(ml[(k * kFewRows + row) * 2] - base);   // 0 for a wave without keys
+            const float e = __builtin_amdgcn_exp2f(ml[(k * kFewRows + row) * 2] - base);   // 0 for a wave without keys
             const float4 v = *(const float4*)(ow + (k * kFewRows + row) * OP + 4 * c);
-            x.den = fmaf(f, ml[(k * kFewRows + row) * 2 + 1], x.den);
-            x.num.x = fmaf(f, v.x, x.num.x); x.num.y = fmaf(f, v.y, x.num.y);
-            x.num.z = fmaf(f, v.z, x.num.z); x.num.w = fmaf(f, v.w, x.num.w);
+            x.den = fmaf(e, ml[(k * kFewRows + row) * 2 + 1], x.den);
+            x.num.x = fmaf(e, v.x, x.num.x); x.num.y = fmaf(e, v.y, x.num.y);
+            x.num.z = fmaf(e, v.z, x.num.z); x.num.w = fmaf(e, v.w, x.num.w);
         }
         if (it.parts > 1) store(it.part, row, c, x, bad_page);
         else write(row, c, x, bad_page);
@@ -736,7 +708,7 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
 template <int D, int PT, int OT>
 __global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets, int slots, int cap) {
     prefetch_kernargs<sizeof(PagedArgs)>();
-    __shared__ __attribute__((aligned(1024))) char lds[FewLds<D, kFewWaves>::BYTES];
+    __shared__ __attribute__((aligned(1024))) char lds[FewLds<D, PT, kFewWaves>::BYTES];
     const FewItem it = few_item(a, blockIdx.x / a.Hkv, slots, kFewWaves);
     if (it.parts > 0) few_piece<D, PT, OT, kFewWaves, false>(a, ws, tickets, cap, it, blockIdx.x % a.Hkv, lds);
 }
@@ -1563,7 +1535,7 @@ constexpr float kFewTime = D == 64 ? 0.16f : 0.22f;
 template <int D, int PT, int OT>
 __global__ void __launch_bounds__(kWaves * 64) paged_mixed_kernel(PagedArgs a, float* __restrict__ ws, float* __restrict__ few_ws, unsigned* tickets, int cap) {
     prefetch_kernargs<sizeof(PagedArgs)>();
-    constexpr int FEW = FewLds<D, kWaves>::BYTES;
+    constexpr int FEW = FewLds<D, PT, kWaves>::BYTES;
     __shared__ __attribute__((aligned(1024))) char lds[ManyLds<D>::BYTES > FEW ? ManyLds<D>::BYTES : FEW];
     __shared__ int marks[2];
     const Seq mine = seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1));

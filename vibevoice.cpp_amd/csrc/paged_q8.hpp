@@ -1,0 +1,277 @@
+// paged_q8.hpp — Q8_0 pages in paged_attn.hip: their loads, their values as
+// operands of v_mfma_f32_32x32x16_f16, and the few rows' walk over them.
+// gfx950 only.  Included inside the anonymous namespace of paged_attn.hip.
+//
+// A run (a page of a head) is page_size rows of D codes, then D / 32 rows of
+// page_size F16 scales.  Codes go into LDS as they are, 16-byte chunk c of row r
+// at chunk c ^ f(r); beside a tile's codes lie its scales, [block][key].
+#pragma once
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+// XORed to the chunk index of a row of codes.  K: 8 lanes read a chunk each of 8
+// rows, which f spreads over all banks; V: the transposing read takes 32 bytes of
+// each of 8 rows (f even: a pair of chunks stays one).
+template <int D> __device__ __forceinline__ int kq_swz(int row) { return D == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
+template <int D> __device__ __forceinline__ int vq_swz(int row) { return D == 128 ? row & 6 : (row >> 1) & 2; }
+
+// 64 lanes' 4 bytes, each from an address of its own, to LDS lds .. lds + 255;
+// as dma16, non-temporal or not.
+template <bool NT>
+__device__ __forceinline__ void dma4(uint64_t addr, uint32_t lds) {
+    if constexpr (NT)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off nt"
+                     :
+                     : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(addr)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off"
+                     :
+                     : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(addr)
+                     : "memory", "m0");
+}
+
+__device__ __forceinline__ h2 as_h2(uint32_t x) {
+    h2 v;
+    __builtin_memcpy(&v, &x, 4);
+    return v;
+}
+__device__ __forceinline__ uint32_t as_bits(h2 v) {
+    uint32_t x;
+    __builtin_memcpy(&x, &v, 4);
+    return x;
+}
+__device__ __forceinline__ h2 q8_scale(uint16_t bits) { return as_h2(bits | ((uint32_t)bits << 16)); }
+
+// 4 codes as two pairs of F16: 1024 + (code + 128) has the code's byte as its
+// last bits, so a byte permutation and an exact subtraction make a pair.
+__device__ __forceinline__ void q8_codes(uint32_t codes, h2& a, h2& b) {
+    const uint32_t x = codes ^ 0x80808080u;
+    const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    a = as_h2(__builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - bias;
+    b = as_h2(__builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - bias;
+}
+// 8 codes (two words) times a pair's scales each, as an operand of 8 F16, and
+// what its rounding left (exact but for the smallest values; the operand is
+// infinite beyond 65504, and the rest of no use)
+struct Q8Frag {
+    u32x4 hi, lo;
+};
+template <bool LO>
+__device__ __forceinline__ Q8Frag q8_frag(uint32_t c0, uint32_t c1, const h2 (&scale)[4]) {
+    h2 c[4];
+    q8_codes(c0, c[0], c[1]);
+    q8_codes(c1, c[2], c[3]);
+    Q8Frag f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const h2 v = c[i] * scale[i];
+        f.hi[i] = as_bits(v);
+        if constexpr (LO) f.lo[i] = as_bits(__builtin_elementwise_fma(c[i], scale[i], -v));
+    }
+    return f;
+}
+// Row r, chunk c (16 dims) of a 16-bit tile from the codes of those dims
+template <int D, bool V>
+__device__ __forceinline__ void q8_store(uint32_t tile, int r, int c, u32x4 codes, uint16_t scale) {
+    const h2 x = q8_scale(scale);
+    const h2 x4[4] = {x, x, x, x};
+    const int z = V ? v_swz<D>(r) : k_swz<D>(r);
+    *lds_vec(tile + r * 2 * D + (((2 * c) ^ z) << 4)) = q8_frag<false>(codes.x, codes.y, x4).hi;
+    *lds_vec(tile + r * 2 * D + (((2 * c + 1) ^ z) << 4)) = q8_frag<false>(codes.z, codes.w, x4).hi;
+}
+// whether either of two scales may take a code's value beyond F16, or is not finite
+__device__ __forceinline__ bool q8_big2(uint32_t x) { return (x & 0x7fffu) >= 0x6000u || ((x >> 16) & 0x7fffu) >= 0x6000u; }
+
+// O += the infinities and NaNs of a tile's V that this lane's row sees (keys k0
+// .. of the tile up to lim).  Codes of N rows at v_lds, scales [block][N] at s_lds.
+template <int D, int N>
+__device__ __forceinline__ void q8_add_not_finite(uint32_t v_lds, uint32_t s_lds, int k0, int lim, int half, f32x16 (&o)[D / 32]) {
+    for (int j = 0; j < N; ++j) {
+        const bool seen = k0 + j <= lim;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+            const h2 s = q8_scale(*(const __attribute__((address_space(3))) uint16_t*)lds_at(s_lds + (dt * N + j) * 2));
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                const uint32_t c = *(const __attribute__((address_space(3))) uint32_t*)lds_at(
+                    v_lds + j * D + (((2 * dt + (q4 >> 1)) ^ vq_swz<D>(j)) << 4) + 8 * (q4 & 1) + 4 * half);
+                h2 x[2];
+                q8_codes(c, x[0], x[1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const _Float16 v = (x[e / 2] * s)[e % 2];
+                    if (seen && !__builtin_isfinite((float)v)) o[dt][4 * q4 + e] += (float)v;
+                }
+            }
+        }
+    }
+}
+
+// The tiles t0 + w, + WAVES, ... below t1 of a piece, as few_stream: of 32 keys,
+// two under way while one is computed (a stage is 8.5 KB: one alone would leave
+// less than half of what the 16-bit tiles have in flight).
+// LO: the rounding of scale times code to F16 goes into the products as well,
+// in a second one with the rest, so that K and V are what the pages hold but for
+// 2^-22: results rounded to F16 show it (error of a 30k-key step 4.1e-4 of its
+// size without, 2.8e-4 with, of which the rounding of the result is 2.1e-4; BF16
+// ones do not).  Against tiles converted to F16 on their way into LDS, one under
+// way: 48 sequences of 500 to 8000 keys (215 MB) 61.4 -> 48.1 us.
+template <int D, int OT, int WAVES>
+__device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D>& r) {
+    using F = Frag<VVA_TYPE_F16>;
+    constexpr int KT = VVA_TYPE_F16;
+    constexpr bool LO = OT == VVA_TYPE_F16;
+    constexpr int NB = D / 32;                     // blocks of a row, 32-dim tiles of the sums
+    constexpr int CB = kFewTile * D, SB = kFewTile * NB * 2;           // codes and scales of a tile
+    constexpr int STAGE = 2 * (CB + SB), QB = FewLds<D, VVA_TYPE_Q8_0, WAVES>::TB;
+    static_assert(QB + WAVES * 2 * STAGE == FewLds<D, VVA_TYPE_Q8_0, WAVES>::RING, "the ring fits");
+    constexpr int NC = CB / 1024, RC = 1024 / D;   // loads of a tile's codes, rows of one
+    constexpr int NL = NC + 1;                     // with its scales
+    constexpr int NV = 16 / RC;                    // loads of 16 keys
+    const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int L = it.q.L, rows = min(it.q.n, a.max_new) * a.G, past = L - it.q.n, t1 = it.t1;
+    const ConstInts table = (ConstInts)(uintptr_t)(a.table + (int64_t)it.q.s * a.table_stride);
+    const int last_page = (L - 1) >> a.page_shift, page = 1 << a.page_shift;
+    const uint32_t qs = (uint32_t)(uintptr_t)(lds_char*)lds, ring = qs + QB + w * 2 * STAGE;
+
+    int koff[NV], voff[NV];                        // codes: from the first slot of 16
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int row = i * RC + lane / (D / 16), c = lane % (D / 16);
+        koff[i] = row * D + ((c ^ kq_swz<D>(row)) << 4);
+        voff[i] = row * D + ((c ^ vq_swz<D>(row)) << 4);
+    }
+    const int soff = page * D + (((lane >> 4) << a.page_shift) + 2 * (lane & 7)) * 2;   // scales: two keys of a block
+    int ids[2];                                    // pages of the two 16-key halves of the next tile to load
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ids[i] = table[min((t * kFewTile + 16 * i) >> a.page_shift, last_page)];
+    };
+    auto issue = [&](int t, uint32_t codes, uint32_t scales, const char* pool, int64_t nb_page, int64_t nb_head, const int (&off)[NV]) {
+        uint64_t run[2];
+        int slot[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool ok = (uint32_t)ids[i] < (uint32_t)a.n_pages;
+            r.bad = r.bad || !ok;
+            run[i] = uniform64((uint64_t)(uintptr_t)pool + (int64_t)(ok ? ids[i] : 0) * nb_page + kvh * nb_head);
+            slot[i] = (t * kFewTile + 16 * i) & (page - 1);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) dma16<true>(run[c / NV] + (uint64_t)slot[c / NV] * D, off[c % NV], codes + c * 1024);
+        const uint64_t s0 = run[0] + 2 * slot[0], s1 = run[1] + 2 * slot[1];
+        if (D == 128 || lane < 32) dma4<true>((lane & 8 ? s1 : s0) + soff, scales);
+    };
+    auto issue_k = [&](int t, uint32_t st) { issue(t, st, st + 2 * CB, a.k, a.k_nb_page, a.k_nb_head, koff); };
+    auto issue_v = [&](int t, uint32_t st) { issue(t, st + CB, st + 2 * CB + SB, a.v, a.v_nb_page, a.v_nb_head, voff); };
+    int t = it.t0 + w;
+    if (t < t1) fetch(t);
+    few_load_q<D, WAVES>(a, it, kvh, rows, qs);
+    if (t < t1) {
+        issue_k(t, ring);
+        issue_v(t, ring);
+        if (t + WAVES < t1) {
+            fetch(t + WAVES);
+            issue_k(t + WAVES, ring + STAGE);
+            issue_v(t + WAVES, ring + STAGE);
+            wait_vm<4 * NL>();                     // Q
+        } else {
+            wait_vm<2 * NL>();
+        }
+    } else {
+        wait_vm<0>();
+    }
+    asm volatile("s_barrier" : : : "memory");
+    // The keys of a tile in the order in which the transposing read of V gives
+    // them: row x of the scores' operand is key x with bits 2 and 3 exchanged,
+    // so a lane's accumulators are keys 16 kk + 8 half + 0 .. 7.  Of a block a lane
+    // reads 16 dims of its key at once, so Q's dims are taken in that order too.
+    const int key = (l32 & 19) | ((l32 & 4) << 1) | ((l32 & 8) >> 1);
+    const int k_off = key * D + ((half ^ kq_swz<D>(key)) << 4);
+    const int v_row = 8 * half + ((lane & 15) >> 1);
+    const int v_off = v_row * D + ((((lane >> 4) & 1) ^ vq_swz<D>(v_row)) << 4) + 8 * (lane & 1);
+    h8 qf[2 * NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) qf[2 * b + e] = q_frag<KT, OT>(lds_read(qs + l32 * 2 * D + (((4 * b + 2 * half + e) ^ k_swz<D>(l32)) << 4)));
+    const int lim = l32 < rows ? min(L - 1, past + div_g(a, l32)) : -1;   // the last key the lane's row sees
+    const float sl2 = a.scale * kLog2e;
+    auto big = [&](uint32_t scales) {              // of a tile's scales (whole wave)
+        return (bool)__any(q8_big2(*(const __attribute__((address_space(3))) uint32_t*)lds_at(scales + (lane & (SB / 4 - 1)) * 4)));
+    };
+    for (uint32_t st = ring; t < t1; t += WAVES, st = st == ring ? ring + STAGE : ring) {
+        const bool one = t + WAVES < t1, two = t + 2 * WAVES < t1;
+        const uint32_t ks = st + 2 * CB, vs = ks + SB;
+        if (two) fetch(t + 2 * WAVES);
+        if (one) wait_vm<3 * NL>();                // K; V and the next tile may still fly
+        else wait_vm<NL>();
+        f32x16 s{};
+        {
+            u32x4 c[NB];
+            uint16_t sc[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                c[b] = lds_read((st + k_off) ^ (b << 5));
+                sc[b] = *(const __attribute__((address_space(3))) uint16_t*)lds_at(ks + b * kFewTile * 2 + key * 2);
+            }
+            const bool lo = LO && !big(ks);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const h2 x = q8_scale(sc[b]);
+                const h2 x4[4] = {x, x, x, x};
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const Q8Frag f = q8_frag<LO>(c[b][2 * e], c[b][2 * e + 1], x4);
+                    s = F::mma(as_vec<h8>(f.hi), qf[2 * b + e], s);
+                    if constexpr (LO) {
+                        if (lo) s = F::mma(as_vec<h8>(f.lo), qf[2 * b + e], s);
+                    }
+                }
+            }
+        }
+        if (two) {
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // K is read
+            issue_k(t + 2 * WAVES, st);
+        }
+        const int k0 = t * kFewTile;
+        const bool masked = k0 + kFewTile - 1 > min(L - 1, past);      // some row must not see some key
+        if (masked) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) s[x] = 16 * (x / 8) + x % 8 > lim - k0 - 8 * half ? -INFINITY : s[x];
+        }
+        uint32_t p[8];
+        [[maybe_unused]] uint32_t none[8];
+        few_probs<D, KT>(s, sl2, r, p, none);
+        if (two) wait_vm<3 * NL>();                // V; what was asked for after it may still fly
+        else if (one) wait_vm<2 * NL>();
+        else wait_vm<0>();
+        bool wide = false;
+        if (LO || masked) wide = big(vs);
+        const bool fix = masked && wide;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const h8 pf = as_vec<h8>(u32x4{p[4 * kk], p[4 * kk + 1], p[4 * kk + 2], p[4 * kk + 3]});
+#pragma unroll
+            for (int dt = 0; dt < NB; ++dt) {
+                const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (__attribute__((address_space(3))) i32x2*)lds_at(((st + CB + v_off) ^ (dt << 5)) + kk * 16 * D));
+                const u32x4 sc = lds_read(vs + dt * kFewTile * 2 + kk * 32 + half * 16);
+                const h2 x4[4] = {as_h2(sc.x), as_h2(sc.y), as_h2(sc.z), as_h2(sc.w)};
+                Q8Frag f = q8_frag<LO>((uint32_t)c.x, (uint32_t)c.y, x4);
+                if (fix) f.hi = u32x4{finite2<KT>(f.hi.x), finite2<KT>(f.hi.y), finite2<KT>(f.hi.z), finite2<KT>(f.hi.w)};
+                r.o[dt] = F::mma(as_vec<h8>(f.hi), pf, r.o[dt]);
+                if constexpr (LO) {
+                    if (!wide) r.o[dt] = F::mma(as_vec<h8>(f.lo), pf, r.o[dt]);
+                }
+            }
+        }
+        if (fix) q8_add_not_finite<D, kFewTile>(st + CB, vs, k0, lim, half, r.o);
+        if (two) {
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // V is read
+            issue_v(t + 2 * WAVES, st);
+        }
+    }
+}
