@@ -945,9 +945,13 @@ __device__ __forceinline__ ManyPieces many_pieces(const PagedArgs& a, const Many
 // takes the wave's ticket: the last of up to kGroup pieces adds them, and of
 // more groups the last adds the groups, in the order of the keys whoever it is
 // (its own sums are read back too, so that they need no registers meanwhile).
-template <int D>
+template <int D, int PT>
 struct ManyLds {
-    static constexpr int BYTES = kStages * 2 * kBN * 2 * D;
+    // Q8_0: tile j + 2 is stored while tile j is computed.  The last two stages of
+    // the 16-bit ring, one of three here, take the rows of Q first.
+    static constexpr int STAGES = PT == VVA_TYPE_Q8_0 ? 3 : kStages;
+    static constexpr int Q_AT = PT == VVA_TYPE_Q8_0 ? 1 : 2;
+    static constexpr int BYTES = STAGES * 2 * kBN * 2 * D;
 };
 template <int D, int PT, int OT>
 __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, const ManyAxis& axis, const ManyPieces& pc, const Seq& mine, int block, int wgs, char* lds, int* marks) {
@@ -960,7 +964,7 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
     constexpr int TB = kBN * ROW;                  // bytes of a K (V) tile
     constexpr int NI = TB / 1024 / kWaves;         // loads of a K (V) tile per wave
     constexpr int RC = 1024 / ROW;                 // rows of a load
-    constexpr int STAGE = 2 * TB;
+    constexpr int STAGE = 2 * TB, STAGES = ManyLds<D, PT>::STAGES, Q_AT = ManyLds<D, PT>::Q_AT;
     constexpr int NLD = 2 * NI;
     constexpr int NID = Q8 ? 1 : NI;               // page ids of a wave's loads of a tile
     constexpr int WAVE_O = DT * 16 * 64 * 4;       // bytes of a wave's sums
@@ -1076,37 +1080,7 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
     // further ones of the sequence, to a stage that nobody reads any more, so
     // that every tile counts the same
     auto issue = [&](const Source& t, int j, int key, const int (&id)[NID]) {
-        if constexpr (Q8) {
-            // 8 rows a wave: K, then V (D = 64: K by the lower lanes, V by the upper)
-            const int ln = lane_id(), page = 1 << t.shift;
-            constexpr int C = D / 16;
-            const int r = 8 * w + (ln / C) % 8, c = ln % C;
-            const bool ok = (uint32_t)id[0] < (uint32_t)t.n_pages;
-            bad = bad || !ok;
-            const int64_t at = ok ? id[0] : 0;
-            const int slot = ((key + 8 * w) & (page - 1)) + r % 8;
-            const uint32_t st = lds0 + (j % kStages) * STAGE;
-            const char* kp = (const char*)(uintptr_t)(t.k + at * t.k_page);
-            const char* vp = (const char*)(uintptr_t)(t.v + at * t.v_page);
-            auto load = [&](const char* p, u32x4& codes, uint16_t& scale) {
-                codes = *(const u32x4*)(p + slot * D + c * 16);
-                scale = *(const uint16_t*)(p + page * D + ((c >> 1) * page + slot) * 2);
-            };
-            u32x4 x, y;
-            uint16_t sx, sy;
-            if constexpr (D == 128) {
-                load(kp, x, sx);
-                load(vp, y, sy);
-                q8_store<D, false>(st, r, c, x, sx);
-                q8_store<D, true>(st + TB, r, c, y, sy);
-            } else {
-                load(ln < 32 ? kp : vp, x, sx);
-                if (ln < 32) q8_store<D, false>(st, r, c, x, sx);
-                else q8_store<D, true>(st + TB, r, c, x, sx);
-            }
-            return;
-        } else {
-        const uint32_t st = lds0 + (j % kStages) * STAGE + w * 1024;
+        const uint32_t st = lds0 + (j % STAGES) * STAGE + w * 1024;
         uint64_t kb[NI], vb[NI];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
@@ -1121,6 +1095,38 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
         for (int i = 0; i < NI; ++i) dma16<false>(kb[i], koff, st + i * kWaves * 1024);
 #pragma unroll
         for (int i = 0; i < NI; ++i) dma16<false>(vb[i], voff, st + TB + i * kWaves * 1024);
+    };
+    // Q8_0: a wave takes 8 rows of a tile (D = 64: K by the lower lanes, V by the
+    // upper), a lane 16 dims of one of K and one of V: loaded a step before they are
+    // converted and stored
+    constexpr int QC = D / 16, QN = D == 128 ? 2 : 1;
+    u32x4 codes[QN];
+    uint16_t scales[QN];
+    auto load_q8 = [&](const Source& t, int key, const int (&id)[NID]) {
+        const int ln = lane_id(), page = 1 << t.shift;
+        const bool ok = (uint32_t)id[0] < (uint32_t)t.n_pages;
+        bad = bad || !ok;
+        const int64_t at = ok ? id[0] : 0;
+        const int slot = ((key + 8 * w) & (page - 1)) + (ln / QC) % 8, c = ln % QC;
+        const char* kp = (const char*)(uintptr_t)uniform64(t.k + at * t.k_page);
+        const char* vp = (const char*)(uintptr_t)uniform64(t.v + at * t.v_page);
+        const int co = slot * D + c * 16, so = page * D + ((c >> 1) * page + slot) * 2;
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const char* p = QN == 2 ? (i == 0 ? kp : vp) : (ln < 32 ? kp : vp);
+            codes[i] = *(const u32x4*)(p + co);
+            scales[i] = *(const uint16_t*)(p + so);
+        }
+    };
+    auto put_q8 = [&](int j) {
+        const int ln = lane_id(), r = 8 * w + (ln / QC) % 8, c = ln % QC;
+        const uint32_t st = lds0 + (j % STAGES) * STAGE;
+        if constexpr (QN == 2) {
+            q8_store<D, false>(st, r, c, codes[0], scales[0]);
+            q8_store<D, true>(st + TB, r, c, codes[1], scales[1]);
+        } else {
+            if (ln < 32) q8_store<D, false>(st, r, c, codes[0], scales[0]);
+            else q8_store<D, true>(st + TB, r, c, codes[0], scales[0]);
         }
     };
     // x = t * G + h for small x (below G + 32): one product
@@ -1135,10 +1141,11 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
         const int G = a.G;
         bad = false;
         const int ln = lane_id();                  // offsets made here, not held from one part to the next
-        int id0[NID], id1[NID];
+        int id0[NID];
+        [[maybe_unused]] int id1[NID];
         fetch(src, c.kb0, id0);
-        fetch(src, c.kb0 + kBN, id1);
-        fetch(src, c.kb0 + 2 * kBN, ids);
+        if constexpr (!Q8) fetch(src, c.kb0 + kBN, id1);
+        fetch(src, c.kb0 + (Q8 ? 1 : 2) * kBN, ids);
         const int wr0 = min(c.rt * kRowsWG + w * kRowsWave, c.rows - 1), live = min(kRowsWave, c.rows - wr0);
         const int t0 = div_g(a, wr0), h0 = wr0 - t0 * G;
         const uint64_t qb = uniform64((uint64_t)(uintptr_t)a.q + (int64_t)(c.q0 + t0) * a.q_nb_t + (int64_t)c.kvh * G * a.q_nb_h);
@@ -1148,10 +1155,14 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
             int t, h;
             small_divide(h0 + (r < live ? r : 0), G, t, h);
             dma16<false>(qb, t * (int)a.q_nb_t + h * (int)a.q_nb_h + (((ln % (D / 8)) ^ k_swz<D>(r)) << 4),
-                         lds0 + 2 * STAGE + w * kRowsWave * ROW + i * 1024);
+                         lds0 + Q_AT * STAGE + w * kRowsWave * ROW + i * 1024);
         }
-        issue(src, 0, c.kb0, id0);
-        issue(src, 1, c.kb0 + kBN, id1);
+        if constexpr (Q8) {
+            load_q8(src, c.kb0, id0);
+        } else {
+            issue(src, 0, c.kb0, id0);
+            issue(src, 1, c.kb0 + kBN, id1);
+        }
     };
 
     int fix_id = 0;
@@ -1183,18 +1194,28 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
         const int l32 = lane_id() & 31;
         small_divide(wr - t0 * G + (wr0 + l32 < rows ? l32 : 0), G, lim, hcol);
         lim = min(L - 1, past + t0 + lim);
+        if constexpr (Q8) put_q8(0);
         wait_vm<Q8 ? 0 : 2 * NLD>();                          // Q has landed
+        if constexpr (Q8) {
+            load_q8(src, kb0 + kBN, ids);
+            fetch(src, kb0 + 2 * kBN, ids);
+        }
         QF qf[DS];
         {
-            const uint32_t qa = lds0 + 2 * STAGE + w * kRowsWave * ROW + k_lane_off<D>(lane_id());
+            const uint32_t qa = lds0 + Q_AT * STAGE + w * kRowsWave * ROW + k_lane_off<D>(lane_id());
 #pragma unroll
             for (int ds = 0; ds < DS; ++ds) qf[ds] = q_frag<KT, OT>(lds_read(qa ^ (ds << 5)));
         }
         // K of tile 0 has landed (its V and tile 1 may still fly), and every wave has its Q
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(Q8 ? 0 : NI + NLD) : "memory");
-        issue(src, 2, kb0 + 2 * kBN, ids);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(Q8 ? 63 : NI + NLD) : "memory");
+        if constexpr (Q8) {
+            put_q8(1);
+            load_q8(src, kb0 + 2 * kBN, ids);
+        } else {
+            issue(src, 2, kb0 + 2 * kBN, ids);
+        }
         fetch(src, kb0 + 3 * kBN, ids);
-        auto stage = [&](int j) { return lds0 + (j % kStages) * STAGE; };
+        auto stage = [&](int j) { return lds0 + (j % STAGES) * STAGE; };
         auto read_k = [&](uint32_t ka, int ds, int kt) { return lds_read((ka ^ (ds << 5)) + kt * 32 * ROW); };
         auto apply_mask = [&](f32x16 (&s)[2], int k0) {
             const int x = lim - k0 - 4 * (lane_id() >> 5);
@@ -1320,8 +1341,13 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
         auto step = [&](int j, const f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
             // K of tile j + 1 and V of tile j have landed, and every wave is done
             // with tile j - 1, whose stage tile j + 3 now takes
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(Q8 ? 0 : NI + NLD) : "memory");
-            issue(src, j + 3, kb0 + (j + 3) * kBN, ids);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(Q8 ? 63 : NI + NLD) : "memory");
+            if constexpr (Q8) {
+                put_q8(j + 2);
+                load_q8(src, kb0 + (j + 3) * kBN, ids);
+            } else {
+                issue(src, j + 3, kb0 + (j + 3) * kBN, ids);
+            }
             fetch(src, kb0 + (j + 4) * kBN, ids);
             if (j < n_live) rescale(mx);                      // wave-uniform
             if (kb0 + j * kBN + kBN - 1 > lim_wg) fix_tile(j);
@@ -1460,7 +1486,7 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
 template <int D, int PT, int OT>
 __global__ void __launch_bounds__(kWaves * 64) paged_many_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets) {
     prefetch_kernargs<sizeof(PagedArgs)>();
-    __shared__ __attribute__((aligned(1024))) char lds[ManyLds<D>::BYTES];
+    __shared__ __attribute__((aligned(1024))) char lds[ManyLds<D, PT>::BYTES];
     __shared__ int marks[2];
     const Seq mine = seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1));
     const ManyAxis axis = many_axis(a, mine);
@@ -1536,7 +1562,7 @@ template <int D, int PT, int OT>
 __global__ void __launch_bounds__(kWaves * 64) paged_mixed_kernel(PagedArgs a, float* __restrict__ ws, float* __restrict__ few_ws, unsigned* tickets, int cap) {
     prefetch_kernargs<sizeof(PagedArgs)>();
     constexpr int FEW = FewLds<D, PT, kWaves>::BYTES;
-    __shared__ __attribute__((aligned(1024))) char lds[ManyLds<D>::BYTES > FEW ? ManyLds<D>::BYTES : FEW];
+    __shared__ __attribute__((aligned(1024))) char lds[ManyLds<D, PT>::BYTES > FEW ? ManyLds<D, PT>::BYTES : FEW];
     __shared__ int marks[2];
     const Seq mine = seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1));
     const ManyAxis axis = many_axis(a, mine);
