@@ -1098,35 +1098,41 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
     };
     // Q8_0: a wave takes 8 rows of a tile (D = 64: K by the lower lanes, V by the
     // upper), a lane 16 dims of one of K and one of V: loaded a step before they are
-    // converted and stored
+    // converted to F16 and stored, at the start of a step.  2048 tokens behind 28672
+    // keys take 915 us so (F16 pages, whose rows go into LDS by themselves, 870); by
+    // half of the waves at the end of the step 934, between the products 960, rows of
+    // 8 dims a lane, whose stores meet on no banks but take two loads each, 928.
     constexpr int QC = D / 16, QN = D == 128 ? 2 : 1;
     u32x4 codes[QN];
     uint16_t scales[QN];
     auto load_q8 = [&](const Source& t, int key, const int (&id)[NID]) {
-        const int ln = lane_id(), page = 1 << t.shift;
+        const uint32_t ln = lane_id(), shift = t.shift;
         const bool ok = (uint32_t)id[0] < (uint32_t)t.n_pages;
         bad = bad || !ok;
         const int64_t at = ok ? id[0] : 0;
-        const int slot = ((key + 8 * w) & (page - 1)) + (ln / QC) % 8, c = ln % QC;
-        const char* kp = (const char*)(uintptr_t)uniform64(t.k + at * t.k_page);
-        const char* vp = (const char*)(uintptr_t)uniform64(t.v + at * t.v_page);
-        const int co = slot * D + c * 16, so = page * D + ((c >> 1) * page + slot) * 2;
+        const uint32_t slot = (uint32_t)(key + 8 * w) & ((1u << shift) - 1);
+        // 8 rows of codes are one run of memory, 16 bytes a lane
+        const uint32_t co = slot * D, so = ((uint32_t)D << shift) + 2 * slot;
+        const uint32_t cl = ln % (8 * QC) * 16, sl = ((ln % QC / 2 << shift) + ln / QC % 8) * 2;
+        const uint64_t kp = uniform64(t.k + at * t.k_page), vp = uniform64(t.v + at * t.v_page);
 #pragma unroll
         for (int i = 0; i < QN; ++i) {
-            const char* p = QN == 2 ? (i == 0 ? kp : vp) : (ln < 32 ? kp : vp);
-            codes[i] = *(const u32x4*)(p + co);
-            scales[i] = *(const uint16_t*)(p + so);
+            const uint64_t p = QN == 2 ? (i == 0 ? kp : vp) : (ln < 32 ? kp : vp);
+            codes[i] = global_load<u32x4>(p + co, cl);
+            scales[i] = global_load<uint16_t>(p + so, sl);
         }
     };
     auto put_q8 = [&](int j) {
-        const int ln = lane_id(), r = 8 * w + (ln / QC) % 8, c = ln % QC;
-        const uint32_t st = lds0 + (j % STAGES) * STAGE;
-        if constexpr (QN == 2) {
-            q8_store<D, false>(st, r, c, codes[0], scales[0]);
-            q8_store<D, true>(st + TB, r, c, codes[1], scales[1]);
-        } else {
-            if (ln < 32) q8_store<D, false>(st, r, c, codes[0], scales[0]);
-            else q8_store<D, true>(st + TB, r, c, codes[0], scales[0]);
+        const uint32_t ln = lane_id(), r = 8 * w + ln / QC % 8, c = 2 * (ln % QC);
+        const uint32_t row = lds0 + (j % STAGES) * STAGE + r * ROW;
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const bool v = QN == 2 ? i == 1 : ln >= 32;
+            const uint32_t to = row + (v ? TB : 0) + ((c ^ (uint32_t)(v ? v_swz<D>(r) : k_swz<D>(r))) << 4);
+            const h2 x = q8_scale(scales[i]);
+            const h2 x4[4] = {x, x, x, x};
+            *lds_vec(to) = q8_frag<false>(codes[i].x, codes[i].y, x4).hi;
+            *lds_vec(to ^ 16) = q8_frag<false>(codes[i].z, codes[i].w, x4).hi;
         }
     };
     // x = t * G + h for small x (below G + 32): one product

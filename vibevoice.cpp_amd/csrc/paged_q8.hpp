@@ -31,6 +31,11 @@ __device__ __forceinline__ void dma4(uint64_t addr, uint32_t lds) {
                      : "memory", "m0");
 }
 
+// a T at base + off (a pointer made of integers alone would be a flat one)
+template <typename T>
+__device__ __forceinline__ T global_load(uint64_t base, uint32_t off) {
+    return *(const __attribute__((address_space(1))) T*)((const __attribute__((address_space(1))) char*)base + off);
+}
 __device__ __forceinline__ h2 as_h2(uint32_t x) {
     h2 v;
     __builtin_memcpy(&v, &x, 4);
@@ -70,15 +75,6 @@ __device__ __forceinline__ Q8Frag q8_frag(uint32_t c0, uint32_t c1, const h2 (&s
         if constexpr (LO) f.lo[i] = as_bits(__builtin_elementwise_fma(c[i], scale[i], -v));
     }
     return f;
-}
-// Row r, chunk c (16 dims) of a 16-bit tile from the codes of those dims
-template <int D, bool V>
-__device__ __forceinline__ void q8_store(uint32_t tile, int r, int c, u32x4 codes, uint16_t scale) {
-    const h2 x = q8_scale(scale);
-    const h2 x4[4] = {x, x, x, x};
-    const int z = V ? v_swz<D>(r) : k_swz<D>(r);
-    *lds_vec(tile + r * 2 * D + (((2 * c) ^ z) << 4)) = q8_frag<false>(codes.x, codes.y, x4).hi;
-    *lds_vec(tile + r * 2 * D + (((2 * c + 1) ^ z) << 4)) = q8_frag<false>(codes.z, codes.w, x4).hi;
 }
 // whether either of two scales may take a code's value beyond F16, or is not finite
 __device__ __forceinline__ bool q8_big2(uint32_t x) { return (x & 0x7fffu) >= 0x6000u || ((x >> 16) & 0x7fffu) >= 0x6000u; }
