@@ -54,6 +54,7 @@
 #include "vva_internal.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace vva {
 
@@ -62,6 +63,8 @@ namespace {
 #include "wave_ops.hpp"
 #include "mfma_ops.hpp"
 #include "paged_ops.hpp"
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLazy = 8.0f;      // running-max slack in log2 units
 // The type that the products take: the pages' own, F16 for Q8_0
@@ -251,7 +254,7 @@ __device__ __forceinline__ const PagedArgs& fresh_args() {
 
 // ------------------------------------------------------------ few rows
 
-constexpr int kFewWaves = 4;       // of a workgroup of paged_few_kernel
+constexpr int kFewWaves = 4;       // of a workgroup of paged_few_kernel (Q8_0 pages, 16 rows: 8)
 constexpr int kFewTile = 32;
 constexpr int kMaxWgs = 256;       // workgroups of the many rows at most
 constexpr int kFewCost = 4;        // what a piece costs beside its keys, in tiles
@@ -363,29 +366,53 @@ constexpr int kFewTickets = kMaxPagedSeqHeads + 4 * kMaxWgs;
 // streams of 1k keys 6.8 -> 7.3, 1 x 32768 keys 23.2 -> 22.2)
 constexpr int kMergeBatch = 8;
 
-// LDS of few_piece: the rows of Q and a wave's tiles (16-bit pages: a K and a V
-// tile, Q8_0: two of each, codes and scales), then the waves' sums
-template <int D, int PT, int WAVES>
+// How few_piece goes over pages of type PT with up to ROWS rows: tiles that a wave
+// has under way, and its LDS: the rows of Q and the waves' tiles (16-bit pages: a K
+// and a V tile, Q8_0: codes and scales of each), then the waves' sums
+template <int D, int PT, int WAVES, int ROWS>
 struct FewLds {
-    static constexpr int TB = kFewTile * 2 * D;    // bytes of a 16-bit K (V) tile, and of the rows of Q
+    static constexpr bool Q8 = PT == VVA_TYPE_Q8_0;
+    static constexpr int STAGES = Q8 && !(ROWS == 16 && D == 128) ? 2 : 1;
+    static constexpr int TILE = Q8 ? kFewTile * (D + D / 16) : kFewTile * 2 * D;   // bytes of a K (V) tile
     static constexpr int OP = D + 4;               // pitch of a row of sums
-    static constexpr int SUMS = WAVES * kFewRows * (OP + 2) * (int)sizeof(float);
-    static constexpr int RING = PT == VVA_TYPE_Q8_0 ? TB + WAVES * 4 * (kFewTile * D + kFewTile * (D / 32) * 2) : (WAVES * 2 + 1) * TB;
+    static constexpr int SUMS = WAVES * ROWS * (OP + 2) * (int)sizeof(float), RING = ROWS * 2 * D + WAVES * STAGES * 2 * TILE;
     static constexpr int BYTES = RING > SUMS ? RING : SUMS;
 };
 
-// What a wave's walk over the tiles of a piece leaves
+// What a wave's walk over the tiles of a piece leaves, for up to ROWS rows
+template <int D, int ROWS> struct FewSums;
 template <int D>
-struct FewSums {
-    f32x16 o[D / 32];
-    float m, lsum;
-    bool bad;                       // a page outside the pool
+struct FewSums<D, 32> {
+    f32x16 o[D / 32] = {};
+    float m = -INFINITY, lsum = 0.0f;
+    bool bad = false;               // a page outside the pool
+    // dims of row `lane % 32` into its row of sums; the row sum over the lanes
+    __device__ __forceinline__ void store(float* row, int lane) const {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+                *(float4*)(row + dt * 32 + 8 * q4 + 4 * (lane >> 5)) =
+                    make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
+    }
+    __device__ __forceinline__ float row_sum() const { return add_swap32(lsum); }
+};
+template <int D>
+struct FewSums<D, 16> {
+    f32x4 o[D / 16] = {};
+    float m = -INFINITY, lsum = 0.0f;
+    bool bad = false;
+    __device__ __forceinline__ void store(float* row, int lane) const {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) *(float4*)(row + i * 16 + 4 * (lane >> 4)) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+    }
+    __device__ __forceinline__ float row_sum() const { return add_swap32(add_swap16(lsum)); }
 };
 // The rows of Q into LDS, a part by each wave, laid out as 16-bit K is; rows that
 // are not there are row 0 again (no one reads their results)
-template <int D, int WAVES>
+template <int D, int WAVES, int ROWS>
 __device__ __forceinline__ void few_load_q(const PagedArgs& a, const FewItem& it, int kvh, int rows, uint32_t qs) {
-    constexpr int NC = kFewRows * 2 * D / 1024, RC = 1024 / (2 * D);
+    constexpr int NC = ROWS * 2 * D / 1024, RC = 1024 / (2 * D);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t qb = uniform64((uint64_t)(uintptr_t)a.q + (int64_t)it.q.q0 * a.q_nb_t + (int64_t)kvh * a.G * a.q_nb_h);
 #pragma unroll
@@ -400,7 +427,7 @@ __device__ __forceinline__ void few_load_q(const PagedArgs& a, const FewItem& it
 // The softmax of a tile's scores: the running max and the sums raised to it, the
 // probabilities packed (BF16: with what their rounding leaves), their sum
 template <int D, int KT>
-__device__ __forceinline__ void few_probs(const f32x16& s, float sl2, FewSums<D>& f, uint32_t (&p)[8], uint32_t (&rest)[8]) {
+__device__ __forceinline__ void few_probs(const f32x16& s, float sl2, FewSums<D, 32>& f, uint32_t (&p)[8], uint32_t (&rest)[8]) {
     float mx = fmaxf(s[0], s[1]);
 #pragma unroll
     for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
@@ -432,13 +459,13 @@ __device__ __forceinline__ void few_probs(const f32x16& s, float sl2, FewSums<D>
 // a barrier: the next K goes out when K is read, the next V when V is, so 16 KB of
 // the wave's loads fly while it waits and 8 while it computes.
 template <int D, int KT, int WAVES>
-__device__ __forceinline__ void few_stream(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D>& f) {
+__device__ __forceinline__ void few_stream(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D, 32>& f) {
     using F = Frag<KT>;
     using QF = typename F::type;
     constexpr int DS = D / 16, DT = D / 32;
     constexpr int NC = kFewTile * 2 * D / 1024;    // loads of a K (V) tile
     constexpr int RC = 1024 / (2 * D);             // rows of a load
-    constexpr int TB = FewLds<D, KT, WAVES>::TB;
+    constexpr int TB = kFewTile * 2 * D;           // bytes of a K (V) tile, and of the rows of Q
 
     const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -480,7 +507,7 @@ __device__ __forceinline__ void few_stream(const PagedArgs& a, const FewItem& it
     auto issue_v = [&](int t) { issue(t, vs, a.v, a.v_nb_page, a.v_nb_head, a.v_nb_slot, voff); };
     int t = t0 + w;
     if (t < t1) fetch(t);
-    few_load_q<D, WAVES>(a, it, kvh, rows, qs);
+    few_load_q<D, WAVES, 32>(a, it, kvh, rows, qs);
     if (t < t1) {
         issue_k(t);
         issue_v(t);
@@ -544,33 +571,25 @@ __device__ __forceinline__ void few_stream(const PagedArgs& a, const FewItem& it
 // A workgroup's piece of a sequence's keys, for one kv head.  The waves' sums
 // meet at the end.  Partials in the workspace, per piece and kv head: [cap
 // rows][D] sums, then [cap] (exponent base, row sum).
-template <int D, int PT, int OT, int WAVES, bool SHARES>
+template <int D, int PT, int OT, int WAVES, int ROWS, bool SHARES>
 __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict__ ws, unsigned* tickets, int cap, const FewItem& it, int kvh, char* lds) {
-    constexpr int DT = D / 32, OP = FewLds<D, PT, WAVES>::OP;
-    const int tid = threadIdx.x, half = (tid & 63) >> 5, l32 = tid & 31;
+    using Lds = FewLds<D, PT, WAVES, ROWS>;
+    constexpr int OP = Lds::OP;
+    const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rows = min(it.q.n, a.max_new) * a.G;
-    FewSums<D> f;
-    f.m = -INFINITY;
-    f.lsum = 0.0f;
-    f.bad = false;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) f.o[dt] = f32x16{};
-    if constexpr (PT == VVA_TYPE_Q8_0) few_stream_q8<D, OT, WAVES>(a, it, kvh, lds, f);
+    FewSums<D, ROWS> f;
+    if constexpr (ROWS == 16) few_stream16_q8<D, OT, WAVES, Lds::STAGES>(a, it, kvh, lds, f);
+    else if constexpr (Lds::Q8) few_stream_q8<D, OT, WAVES>(a, it, kvh, lds, f);
     else few_stream<D, PT, WAVES>(a, it, kvh, lds, f);
     // ---- the waves' sums, in LDS, added in wave order
-    const float lt = add_swap32(f.lsum);
+    const float lt = f.row_sum();
     __syncthreads();
     float* const ow = (float*)lds;
-    float* const ml = ow + WAVES * kFewRows * OP;
-    if (l32 < rows) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4)
-                *(float4*)(ow + (w * kFewRows + l32) * OP + dt * 32 + 8 * q4 + 4 * half) =
-                    make_float4(f.o[dt][4 * q4], f.o[dt][4 * q4 + 1], f.o[dt][4 * q4 + 2], f.o[dt][4 * q4 + 3]);
-        if (half == 0) *(float2*)(ml + (w * kFewRows + l32) * 2) = make_float2(f.m, lt);
+    float* const ml = ow + WAVES * ROWS * OP;
+    if (lane % ROWS < rows) {
+        f.store(ow + (w * ROWS + lane % ROWS) * OP, lane);
+        if (lane < ROWS) *(float2*)(ml + (w * ROWS + lane) * 2) = make_float2(f.m, lt);
     }
     const bool bad_page = __syncthreads_or(f.bad);
     const PagedArgs& args = fresh_args();
@@ -609,13 +628,13 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
         const int row = i / (D / 4), c = i % (D / 4);
         Sum x{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) x.M = fmaxf(x.M, ml[(k * kFewRows + row) * 2]);
+        for (int k = 0; k < WAVES; ++k) x.M = fmaxf(x.M, ml[(k * ROWS + row) * 2]);
         const float base = x.M == -INFINITY ? 0.0f : x.M;
 #pragma unroll
         for (int k = 0; k < WAVES; ++k) {
-            const float e = __builtin_amdgcn_exp2f(ml[(k * kFewRows + row) * 2] - base);   // 0 for a wave without keys
-            const float4 v = *(const float4*)(ow + (k * kFewRows + row) * OP + 4 * c);
-            x.den = fmaf(e, ml[(k * kFewRows + row) * 2 + 1], x.den);
+            const float e = __builtin_amdgcn_exp2f(ml[(k * ROWS + row) * 2] - base);   // 0 for a wave without keys
+            const float4 v = *(const float4*)(ow + (k * ROWS + row) * OP + 4 * c);
+            x.den = fmaf(e, ml[(k * ROWS + row) * 2 + 1], x.den);
             x.num.x = fmaf(e, v.x, x.num.x); x.num.y = fmaf(e, v.y, x.num.y);
             x.num.z = fmaf(e, v.z, x.num.z); x.num.w = fmaf(e, v.w, x.num.w);
         }
@@ -705,12 +724,12 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
 }
 
 // One workgroup per (piece, kv head), two of them (D = 64: four) on a CU.
-template <int D, int PT, int OT>
-__global__ void __launch_bounds__(kFewWaves * 64, 2) paged_few_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets, int slots, int cap) {
+template <int D, int PT, int OT, int WAVES, int ROWS>
+__global__ void __launch_bounds__(WAVES * 64, WAVES == 8 ? 4 : 2) paged_few_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets, int slots, int cap) {
     prefetch_kernargs<sizeof(PagedArgs)>();
-    __shared__ __attribute__((aligned(1024))) char lds[FewLds<D, PT, kFewWaves>::BYTES];
-    const FewItem it = few_item(a, blockIdx.x / a.Hkv, slots, kFewWaves);
-    if (it.parts > 0) few_piece<D, PT, OT, kFewWaves, false>(a, ws, tickets, cap, it, blockIdx.x % a.Hkv, lds);
+    __shared__ __attribute__((aligned(1024))) char lds[FewLds<D, PT, WAVES, ROWS>::BYTES];
+    const FewItem it = few_item(a, blockIdx.x / a.Hkv, slots, WAVES);
+    if (it.parts > 0) few_piece<D, PT, OT, WAVES, ROWS, false>(a, ws, tickets, cap, it, blockIdx.x % a.Hkv, lds);
 }
 
 // ----------------------------------------------------------- many rows
@@ -1545,7 +1564,7 @@ __device__ __forceinline__ bool few_share(const PagedArgs& a, float* __restrict_
         it.part = g - it.first;
         it.t0 = max(0, off - kFewCost);            // a cut is more than kFewCost from the ends, or at one
         it.t1 = min(off_end - kFewCost, (it.q.L + kFewTile - 1) / kFewTile);   // no keys: none
-        few_piece<D, PT, OT, kWaves, true>(a, ws, tickets, cap, it, kvh, lds);
+        few_piece<D, PT, OT, kWaves, 32, true>(a, ws, tickets, cap, it, kvh, lds);
         __syncthreads();                           // the next piece's rows of Q go where this one's sums are
     }
     return true;
@@ -1567,7 +1586,7 @@ constexpr float kFewTime = D == 64 ? 0.16f : 0.22f;
 template <int D, int PT, int OT>
 __global__ void __launch_bounds__(kWaves * 64) paged_mixed_kernel(PagedArgs a, float* __restrict__ ws, float* __restrict__ few_ws, unsigned* tickets, int cap) {
     prefetch_kernargs<sizeof(PagedArgs)>();
-    constexpr int FEW = FewLds<D, PT, kWaves>::BYTES;
+    constexpr int FEW = FewLds<D, PT, kWaves, 32>::BYTES;
     __shared__ __attribute__((aligned(1024))) char lds[ManyLds<D, PT>::BYTES > FEW ? ManyLds<D, PT>::BYTES : FEW];
     __shared__ int marks[2];
     const Seq mine = seq_of(a, min((int)threadIdx.x & 63, a.n_seq - 1));
@@ -1601,7 +1620,14 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, float* ws, unsig
     } else if (p.many_wgs > 0) {
         hipLaunchKernelGGL((paged_many_kernel<D, PT, OT>), dim3(p.many_wgs), dim3(kWaves * 64), 0, s, a, ws, tickets);
     } else {
-        hipLaunchKernelGGL((paged_few_kernel<D, PT, OT>), dim3(p.few_pieces * a.Hkv), dim3(kFewWaves * 64), 0, s, a, ws, tickets, p.few_slots, p.few_cap);
+        const dim3 g(p.few_pieces * a.Hkv), b(p.few_waves * 64);
+        if constexpr (PT == VVA_TYPE_Q8_0) {
+            if (p.few_waves == 8) {
+                hipLaunchKernelGGL((paged_few_kernel<D, PT, OT, 8, 16>), g, b, 0, s, a, ws, tickets, p.few_slots, p.few_cap);
+                return hipGetLastError();
+            }
+        }
+        hipLaunchKernelGGL((paged_few_kernel<D, PT, OT, kFewWaves, 32>), g, b, 0, s, a, ws, tickets, p.few_slots, p.few_cap);
     }
     return hipGetLastError();
 }
@@ -1637,11 +1663,13 @@ PagedPlan paged_plan(const PagedArgs& a, int n_cu) {
         // no CU's share of the bytes is less (1 x 32768 keys 29.3 -> 22.3 us, 64 x 4096
         // 88.8 -> 83.8); all of them where the sequences are too many to be cut evenly
         // into that few (48 of 500 to 8000 keys: 94.2 -> 79.3)
-        const int slots = std::min(n_cu, kMaxWgs) * (a.d == 64 ? 2 : 1);
+        // Q8_0 pages and at most 16 rows: twice the waves in a workgroup
+        p.few_waves = a.type == VVA_TYPE_Q8_0 && rows <= 16 ? 8 : kFewWaves;
+        const int slots = std::min(n_cu, kMaxWgs) * (a.d == 64 && p.few_waves == kFewWaves ? 2 : 1);
         p.few_slots = std::max(1, (2 * a.n_seq * a.Hkv > slots ? 2 : 1) * slots / a.Hkv);
         const int64_t seq_tiles = (max_keys + kFewTile - 1) / kFewTile;
-        p.few_split = seq_tiles > kFewWaves;
-        p.few_pieces = (int)std::min<int64_t>(p.few_slots + (int64_t)a.n_seq, a.n_seq * ((seq_tiles + kFewWaves - 1) / kFewWaves));
+        p.few_split = seq_tiles > (p.many_wgs > 0 ? kFewWaves : p.few_waves);
+        p.few_pieces = (int)std::min<int64_t>(p.few_slots + (int64_t)a.n_seq, a.n_seq * ((seq_tiles + p.few_waves - 1) / p.few_waves));
     }
     return p;
 }

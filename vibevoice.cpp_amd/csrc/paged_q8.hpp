@@ -79,6 +79,17 @@ __device__ __forceinline__ Q8Frag q8_frag(uint32_t c0, uint32_t c1, const h2 (&s
 // whether either of two scales may take a code's value beyond F16, or is not finite
 __device__ __forceinline__ bool q8_big2(uint32_t x) { return (x & 0x7fffu) >= 0x6000u || ((x >> 16) & 0x7fffu) >= 0x6000u; }
 
+// add(e, v) for each of 4 codes whose value v is infinite or NaN, where it is seen
+template <typename F>
+__device__ __forceinline__ void q8_add_not_finite4(uint32_t codes, h2 scale, bool seen, F add) {
+    h2 x[2];
+    q8_codes(codes, x[0], x[1]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float v = (float)(x[e / 2] * scale)[e % 2];
+        if (seen && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) add(e, v);
+    }
+}
 // O += the infinities and NaNs of a tile's V that this lane's row sees (keys k0
 // .. of the tile up to lim).  Codes of N rows at v_lds, scales [block][N] at s_lds.
 template <int D, int N>
@@ -92,13 +103,7 @@ __device__ __forceinline__ void q8_add_not_finite(uint32_t v_lds, uint32_t s_lds
             for (int q4 = 0; q4 < 4; ++q4) {
                 const uint32_t c = *(const __attribute__((address_space(3))) uint32_t*)lds_at(
                     v_lds + j * D + (((2 * dt + (q4 >> 1)) ^ vq_swz<D>(j)) << 4) + 8 * (q4 & 1) + 4 * half);
-                h2 x[2];
-                q8_codes(c, x[0], x[1]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const _Float16 v = (x[e / 2] * s)[e % 2];
-                    if (seen && !__builtin_isfinite((float)v)) o[dt][4 * q4 + e] += (float)v;
-                }
+                q8_add_not_finite4(c, s, seen, [&](int e, float v) { o[dt][4 * q4 + e] += v; });
             }
         }
     }
@@ -114,14 +119,13 @@ __device__ __forceinline__ void q8_add_not_finite(uint32_t v_lds, uint32_t s_lds
 // ones do not).  Against tiles converted to F16 on their way into LDS, one under
 // way: 48 sequences of 500 to 8000 keys (215 MB) 61.4 -> 48.1 us.
 template <int D, int OT, int WAVES>
-__device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D>& r) {
+__device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D, 32>& r) {
     using F = Frag<VVA_TYPE_F16>;
     constexpr int KT = VVA_TYPE_F16;
     constexpr bool LO = OT == VVA_TYPE_F16;
     constexpr int NB = D / 32;                     // blocks of a row, 32-dim tiles of the sums
     constexpr int CB = kFewTile * D, SB = kFewTile * NB * 2;           // codes and scales of a tile
-    constexpr int STAGE = 2 * (CB + SB), QB = FewLds<D, VVA_TYPE_Q8_0, WAVES>::TB;
-    static_assert(QB + WAVES * 2 * STAGE == FewLds<D, VVA_TYPE_Q8_0, WAVES>::RING, "the ring fits");
+    constexpr int STAGE = 2 * (CB + SB), QB = 32 * 2 * D;
     constexpr int NC = CB / 1024, RC = 1024 / D;   // loads of a tile's codes, rows of one
     constexpr int NL = NC + 1;                     // with its scales
     constexpr int NV = 16 / RC;                    // loads of 16 keys
@@ -164,7 +168,7 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
     auto issue_v = [&](int t, uint32_t st) { issue(t, st + CB, st + 2 * CB + SB, a.v, a.v_nb_page, a.v_nb_head, voff); };
     int t = it.t0 + w;
     if (t < t1) fetch(t);
-    few_load_q<D, WAVES>(a, it, kvh, rows, qs);
+    few_load_q<D, WAVES, 32>(a, it, kvh, rows, qs);
     if (t < t1) {
         issue_k(t, ring);
         issue_v(t, ring);
@@ -213,19 +217,24 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
                 c[b] = lds_read((st + k_off) ^ (b << 5));
                 sc[b] = *(const __attribute__((address_space(3))) uint16_t*)lds_at(ks + b * kFewTile * 2 + key * 2);
             }
-            const bool lo = LO && !big(ks);
+            auto scores = [&](auto rest) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const h2 x = q8_scale(sc[b]);
-                const h2 x4[4] = {x, x, x, x};
+                for (int b = 0; b < NB; ++b) {
+                    const h2 x = q8_scale(sc[b]);
+                    const h2 x4[4] = {x, x, x, x};
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const Q8Frag f = q8_frag<LO>(c[b][2 * e], c[b][2 * e + 1], x4);
-                    s = F::mma(as_vec<h8>(f.hi), qf[2 * b + e], s);
-                    if constexpr (LO) {
-                        if (lo) s = F::mma(as_vec<h8>(f.lo), qf[2 * b + e], s);
+                    for (int e = 0; e < 2; ++e) {
+                        const Q8Frag f = q8_frag<decltype(rest)::value>(c[b][2 * e], c[b][2 * e + 1], x4);
+                        s = F::mma(as_vec<h8>(f.hi), qf[2 * b + e], s);
+                        if constexpr (decltype(rest)::value) s = F::mma(as_vec<h8>(f.lo), qf[2 * b + e], s);
                     }
                 }
+            };
+            if constexpr (LO) {
+                if (!big(ks)) scores(std::true_type{});
+                else scores(std::false_type{});
+            } else {
+                scores(std::false_type{});
             }
         }
         if (two) {
@@ -244,30 +253,241 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
         if (two) wait_vm<3 * NL>();                // V; what was asked for after it may still fly
         else if (one) wait_vm<2 * NL>();
         else wait_vm<0>();
-        bool wide = false;
-        if (LO || masked) wide = big(vs);
-        const bool fix = masked && wide;
+        // the products straight through; a tile with a value that is not finite, or
+        // near the end of F16, by a path of its own
+        auto values = [&](auto rest, auto fix) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const h8 pf = as_vec<h8>(u32x4{p[4 * kk], p[4 * kk + 1], p[4 * kk + 2], p[4 * kk + 3]});
+            for (int kk = 0; kk < 2; ++kk) {
+                const h8 pf = as_vec<h8>(u32x4{p[4 * kk], p[4 * kk + 1], p[4 * kk + 2], p[4 * kk + 3]});
 #pragma unroll
-            for (int dt = 0; dt < NB; ++dt) {
-                const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (__attribute__((address_space(3))) i32x2*)lds_at(((st + CB + v_off) ^ (dt << 5)) + kk * 16 * D));
-                const u32x4 sc = lds_read(vs + dt * kFewTile * 2 + kk * 32 + half * 16);
-                const h2 x4[4] = {as_h2(sc.x), as_h2(sc.y), as_h2(sc.z), as_h2(sc.w)};
-                Q8Frag f = q8_frag<LO>((uint32_t)c.x, (uint32_t)c.y, x4);
-                if (fix) f.hi = u32x4{finite2<KT>(f.hi.x), finite2<KT>(f.hi.y), finite2<KT>(f.hi.z), finite2<KT>(f.hi.w)};
-                r.o[dt] = F::mma(as_vec<h8>(f.hi), pf, r.o[dt]);
-                if constexpr (LO) {
-                    if (!wide) r.o[dt] = F::mma(as_vec<h8>(f.lo), pf, r.o[dt]);
+                for (int dt = 0; dt < NB; ++dt) {
+                    const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                        (__attribute__((address_space(3))) i32x2*)lds_at(((st + CB + v_off) ^ (dt << 5)) + kk * 16 * D));
+                    const u32x4 sc = lds_read(vs + dt * kFewTile * 2 + kk * 32 + half * 16);
+                    const h2 x4[4] = {as_h2(sc.x), as_h2(sc.y), as_h2(sc.z), as_h2(sc.w)};
+                    Q8Frag f = q8_frag<decltype(rest)::value>((uint32_t)c.x, (uint32_t)c.y, x4);
+                    if constexpr (decltype(fix)::value) {
+                        if (masked) f.hi = u32x4{finite2<KT>(f.hi.x), finite2<KT>(f.hi.y), finite2<KT>(f.hi.z), finite2<KT>(f.hi.w)};
+                    }
+                    r.o[dt] = F::mma(as_vec<h8>(f.hi), pf, r.o[dt]);
+                    if constexpr (decltype(rest)::value) r.o[dt] = F::mma(as_vec<h8>(f.lo), pf, r.o[dt]);
                 }
             }
+        };
+        if ((LO || masked) && big(vs)) {
+            values(std::false_type{}, std::true_type{});
+            if (masked) q8_add_not_finite<D, kFewTile>(st + CB, vs, k0, lim, half, r.o);
+        } else {
+            values(std::integral_constant<bool, LO>{}, std::false_type{});
         }
-        if (fix) q8_add_not_finite<D, kFewTile>(st + CB, vs, k0, lim, half, r.o);
         if (two) {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // V is read
             issue_v(t + 2 * WAVES, st);
+        }
+    }
+}
+
+// The same for at most 16 rows (single tokens of up to 16 heads a group), with
+// v_mfma_f32_16x16x32_f16: half the scores and sums a lane holds, so twice the
+// waves fit and the conversions, which are the most of a tile's arithmetic, have
+// other waves' waits to run in.  One tile of 128 dims a wave is under way then
+// (two of 64), 4 waves per SIMD.  Against 32 rows and half the waves, us: 30k keys
+// 17.4 -> 14.9; 12 sequences of up to 8000 keys 20.5 -> 16.4, 48 48.1 -> 46.3; 24 of
+// the 1.5B model 20.0 -> 16.0.  In workgroups of one per CU, beside many rows, it was
+// slower (48 sequences 51 -> 57): those keep 32 rows.  Layouts (lane l, l16 = l % 16, g = l / 16):
+//   A (16 x 32): row l16, k = 8 g .. 8 g + 7     B (32 x 16): column l16, the same k
+//   C (16 x 16): column l16, register r holds row 4 g + r
+// Row x of score tile mt is key 8 (x / 4) + 4 mt + x % 4, so a lane's 8 scores are
+// keys 8 g .. 8 g + 7, the ones that the transposing read gives of a dim of V.
+template <int D> __device__ __forceinline__ int kq16_swz(int row) {
+    return D == 128 ? (row >> 2 & 6) | (row >> 1 & 1) : row >> 3 & 3;
+}
+template <int D, int OT, int WAVES, int STAGES>
+__device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D, 16>& r) {
+    constexpr int KT = VVA_TYPE_F16;
+    constexpr bool LO = OT == VVA_TYPE_F16;
+    constexpr int NB = D / 32;                     // blocks of a row
+    constexpr int CB = kFewTile * D, SB = kFewTile * NB * 2;           // codes and scales of a tile
+    constexpr int STAGE = 2 * (CB + SB), QB = 16 * 2 * D;
+    constexpr int NC = CB / 1024, RC = 1024 / D;   // loads of a tile's codes, rows of one
+    constexpr int NL = NC + 1;                     // with its scales
+    constexpr int NV = 16 / RC;                    // loads of 16 keys
+    const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int L = it.q.L, rows = min(it.q.n, a.max_new) * a.G, past = L - it.q.n, t1 = it.t1;
+    const ConstInts table = (ConstInts)(uintptr_t)(a.table + (int64_t)it.q.s * a.table_stride);
+    const int last_page = (L - 1) >> a.page_shift, page = 1 << a.page_shift;
+    const uint32_t qs = (uint32_t)(uintptr_t)(lds_char*)lds, ring = qs + QB + w * STAGES * STAGE;
+
+    int koff[NV], voff[NV];                        // codes: from the first slot of 16
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int row = i * RC + lane / (D / 16), c = lane % (D / 16);
+        koff[i] = row * D + ((c ^ kq16_swz<D>(row)) << 4);
+        voff[i] = row * D + ((c ^ kq_swz<D>(row)) << 4);
+    }
+    const int soff = page * D + (((lane >> 4) << a.page_shift) + 2 * (lane & 7)) * 2;   // scales: two keys of a block
+    int ids[2];                                    // pages of the two 16-key halves of the next tile to load
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ids[i] = table[min((t * kFewTile + 16 * i) >> a.page_shift, last_page)];
+    };
+    // turn: what the swizzle of the upper 16 rows adds to that of the lower ones
+    auto issue = [&](int t, uint32_t codes, uint32_t scales, const char* pool, int64_t nb_page, int64_t nb_head, const int (&off)[NV], int turn) {
+        uint64_t run[2];
+        int slot[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool ok = (uint32_t)ids[i] < (uint32_t)a.n_pages;
+            r.bad = r.bad || !ok;
+            run[i] = uniform64((uint64_t)(uintptr_t)pool + (int64_t)(ok ? ids[i] : 0) * nb_page + kvh * nb_head);
+            slot[i] = (t * kFewTile + 16 * i) & (page - 1);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            dma16<true>(run[c / NV] + (uint64_t)slot[c / NV] * D, off[c % NV] ^ (c / NV ? turn : 0), codes + c * 1024);
+        const uint64_t s0 = run[0] + 2 * slot[0], s1 = run[1] + 2 * slot[1];
+        if (D == 128 || lane < 32) dma4<true>((lane & 8 ? s1 : s0) + soff, scales);
+    };
+    auto issue_k = [&](int t, uint32_t st) { issue(t, st, st + 2 * CB, a.k, a.k_nb_page, a.k_nb_head, koff, kq16_swz<D>(16) << 4); };
+    auto issue_v = [&](int t, uint32_t st) { issue(t, st + CB, st + 2 * CB + SB, a.v, a.v_nb_page, a.v_nb_head, voff, 0); };
+    int t = it.t0 + w;
+    if (t < t1) fetch(t);
+    few_load_q<D, WAVES, 16>(a, it, kvh, rows, qs);
+    if (t < t1) {
+        issue_k(t, ring);
+        issue_v(t, ring);
+        if (STAGES == 2 && t + WAVES < t1) {
+            fetch(t + WAVES);
+            issue_k(t + WAVES, ring + STAGE);
+            issue_v(t + WAVES, ring + STAGE);
+            wait_vm<4 * NL>();                     // Q
+        } else {
+            wait_vm<2 * NL>();
+        }
+    } else {
+        wait_vm<0>();
+    }
+    asm volatile("s_barrier" : : : "memory");
+    const int key = 8 * (l16 >> 2) + (l16 & 3);
+    const int k_off = key * D + (((g >> 1) ^ kq16_swz<D>(key)) << 4) + 8 * (g & 1);
+    const int v_row = 8 * g + (l16 >> 1);
+    const int v_off = v_row * D + (kq_swz<D>(v_row) << 4) + 8 * (lane & 1);
+    h8 qf[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) qf[b] = q_frag<KT, OT>(lds_read(qs + l16 * 2 * D + (((4 * b + g) ^ k_swz<D>(l16)) << 4)));
+    const int lim = l16 < rows ? min(L - 1, past + div_g(a, l16)) : -1;   // the last key the lane's row sees
+    const float sl2 = a.scale * kLog2e;
+    auto big = [&](uint32_t scales) {              // of a tile's scales (whole wave)
+        return (bool)__any(q8_big2(*(const __attribute__((address_space(3))) uint32_t*)lds_at(scales + (lane & (SB / 4 - 1)) * 4)));
+    };
+    for (uint32_t st = ring; t < t1; t += WAVES, st = STAGES == 1 || st != ring ? ring : ring + STAGE) {
+        const bool one = t + WAVES < t1, next = t + STAGES * WAVES < t1;
+        const uint32_t ks = st + 2 * CB, vs = ks + SB;
+        if (next) fetch(t + STAGES * WAVES);
+        if (STAGES == 2 && one) wait_vm<3 * NL>(); // K; V and the next tile may still fly
+        else wait_vm<NL>();
+        f32x4 s[2] = {};
+        {
+            u32x2 c[NB][2];
+            uint16_t sc[NB][2];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt) {
+                    c[b][mt] = *(const __attribute__((address_space(3))) u32x2*)lds_at(((st + k_off) ^ (b << 5)) + mt * 4 * D);
+                    sc[b][mt] = *(const __attribute__((address_space(3))) uint16_t*)lds_at(ks + b * kFewTile * 2 + (key + 4 * mt) * 2);
+                }
+            auto scores = [&](auto rest) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt) {
+                        const h2 x = q8_scale(sc[b][mt]);
+                        const h2 x4[4] = {x, x, x, x};
+                        const Q8Frag f = q8_frag<decltype(rest)::value>(c[b][mt].x, c[b][mt].y, x4);
+                        s[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_vec<h8>(f.hi), qf[b], s[mt], 0, 0, 0);
+                        if constexpr (decltype(rest)::value) s[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_vec<h8>(f.lo), qf[b], s[mt], 0, 0, 0);
+                    }
+            };
+            if constexpr (LO) {
+                if (!big(ks)) scores(std::true_type{});
+                else scores(std::false_type{});
+            } else {
+                scores(std::false_type{});
+            }
+        }
+        if (next) {
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // K is read
+            issue_k(t + STAGES * WAVES, st);
+        }
+        const int k0 = t * kFewTile;
+        const bool masked = k0 + kFewTile - 1 > min(L - 1, past);      // some row must not see some key
+        if (masked) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) s[x / 4][x % 4] = x > lim - k0 - 8 * g ? -INFINITY : s[x / 4][x % 4];
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = max_swap32(max_swap16(mx)) * sl2;
+        if (__any(mx > r.m + kLazy)) {
+            if (mx > r.m + kLazy) {
+                const float alpha = __builtin_amdgcn_exp2f(r.m - mx);  // 0 while m = -inf
+                r.lsum *= alpha;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) r.o[i] *= alpha;
+                r.m = mx;
+            }
+        }
+        const float nb = kLift<KT> - (r.m == -INFINITY ? 0.0f : r.m);
+        u32x4 p;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            p[x] = pack2<KT>(__builtin_amdgcn_exp2f(fmaf(s[x / 2][2 * (x % 2)], sl2, nb)), __builtin_amdgcn_exp2f(fmaf(s[x / 2][2 * (x % 2) + 1], sl2, nb)));
+            r.lsum = sum2<KT>(p[x], r.lsum);
+        }
+        const h8 pf = as_vec<h8>(p);
+        if (STAGES == 2 && next) wait_vm<3 * NL>();                    // V; what was asked for after it may still fly
+        else if (STAGES == 2 && one) wait_vm<2 * NL>();
+        else if (STAGES == 1 && next) wait_vm<NL>();
+        else wait_vm<0>();
+        // the products straight through; a tile with a value that is not finite, or
+        // near the end of F16, by a path of its own
+        auto values = [&](auto rest, auto fix) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const u32x4 sc = lds_read(vs + b * kFewTile * 2 + g * 16);
+                const h2 x4[4] = {as_h2(sc.x), as_h2(sc.y), as_h2(sc.z), as_h2(sc.w)};
+#pragma unroll
+                for (int i = 2 * b; i < 2 * b + 2; ++i) {
+                    const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)lds_at((st + CB + v_off) ^ (i << 4)));
+                    Q8Frag f = q8_frag<decltype(rest)::value>((uint32_t)c.x, (uint32_t)c.y, x4);
+                    if constexpr (decltype(fix)::value) {
+                        if (masked) f.hi = u32x4{finite2<KT>(f.hi.x), finite2<KT>(f.hi.y), finite2<KT>(f.hi.z), finite2<KT>(f.hi.w)};
+                    }
+                    r.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_vec<h8>(f.hi), pf, r.o[i], 0, 0, 0);
+                    if constexpr (decltype(rest)::value) r.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_vec<h8>(f.lo), pf, r.o[i], 0, 0, 0);
+                }
+            }
+        };
+        if ((LO || masked) && big(vs)) {
+            values(std::false_type{}, std::true_type{});
+            if (masked) {                          // a lane's dims of tile i: 16 i + 4 g ..
+                for (int j = 0; j < kFewTile; ++j) {
+                    const bool seen = k0 + j <= lim;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const h2 sc = q8_scale(*(const __attribute__((address_space(3))) uint16_t*)lds_at(vs + ((i / 2) * kFewTile + j) * 2));
+                        const uint32_t c = *(const __attribute__((address_space(3))) uint32_t*)lds_at(st + CB + j * D + ((i ^ kq_swz<D>(j)) << 4) + 4 * g);
+                        q8_add_not_finite4(c, sc, seen, [&](int e, float v) { r.o[i][e] += v; });
+                    }
+                }
+            }
+        } else {
+            values(std::integral_constant<bool, LO>{}, std::false_type{});
+        }
+        if (next) {
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // V is read
+            issue_v(t + STAGES * WAVES, st);
         }
     }
 }

@@ -249,6 +249,7 @@ hipError_t launch_paged_read(const PagedReadArgs& a, hipStream_t s);
 struct PagedPlan {
     int many_wgs;                              // workgroups of paged_many_kernel (0: no launch)
     int few_pieces, few_slots, few_cap;        // few rows: pieces per kv head (0: none), how many run at once, rows of a partial
+    int few_waves;                             // of a workgroup, where they are alone
     bool few_split;                            // whether pieces may leave partials
 };
 PagedPlan paged_plan(const PagedArgs& a, int n_cu);
