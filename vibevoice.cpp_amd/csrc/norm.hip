@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(256) norm_kernel(NormArgs a) {
         const int q = (k % kQK8) / 2;
         if (q == 0) blk[0] = q8.scale;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) blk[1 + q + e] = (uint16_t)(q8.code(z[2 * e]) | (q8.code(z[2 * e + 1]) << 8));
+        for (int e = 0; e < 4; ++e) blk[1 + q + e] = (uint16_t)((q8.code(z[2 * e]) & 0xff) | (q8.code(z[2 * e + 1]) << 8));
     }
 }
 

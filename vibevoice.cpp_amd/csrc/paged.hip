@@ -53,13 +53,10 @@ __device__ __forceinline__ void store8(char* p, int type, const float (&y)[8]) {
 // d bytes a slot, the scales of a block `page` F16 behind all of them
 __device__ __forceinline__ void store8_q8(char* tile, int d, int page_shift, int slot, int i, const float (&y)[8]) {
     const Q8Block b = q8_block(y);
-    uint2 c = {0u, 0u};
+    int c[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        c.x |= (uint32_t)b.code(y[e]) << (8 * e);
-        c.y |= (uint32_t)b.code(y[e + 4]) << (8 * e);
-    }
-    *(uint2*)(tile + slot * d + i) = c;
+    for (int e = 0; e < 8; ++e) c[e] = b.code(y[e]);
+    *(uint2*)(tile + slot * d + i) = make_uint2(q8_pack(c[0], c[1], c[2], c[3]), q8_pack(c[4], c[5], c[6], c[7]));
     if (i % kQK8 == 0) *(uint16_t*)(tile + (d << page_shift) + (((i / kQK8) << page_shift) + slot) * 2) = b.scale;
 }
 
@@ -68,7 +65,8 @@ __device__ __forceinline__ void store8_q8(char* tile, int d, int page_shift, int
 // HBM-bound (4k tokens 78 -> 33 us against one pair per thread); a short call
 // is a chain of two round trips: the batch, with the token's own rows under
 // way, then the page id and the row of the rope table.
-template <bool Q8>
+// IO: the type of q, k and v where it is one, else -1
+template <bool Q8, int IO>
 __global__ void __launch_bounds__(512) paged_append_kernel(PagedAppendArgs a) {
     prefetch_kernargs<sizeof(PagedAppendArgs)>();
     const PagedArgs& p = a.p;
@@ -99,9 +97,9 @@ __global__ void __launch_bounds__(512) paged_append_kernel(PagedAppendArgs a) {
     int w = threadIdx.x;
     Item it = item(min(w, items - 1));
     auto load = [&](const Item& t, Raw8& lo, Raw8& hi) {
-        const int es = t.type == VVA_TYPE_F32 ? 4 : 2;
-        lo = load_raw8(t.src + t.e * es, t.type);
-        hi = load_raw8(t.src + (t.e + P) * es, t.type);
+        const int type = IO >= 0 ? IO : t.type, es = type == VVA_TYPE_F32 ? 4 : 2;
+        lo = load_raw8(t.src + t.e * es, type);
+        hi = load_raw8(t.src + (t.e + P) * es, type);
     };
     Raw8 lo, hi;
     load(it, lo, hi);
@@ -126,8 +124,8 @@ __global__ void __launch_bounds__(512) paged_append_kernel(PagedAppendArgs a) {
     const int slot = i & ((1 << p.page_shift) - 1);
     while (w < items) {
         float x0[8], x1[8], y0[8], y1[8];
-        raw8_to_f32(lo, it.type, x0);
-        raw8_to_f32(hi, it.type, x1);
+        raw8_to_f32(lo, IO >= 0 ? IO : it.type, x0);
+        raw8_to_f32(hi, IO >= 0 ? IO : it.type, x1);
         const Item t = it;
         if (t.h < p.Hq + p.Hkv) {
 #pragma unroll
@@ -246,13 +244,21 @@ __global__ void __launch_bounds__(kReadWaves * 64) paged_read_kernel(PagedReadAr
     }
 }
 
+template <bool Q8>
+void launch_append(const PagedAppendArgs& a, dim3 g, dim3 b, hipStream_t s) {
+    if (a.q_type != a.k_type || a.k_type != a.v_type) hipLaunchKernelGGL((paged_append_kernel<Q8, -1>), g, b, 0, s, a);
+    else if (a.q_type == VVA_TYPE_F32) hipLaunchKernelGGL((paged_append_kernel<Q8, VVA_TYPE_F32>), g, b, 0, s, a);
+    else if (a.q_type == VVA_TYPE_F16) hipLaunchKernelGGL((paged_append_kernel<Q8, VVA_TYPE_F16>), g, b, 0, s, a);
+    else hipLaunchKernelGGL((paged_append_kernel<Q8, VVA_TYPE_BF16>), g, b, 0, s, a);
+}
+
 }  // namespace
 
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
     const int items = (a.p.Hq + 2 * a.p.Hkv) * (a.p.d / 16);
     const dim3 g(a.p.n_tok), b(std::min(512, (items + 63) / 64 * 64));
-    if (a.p.type == VVA_TYPE_Q8_0) hipLaunchKernelGGL(paged_append_kernel<true>, g, b, 0, s, a);
-    else hipLaunchKernelGGL(paged_append_kernel<false>, g, b, 0, s, a);
+    if (a.p.type == VVA_TYPE_Q8_0) launch_append<true>(a, g, b, s);
+    else launch_append<false>(a, g, b, s);
     return hipGetLastError();
 }
 

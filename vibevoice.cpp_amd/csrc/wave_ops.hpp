@@ -124,8 +124,18 @@ struct Q8Block {
     float inv;
     bool finite;
     uint16_t scale;                                    // F16 bits
-    __device__ __forceinline__ uint8_t code(float z) const { return (uint8_t)(int8_t)roundf(finite ? z * inv : 1.0f); }
+    // round(z / scale), halves away from zero: cut after adding the largest float
+    // below a half (a half itself would take 0.5 - 2^-25 up to 1)
+    __device__ __forceinline__ int code(float z) const {
+        const float x = finite ? z * inv : 1.0f;
+        return (int)(x + copysignf(0x1.fffffep-2f, x));
+    }
 };
+// The low bytes of 4 codes in a word
+__device__ __forceinline__ uint32_t q8_pack(int a, int b, int c, int d) {
+    const uint32_t ab = __builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x0c0c0400u), cd = __builtin_amdgcn_perm((uint32_t)d, (uint32_t)c, 0x04000c0cu);
+    return ab | cd;
+}
 __device__ __forceinline__ Q8Block q8_block(const float (&z)[8]) {
     uint32_t ab = 0;
 #pragma unroll
