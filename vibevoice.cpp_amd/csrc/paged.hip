@@ -116,8 +116,9 @@ __global__ void __launch_bounds__(512) paged_append_kernel(PagedAppendArgs a) {
         }
     }
     if (s < 0) return;
-    const int page = i >= 0 ? p.table[s * p.table_stride + (i >> p.page_shift)] : -1;
-    const int pos = a.pos ? a.pos[n] : i;
+    // (uniform: what goes by them are scalar branches and bases)
+    const int page = __builtin_amdgcn_readfirstlane(i >= 0 ? p.table[s * p.table_stride + (i >> p.page_shift)] : -1);
+    const int pos = __builtin_amdgcn_readfirstlane(a.pos ? a.pos[n] : i);
     const bool in_table = pos >= 0 && pos < a.n_pos;
     const float* cs = (const float*)(a.rope + (int64_t)(in_table ? pos : 0) * a.rope_nb);
     const bool live = page >= 0 && page < p.n_pages;
@@ -134,10 +135,13 @@ __global__ void __launch_bounds__(512) paged_append_kernel(PagedAppendArgs a) {
                 const float c[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    y0[4 * v + e] = in_table ? fmaf(x0[4 * v + e], c[e], -(x1[4 * v + e] * sn[e])) : __builtin_nanf("");
-                    y1[4 * v + e] = in_table ? fmaf(x0[4 * v + e], sn[e], x1[4 * v + e] * c[e]) : __builtin_nanf("");
+                    y0[4 * v + e] = fmaf(x0[4 * v + e], c[e], -(x1[4 * v + e] * sn[e]));
+                    y1[4 * v + e] = fmaf(x0[4 * v + e], sn[e], x1[4 * v + e] * c[e]);
                 }
             }
+            if (!in_table)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y0[e] = y1[e] = __builtin_nanf("");
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
