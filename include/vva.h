@@ -403,8 +403,10 @@ VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, 
  * Hq / Hkv are at most 32 (not in calls of n_seq * max_new tokens whose max_new
  * times that is more).
  * Over Q8_0 pages the products and probabilities are those of F16 pages that
- * hold scale times code rounded to F16 (infinite beyond 65504), and BF16 q are
- * taken as F16 too (their 8 bits are kept from 2^-17 to 65504).
+ * hold scale times code rounded to F16 (2^-11; infinite beyond 65504), and BF16 q
+ * are taken as F16 too (their 8 bits are kept from 2^-17 to 65504).  With F16 q,
+ * what that rounding of K and V leaves goes into the products as well where a
+ * sequence's new tokens times Hq / Hkv are at most 32 (as above).
  * Every row of q and out and every page row starts on 16 bytes.
  * Partial sums go through the context's workspace, as those of the other
  * calls: under stream capture a call larger than any before it is refused

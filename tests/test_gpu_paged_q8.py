@@ -278,6 +278,21 @@ def test_attention_head_layouts(ctx, torch_gpu, Hq, Hkv, d, lens):
     run_attn(ctx, Q8Pages(torch_gpu, lens, Hq, Hkv, d, vva.F16, 16, seed=Hq, extra_rows=1))
 
 
+@pytest.mark.parametrize("t", [vva.F16, vva.BF16])
+@pytest.mark.parametrize("n,Hq,Hkv,d", [(1, 16, 1, 128), (1, 17, 1, 128), (2, 8, 1, 64), (2, 16, 2, 64), (1, 1, 1, 128), (2, 9, 1, 64),
+                                        (4, 8, 1, 128), (16, 2, 2, 64), (32, 3, 3, 128), (17, 1, 1, 64)])
+def test_attention_of_one_to_thirty_two_rows(ctx, torch_gpu, n, Hq, Hkv, d, t):
+    """Rows of a sequence and kv head on both sides of 16, tiles in one piece and in many."""
+    print(n, Hq, Hkv, d, t, flush=True)
+    run_attn(ctx, Q8Pages(torch_gpu, [(n, 40), (n, n), (n, 1500), (n, 257), (n, 7001)], Hq, Hkv, d, t, 32, seed=n + Hq, extra_rows=0))
+
+
+@pytest.mark.parametrize("heads,t", [(H7, vva.BF16), (H05, vva.F16)])
+def test_single_tokens_of_many_sequences(ctx, torch_gpu, heads, t):
+    """More sequences than lanes of a wave, in one kernel for single tokens."""
+    run_attn(ctx, Q8Pages(torch_gpu, [(1, 1 + (97 * i) % 1301) for i in range(130)], *heads, t, 16, seed=7))
+
+
 @pytest.mark.parametrize("lens,heads,t,page", [
     ([(1, 20011)], H7, vva.F16, 16),
     ([(1, 9000), (1, 40), (2, 6001)], H7, vva.BF16, 1024),
