@@ -17,7 +17,9 @@
 //
 // Reached, of a copy's 4.9 TB/s and a large product's 1175 TFLOP/s: single
 // tokens 5.5 TB/s (48 sequences of 500 to 8000 keys, 405 MB, 73 us); 2048 tokens
-// behind 28672 keys 991 TFLOP/s (880 us), 512 behind 15872 858 (138 us).
+// behind 28672 keys 991 TFLOP/s (880 us), 512 behind 15872 858 (138 us).  Over
+// Q8_0 pages: the 48 sequences (216 MB) 46.4 us, one of 30k keys 14.5 (16-bit pages
+// 17.4); the chunks 885 and 142 us where 16-bit pages take 852 and 136.
 //
 // Both compute, per 32 rows and a tile of keys, with
 // v_mfma_f32_32x32x16_{f16,bf16} (layouts in mfma_ops.hpp):
@@ -51,6 +53,12 @@
 // -inf by a select, and where such a tile holds a V that is not finite (a
 // stale slot behind the sequence, a later token's overflow) its products leave
 // those values out and add them to the rows that see them (0 * inf is not 0).
+//
+// Q8_0 pages (paged_q8.hpp) take the F16 products.  Few rows keep the codes in LDS
+// and convert them as operands; many rows convert each tile once, into the LDS tile
+// that F16 pages are loaded into, so K and V are rounded to F16 there (a relative
+// 2^-11 at most; with the probabilities' and the result's rounding an F16 result is
+// off by 4.2e-4 of its size, of which the last alone is 2.1e-4).
 #include "vva_internal.hpp"
 
 #include <algorithm>

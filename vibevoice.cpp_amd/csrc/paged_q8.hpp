@@ -9,28 +9,22 @@
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
-// XORed to the chunk index of a row of codes.  K: 8 lanes read a chunk each of 8
-// rows, which f spreads over all banks; V: the transposing read takes 32 bytes of
-// each of 8 rows (f even: a pair of chunks stays one).
+// XORed to the chunk index of a row of codes, so that what a phase of a read takes
+// lies on different banks: K in chunks of 8 rows; V in 32 bytes of each of 8 rows (f
+// even: a pair of chunks stays one); with 16-row products, K in half chunks of rows
+// 8 i + 0 .. 3, and V as K is in the first case
 template <int D> __device__ __forceinline__ int kq_swz(int row) { return D == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
 template <int D> __device__ __forceinline__ int vq_swz(int row) { return D == 128 ? row & 6 : (row >> 1) & 2; }
+template <int D> __device__ __forceinline__ int kq16_swz(int row) { return D == 128 ? (row >> 2 & 6) | (row >> 1 & 1) : row >> 3 & 3; }
 
-// 64 lanes' 4 bytes, each from an address of its own, to LDS lds .. lds + 255;
-// as dma16, non-temporal or not.
-template <bool NT>
+// 64 lanes' 4 bytes, each from an address of its own, to LDS lds .. lds + 255; as
+// dma16, non-temporal
 __device__ __forceinline__ void dma4(uint64_t addr, uint32_t lds) {
-    if constexpr (NT)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off nt"
-                     :
-                     : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(addr)
-                     : "memory", "m0");
-    else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off"
-                     :
-                     : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(addr)
-                     : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off nt"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(addr)
+                 : "memory", "m0");
 }
-
 // a T at base + off (a pointer made of integers alone would be a flat one)
 template <typename T>
 __device__ __forceinline__ T global_load(uint64_t base, uint32_t off) {
@@ -109,6 +103,90 @@ __device__ __forceinline__ void q8_add_not_finite(uint32_t v_lds, uint32_t s_lds
     }
 }
 
+// A wave's tiles of 32 keys of a sequence and kv head, from the pages into LDS
+// stages: the codes of K, of V, then the scales of K, of V.  ROWS16: for products of
+// 16 rows.
+template <int D, bool ROWS16>
+struct Q8Tiles {
+    static constexpr int NB = D / 32;              // blocks of a row
+    static constexpr int CB = kFewTile * D, SB = kFewTile * NB * 2;    // codes and scales of a tile
+    static constexpr int STAGE = 2 * (CB + SB);
+    static constexpr int NC = CB / 1024, RC = 1024 / D;                // loads of a tile's codes, rows of one
+    static constexpr int NL = NC + 1;              // with its scales
+    static constexpr int NV = 16 / RC;             // loads of 16 keys
+
+    const PagedArgs& a;
+    const ConstInts table;
+    const int kvh, last_page, lane;
+    int koff[NV], voff[NV];                        // codes: from the first slot of 16
+    int soff;                                      // scales: two keys of a block
+    int ids[2];                                    // pages of the two 16-key halves of the next tile to load
+    bool bad = false;
+
+    static __device__ __forceinline__ int k_swz(int row) { return ROWS16 ? kq16_swz<D>(row) : kq_swz<D>(row); }
+    static __device__ __forceinline__ int v_swz(int row) { return ROWS16 ? kq_swz<D>(row) : vq_swz<D>(row); }
+
+    __device__ __forceinline__ Q8Tiles(const PagedArgs& args, const FewItem& it, int head, int l)
+        : a(args), table((ConstInts)(uintptr_t)(args.table + (int64_t)it.q.s * args.table_stride)), kvh(head),
+          last_page((it.q.L - 1) >> args.page_shift), lane(l) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int row = i * RC + lane / (D / 16), c = lane % (D / 16);
+            koff[i] = row * D + ((c ^ k_swz(row)) << 4);
+            voff[i] = row * D + ((c ^ v_swz(row)) << 4);
+        }
+        soff = (D << a.page_shift) + (((lane >> 4) << a.page_shift) + 2 * (lane & 7)) * 2;
+    }
+    __device__ __forceinline__ void fetch(int t) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ids[i] = table[min((t * kFewTile + 16 * i) >> a.page_shift, last_page)];
+    }
+    // turn: what the swizzle of the upper 16 rows adds to that of the lower ones
+    __device__ __forceinline__ void issue(int t, uint32_t codes, uint32_t scales, const char* pool, int64_t nb_page, int64_t nb_head, const int (&off)[NV], int turn) {
+        uint64_t run[2];
+        int slot[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool ok = (uint32_t)ids[i] < (uint32_t)a.n_pages;
+            bad = bad || !ok;
+            run[i] = uniform64((uint64_t)(uintptr_t)pool + (int64_t)(ok ? ids[i] : 0) * nb_page + kvh * nb_head);
+            slot[i] = (t * kFewTile + 16 * i) & ((1 << a.page_shift) - 1);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            dma16<true>(run[c / NV] + (uint64_t)slot[c / NV] * D, off[c % NV] ^ (c / NV ? turn : 0), codes + c * 1024);
+        const uint64_t s0 = run[0] + 2 * slot[0], s1 = run[1] + 2 * slot[1];
+        if (D == 128 || lane < 32) dma4((lane & 8 ? s1 : s0) + soff, scales);
+    }
+    __device__ __forceinline__ void issue_k(int t, uint32_t st) { issue(t, st, st + 2 * CB, a.k, a.k_nb_page, a.k_nb_head, koff, k_swz(16) << 4); }
+    __device__ __forceinline__ void issue_v(int t, uint32_t st) { issue(t, st + CB, st + 2 * CB + SB, a.v, a.v_nb_page, a.v_nb_head, voff, v_swz(16) << 4); }
+    // The rows of Q, and the first tiles (t, t + WAVES) into the ring's stages, until Q has landed
+    template <int WAVES, int ROWS, int STAGES>
+    __device__ __forceinline__ void begin(const FewItem& it, int rows, int t, uint32_t qs, uint32_t ring) {
+        if (t < it.t1) fetch(t);
+        few_load_q<D, WAVES, ROWS>(a, it, kvh, rows, qs);
+        if (t < it.t1) {
+            issue_k(t, ring);
+            issue_v(t, ring);
+            if (STAGES == 2 && t + WAVES < it.t1) {
+                fetch(t + WAVES);
+                issue_k(t + WAVES, ring + STAGE);
+                issue_v(t + WAVES, ring + STAGE);
+                wait_vm<4 * NL>();
+            } else {
+                wait_vm<2 * NL>();
+            }
+        } else {
+            wait_vm<0>();
+        }
+        asm volatile("s_barrier" : : : "memory");
+    }
+    // whether a tile's scales may take a value beyond F16 or are not finite (whole wave)
+    __device__ __forceinline__ bool big(uint32_t scales) const {
+        return (bool)__any(q8_big2(*(const __attribute__((address_space(3))) uint32_t*)lds_at(scales + (lane & (SB / 4 - 1)) * 4)));
+    }
+};
+
 // The tiles t0 + w, + WAVES, ... below t1 of a piece, as few_stream: of 32 keys,
 // two under way while one is computed (a stage is 8.5 KB: one alone would leave
 // less than half of what the 16-bit tiles have in flight).
@@ -121,69 +199,17 @@ __device__ __forceinline__ void q8_add_not_finite(uint32_t v_lds, uint32_t s_lds
 template <int D, int OT, int WAVES>
 __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D, 32>& r) {
     using F = Frag<VVA_TYPE_F16>;
+    using T = Q8Tiles<D, false>;
     constexpr int KT = VVA_TYPE_F16;
     constexpr bool LO = OT == VVA_TYPE_F16;
-    constexpr int NB = D / 32;                     // blocks of a row, 32-dim tiles of the sums
-    constexpr int CB = kFewTile * D, SB = kFewTile * NB * 2;           // codes and scales of a tile
-    constexpr int STAGE = 2 * (CB + SB), QB = 32 * 2 * D;
-    constexpr int NC = CB / 1024, RC = 1024 / D;   // loads of a tile's codes, rows of one
-    constexpr int NL = NC + 1;                     // with its scales
-    constexpr int NV = 16 / RC;                    // loads of 16 keys
+    constexpr int NB = T::NB, CB = T::CB, SB = T::SB, STAGE = T::STAGE, NL = T::NL;
     const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int L = it.q.L, rows = min(it.q.n, a.max_new) * a.G, past = L - it.q.n, t1 = it.t1;
-    const ConstInts table = (ConstInts)(uintptr_t)(a.table + (int64_t)it.q.s * a.table_stride);
-    const int last_page = (L - 1) >> a.page_shift, page = 1 << a.page_shift;
-    const uint32_t qs = (uint32_t)(uintptr_t)(lds_char*)lds, ring = qs + QB + w * 2 * STAGE;
-
-    int koff[NV], voff[NV];                        // codes: from the first slot of 16
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int row = i * RC + lane / (D / 16), c = lane % (D / 16);
-        koff[i] = row * D + ((c ^ kq_swz<D>(row)) << 4);
-        voff[i] = row * D + ((c ^ vq_swz<D>(row)) << 4);
-    }
-    const int soff = page * D + (((lane >> 4) << a.page_shift) + 2 * (lane & 7)) * 2;   // scales: two keys of a block
-    int ids[2];                                    // pages of the two 16-key halves of the next tile to load
-    auto fetch = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) ids[i] = table[min((t * kFewTile + 16 * i) >> a.page_shift, last_page)];
-    };
-    auto issue = [&](int t, uint32_t codes, uint32_t scales, const char* pool, int64_t nb_page, int64_t nb_head, const int (&off)[NV]) {
-        uint64_t run[2];
-        int slot[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const bool ok = (uint32_t)ids[i] < (uint32_t)a.n_pages;
-            r.bad = r.bad || !ok;
-            run[i] = uniform64((uint64_t)(uintptr_t)pool + (int64_t)(ok ? ids[i] : 0) * nb_page + kvh * nb_head);
-            slot[i] = (t * kFewTile + 16 * i) & (page - 1);
-        }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) dma16<true>(run[c / NV] + (uint64_t)slot[c / NV] * D, off[c % NV], codes + c * 1024);
-        const uint64_t s0 = run[0] + 2 * slot[0], s1 = run[1] + 2 * slot[1];
-        if (D == 128 || lane < 32) dma4<true>((lane & 8 ? s1 : s0) + soff, scales);
-    };
-    auto issue_k = [&](int t, uint32_t st) { issue(t, st, st + 2 * CB, a.k, a.k_nb_page, a.k_nb_head, koff); };
-    auto issue_v = [&](int t, uint32_t st) { issue(t, st + CB, st + 2 * CB + SB, a.v, a.v_nb_page, a.v_nb_head, voff); };
+    const uint32_t qs = (uint32_t)(uintptr_t)(lds_char*)lds, ring = qs + 32 * 2 * D + w * 2 * STAGE;
+    T tiles(a, it, kvh, lane);
     int t = it.t0 + w;
-    if (t < t1) fetch(t);
-    few_load_q<D, WAVES, 32>(a, it, kvh, rows, qs);
-    if (t < t1) {
-        issue_k(t, ring);
-        issue_v(t, ring);
-        if (t + WAVES < t1) {
-            fetch(t + WAVES);
-            issue_k(t + WAVES, ring + STAGE);
-            issue_v(t + WAVES, ring + STAGE);
-            wait_vm<4 * NL>();                     // Q
-        } else {
-            wait_vm<2 * NL>();
-        }
-    } else {
-        wait_vm<0>();
-    }
-    asm volatile("s_barrier" : : : "memory");
+    tiles.template begin<WAVES, 32, 2>(it, rows, t, qs, ring);
     // The keys of a tile in the order in which the transposing read of V gives
     // them: row x of the scores' operand is key x with bits 2 and 3 exchanged,
     // so a lane's accumulators are keys 16 kk + 8 half + 0 .. 7.  Of a block a lane
@@ -199,13 +225,10 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
         for (int e = 0; e < 2; ++e) qf[2 * b + e] = q_frag<KT, OT>(lds_read(qs + l32 * 2 * D + (((4 * b + 2 * half + e) ^ k_swz<D>(l32)) << 4)));
     const int lim = l32 < rows ? min(L - 1, past + div_g(a, l32)) : -1;   // the last key the lane's row sees
     const float sl2 = a.scale * kLog2e;
-    auto big = [&](uint32_t scales) {              // of a tile's scales (whole wave)
-        return (bool)__any(q8_big2(*(const __attribute__((address_space(3))) uint32_t*)lds_at(scales + (lane & (SB / 4 - 1)) * 4)));
-    };
     for (uint32_t st = ring; t < t1; t += WAVES, st = st == ring ? ring + STAGE : ring) {
         const bool one = t + WAVES < t1, two = t + 2 * WAVES < t1;
         const uint32_t ks = st + 2 * CB, vs = ks + SB;
-        if (two) fetch(t + 2 * WAVES);
+        if (two) tiles.fetch(t + 2 * WAVES);
         if (one) wait_vm<3 * NL>();                // K; V and the next tile may still fly
         else wait_vm<NL>();
         f32x16 s{};
@@ -231,7 +254,7 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
                 }
             };
             if constexpr (LO) {
-                if (!big(ks)) scores(std::true_type{});
+                if (!tiles.big(ks)) scores(std::true_type{});
                 else scores(std::false_type{});
             } else {
                 scores(std::false_type{});
@@ -239,7 +262,7 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
         }
         if (two) {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // K is read
-            issue_k(t + 2 * WAVES, st);
+            tiles.issue_k(t + 2 * WAVES, st);
         }
         const int k0 = t * kFewTile;
         const bool masked = k0 + kFewTile - 1 > min(L - 1, past);      // some row must not see some key
@@ -274,7 +297,7 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
                 }
             }
         };
-        if ((LO || masked) && big(vs)) {
+        if ((LO || masked) && tiles.big(vs)) {
             values(std::false_type{}, std::true_type{});
             if (masked) q8_add_not_finite<D, kFewTile>(st + CB, vs, k0, lim, half, r.o);
         } else {
@@ -282,9 +305,10 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
         }
         if (two) {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // V is read
-            issue_v(t + 2 * WAVES, st);
+            tiles.issue_v(t + 2 * WAVES, st);
         }
     }
+    r.bad = tiles.bad;
 }
 
 // The same for at most 16 rows (single tokens of up to 16 heads a group), with
@@ -299,76 +323,19 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
 //   C (16 x 16): column l16, register r holds row 4 g + r
 // Row x of score tile mt is key 8 (x / 4) + 4 mt + x % 4, so a lane's 8 scores are
 // keys 8 g .. 8 g + 7, the ones that the transposing read gives of a dim of V.
-template <int D> __device__ __forceinline__ int kq16_swz(int row) {
-    return D == 128 ? (row >> 2 & 6) | (row >> 1 & 1) : row >> 3 & 3;
-}
 template <int D, int OT, int WAVES, int STAGES>
 __device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D, 16>& r) {
+    using T = Q8Tiles<D, true>;
     constexpr int KT = VVA_TYPE_F16;
     constexpr bool LO = OT == VVA_TYPE_F16;
-    constexpr int NB = D / 32;                     // blocks of a row
-    constexpr int CB = kFewTile * D, SB = kFewTile * NB * 2;           // codes and scales of a tile
-    constexpr int STAGE = 2 * (CB + SB), QB = 16 * 2 * D;
-    constexpr int NC = CB / 1024, RC = 1024 / D;   // loads of a tile's codes, rows of one
-    constexpr int NL = NC + 1;                     // with its scales
-    constexpr int NV = 16 / RC;                    // loads of 16 keys
+    constexpr int NB = T::NB, CB = T::CB, SB = T::SB, STAGE = T::STAGE, NL = T::NL;
     const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int L = it.q.L, rows = min(it.q.n, a.max_new) * a.G, past = L - it.q.n, t1 = it.t1;
-    const ConstInts table = (ConstInts)(uintptr_t)(a.table + (int64_t)it.q.s * a.table_stride);
-    const int last_page = (L - 1) >> a.page_shift, page = 1 << a.page_shift;
-    const uint32_t qs = (uint32_t)(uintptr_t)(lds_char*)lds, ring = qs + QB + w * STAGES * STAGE;
-
-    int koff[NV], voff[NV];                        // codes: from the first slot of 16
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int row = i * RC + lane / (D / 16), c = lane % (D / 16);
-        koff[i] = row * D + ((c ^ kq16_swz<D>(row)) << 4);
-        voff[i] = row * D + ((c ^ kq_swz<D>(row)) << 4);
-    }
-    const int soff = page * D + (((lane >> 4) << a.page_shift) + 2 * (lane & 7)) * 2;   // scales: two keys of a block
-    int ids[2];                                    // pages of the two 16-key halves of the next tile to load
-    auto fetch = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) ids[i] = table[min((t * kFewTile + 16 * i) >> a.page_shift, last_page)];
-    };
-    // turn: what the swizzle of the upper 16 rows adds to that of the lower ones
-    auto issue = [&](int t, uint32_t codes, uint32_t scales, const char* pool, int64_t nb_page, int64_t nb_head, const int (&off)[NV], int turn) {
-        uint64_t run[2];
-        int slot[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const bool ok = (uint32_t)ids[i] < (uint32_t)a.n_pages;
-            r.bad = r.bad || !ok;
-            run[i] = uniform64((uint64_t)(uintptr_t)pool + (int64_t)(ok ? ids[i] : 0) * nb_page + kvh * nb_head);
-            slot[i] = (t * kFewTile + 16 * i) & (page - 1);
-        }
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-            dma16<true>(run[c / NV] + (uint64_t)slot[c / NV] * D, off[c % NV] ^ (c / NV ? turn : 0), codes + c * 1024);
-        const uint64_t s0 = run[0] + 2 * slot[0], s1 = run[1] + 2 * slot[1];
-        if (D == 128 || lane < 32) dma4<true>((lane & 8 ? s1 : s0) + soff, scales);
-    };
-    auto issue_k = [&](int t, uint32_t st) { issue(t, st, st + 2 * CB, a.k, a.k_nb_page, a.k_nb_head, koff, kq16_swz<D>(16) << 4); };
-    auto issue_v = [&](int t, uint32_t st) { issue(t, st + CB, st + 2 * CB + SB, a.v, a.v_nb_page, a.v_nb_head, voff, 0); };
+    const uint32_t qs = (uint32_t)(uintptr_t)(lds_char*)lds, ring = qs + 16 * 2 * D + w * STAGES * STAGE;
+    T tiles(a, it, kvh, lane);
     int t = it.t0 + w;
-    if (t < t1) fetch(t);
-    few_load_q<D, WAVES, 16>(a, it, kvh, rows, qs);
-    if (t < t1) {
-        issue_k(t, ring);
-        issue_v(t, ring);
-        if (STAGES == 2 && t + WAVES < t1) {
-            fetch(t + WAVES);
-            issue_k(t + WAVES, ring + STAGE);
-            issue_v(t + WAVES, ring + STAGE);
-            wait_vm<4 * NL>();                     // Q
-        } else {
-            wait_vm<2 * NL>();
-        }
-    } else {
-        wait_vm<0>();
-    }
-    asm volatile("s_barrier" : : : "memory");
+    tiles.template begin<WAVES, 16, STAGES>(it, rows, t, qs, ring);
     const int key = 8 * (l16 >> 2) + (l16 & 3);
     const int k_off = key * D + (((g >> 1) ^ kq16_swz<D>(key)) << 4) + 8 * (g & 1);
     const int v_row = 8 * g + (l16 >> 1);
@@ -378,13 +345,10 @@ __device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewIte
     for (int b = 0; b < NB; ++b) qf[b] = q_frag<KT, OT>(lds_read(qs + l16 * 2 * D + (((4 * b + g) ^ k_swz<D>(l16)) << 4)));
     const int lim = l16 < rows ? min(L - 1, past + div_g(a, l16)) : -1;   // the last key the lane's row sees
     const float sl2 = a.scale * kLog2e;
-    auto big = [&](uint32_t scales) {              // of a tile's scales (whole wave)
-        return (bool)__any(q8_big2(*(const __attribute__((address_space(3))) uint32_t*)lds_at(scales + (lane & (SB / 4 - 1)) * 4)));
-    };
     for (uint32_t st = ring; t < t1; t += WAVES, st = STAGES == 1 || st != ring ? ring : ring + STAGE) {
         const bool one = t + WAVES < t1, next = t + STAGES * WAVES < t1;
         const uint32_t ks = st + 2 * CB, vs = ks + SB;
-        if (next) fetch(t + STAGES * WAVES);
+        if (next) tiles.fetch(t + STAGES * WAVES);
         if (STAGES == 2 && one) wait_vm<3 * NL>(); // K; V and the next tile may still fly
         else wait_vm<NL>();
         f32x4 s[2] = {};
@@ -411,7 +375,7 @@ __device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewIte
                     }
             };
             if constexpr (LO) {
-                if (!big(ks)) scores(std::true_type{});
+                if (!tiles.big(ks)) scores(std::true_type{});
                 else scores(std::false_type{});
             } else {
                 scores(std::false_type{});
@@ -419,7 +383,7 @@ __device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewIte
         }
         if (next) {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // K is read
-            issue_k(t + STAGES * WAVES, st);
+            tiles.issue_k(t + STAGES * WAVES, st);
         }
         const int k0 = t * kFewTile;
         const bool masked = k0 + kFewTile - 1 > min(L - 1, past);      // some row must not see some key
@@ -469,7 +433,7 @@ __device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewIte
                 }
             }
         };
-        if ((LO || masked) && big(vs)) {
+        if ((LO || masked) && tiles.big(vs)) {
             values(std::false_type{}, std::true_type{});
             if (masked) {                          // a lane's dims of tile i: 16 i + 4 g ..
                 for (int j = 0; j < kFewTile; ++j) {
@@ -487,7 +451,8 @@ __device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewIte
         }
         if (next) {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // V is read
-            issue_v(t + STAGES * WAVES, st);
+            tiles.issue_v(t + STAGES * WAVES, st);
         }
     }
+    r.bad = tiles.bad;
 }
