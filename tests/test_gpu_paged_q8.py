@@ -383,6 +383,30 @@ def test_value_scale_that_is_not_finite_stays_with_the_rows_that_see_it(ctx, tor
     check_rows(out[:, :, keep], ref[:, :, keep], tol[:, :, keep])
 
 
+@pytest.mark.parametrize("lens,heads", [([(1, 70), (1, 33), (1, 2000)], H7), ([(4, 70), (2, 1)], H05), ([(4, 40)], H7), ([(60, 200), (1, 75)], H05), ([(300, 310)], H7)])
+@pytest.mark.parametrize("t", [vva.F16, vva.BF16])
+def test_what_lies_behind_a_sequence_does_not_change_a_bit(ctx, torch_gpu, lens, heads, t):
+    """Slots behind the keys: NaN scales, large ones, zeros; and later tokens' values past F16 leave the rows before them."""
+    torch = torch_gpu
+    P = Q8Pages(torch, lens, *heads, t, 16, seed=5)
+    outs = []
+    for scale in (float("nan"), 6e4, 0.0, float("inf")):
+        for s, (_, L) in enumerate(lens):
+            if L % 16:
+                for raw in P.raw:
+                    parts(raw, P.d)[1][int(P.table_host[s, L // 16]), :, :, L % 16:] = scale
+        outs.append(run_attn(ctx, P))
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
+    n, L = lens[0]
+    if n > 1:
+        for raw in P.raw:                                  # the last token's own row
+            parts(raw, P.d)[1][int(P.table_host[0, (L - 1) // 16]), :, :, (L - 1) % 16] = 6e4
+        out = torch.empty_like(P.q)
+        ctx.paged_attn(P.q, P.k, P.v, P.batch(), P.d ** -0.5, out)
+        torch.cuda.synchronize()
+        assert torch.equal(out[:n - 1], outs[0][:n - 1])
+
+
 @pytest.mark.parametrize("lens", [[(4, 70)], [(60, 200)]])
 def test_key_scale_that_is_not_finite_reaches_the_rows_that_see_it(ctx, torch_gpu, lens):
     torch = torch_gpu

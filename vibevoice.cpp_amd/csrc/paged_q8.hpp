@@ -70,6 +70,14 @@ __device__ __forceinline__ Q8Frag q8_frag(uint32_t c0, uint32_t c1, const h2 (&s
     }
     return f;
 }
+// The rest beside an operand whose values may be infinite or NaN: none where they are
+__device__ __forceinline__ u32x4 q8_rest(u32x4 hi, u32x4 lo) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r[i] = ((hi[i] & 0x7c00u) == 0x7c00u ? 0u : lo[i] & 0xffffu) | ((hi[i] & 0x7c000000u) == 0x7c000000u ? 0u : lo[i] & 0xffff0000u);
+    return r;
+}
 // whether either of two scales may take a code's value beyond F16, or is not finite
 __device__ __forceinline__ bool q8_big2(uint32_t x) { return (x & 0x7fffu) >= 0x6000u || ((x >> 16) & 0x7fffu) >= 0x6000u; }
 
@@ -240,21 +248,22 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
                 c[b] = lds_read((st + k_off) ^ (b << 5));
                 sc[b] = *(const __attribute__((address_space(3))) uint16_t*)lds_at(ks + b * kFewTile * 2 + key * 2);
             }
-            auto scores = [&](auto rest) {
+            auto scores = [&](auto care) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const h2 x = q8_scale(sc[b]);
                     const h2 x4[4] = {x, x, x, x};
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const Q8Frag f = q8_frag<decltype(rest)::value>(c[b][2 * e], c[b][2 * e + 1], x4);
+                        Q8Frag f = q8_frag<LO>(c[b][2 * e], c[b][2 * e + 1], x4);
+                        if constexpr (decltype(care)::value) f.lo = q8_rest(f.hi, f.lo);
                         s = F::mma(as_vec<h8>(f.hi), qf[2 * b + e], s);
-                        if constexpr (decltype(rest)::value) s = F::mma(as_vec<h8>(f.lo), qf[2 * b + e], s);
+                        if constexpr (LO) s = F::mma(as_vec<h8>(f.lo), qf[2 * b + e], s);
                     }
                 }
             };
             if constexpr (LO) {
-                if (!tiles.big(ks)) scores(std::true_type{});
+                if (tiles.big(ks)) scores(std::true_type{});
                 else scores(std::false_type{});
             } else {
                 scores(std::false_type{});
@@ -278,7 +287,7 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
         else wait_vm<0>();
         // the products straight through; a tile with a value that is not finite, or
         // near the end of F16, by a path of its own
-        auto values = [&](auto rest, auto fix) {
+        auto values = [&](auto care) {
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 const h8 pf = as_vec<h8>(u32x4{p[4 * kk], p[4 * kk + 1], p[4 * kk + 2], p[4 * kk + 3]});
@@ -288,20 +297,21 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
                         (__attribute__((address_space(3))) i32x2*)lds_at(((st + CB + v_off) ^ (dt << 5)) + kk * 16 * D));
                     const u32x4 sc = lds_read(vs + dt * kFewTile * 2 + kk * 32 + half * 16);
                     const h2 x4[4] = {as_h2(sc.x), as_h2(sc.y), as_h2(sc.z), as_h2(sc.w)};
-                    Q8Frag f = q8_frag<decltype(rest)::value>((uint32_t)c.x, (uint32_t)c.y, x4);
-                    if constexpr (decltype(fix)::value) {
+                    Q8Frag f = q8_frag<LO>((uint32_t)c.x, (uint32_t)c.y, x4);
+                    if constexpr (decltype(care)::value) {
+                        if constexpr (LO) f.lo = q8_rest(f.hi, f.lo);
                         if (masked) f.hi = u32x4{finite2<KT>(f.hi.x), finite2<KT>(f.hi.y), finite2<KT>(f.hi.z), finite2<KT>(f.hi.w)};
                     }
                     r.o[dt] = F::mma(as_vec<h8>(f.hi), pf, r.o[dt]);
-                    if constexpr (decltype(rest)::value) r.o[dt] = F::mma(as_vec<h8>(f.lo), pf, r.o[dt]);
+                    if constexpr (LO) r.o[dt] = F::mma(as_vec<h8>(f.lo), pf, r.o[dt]);
                 }
             }
         };
         if ((LO || masked) && tiles.big(vs)) {
-            values(std::false_type{}, std::true_type{});
+            values(std::true_type{});
             if (masked) q8_add_not_finite<D, kFewTile>(st + CB, vs, k0, lim, half, r.o);
         } else {
-            values(std::integral_constant<bool, LO>{}, std::false_type{});
+            values(std::false_type{});
         }
         if (two) {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // V is read
@@ -362,20 +372,21 @@ __device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewIte
                     c[b][mt] = *(const __attribute__((address_space(3))) u32x2*)lds_at(((st + k_off) ^ (b << 5)) + mt * 4 * D);
                     sc[b][mt] = *(const __attribute__((address_space(3))) uint16_t*)lds_at(ks + b * kFewTile * 2 + (key + 4 * mt) * 2);
                 }
-            auto scores = [&](auto rest) {
+            auto scores = [&](auto care) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt) {
                         const h2 x = q8_scale(sc[b][mt]);
                         const h2 x4[4] = {x, x, x, x};
-                        const Q8Frag f = q8_frag<decltype(rest)::value>(c[b][mt].x, c[b][mt].y, x4);
+                        Q8Frag f = q8_frag<LO>(c[b][mt].x, c[b][mt].y, x4);
+                        if constexpr (decltype(care)::value) f.lo = q8_rest(f.hi, f.lo);
                         s[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_vec<h8>(f.hi), qf[b], s[mt], 0, 0, 0);
-                        if constexpr (decltype(rest)::value) s[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_vec<h8>(f.lo), qf[b], s[mt], 0, 0, 0);
+                        if constexpr (LO) s[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_vec<h8>(f.lo), qf[b], s[mt], 0, 0, 0);
                     }
             };
             if constexpr (LO) {
-                if (!tiles.big(ks)) scores(std::true_type{});
+                if (tiles.big(ks)) scores(std::true_type{});
                 else scores(std::false_type{});
             } else {
                 scores(std::false_type{});
@@ -416,7 +427,7 @@ __device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewIte
         else wait_vm<0>();
         // the products straight through; a tile with a value that is not finite, or
         // near the end of F16, by a path of its own
-        auto values = [&](auto rest, auto fix) {
+        auto values = [&](auto care) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const u32x4 sc = lds_read(vs + b * kFewTile * 2 + g * 16);
@@ -424,17 +435,18 @@ __device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewIte
 #pragma unroll
                 for (int i = 2 * b; i < 2 * b + 2; ++i) {
                     const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)lds_at((st + CB + v_off) ^ (i << 4)));
-                    Q8Frag f = q8_frag<decltype(rest)::value>((uint32_t)c.x, (uint32_t)c.y, x4);
-                    if constexpr (decltype(fix)::value) {
+                    Q8Frag f = q8_frag<LO>((uint32_t)c.x, (uint32_t)c.y, x4);
+                    if constexpr (decltype(care)::value) {
+                        if constexpr (LO) f.lo = q8_rest(f.hi, f.lo);
                         if (masked) f.hi = u32x4{finite2<KT>(f.hi.x), finite2<KT>(f.hi.y), finite2<KT>(f.hi.z), finite2<KT>(f.hi.w)};
                     }
                     r.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_vec<h8>(f.hi), pf, r.o[i], 0, 0, 0);
-                    if constexpr (decltype(rest)::value) r.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_vec<h8>(f.lo), pf, r.o[i], 0, 0, 0);
+                    if constexpr (LO) r.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_vec<h8>(f.lo), pf, r.o[i], 0, 0, 0);
                 }
             }
         };
         if ((LO || masked) && tiles.big(vs)) {
-            values(std::false_type{}, std::true_type{});
+            values(std::true_type{});
             if (masked) {                          // a lane's dims of tile i: 16 i + 4 g ..
                 for (int j = 0; j < kFewTile; ++j) {
                     const bool seen = k0 + j <= lim;
@@ -447,7 +459,7 @@ __device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewIte
                 }
             }
         } else {
-            values(std::integral_constant<bool, LO>{}, std::false_type{});
+            values(std::false_type{});
         }
         if (next) {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // V is read
