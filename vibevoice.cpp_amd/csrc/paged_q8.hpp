@@ -113,8 +113,9 @@ __device__ __forceinline__ void q8_add_not_finite(uint32_t v_lds, uint32_t s_lds
 
 // A wave's tiles of 32 keys of a sequence and kv head, from the pages into LDS
 // stages: the codes of K, of V, then the scales of K, of V.  ROWS16: for products of
-// 16 rows.
-template <int D, bool ROWS16>
+// 16 rows.  HOLD: the lane's offsets stay in registers through the tiles, where there
+// are any left (made anew for each tile: 48 sequences 46.2 -> 46.8 us).
+template <int D, bool ROWS16, bool HOLD>
 struct Q8Tiles {
     static constexpr int NB = D / 32;              // blocks of a row
     static constexpr int CB = kFewTile * D, SB = kFewTile * NB * 2;    // codes and scales of a tile
@@ -125,32 +126,23 @@ struct Q8Tiles {
 
     const PagedArgs& a;
     const ConstInts table;
-    const int kvh, last_page, lane;
-    int koff[NV], voff[NV];                        // codes: from the first slot of 16
-    int soff;                                      // scales: two keys of a block
+    const int kvh, last_page, held;
     int ids[2];                                    // pages of the two 16-key halves of the next tile to load
     bool bad = false;
 
     static __device__ __forceinline__ int k_swz(int row) { return ROWS16 ? kq16_swz<D>(row) : kq_swz<D>(row); }
     static __device__ __forceinline__ int v_swz(int row) { return ROWS16 ? kq_swz<D>(row) : vq_swz<D>(row); }
 
-    __device__ __forceinline__ Q8Tiles(const PagedArgs& args, const FewItem& it, int head, int l)
+    __device__ __forceinline__ Q8Tiles(const PagedArgs& args, const FewItem& it, int head, int lane)
         : a(args), table((ConstInts)(uintptr_t)(args.table + (int64_t)it.q.s * args.table_stride)), kvh(head),
-          last_page((it.q.L - 1) >> args.page_shift), lane(l) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int row = i * RC + lane / (D / 16), c = lane % (D / 16);
-            koff[i] = row * D + ((c ^ k_swz(row)) << 4);
-            voff[i] = row * D + ((c ^ v_swz(row)) << 4);
-        }
-        soff = (D << a.page_shift) + (((lane >> 4) << a.page_shift) + 2 * (lane & 7)) * 2;
-    }
+          last_page((it.q.L - 1) >> args.page_shift), held(lane) {}
     __device__ __forceinline__ void fetch(int t) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) ids[i] = table[min((t * kFewTile + 16 * i) >> a.page_shift, last_page)];
     }
-    // turn: what the swizzle of the upper 16 rows adds to that of the lower ones
-    __device__ __forceinline__ void issue(int t, uint32_t codes, uint32_t scales, const char* pool, int64_t nb_page, int64_t nb_head, const int (&off)[NV], int turn) {
+    template <bool V>
+    __device__ __forceinline__ void issue(int t, uint32_t codes, uint32_t scales, const char* pool, int64_t nb_page, int64_t nb_head) {
+        const int lane = HOLD ? held : lane_id();
         uint64_t run[2];
         int slot[2];
 #pragma unroll
@@ -161,13 +153,19 @@ struct Q8Tiles {
             slot[i] = (t * kFewTile + 16 * i) & ((1 << a.page_shift) - 1);
         }
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-            dma16<true>(run[c / NV] + (uint64_t)slot[c / NV] * D, off[c % NV] ^ (c / NV ? turn : 0), codes + c * 1024);
+        for (int c = 0; c < NC; ++c) {
+            // of the load's rows, in their 16-key half; the swizzle of the upper half is the lower one's with bits turned
+            const int row = c % NV * RC + lane / (D / 16), chunk = (lane % (D / 16)) ^ (V ? v_swz(row) : k_swz(row));
+            const int turn = c / NV ? (V ? v_swz(16) : k_swz(16)) : 0;
+            dma16<true>(run[c / NV] + (uint64_t)slot[c / NV] * D, (row * D + chunk * 16) ^ (turn << 4), codes + c * 1024);
+        }
+        // two keys of a block a lane
         const uint64_t s0 = run[0] + 2 * slot[0], s1 = run[1] + 2 * slot[1];
+        const int soff = (D << a.page_shift) + (((lane >> 4) << a.page_shift) + 2 * (lane & 7)) * 2;
         if (D == 128 || lane < 32) dma4((lane & 8 ? s1 : s0) + soff, scales);
     }
-    __device__ __forceinline__ void issue_k(int t, uint32_t st) { issue(t, st, st + 2 * CB, a.k, a.k_nb_page, a.k_nb_head, koff, k_swz(16) << 4); }
-    __device__ __forceinline__ void issue_v(int t, uint32_t st) { issue(t, st + CB, st + 2 * CB + SB, a.v, a.v_nb_page, a.v_nb_head, voff, v_swz(16) << 4); }
+    __device__ __forceinline__ void issue_k(int t, uint32_t st) { issue<false>(t, st, st + 2 * CB, a.k, a.k_nb_page, a.k_nb_head); }
+    __device__ __forceinline__ void issue_v(int t, uint32_t st) { issue<true>(t, st + CB, st + 2 * CB + SB, a.v, a.v_nb_page, a.v_nb_head); }
     // The rows of Q, and the first tiles (t, t + WAVES) into the ring's stages, until Q has landed
     template <int WAVES, int ROWS, int STAGES>
     __device__ __forceinline__ void begin(const FewItem& it, int rows, int t, uint32_t qs, uint32_t ring) {
@@ -191,7 +189,7 @@ struct Q8Tiles {
     }
     // whether a tile's scales may take a value beyond F16 or are not finite (whole wave)
     __device__ __forceinline__ bool big(uint32_t scales) const {
-        return (bool)__any(q8_big2(*(const __attribute__((address_space(3))) uint32_t*)lds_at(scales + (lane & (SB / 4 - 1)) * 4)));
+        return (bool)__any(q8_big2(*(const __attribute__((address_space(3))) uint32_t*)lds_at(scales + ((HOLD ? held : lane_id()) & (SB / 4 - 1)) * 4)));
     }
 };
 
@@ -207,9 +205,9 @@ struct Q8Tiles {
 template <int D, int OT, int WAVES>
 __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D, 32>& r) {
     using F = Frag<VVA_TYPE_F16>;
-    using T = Q8Tiles<D, false>;
     constexpr int KT = VVA_TYPE_F16;
     constexpr bool LO = OT == VVA_TYPE_F16;
+    using T = Q8Tiles<D, false, true>;
     constexpr int NB = T::NB, CB = T::CB, SB = T::SB, STAGE = T::STAGE, NL = T::NL;
     const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -335,9 +333,9 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
 // keys 8 g .. 8 g + 7, the ones that the transposing read gives of a dim of V.
 template <int D, int OT, int WAVES, int STAGES>
 __device__ __forceinline__ void few_stream16_q8(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D, 16>& r) {
-    using T = Q8Tiles<D, true>;
     constexpr int KT = VVA_TYPE_F16;
     constexpr bool LO = OT == VVA_TYPE_F16;
+    using T = Q8Tiles<D, true, !(LO && D == 128)>;
     constexpr int NB = T::NB, CB = T::CB, SB = T::SB, STAGE = T::STAGE, NL = T::NL;
     const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
