@@ -147,4 +147,5 @@ def quantise(x: np.ndarray):
         z = b * np.where(d > 0, np.float32(1) / d, np.float32(0))
     low = np.floor(np.abs(z))
     codes = np.sign(z) * (low + (np.abs(z) - low >= 0.5))
-    return codes.astype(np.int8).reshape(x.shape), d[..., 0].astype(np.float16)
+    with np.errstate(over="ignore"):                      # scales beyond F16 are infinite
+        return codes.astype(np.int8).reshape(x.shape), d[..., 0].astype(np.float16)
