@@ -407,7 +407,7 @@ VVA_API vva_status vva_paged_rope_append(vva_context* ctx, const vva_tensor* q, 
  * are taken as F16 too (their 8 bits are kept from 2^-17 to 65504).  With F16 q,
  * what that rounding of K and V leaves goes into the products as well where a
  * sequence's new tokens times Hq / Hkv are at most 32 (as above).
- * Every row of q and out and every page row starts on 16 bytes.
+ * Every row of q and out and every page row (Q8_0: run) starts on 16 bytes.
  * Partial sums go through the context's workspace, as those of the other
  * calls: under stream capture a call larger than any before it is refused
  * (VVA_ERR_INVALID_ARG), and graphs captured from one context are replayed one
