@@ -731,7 +731,8 @@ __device__ __forceinline__ void few_piece(const PagedArgs& a, float* __restrict_
     }
 }
 
-// One workgroup per (piece, kv head), two of them (D = 64: four) on a CU.
+// One workgroup per (piece, kv head), two of them on a CU (D = 64, 4 waves: four over
+// 16-bit pages, three over Q8_0 ones).
 template <int D, int PT, int OT, int WAVES, int ROWS>
 __global__ void __launch_bounds__(WAVES * 64, WAVES == 8 ? 4 : 2) paged_few_kernel(PagedArgs a, float* __restrict__ ws, unsigned* tickets, int slots, int cap) {
     prefetch_kernargs<sizeof(PagedArgs)>();
@@ -1673,8 +1674,12 @@ PagedPlan paged_plan(const PagedArgs& a, int n_cu) {
         // into that few (48 of 500 to 8000 keys: 94.2 -> 79.3)
         // Q8_0 pages and at most 16 rows: twice the waves in a workgroup
         p.few_waves = a.type == VVA_TYPE_Q8_0 && rows <= 16 ? 8 : kFewWaves;
+        // of 17 to 32 rows of 64 dims over Q8_0 pages three fit, by their registers: two are
+        // taken, for many sequences too (0.5B heads, 4 tokens, us with 4, 3 and 2: 130 sequences
+        // of up to 4000 keys 36.9, 37.6, 32.8, 256 of up to 1000 28.7, 27.1, 22.0)
+        const bool two = a.type == VVA_TYPE_Q8_0 && a.d == 64 && p.few_waves == kFewWaves;
         const int slots = std::min(n_cu, kMaxWgs) * (a.d == 64 && p.few_waves == kFewWaves ? 2 : 1);
-        p.few_slots = std::max(1, (2 * a.n_seq * a.Hkv > slots ? 2 : 1) * slots / a.Hkv);
+        p.few_slots = std::max(1, (2 * a.n_seq * a.Hkv > slots && !two ? 2 : 1) * slots / a.Hkv);
         const int64_t seq_tiles = (max_keys + kFewTile - 1) / kFewTile;
         p.few_split = seq_tiles > (p.many_wgs > 0 ? kFewWaves : p.few_waves);
         p.few_pieces = (int)std::min<int64_t>(p.few_slots + (int64_t)a.n_seq, a.n_seq * ((seq_tiles + p.few_waves - 1) / p.few_waves));
