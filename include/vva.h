@@ -425,7 +425,13 @@ VVA_API vva_status vva_paged_attn(vva_context* ctx, const vva_tensor* q, const v
  * kv_len[s] the whole sequence.  Rows whose page id is outside the pool, and
  * those of keys before key 0, get NaN; rows of no sequence are left as they were.
  * All tokens of a sequence are read, whatever max_new is.  The outputs lie apart
- * from the pages, the batch and each other (k and v may interleave). */
+ * from the pages, the batch and each other (k and v may interleave).
+ * Rows go back into pages by vva_paged_rope_append with a table of one row, d / 2
+ * ones and d / 2 zeros, and pos 0 for each (q: k itself; q_out: scratch of as
+ * many rows): finite rows are stored as they are.  Blocks of Q8_0 pages that the
+ * append wrote come back bit for bit from F32 rows where their scale is finite
+ * and above 0, or they hold zeros or an infinity or NaN; not those whose scale
+ * rounded to 0 (all codes 0) or to infinity (NaN). */
 VVA_API vva_status vva_paged_read(vva_context* ctx, const vva_batch* batch, const vva_tensor* k_pages,
                                   const vva_tensor* v_pages, const vva_tensor* k, const vva_tensor* v);
 
