@@ -1,9 +1,10 @@
-"""Rows read back out of Q8_0 pages go into pages again, bit for bit: vva_paged_rope_append with one row of the rope table, of
+"""Rows read back out of pages go into pages again, bit for bit: vva_paged_rope_append with one row of the rope table, of
 ones, then zeros, for every token (a rotation by nothing)."""
 import pytest
 
 import vva
 from paged_q8_util import Q8Pages, parts
+from paged_util import Pages
 from test_gpu_paged_q8 import append
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +89,20 @@ def test_16_bit_rows_round_the_values_once_more(ctx, torch_gpu):
     for which in (0, 1):
         (c, s), (c2, s2) = rows(P, which), rows(to, which)
         assert torch.equal(c, c2) and int((s.int() - s2.int()).abs().max()) <= 1
+
+
+@pytest.mark.parametrize("t", [vva.F16, vva.BF16])
+def test_16_bit_pages_come_back(ctx, torch_gpu, t):
+    torch = torch_gpu
+    lens = [(40, 40), (1, 1), (77, 77)]
+    P, to = Pages(torch, lens, *H05, t, 16, seed=3), Pages(torch, lens, 2, 2, 64, t, 32, seed=4)
+    k, v = (torch.empty(P.n_tok, 2, 64, dtype=P.q.dtype, device="cuda") for _ in range(2))
+    ctx.paged_read(P.batch(), P.k, P.v, k=k, v=v)
+    rope = torch.zeros(1, 64, device="cuda")
+    rope[:, :32] = 1.0
+    pos = torch.zeros(P.n_tok, dtype=torch.int32, device="cuda")
+    ctx.paged_rope_append(k, k, v, rope, to.batch(), to.k, to.v, torch.empty_like(k), pos=pos)
+    torch.cuda.synchronize()
+    for s in range(3):
+        for kvh in range(2):
+            assert torch.equal(P.keys(s, P.k, kvh), to.keys(s, to.k, kvh)) and torch.equal(P.keys(s, P.v, kvh), to.keys(s, to.v, kvh))
