@@ -62,8 +62,9 @@ __device__ __forceinline__ void store8_q8(char* tile, int d, int page_shift, int
 
 // One workgroup per token row, a thread per 8 rotation pairs (elements i ..
 // i + 7 and i + P .. of a head); no head's item crosses a wave's table lookup.
-// HBM-bound (4k tokens, F32 rows of 7B heads: 27.4 us, 4.7 TB/s, 28.1 into Q8_0
-// pages; one pair per thread 78); a short call is a chain of two round trips: the
+// HBM-bound (4k tokens, F32 rows of 7B heads, three sets of tensors by turns: 27.4 us,
+// 4.7 TB/s, 28.2 into Q8_0 pages, 23.3 over one set that the last-level cache holds;
+// one pair per thread 78); a short call is a chain of two round trips: the
 // batch, with the token's own rows under way, then the page id and the row of the
 // rope table.
 // IO: the type of q, k and v where it is one, else -1 (types looked up by the lane
@@ -183,8 +184,8 @@ __global__ void __launch_bounds__(512) paged_append_kernel(PagedAppendArgs a) {
 
 // Rows read back: one workgroup per kReadTokens token rows, a wave for every
 // fourth of them, whose loads go out together; a lane takes 8 elements of a K or V
-// row at a time.  HBM-bound: 20k tokens of 7B heads from Q8_0 pages to BF16 (63 MB)
-// 12.8 us, a copy's 4.9 TB/s; a short call is the launch and three round trips
+// row at a time.  HBM-bound: 20k tokens of 7B heads to BF16, from Q8_0 pages (63 MB)
+// 12.8 us, a copy's 4.9 TB/s, from F16 pages (82 MB) 18.0, 4.6; a short call is the launch and three round trips
 // (333 tokens 4.3 us).
 constexpr int kReadTokens = 16, kReadWaves = 4;
 

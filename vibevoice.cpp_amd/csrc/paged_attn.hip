@@ -17,9 +17,9 @@
 //
 // Reached, of a copy's 4.9 TB/s and a large product's 1175 TFLOP/s: single
 // tokens 5.5 TB/s (48 sequences of 500 to 8000 keys, 405 MB, 73 us); 2048 tokens
-// behind 28672 keys 991 TFLOP/s (880 us), 512 behind 15872 858 (138 us).  Over
-// Q8_0 pages: the 48 sequences (216 MB) 46.4 us, one of 30k keys 14.5 (16-bit pages
-// 17.4); the chunks 885 and 142 us where 16-bit pages take 852 and 136.
+// behind 28672 keys 976 to 1026 TFLOP/s from GPU to GPU (893 to 850 us), 512 behind
+// 15872 829 to 868 (143 to 136).  Over Q8_0 pages: the 48 sequences (216 MB) 46.4 us,
+// one of 30k keys 14.5 (16-bit pages 17.4); the chunks 880 to 922 and 142 to 147 us.
 //
 // Both compute, per 32 rows and a tile of keys, with
 // v_mfma_f32_32x32x16_{f16,bf16} (layouts in mfma_ops.hpp):
@@ -1126,9 +1126,9 @@ __device__ __forceinline__ void many_share(const PagedArgs& a, float* __restrict
     };
     // Q8_0: a wave takes 8 rows of a tile (D = 64: K by the lower lanes, V by the
     // upper), a lane 16 dims of one of K and one of V: loaded a step before they are
-    // converted to F16 and stored, at the start of a step.  2048 tokens behind 28672
-    // keys take 915 us so (F16 pages, whose rows go into LDS by themselves, 870); by
-    // half of the waves at the end of the step 934, between the products 960, rows of
+    // converted to F16 and stored, at the start of a step.  On one GPU, 2048 tokens
+    // behind 28672 keys: 915 us so (F16 pages, whose rows go into LDS by themselves,
+    // 870); by half of the waves at the end of the step 934, between the products 960, rows of
     // 8 dims a lane, whose stores meet on no banks but take two loads each, 928.
     constexpr int QC = D / 16, QN = D == 128 ? 2 : 1;
     u32x4 codes[QN];
@@ -1589,7 +1589,9 @@ __device__ __forceinline__ bool few_share(const PagedArgs& a, float* __restrict_
 // have brought more 10 -> 13, 64 x 4096 alone 90 -> 85.
 // Time of a few-row tile to that of a key tile of a row tile (0.16 and 0.22: D =
 // 64, 64 x 2000 keys and 512 tokens 21.9 and 25.4 us; D = 128, 60 sequences of up
-// to 8000 and 700 behind 2000 105 and 97):
+// to 8000 and 700 behind 2000 105 and 97), over 16-bit pages.  Q8_0 ones take the
+// same: neither it nor the costs that are counted in tiles (kFewCost, kFewSnap,
+// kRowTileCost) was fitted for them.
 template <int D>
 constexpr float kFewTime = D == 64 ? 0.16f : 0.22f;
 template <int D, int PT, int OT>

@@ -199,9 +199,11 @@ struct Q8Tiles {
 // LO: the rounding of scale times code to F16 goes into the products as well,
 // in a second one with the rest, so that K and V are what the pages hold but for
 // 2^-22: results rounded to F16 show it (error of a 30k-key step 4.1e-4 of its
-// size without, 2.8e-4 with, of which the rounding of the result is 2.1e-4; BF16
+// size without, 2.7e-4 with, of which the rounding of the result is 2.1e-4; BF16
 // ones do not).  Against tiles converted to F16 on their way into LDS, one under
-// way: 48 sequences of 500 to 8000 keys (215 MB) 61.4 -> 48.1 us.
+// way: 48 sequences of 500 to 8000 keys (216 MB) 61.4 -> 48.1 us.  4 tokens a
+// sequence, 7B heads: 48 of them 51.7 us (BF16), 60.2 (F16, whose second products
+// show), one behind 30k keys 24.9.
 template <int D, int OT, int WAVES>
 __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem& it, int kvh, char* lds, FewSums<D, 32>& r) {
     using F = Frag<VVA_TYPE_F16>;
@@ -326,7 +328,9 @@ __device__ __forceinline__ void few_stream_q8(const PagedArgs& a, const FewItem&
 // (two of 64), 4 waves per SIMD.  Against 32 rows and half the waves, us: 30k keys
 // 17.4 -> 14.9; 12 sequences of up to 8000 keys 20.5 -> 16.4, 48 48.1 -> 46.3; 24 of
 // the 1.5B model 20.0 -> 16.0.  In workgroups of one per CU, beside many rows, it was
-// slower (48 sequences 51 -> 57): those keep 32 rows.  Layouts (lane l, l16 = l % 16, g = l / 16):
+// slower (48 sequences 51 -> 57): those keep 32 rows.  Of 128 dims it takes 128 of 128
+// VGPRs and one spilled register, 8 bytes of scratch a lane: built with 162 and none
+// spilled, on as many workgroups, 30k keys 15.1 -> 15.6 us, 40 keys 6.1 -> 6.4.  Layouts (lane l, l16 = l % 16, g = l / 16):
 //   A (16 x 32): row l16, k = 8 g .. 8 g + 7     B (32 x 16): column l16, the same k
 //   C (16 x 16): column l16, register r holds row 4 g + r
 // Row x of score tile mt is key 8 (x / 4) + 4 mt + x % 4, so a lane's 8 scores are
